@@ -39,6 +39,7 @@ extern "C" {
 #define WRS_F32 0
 #define WRS_F16 1
 #define WRS_BF16 2
+#define WRS_MX4 3 /* packed MXFP4 rows: input of wrs_linear_mx4 only */
 
 typedef struct wrs_attn_ctx wrs_attn_ctx;
 typedef struct wrs_kv wrs_kv;
@@ -93,7 +94,7 @@ const char *wrs_attn_status_string(int status);
  * reference allocates per call on the host). Device-resident entry points
  * never allocate once their sizes are reserved; a call that would grow
  * scratch while the context's stream records a graph fails with
- * WRS_ECAPTURE instead. Three exceptions need no reservation:
+ * WRS_ECAPTURE instead. Four exceptions need no reservation:
  * 16-bit prefill grids of fewer 128-query blocks than half the CUs merge
  * blocks split over two workgroups through a fixed context buffer (~9 MB on
  * 256 CUs), allocated by the first such call outside capture; during capture
@@ -101,7 +102,9 @@ const char *wrs_attn_status_string(int status);
  * than 8 rows over n_in >= 2048 whose tiles cover less than half the CUs, which
  * split k through another fixed buffer (~8 MB on 256 CUs) under the same rule;
  * and fused norms of decode rows over many features (wrs_linear_fused), likewise
- * (reserving linear_tokens allocates both). Switching streams
+ * (reserving linear_tokens allocates both). Tree attention splits long caches through
+ * a third one (~9 MB, which reserving heads with decode rows and keys allocates too)
+ * and, captured before it exists, runs unsplit. Switching streams
  * (wrs_attn_set_stream) drains the old stream unless either stream is
  * recording a graph. Zero fields are ignored; reserving never shrinks.
  * Synchronous. */
@@ -226,6 +229,17 @@ int wrs_kv_slide_to_fit(wrs_kv *kv, size_t slot, size_t n_new, size_t max_ctx, s
 int wrs_kv_append(wrs_kv *kv, size_t layer, size_t slot, const float *k_rows,
                   const float *v_rows, size_t n, int src_on_host);
 int wrs_kv_advance(wrs_kv *kv, size_t slot, size_t n);
+/* The rows of an accepted path of a drafted tree (wrs_attn_tree_self) come
+ * together behind their slot's history: for every layer and head, K and V, row
+ * slot_len + j becomes what row slot_len + rows[j] held. counts[i] rows of
+ * slots[i], packed in `rows` (host arrays), rising within a slot; each slot once.
+ * Rows behind the kept ones are undefined afterwards; slot lengths are left, so
+ * that wrs_kv_advance takes the path in. n_rows is the sum of counts; a row lies
+ * within max_ctx and at most 65535 past the length. Every argument is checked
+ * before any row moves. No reference counterpart: the reference's cache keeps one
+ * candidate per slot. */
+int wrs_kv_keep_rows(wrs_kv *kv, const size_t *slots, const size_t *counts, size_t n_slots,
+                     const size_t *rows, size_t n_rows);
 /* Store of precompute_cross_attn (decoder.rs:423-447): f32 [n_audio][d_model]
  * K and V of one layer, into the head planes (converted to f16, or copied). */
 int wrs_kv_set_cross(wrs_kv *kv, size_t layer, const float *k, const float *v, size_t n_audio,
@@ -281,6 +295,24 @@ int wrs_attn_prefill_self(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, size_t sl
                           const float *q, size_t n_tokens, float *out);
 int wrs_attn_prefill_cross(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const float *q,
                            size_t n_tokens, float *out); /* q 16-byte aligned */
+/* Self-attention of drafted tokens: what decoder.rs:613-647 computes for a chain,
+ * for trees of drafted continuations, so that one pass over the weights checks
+ * several of them. Tree i holds n_nodes[i] rows (0..256) of slots[i] (host arrays;
+ * a slot may carry several trees), whose K/V rows wrs_kv_append stored at the
+ * slot's length (not advanced). `parents` is a device array of int32, one per row
+ * in the order of q, read when the call runs (a replayed graph takes new trees):
+ * row r of a tree hangs from row parents[r] of the same tree if that is in [0, r),
+ * from the last cached token otherwise, and attends the slot's slot_len rows, its
+ * ancestors and itself. Rows of q and out ([sum of n_nodes][d_model] f32, device)
+ * lie q_row_stride and out_row_stride elements apart, so that q may lie in wider
+ * rows. Values of rows that a row does not see never reach it, infinities and NaN
+ * among them; a row whose visible scores are all -infinity is zero, and one with
+ * a NaN among them NaN. Any arena, up to 2^24 - 4096 keys. No reference counterpart:
+ * the reference decodes one token per beam and step. */
+int wrs_attn_tree_self(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const size_t *slots,
+                       const size_t *n_nodes, size_t n_trees, const void *parents,
+                       size_t parents_len, const float *q, int64_t q_row_stride, float *out,
+                       int64_t out_row_stride);
 /* wrs_attn_prefill_cross (the multi_head_attention call of decoder.rs:698-708)
  * that also writes each row's softmax statistics for
  * wrs_attn_capture_cross_heads_lse: lse is an f32
@@ -385,6 +417,40 @@ int wrs_layer_norm(wrs_attn_ctx *ctx, const float *x, size_t x_len, const float 
 /* pub fn gelu_inplace(data) -- crates/tensor/src/ops/gelu.rs:11-23, tanh form,
  * in place on device f32. */
 int wrs_gelu_inplace(wrs_attn_ctx *ctx, float *data, size_t n);
+
+/* ---- projections with MXFP4 weights (asynchronous) ----------------------
+ * Rows of 4-bit values in blocks of 32 that share a scale (OCP Microscaling
+ * Formats v1.0, MXFP4): 17/32 byte a weight, 3.76 times fewer than f16, for decode
+ * steps that the weight stream bounds. The reference's own 4-bit weights are ggml's
+ * (LinearWeight, crates/tensor/src/weight.rs:116-137); this is the format whose
+ * products the GPU's matrix pipe takes as they are.
+ * Rows are packed: codes [n_rows][n_cols / 2] bytes, the even column in the low
+ * half (e2m1: 0 .5 1 1.5 2 3 4 6, bit 3 the sign), scales [n_rows][n_cols / 32]
+ * bytes (e8m0: 2^(byte - 127), 255 NaN). Codes and the f32 / f16 / bf16 rows are
+ * 16-byte aligned device memory; row strides and lengths in elements (codes_len,
+ * scales_len in bytes).
+ * wrs_mx4_quantize: per block the scale 2^(floor(log2(largest)) - 2), at least
+ * 2^-127, and the nearest codes, ties to the even one, 6 the largest; a block with
+ * an infinity or NaN gets the NaN scale and codes of 0. n_cols % 32 == 0.
+ * wrs_mx4_dequantize: the values, rounded once to out_dtype. */
+int wrs_mx4_quantize(wrs_attn_ctx *ctx, int x_dtype, const void *x, size_t x_len,
+                     int64_t x_row_stride, size_t n_rows, size_t n_cols, void *codes,
+                     size_t codes_len, void *scales, size_t scales_len);
+int wrs_mx4_dequantize(wrs_attn_ctx *ctx, const void *codes, size_t codes_len, const void *scales,
+                       size_t scales_len, size_t n_rows, size_t n_cols, int out_dtype, void *out,
+                       size_t out_len, int64_t out_row_stride);
+/* out[g](t, r) = act(w[g][r] . x[t] + bias[g][r]) for up to 8 weight matrices of one
+ * shape (w[g], w_scales[g]: MXFP4 rows [n_out][n_in]) in one launch, in the layout
+ * and with the activations of wrs_linear_fused; sums in f32, one rounding to
+ * out_dtype (WRS_F32, WRS_F16, WRS_BF16). x is f32, f16 or bf16 rows x_row_stride
+ * apart (x_scales NULL), or with x_dtype WRS_MX4 packed MXFP4 rows (x_row_stride ==
+ * n_in, x_len in values). bias may be NULL, or hold NULL entries. n_in % 64 == 0;
+ * any n_out. */
+int wrs_linear_mx4(wrs_attn_ctx *ctx, int x_dtype, const void *x, const void *x_scales,
+                   size_t x_len, int64_t x_row_stride, size_t n_groups, const void *const *w,
+                   const void *const *w_scales, const float *const *bias, size_t n_tokens,
+                   size_t n_in, size_t n_out, int activation, int out_dtype, void *const *out,
+                   const size_t *out_len, int64_t out_row_stride, int64_t out_head_stride);
 
 /* WhisperDecoder::precompute_cross_attn (crates/whisper/src/decoder.rs:423-447)
  * straight into the arena: for every layer l, K = enc . w_k[l]^T and

@@ -76,6 +76,7 @@ pub mod ffi {
     pub const WRS_F32: c_int = 0;
     pub const WRS_F16: c_int = 1;
     pub const WRS_BF16: c_int = 2;
+    pub const WRS_MX4: c_int = 3;
 
     pub const WRS_ACT_NONE: c_int = 0;
     pub const WRS_ACT_GELU: c_int = 1;
@@ -142,6 +143,9 @@ pub mod ffi {
         pub fn wrs_kv_append(kv: *mut WrsKv, layer: usize, slot: usize, k_rows: *const f32,
             v_rows: *const f32, n: usize, src_on_host: c_int) -> c_int;
         pub fn wrs_kv_advance(kv: *mut WrsKv, slot: usize, n: usize) -> c_int;
+        // drafted trees (no reference counterpart): an accepted path's rows
+        pub fn wrs_kv_keep_rows(kv: *mut WrsKv, slots: *const usize, counts: *const usize,
+            n_slots: usize, rows: *const usize, n_rows: usize) -> c_int;
         pub fn wrs_kv_set_cross(kv: *mut WrsKv, layer: usize, k: *const f32, v: *const f32,
             n_audio: usize, src_on_host: c_int) -> c_int;
         pub fn wrs_kv_cross_len(kv: *mut WrsKv, layer: usize, n_audio: *mut usize) -> c_int;
@@ -163,7 +167,12 @@ pub mod ffi {
             slot: usize, q: *const f32, n_tokens: usize, out: *mut f32) -> c_int;
         pub fn wrs_attn_prefill_cross(ctx: *mut WrsCtx, kv: *mut WrsKv, layer: usize,
             q: *const f32, n_tokens: usize, out: *mut f32) -> c_int;
-        // the same, also writing the rows' softmax statistics for the one-pass capture
+        // drafted trees over the cache (no reference counterpart); parents: device int32
+        pub fn wrs_attn_tree_self(ctx: *mut WrsCtx, kv: *mut WrsKv, layer: usize,
+            slots: *const usize, n_nodes: *const usize, n_trees: usize, parents: *const c_void,
+            parents_len: usize, q: *const f32, q_row_stride: i64, out: *mut f32,
+            out_row_stride: i64) -> c_int;
+        // prefill_cross, also writing the rows' softmax statistics for the one-pass capture
         pub fn wrs_attn_prefill_cross_lse(ctx: *mut WrsCtx, kv: *mut WrsKv, layer: usize,
             q: *const f32, n_tokens: usize, out: *mut f32, lse: *mut f32) -> c_int;
 
@@ -197,6 +206,19 @@ pub mod ffi {
             out: *const *mut c_void, out_len: *const usize, out_row_stride: i64,
             out_head_stride: i64) -> c_int;
         // norm.rs:116-143 and gelu.rs:11-23 over device f32 rows
+        // MXFP4 rows and the projections with them
+        pub fn wrs_mx4_quantize(ctx: *mut WrsCtx, x_dtype: c_int, x: *const c_void, x_len: usize,
+            x_row_stride: i64, n_rows: usize, n_cols: usize, codes: *mut c_void,
+            codes_len: usize, scales: *mut c_void, scales_len: usize) -> c_int;
+        pub fn wrs_mx4_dequantize(ctx: *mut WrsCtx, codes: *const c_void, codes_len: usize,
+            scales: *const c_void, scales_len: usize, n_rows: usize, n_cols: usize,
+            out_dtype: c_int, out: *mut c_void, out_len: usize, out_row_stride: i64) -> c_int;
+        pub fn wrs_linear_mx4(ctx: *mut WrsCtx, x_dtype: c_int, x: *const c_void,
+            x_scales: *const c_void, x_len: usize, x_row_stride: i64, n_groups: usize,
+            w: *const *const c_void, w_scales: *const *const c_void,
+            bias: *const *const f32, n_tokens: usize, n_in: usize, n_out: usize,
+            activation: c_int, out_dtype: c_int, out: *const *mut c_void,
+            out_len: *const usize, out_row_stride: i64, out_head_stride: i64) -> c_int;
         pub fn wrs_layer_norm(ctx: *mut WrsCtx, x: *const f32, x_len: usize,
             gamma: *const f32, beta: *const f32, eps: f32, n_tokens: usize, d_model: usize,
             out_dtype: c_int, out: *mut c_void, out_len: usize) -> c_int;

@@ -13,7 +13,10 @@ Host-side mirror of the reference's attention interface over the C ABI of
   and the stream; every FLOP runs in this package's HIP kernels):
   ``prefill`` and the ``KvArena`` (DecoderKvCache, decoder.rs:131-264) with
   its ``decode_self`` / ``decode_cross`` / ``prefill_self`` / ``prefill_cross``
-  and the DTW alignment-head capture ``capture_cross_heads``.
+  and the DTW alignment-head capture ``capture_cross_heads``;
+* drafted tokens: ``KvArena.tree_self`` checks trees of them in one pass and
+  ``KvArena.keep_rows`` keeps the accepted path; MXFP4 weights: ``mx4_quantize``,
+  ``mx4_dequantize`` and ``linear_mx4`` on :class:`Mx4` rows.
 
 There is no CPU fallback: without the built library every call raises.
 """
@@ -25,8 +28,8 @@ import threading
 import numpy as np
 
 from . import _lib as _L
-from ._lib import (WRS_BF16, WRS_EINVAL, WRS_F16, WRS_F32, WRS_OK, ExtensionMissing, Layout,
-                   header_symbols)
+from ._lib import (WRS_BF16, WRS_EINVAL, WRS_F16, WRS_F32, WRS_MX4, WRS_OK, ExtensionMissing,
+                   Layout, header_symbols)
 
 Q_TILE = 128  # crates/tensor/src/ops/attention.rs:13 (reference tile constants)
 KV_TILE = 128  # crates/tensor/src/ops/attention.rs:26
@@ -35,7 +38,8 @@ __all__ = [
     "Context", "KvArena", "ExtensionMissing", "Layout", "flash_attention_2",
     "multi_head_attention", "single_token_mha_d64", "mha_with_cache", "prefill",
     "token_major", "default_context", "header_symbols", "Q_TILE", "KV_TILE", "linear",
-    "linear_group", "linear_fused", "layer_norm", "gelu_inplace",
+    "linear_group", "linear_fused", "layer_norm", "gelu_inplace", "Mx4", "mx4_quantize",
+    "mx4_dequantize", "linear_mx4",
 ]
 
 
@@ -298,6 +302,119 @@ def linear_fused(x, ws, biases, outs, *, ln=None, act=None, out_row_stride=None,
         o_arr, len_arr, rs, out_head_stride), "linear_fused")
 
 
+def _on_device(ctx, what, *tensors):
+    """Every tensor lies on the context's GPU."""
+    for t in tensors:
+        if not t.is_cuda or t.get_device() != ctx.device:
+            raise TypeError(f"{what}: tensors must be on cuda:{ctx.device}, got {t.device}")
+
+
+def _rows(t, what):
+    """(rows, columns, row stride) of a 2-D tensor with adjacent columns."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise TypeError(f"{what}: rows of adjacent values expected, got {tuple(t.shape)} "
+                        f"with strides {t.stride()}")
+    n, d = t.shape
+    return n, d, (t.stride(0) if n > 1 else d)
+
+
+class Mx4:
+    """Packed MXFP4 rows (OCP Microscaling Formats v1.0): ``codes`` uint8
+    [rows][cols / 2], two e2m1 codes to a byte with the even column in the low
+    half, and ``scales`` uint8 [rows][cols / 32], e8m0."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes, scales):
+        for t in (codes, scales):
+            if str(t.dtype) != "torch.uint8" or t.dim() != 2 or not t.is_contiguous():
+                raise TypeError("Mx4: codes and scales are contiguous 2-D uint8 tensors")
+        if codes.device != scales.device:
+            raise TypeError("Mx4: codes and scales on two devices")
+        assert codes.shape[0] == scales.shape[0] and codes.shape[1] == 16 * scales.shape[1]
+        self.codes, self.scales = codes, scales
+        self.shape = (codes.shape[0], 2 * codes.shape[1])
+
+    @classmethod
+    def empty(cls, rows, cols, device="cuda"):
+        """Room for ``rows`` rows of ``cols`` values (a multiple of 32)."""
+        import torch
+        assert cols % 32 == 0
+        return cls(torch.empty((rows, cols // 2), dtype=torch.uint8, device=device),
+                   torch.empty((rows, cols // 32), dtype=torch.uint8, device=device))
+
+
+def mx4_quantize(x, out=None, ctx=None):
+    """Rows of a float32, float16 or bfloat16 CUDA tensor as MXFP4 (into ``out``, or a
+    new :class:`Mx4`): scales 2^(floor(log2(largest of 32)) - 2), nearest codes, ties
+    to the even one (``wrs_mx4_quantize``). Asynchronous on ctx's stream."""
+    ctx = ctx or default_context()
+    n, d, rs = _rows(x, "mx4_quantize")
+    if out is None:
+        out = Mx4.empty(n, d, device=x.device)
+    assert out.shape == (n, d)
+    _on_device(ctx, "mx4_quantize", x, out.codes)
+    ctx.check(ctx._lib.wrs_mx4_quantize(ctx.handle, _dtype_code(x), x.data_ptr(), _span(x), rs, n,
+                                        d, out.codes.data_ptr(), out.codes.numel(),
+                                        out.scales.data_ptr(), out.scales.numel()),
+              "mx4_quantize")
+    return out
+
+
+def mx4_dequantize(x, out, ctx=None):
+    """The values of the :class:`Mx4` rows ``x``, rounded once to the type of ``out``
+    (float32, float16 or bfloat16 rows; ``wrs_mx4_dequantize``)."""
+    ctx = ctx or default_context()
+    n, d, rs = _rows(out, "mx4_dequantize")
+    assert x.shape == (n, d)
+    _on_device(ctx, "mx4_dequantize", out, x.codes)
+    ctx.check(ctx._lib.wrs_mx4_dequantize(ctx.handle, x.codes.data_ptr(), x.codes.numel(),
+                                          x.scales.data_ptr(), x.scales.numel(), n, d,
+                                          _dtype_code(out), out.data_ptr(), _span(out), rs),
+              "mx4_dequantize")
+
+
+def linear_mx4(x, ws, biases, outs, *, act=None, out_row_stride=None, out_head_stride=64,
+               ctx=None):
+    """Projections with MXFP4 weights: ``outs[g]`` = act(``x`` W_g^T + ``biases[g]``), up
+    to 8 weight matrices of one shape in one launch (``wrs_linear_mx4``).
+
+    ``x`` [n_tokens][n_in] float32, float16 or bfloat16 rows, or :class:`Mx4` rows;
+    ``ws`` :class:`Mx4` [n_out][n_in]; ``biases`` None or a list with float32 tensors or
+    None entries; ``outs`` of one dtype (float32, float16 or bfloat16), laid out as in
+    :func:`linear`; ``act`` None or "gelu"."""
+    ctx = ctx or default_context()
+    n = len(ws)
+    assert n == len(outs) and n > 0
+    (n_out, n_in), o = ws[0].shape, outs[0]
+    if isinstance(x, Mx4):
+        (n_tokens, d), rs_x = x.shape, n_in
+        code, xp, xs, x_len = WRS_MX4, x.codes, x.scales.data_ptr(), 2 * x.codes.numel()
+    else:
+        n_tokens, d, rs_x = _rows(x, "linear_mx4")
+        code, xp, xs, x_len = _dtype_code(x), x, None, _span(x)
+    assert d == n_in
+    _on_device(ctx, "linear_mx4", xp)
+    biases = list(biases) if biases is not None else [None] * n
+    assert len(biases) == n
+    for w, b, t in zip(ws, biases, outs):
+        assert w.shape == (n_out, n_in) and t.dtype == o.dtype
+        _on_device(ctx, "linear_mx4", w.codes, t)
+        if b is not None:
+            assert b.numel() == n_out and str(b.dtype) == "torch.float32" and b.is_contiguous()
+            _on_device(ctx, "linear_mx4", b)
+    codes = {None: 0, "gelu": 1}
+    rs = n_out if out_row_stride is None else out_row_stride
+    vp = ctypes.c_void_p
+    arr = vp * n
+    ctx.check(ctx._lib.wrs_linear_mx4(
+        ctx.handle, code, xp.data_ptr(), xs, x_len, rs_x, n, arr(*[w.codes.data_ptr() for w in ws]),
+        arr(*[w.scales.data_ptr() for w in ws]),
+        arr(*[None if b is None else b.data_ptr() for b in biases]), n_tokens, n_in, n_out,
+        codes[act], _dtype_code(o), arr(*[t.data_ptr() for t in outs]),
+        (ctypes.c_size_t * n)(*[_span(t) for t in outs]), rs, out_head_stride), "linear_mx4")
+
+
 def layer_norm(x, gamma, beta, eps, out, ctx=None):
     """layer_norm (crates/tensor/src/ops/norm.rs:116-143) over the rows of the
     float32 CUDA tensor x ([num_tokens][d_model]); out float32/float16/bfloat16."""
@@ -458,6 +575,40 @@ class KvArena:
         self._c(self._lib.wrs_attn_prefill_self(self.ctx.handle, self.handle, layer, slot,
                                                 q.data_ptr(), q.shape[0], out.data_ptr()),
                 "prefill_self")
+
+    def tree_self(self, layer, slots, counts, parents, q, out):
+        """Self-attention of drafted trees (``wrs_attn_tree_self``): ``counts[i]`` rows of
+        ``slots[i]``, appended and not advanced, each against the slot's history, its
+        ancestors and itself. ``parents`` int32 CUDA tensor, one per row: the parent's
+        index within the tree, or -1 for a child of the last cached token. ``q`` and
+        ``out`` float32 [sum(counts)][d_model], rows of any stride."""
+        n, d, q_rs = _rows(q, "tree_self")
+        no, do, o_rs = _rows(out, "tree_self")
+        trees = len(slots)
+        assert d == do == self.d_model and n == no and trees == len(counts)
+        for t, want in ((q, "float32"), (out, "float32"), (parents, "int32")):
+            if str(t.dtype) != "torch." + want:
+                raise TypeError(f"tree_self: {want} expected, got {t.dtype}")
+        if sum(counts) != n or not parents.is_contiguous():
+            raise AssertionError("tree_self: one row and one parent per drafted token")
+        _on_device(self.ctx, "tree_self", q, out, parents)
+        arr = ctypes.c_size_t * trees
+        self._c(self._lib.wrs_attn_tree_self(self.ctx.handle, self.handle, layer, arr(*slots),
+                                             arr(*counts), trees, parents.data_ptr(),
+                                             parents.numel(), q.data_ptr(), q_rs, out.data_ptr(),
+                                             o_rs), "tree_self")
+
+    def keep_rows(self, slots, counts, rows):
+        """Moves the rows of an accepted path together (``wrs_kv_keep_rows``): for every
+        slot, layer and head, row slot_len + j becomes what row slot_len + r_j held, for
+        the slot's ``counts[i]`` entries of ``rows`` (offsets past its length, rising).
+        :meth:`advance` then takes them into the history."""
+        n = len(slots)
+        assert n == len(counts)
+        arr = ctypes.c_size_t * n
+        self._c(self._lib.wrs_kv_keep_rows(self.handle, arr(*slots), arr(*counts), n,
+                                           (ctypes.c_size_t * len(rows))(*rows), len(rows)),
+                "keep_rows")
 
     def prefill_cross(self, layer, q, out, lse=None):
         """Cross-attention of prompt rows (decoder.rs:698-708). With ``lse`` (a

@@ -111,6 +111,33 @@ __global__ __launch_bounds__(256) void kv_copy_planes(const _Float16* k_src, _Fl
   }
 }
 
+// K12 (kv_keep_rows): the rows of an accepted path of a drafted tree come together
+// behind their slot's history, in every (layer, head) plane of K and V. One wave per
+// plane: 8 f16 (4 f32) rows a pass, each pass loaded whole before it is stored. In place
+// and in order this is safe: sources rise and are at or above their destinations, so no
+// pass writes a row that a later one reads.
+constexpr int kKeepWaves = 4;
+__global__ __launch_bounds__(64 * kKeepWaves) void kv_keep_rows(KeepArgs a) {
+  const int64_t planes = static_cast<int64_t>(a.n_layers) * a.n_heads * 2;
+  const int64_t p = static_cast<int64_t>(blockIdx.x) * kKeepWaves + (threadIdx.x >> 6);
+  if (p >= planes) return;  // whole wave
+  const int u = blockIdx.y, lane = threadIdx.x & 63;
+  const int64_t lh = p >> 1;
+  const int h = static_cast<int>(lh % a.n_heads);
+  const int64_t layer = lh / a.n_heads;
+  u32x4* const base = static_cast<u32x4*>((p & 1) ? a.v : a.k) + a.off[u] +
+                      layer * a.layer_stride + h * a.plane_stride +
+                      static_cast<int64_t>(a.past[u]) * a.units;
+  const int i0 = a.first[u], i1 = a.first[u + 1];
+  const int per = 64 / a.units, sub = lane / a.units, c = lane % a.units;
+  for (int i = i0; i < i1; i += per) {
+    const int j = i + sub;
+    u32x4 x = {0, 0, 0, 0};
+    if (j < i1) x = base[static_cast<int64_t>(a.src[j]) * a.units + c];
+    if (j < i1) base[static_cast<int64_t>(a.dst0[u] + j - i0) * a.units + c] = x;
+  }
+}
+
 // Zero fill of a strided [batch][head][row][cols] f32 region (replaces
 // memset nodes, which must not be recorded into captured graphs): one thread
 // per value.
@@ -186,6 +213,16 @@ hipError_t launch_kv_copy_planes(const _Float16* k_src, _Float16* k_dst, const _
   hipLaunchKernelGGL(kv_copy_planes, dim3(n_heads, n_layers, static_cast<unsigned>(2 * parts)),
                      dim3(256), 0, s, k_src, k_dst, v_src, v_dst, layer_stride, plane_stride, len,
                      parts);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_keep_rows(const KeepArgs& a, hipStream_t s) {
+  if (a.n_slots <= 0 || a.n_layers <= 0 || a.n_heads <= 0) return hipSuccess;
+  const int64_t planes = static_cast<int64_t>(a.n_layers) * a.n_heads * 2;
+  const int64_t blocks = (planes + kKeepWaves - 1) / kKeepWaves;
+  if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL(kv_keep_rows, dim3(static_cast<unsigned>(blocks), a.n_slots),
+                     dim3(64 * kKeepWaves), 0, s, a);
   return hipGetLastError();
 }
 

@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -73,6 +74,12 @@ struct wrs_attn_ctx {
   size_t split_part_bytes = 0;
   unsigned* split_counters = nullptr;
   size_t split_counter_bytes = 0;
+  // Tree attention whose keys split over workgroups: partials and merge counters
+  // (kept zero between launches), of one size from the first such call on.
+  float* tree_part = nullptr;
+  size_t tree_part_bytes = 0;
+  unsigned* tree_counters = nullptr;
+  size_t tree_counter_bytes = 0;
   // Prefill schedule overrides (wrs_attn_set_schedule).
   int prefill_queries = 0;
   int f32_split = -1;
@@ -275,6 +282,15 @@ int linear_scratch(wrs_attn_ctx* c) {
   if (rc) return rc;
   return grow(c, reinterpret_cast<void**>(&c->lin_counters), &c->lin_counter_bytes,
               wrs::linear_split_words() * sizeof(unsigned), true);
+}
+// And for tree attention, which runs unsplit when captured before it exists.
+int tree_scratch(wrs_attn_ctx* c) {
+  if (c->tree_counters || capturing(c)) return WRS_OK;
+  int rc = grow(c, reinterpret_cast<void**>(&c->tree_part), &c->tree_part_bytes,
+                wrs::kTreePartFloats * sizeof(float), false);
+  if (rc) return rc;
+  return grow(c, reinterpret_cast<void**>(&c->tree_counters), &c->tree_counter_bytes,
+              wrs::kTreeCounterWords * sizeof(unsigned), true);
 }
 // And for the rows of fused decode projections that are normalized first.
 int ln_rows_scratch(wrs_attn_ctx* c) {
@@ -583,6 +599,8 @@ void wrs_attn_destroy(wrs_attn_ctx* c) {
   if (c->ln_rows) (void)hipFree(c->ln_rows);
   if (c->exact_scores) (void)hipFree(c->exact_scores);
   if (c->exact_counters) (void)hipFree(c->exact_counters);
+  if (c->tree_part) (void)hipFree(c->tree_part);
+  if (c->tree_counters) (void)hipFree(c->tree_counters);
   if (c->split_part) (void)hipFree(c->split_part);
   if (c->split_counters) (void)hipFree(c->split_counters);
   if (c->own_stream) (void)hipStreamDestroy(c->own_stream);
@@ -703,6 +721,10 @@ int wrs_attn_reserve(wrs_attn_ctx* c, const wrs_reserve* r) {
     if (rc) return rc;
     rc = grow(c, reinterpret_cast<void**>(&c->counters), &c->counter_bytes,
               wrs::decode_counter_words(groups, heads) * sizeof(unsigned), true);
+    if (rc) return rc;
+  }
+  if (heads && r->decode_rows && r->decode_keys) {
+    rc = tree_scratch(c);
     if (rc) return rc;
   }
   if (r->capture_tokens && r->capture_keys) {
@@ -1163,6 +1185,82 @@ int wrs_kv_advance(wrs_kv* kv, size_t slot, size_t n) {
   return WRS_OK;
 }
 
+int wrs_kv_keep_rows(wrs_kv* kv, const size_t* slots, const size_t* counts, size_t n_slots,
+                     const size_t* rows, size_t n_rows) {
+  if (!kv) return WRS_EINVAL;
+  wrs_attn_ctx* c = kv->ctx;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (n_slots == 0) return n_rows ? fail(c, WRS_EINVAL, "keep_rows: rows of no slot") : WRS_OK;
+  if (!slots || !counts || (n_rows && !rows)) return fail(c, WRS_EINVAL, "null argument");
+  // Everything is checked before any row moves.
+  size_t at = 0;
+  try {
+    std::vector<bool> seen(kv->n_slots, false);
+    for (size_t i = 0; i < n_slots; ++i) {
+      if (slots[i] >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
+      if (seen[slots[i]]) return fail(c, WRS_EINVAL, "keep_rows: the same slot twice");
+      seen[slots[i]] = true;
+      if (counts[i] > n_rows - at)
+        return fail(c, WRS_EINVAL, "keep_rows: fewer rows than the slots' counts");
+      const size_t room = kv->max_ctx - kv->len[slots[i]];
+      for (size_t j = 0; j < counts[i]; ++j) {
+        if (j && rows[at + j] <= rows[at + j - 1])
+          return fail(c, WRS_EINVAL, "keep_rows: a slot's rows must rise");
+        if (rows[at + j] >= room) return fail(c, WRS_ERANGE, "keep_rows: row past max_ctx");
+        if (rows[at + j] > 0xffff)
+          return fail(c, WRS_ERANGE, "keep_rows: row more than 65535 past the slot's length");
+      }
+      at += counts[i];
+    }
+  } catch (const std::bad_alloc&) {
+    return fail(c, WRS_ENOMEM, "out of host memory");
+  }
+  if (at != n_rows) return fail(c, WRS_EINVAL, "keep_rows: more rows than the slots' counts");
+  DeviceGuard g(c->device);
+  const size_t units = 4 * kv->esize();  // 16-byte units of a row of 64
+  wrs::KeepArgs a;
+  a.k = kv->k_self;
+  a.v = kv->v_self;
+  a.layer_stride = static_cast<int64_t>(kv->n_slots * kv->n_heads * kv->max_ctx * units);
+  a.plane_stride = static_cast<int64_t>(kv->max_ctx * units);
+  a.n_layers = static_cast<int>(kv->n_layers);
+  a.n_heads = static_cast<int>(kv->n_heads);
+  a.units = static_cast<int>(units);
+  a.n_slots = 0;
+  a.first[0] = 0;
+  auto flush = [&]() {
+    const hipError_t e = wrs::launch_kv_keep_rows(a, c->stream);
+    a.n_slots = 0;
+    return e;
+  };
+  at = 0;
+  for (size_t i = 0; i < n_slots; at += counts[i++]) {
+    // Rows already in place are the first ones; the others go in order, as many to a
+    // launch as its arguments hold.
+    size_t j = 0;
+    while (j < counts[i] && rows[at + j] == j) ++j;
+    while (j < counts[i]) {
+      const size_t used = a.n_slots ? a.first[a.n_slots] : 0;
+      if (a.n_slots == wrs::kKeepSlots || used == static_cast<size_t>(wrs::kKeepMoves)) {
+        WRS_HIP(c, flush());
+        continue;
+      }
+      const size_t n = std::min(counts[i] - j, wrs::kKeepMoves - used);
+      const int u = a.n_slots++;
+      a.off[u] = static_cast<int64_t>(kv->self_off(0, slots[i]) / 64 * units);
+      a.past[u] = static_cast<int>(kv->len[slots[i]]);
+      a.dst0[u] = static_cast<int>(j);
+      for (size_t x = 0; x < n; ++x) a.src[used + x] = static_cast<uint16_t>(rows[at + j + x]);
+      a.first[u + 1] = static_cast<uint16_t>(used + n);
+      j += n;
+      // A slot's next rows wait for these: they go in a launch of their own.
+      if (j < counts[i]) WRS_HIP(c, flush());
+    }
+  }
+  WRS_HIP(c, flush());
+  return WRS_OK;
+}
+
 int wrs_kv_set_cross(wrs_kv* kv, size_t layer, const float* k, const float* v, size_t n_audio,
                      int src_on_host) {
   if (!kv) return WRS_EINVAL;
@@ -1470,6 +1568,73 @@ int wrs_attn_prefill_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, size_t slot
                       n_tokens, keys, 64, 1, t_past);
 }
 
+int wrs_attn_tree_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t* slots,
+                       const size_t* n_nodes, size_t n_trees, const void* parents,
+                       size_t parents_len, const float* q, int64_t q_row_stride, float* out,
+                       int64_t out_row_stride) {
+  if (!c || !kv) return WRS_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (layer >= kv->n_layers) return fail(c, WRS_ERANGE, "layer out of range");
+  if (kv->ctx->device != c->device) return fail(c, WRS_EINVAL, "arena of another device");
+  if (n_trees == 0) return WRS_OK;
+  if (!slots || !n_nodes) return fail(c, WRS_EINVAL, "null argument");
+  size_t rows = 0;
+  for (size_t i = 0; i < n_trees; ++i) {
+    if (slots[i] >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
+    if (n_nodes[i] > static_cast<size_t>(wrs::kTreeMaxNodes))
+      return fail(c, WRS_EUNSUPPORTED, "a tree holds at most 256 nodes");
+    // The drafted rows are appended, not yet advanced.
+    if (n_nodes[i] > kv->max_ctx - kv->len[slots[i]])
+      return fail(c, WRS_ERANGE, "drafted rows past max_ctx");
+    if (n_nodes[i] && kv->len[slots[i]] + n_nodes[i] >= wrs::kRowsMaxKeys)
+      return fail(c, WRS_EUNSUPPORTED, "cache too long for tree attention");
+    rows += n_nodes[i];
+  }
+  if (rows == 0) return WRS_OK;
+  if (!parents || !q || !out) return fail(c, WRS_EINVAL, "null argument");
+  if (parents_len != rows) return fail(c, WRS_EINVAL, "one parent per drafted row");
+  if (!fits_int(rows)) return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+  const int64_t dm = static_cast<int64_t>(kv->d_model());
+  if (rows > 1 && (q_row_stride < dm || out_row_stride < dm))
+    return fail(c, WRS_EINVAL, "row stride below d_model");
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
+        reinterpret_cast<uintptr_t>(parents)) & 3))
+    return fail(c, WRS_EINVAL, "tensors must be aligned to their elements");
+  DeviceGuard g(c->device);
+  wrs::TreeArgs a;
+  a.q = q;
+  a.o = out;
+  a.k = kv->k_self;
+  a.v = kv->v_self;
+  a.parents = static_cast<const int*>(parents);
+  a.q_rs = q_row_stride;
+  a.o_rs = out_row_stride;
+  a.kv_hs = static_cast<int64_t>(kv->plane());
+  a.n_heads = static_cast<int>(kv->n_heads);
+  a.scale_log2 = 0.125f * 1.4426950408889634f;
+  size_t row = 0;
+  for (size_t i = 0; i < n_trees;) {
+    a.n_trees = 0;
+    for (; i < n_trees && a.n_trees < wrs::kTreeMaxTrees; ++i) {
+      if (n_nodes[i] == 0) continue;
+      const int t = a.n_trees++;
+      a.off[t] = static_cast<int64_t>(kv->self_off(layer, slots[i]));
+      a.row0[t] = static_cast<int64_t>(row);
+      a.past[t] = static_cast<int>(kv->len[slots[i]]);
+      a.nodes[t] = static_cast<int>(n_nodes[i]);
+      row += n_nodes[i];
+    }
+    if (a.n_trees == 0) break;
+    const int rc = tree_scratch(c);
+    if (rc) return rc;
+    a.part = c->tree_part;
+    a.counters = c->tree_counters;
+    const int64_t wgs = wrs::tree_plan(a, c->tree_counters != nullptr);
+    WRS_HIP(c, wrs::launch_tree_attend(a, kv->f32() ? wrs::kF32 : wrs::kF16, wgs, c->stream));
+  }
+  return WRS_OK;
+}
+
 int wrs_attn_prefill_cross(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const float* q,
                            size_t n_tokens, float* out) {
   if (!c || !kv) return WRS_EINVAL;
@@ -1653,6 +1818,39 @@ bool aligned_out(const void* p, int dt, int64_t rs, int64_t hs) {
   return (reinterpret_cast<uintptr_t>(p) % need) == 0 && rs % 4 == 0 && hs % 4 == 0;
 }
 
+// The checks that quantisation and its inverse share: values of `dtype` in n_rows rows
+// of n_cols, row_stride apart, against packed codes and scales.
+int mx4_rows(wrs_attn_ctx* c, int dtype, const void* values, size_t len, int64_t row_stride,
+             size_t n_rows, size_t n_cols, const void* codes, size_t codes_len,
+             const void* scales, size_t scales_len) {
+  if (dtype != WRS_F32 && dtype != WRS_F16 && dtype != WRS_BF16)
+    return fail(c, WRS_EINVAL, "MX4 rows come from f32, f16 or bf16");
+  if (n_cols % wrs::kMx4Block)
+    return fail(c, WRS_EUNSUPPORTED, "MX4 rows are multiples of 32 values");
+  if (n_rows == 0 || n_cols == 0) return WRS_OK;
+  if (!values || !codes || !scales) return fail(c, WRS_EINVAL, "null argument");
+  if (!fits_int(n_rows) || !fits_int(n_cols))
+    return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+  if (row_stride < 0 || (n_rows > 1 && row_stride < static_cast<int64_t>(n_cols)))
+    return fail(c, WRS_EINVAL, "row stride < n_cols");
+  if (len < (n_rows - 1) * static_cast<size_t>(row_stride) + n_cols)
+    return fail(c, WRS_EINVAL, "values shorter than n_rows rows of n_cols");
+  if (codes_len < n_rows * n_cols / 2 || scales_len < n_rows * (n_cols / wrs::kMx4Block))
+    return fail(c, WRS_EINVAL, "codes or scales shorter than the rows");
+  if ((reinterpret_cast<uintptr_t>(values) & 15) || (reinterpret_cast<uintptr_t>(codes) & 15) ||
+      (n_rows > 1 && row_stride % (dtype == WRS_F32 ? 4 : 8)))
+    return fail(c, WRS_EUNSUPPORTED, "rows and codes must be 16-byte aligned");
+  return WRS_OK;
+}
+
+// Offset of the last element that a projection writes.
+size_t last_out(size_t n_tokens, size_t n_out, int64_t out_rs, int64_t out_hs) {
+  const size_t last_g = (n_out - 1) / 64;
+  return (n_tokens - 1) * static_cast<size_t>(out_rs) +
+         std::max(last_g * static_cast<size_t>(out_hs) + (n_out - 1) % 64,
+                  last_g ? (last_g - 1) * static_cast<size_t>(out_hs) + 63 : 0);
+}
+
 // W_g x + bias_g for g < n_groups weight matrices of one shape against one
 // input, in one launch (the caller holds c->mu). bias may be NULL, or hold
 // NULL entries.
@@ -1671,11 +1869,7 @@ int linear_impl(wrs_attn_ctx* c, int x_dtype, const void* x, size_t x_len, int64
     return fail(c, WRS_EINVAL, "negative stride");
   if (x_len < (n_tokens - 1) * static_cast<size_t>(x_row_stride) + n_in)
     return fail(c, WRS_EINVAL, "x shorter than n_tokens rows of n_in");
-  const size_t last_g = (n_out - 1) / 64;
-  const size_t max_off =
-      (n_tokens - 1) * static_cast<size_t>(out_row_stride) +
-      std::max(last_g * static_cast<size_t>(out_head_stride) + (n_out - 1) % 64,
-               last_g ? (last_g - 1) * static_cast<size_t>(out_head_stride) + 63 : 0);
+  const size_t max_off = last_out(n_tokens, n_out, out_row_stride, out_head_stride);
   for (int gi = 0; gi < n_groups; ++gi)
     if (out_len[gi] <= max_off) return fail(c, WRS_EINVAL, "out shorter than the written range");
   if (out_dtype != WRS_F32 && out_dtype != WRS_F16 && out_dtype != WRS_BF16)
@@ -1922,6 +2116,106 @@ int wrs_kv_set_cross_proj(wrs_kv* kv, int x_dtype, const void* enc, size_t enc_l
     }
   }
   for (size_t l = 0; l < kv->n_layers; ++l) kv->cross_len[l] = n_audio;
+  return WRS_OK;
+}
+
+int wrs_mx4_quantize(wrs_attn_ctx* c, int x_dtype, const void* x, size_t x_len,
+                     int64_t x_row_stride, size_t n_rows, size_t n_cols, void* codes,
+                     size_t codes_len, void* scales, size_t scales_len) {
+  if (!c) return WRS_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  const int rc = mx4_rows(c, x_dtype, x, x_len, x_row_stride, n_rows, n_cols, codes, codes_len,
+                          scales, scales_len);
+  if (rc || n_rows == 0 || n_cols == 0) return rc;
+  DeviceGuard g(c->device);
+  WRS_HIP(c, wrs::launch_mx4_quantize(static_cast<wrs::DType>(x_dtype), x, x_row_stride,
+                                      static_cast<int64_t>(n_rows), static_cast<int>(n_cols),
+                                      static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales),
+                                      c->stream));
+  return WRS_OK;
+}
+
+int wrs_mx4_dequantize(wrs_attn_ctx* c, const void* codes, size_t codes_len, const void* scales,
+                       size_t scales_len, size_t n_rows, size_t n_cols, int out_dtype, void* out,
+                       size_t out_len, int64_t out_row_stride) {
+  if (!c) return WRS_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  const int rc = mx4_rows(c, out_dtype, out, out_len, out_row_stride, n_rows, n_cols, codes,
+                          codes_len, scales, scales_len);
+  if (rc || n_rows == 0 || n_cols == 0) return rc;
+  DeviceGuard g(c->device);
+  WRS_HIP(c, wrs::launch_mx4_dequantize(static_cast<const uint8_t*>(codes),
+                                        static_cast<const uint8_t*>(scales),
+                                        static_cast<int64_t>(n_rows), static_cast<int>(n_cols),
+                                        static_cast<wrs::DType>(out_dtype), out, out_row_stride,
+                                        c->stream));
+  return WRS_OK;
+}
+
+int wrs_linear_mx4(wrs_attn_ctx* c, int x_dtype, const void* x, const void* x_scales,
+                   size_t x_len, int64_t x_row_stride, size_t n_groups, const void* const* w,
+                   const void* const* w_scales, const float* const* bias, size_t n_tokens,
+                   size_t n_in, size_t n_out, int activation, int out_dtype, void* const* out,
+                   const size_t* out_len, int64_t out_row_stride, int64_t out_head_stride) {
+  if (!c) return WRS_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (n_groups == 0 || n_tokens == 0 || n_out == 0) return WRS_OK;
+  if (!x || !w || !w_scales || !out || !out_len) return fail(c, WRS_EINVAL, "null argument");
+  if (n_groups > static_cast<size_t>(wrs::kMx4Groups))
+    return fail(c, WRS_EINVAL, "more weight matrices than one launch takes");
+  const bool both = x_dtype == WRS_MX4;
+  if (!both && x_dtype != WRS_F32 && x_dtype != WRS_F16 && x_dtype != WRS_BF16)
+    return fail(c, WRS_EINVAL, "unknown input dtype");
+  if (out_dtype != WRS_F32 && out_dtype != WRS_F16 && out_dtype != WRS_BF16)
+    return fail(c, WRS_EINVAL, "unknown output dtype");
+  if (activation != WRS_ACT_NONE && activation != WRS_ACT_GELU)
+    return fail(c, WRS_EINVAL, "unknown activation");
+  if (both != (x_scales != nullptr))
+    return fail(c, WRS_EINVAL, "x scales go with MX4 rows, and only with them");
+  if (n_in == 0 || n_in % wrs::kLinearK != 0)
+    return fail(c, WRS_EUNSUPPORTED, "n_in must be a positive multiple of 64");
+  if (n_tokens > static_cast<size_t>(INT32_MAX / 2) || n_in > (1u << 20) ||
+      n_out > static_cast<size_t>(INT32_MAX / 2))
+    return fail(c, WRS_EINVAL, "projection shape too large");
+  if (x_row_stride < 0 || out_row_stride < 0 || out_head_stride < 0)
+    return fail(c, WRS_EINVAL, "negative stride");
+  if (both && x_row_stride != static_cast<int64_t>(n_in))
+    return fail(c, WRS_EUNSUPPORTED, "MX4 rows are packed");
+  if (n_tokens > 1 && x_row_stride < static_cast<int64_t>(n_in))
+    return fail(c, WRS_EINVAL, "x row stride < n_in");
+  if (x_len < (n_tokens - 1) * static_cast<size_t>(x_row_stride) + n_in)
+    return fail(c, WRS_EINVAL, "x shorter than n_tokens rows of n_in");
+  if ((reinterpret_cast<uintptr_t>(x) & 15) ||
+      (n_tokens > 1 && x_row_stride % (x_dtype == WRS_F32 ? 4 : 8)))
+    return fail(c, WRS_EUNSUPPORTED, "x rows must be 16-byte aligned");
+  const size_t max_off = last_out(n_tokens, n_out, out_row_stride, out_head_stride);
+  wrs::Mx4LinearArgs a{};
+  for (size_t gi = 0; gi < n_groups; ++gi) {
+    if (!w[gi] || !w_scales[gi] || !out[gi]) return fail(c, WRS_EINVAL, "null argument");
+    if (out_len[gi] <= max_off) return fail(c, WRS_EINVAL, "out shorter than the written range");
+    if (reinterpret_cast<uintptr_t>(w[gi]) & 15)
+      return fail(c, WRS_EUNSUPPORTED, "codes need 16-byte alignment");
+    if ((reinterpret_cast<uintptr_t>(out[gi]) & (out_dtype == WRS_F32 ? 3 : 1)) ||
+        (bias && (reinterpret_cast<uintptr_t>(bias[gi]) & 3)))
+      return fail(c, WRS_EINVAL, "tensors must be aligned to their elements");
+    a.w[gi] = static_cast<const uint8_t*>(w[gi]);
+    a.w_scales[gi] = static_cast<const uint8_t*>(w_scales[gi]);
+    a.bias[gi] = bias ? bias[gi] : nullptr;
+    a.out[gi] = out[gi];
+  }
+  a.x = x;
+  a.x_scales = static_cast<const uint8_t*>(x_scales);
+  a.x_rs = x_row_stride;
+  a.n_tokens = static_cast<int>(n_tokens);
+  a.n_in = static_cast<int>(n_in);
+  a.n_out = static_cast<int>(n_out);
+  a.n_groups = static_cast<int>(n_groups);
+  a.out_rs = out_row_stride;
+  a.out_hs = out_head_stride;
+  a.act = activation == WRS_ACT_GELU ? wrs::kActGelu : wrs::kActNone;
+  DeviceGuard g(c->device);
+  WRS_HIP(c, wrs::launch_linear_mx4(a, both ? wrs::kF32 : static_cast<wrs::DType>(x_dtype),
+                                    static_cast<wrs::DType>(out_dtype), c->stream));
   return WRS_OK;
 }
 

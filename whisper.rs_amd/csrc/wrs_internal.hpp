@@ -214,6 +214,40 @@ hipError_t launch_attend_rows(const RowsArgs& a, hipStream_t s);
 // One past the keys a launch takes (32-bit plane offsets).
 constexpr size_t kRowsMaxKeys = (size_t{1} << 24) - 4095;
 
+// Attention of drafted trees: tree t's nodes[t] query rows (row row0[t] + i, head h
+// at q + row*q_rs + h*64, any dword) against the plane set at element off[t] of k
+// and v (f16 or f32; head h at + h*kv_hs, key j at + j*64): its `past` keys, and of
+// the drafted rows behind them each row and its ancestors. parents[row0 + i] is
+// row i's parent if it is in [0, i), otherwise the row hangs from the last cached
+// token. tree_plan fills chunk and wg0 and returns the launch's workgroups; with
+// `split` it may deal a block's keys over several, which then need part
+// (kTreePartFloats) and counters (kTreeCounterWords, zero between launches).
+constexpr int kTreeMaxTrees = 64;   // per launch
+constexpr int kTreeMaxNodes = 256;  // of one tree
+constexpr int kTreeMaxRows = 32;    // query rows of a workgroup, at most
+constexpr int kTreeMaxWgs = 1024;   // workgroups of a launch that splits keys
+constexpr int kTreePart = 66;       // floats of a partial row: max, sum, 64 sums
+constexpr size_t kTreePartFloats = size_t{kTreeMaxWgs} * kTreeMaxRows * kTreePart;
+constexpr size_t kTreeCounterWords = size_t{kTreeMaxWgs} * 32;
+struct TreeArgs {
+  const float* q;
+  float* o;  // row r at o + r*o_rs
+  const void* k;
+  const void* v;
+  const int* parents;
+  int64_t q_rs, o_rs, kv_hs;
+  int n_heads, n_trees, chunk;
+  float scale_log2;  // (1/8) * log2(e)
+  float* part;
+  unsigned* counters;
+  int64_t off[kTreeMaxTrees];
+  int64_t row0[kTreeMaxTrees];
+  int past[kTreeMaxTrees], nodes[kTreeMaxTrees];  // nodes >= 1
+  int wg0[kTreeMaxTrees];
+};
+int64_t tree_plan(TreeArgs& a, bool split);
+hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStream_t s);
+
 // Measurement: a streaming read of `bytes` (multiple of 16, 16-byte aligned)
 // with the split-K decode's grid shape (512 threads x 64 bytes per
 // workgroup); sink receives stream_read_blocks(bytes) floats.
@@ -253,6 +287,33 @@ size_t capture_part_floats(int n_pairs, int n_tokens, int n_audio);
 hipError_t launch_capture_cross_f16(const CaptureArgs& a, hipStream_t s);
 // Over f32 planes (k32, scale; no part, no lse): one workgroup per (row, pair).
 hipError_t launch_capture_cross_f32(const CaptureArgs& a, hipStream_t s);
+
+// MXFP4: blocks of 32 values of a row share a power of two 2^(scale byte - 127) (255:
+// NaN), each value an e2m1 code of 4 bits (0 .5 1 1.5 2 3 4 6, bit 3 the sign), two to
+// a byte, the even column in the low half. Rows of codes and scales are packed.
+constexpr int kMx4Block = 32;
+hipError_t launch_mx4_quantize(DType x_dt, const void* x, int64_t x_rs, int64_t n_rows, int n_cols,
+                               uint8_t* codes, uint8_t* scales, hipStream_t s);
+hipError_t launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t n_rows,
+                                 int n_cols, DType out_dt, void* out, int64_t out_rs,
+                                 hipStream_t s);
+// Projections with MXFP4 weights: out[g](t, r) = act(w[g][r] . x[t] + bias[g][r]) at
+// out[g] + t*out_rs + (r/64)*out_hs + r%64, x f32 / f16 / bf16 rows or (x_scales set)
+// packed MXFP4 rows.
+constexpr int kMx4Groups = 8;  // weight matrices per launch
+struct Mx4LinearArgs {
+  const void* x;
+  const uint8_t* x_scales;
+  int64_t x_rs;
+  int n_tokens, n_in, n_out, n_groups;
+  int64_t out_rs, out_hs;
+  int act;  // Act, applied after the bias
+  const uint8_t* w[kMx4Groups];
+  const uint8_t* w_scales[kMx4Groups];
+  const float* bias[kMx4Groups];  // nullable entries
+  void* out[kMx4Groups];
+};
+hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s);
 
 // Projections with f16 weights (quant.rs:415-473 semantics):
 // out(t, r) = row_scale[t] * (W[r] . x'[t]) + bias[r] with W [n_out][n_in] f16
@@ -358,5 +419,22 @@ hipError_t launch_kv_slide(_Float16* k, _Float16* v, int64_t layer_stride, int64
 hipError_t launch_kv_copy_planes(const _Float16* k_src, _Float16* k_dst, const _Float16* v_src,
                                  _Float16* v_dst, int64_t layer_stride, int64_t plane_stride,
                                  int n_layers, int n_heads, int len, hipStream_t s);
+// Rows of a plane that come together: of slot u, at element off[u] of k and v, rows
+// past[u] + src[i] move to past[u] + dst0[u] + i - first[u], for i in [first[u],
+// first[u + 1]) in order; src rises and is at least its destination. Plane (l, h) at +
+// l*layer_stride + h*plane_stride, rows of `units` 16-byte units.
+constexpr int kKeepSlots = 64;   // per launch
+constexpr int kKeepMoves = 768;  // per launch, of all slots
+struct KeepArgs {
+  void* k;
+  void* v;
+  int64_t layer_stride, plane_stride;  // in 16-byte units, as off
+  int n_layers, n_heads, n_slots, units;
+  int64_t off[kKeepSlots];
+  int past[kKeepSlots], dst0[kKeepSlots];
+  uint16_t first[kKeepSlots + 1];
+  uint16_t src[kKeepMoves];
+};
+hipError_t launch_kv_keep_rows(const KeepArgs& a, hipStream_t s);
 
 }  // namespace wrs
