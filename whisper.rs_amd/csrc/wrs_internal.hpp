@@ -301,6 +301,7 @@ hipError_t launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, in
 // out[g] + t*out_rs + (r/64)*out_hs + r%64, x f32 / f16 / bf16 rows or (x_scales set)
 // packed MXFP4 rows.
 constexpr int kMx4Groups = 8;  // weight matrices per launch
+constexpr int kMx4Rows = 16;   // rows of x that the weight stream takes
 struct Mx4LinearArgs {
   const void* x;
   const uint8_t* x_scales;
