@@ -213,6 +213,16 @@ def test_outputs_groups_and_gelu(wrs, ctx, rows, out, x_dtype):
 
 
 @pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
+@pytest.mark.parametrize("rows", [1, 6, 10, 12, 16])
+@pytest.mark.parametrize("n_in,n_out,groups", [(1280, 1280, 3), (5120, 1280, 1), (8192, 16, 1),
+                                               (512, 40000, 1), (2624, 20000, 1)])
+def test_few_rows_of_every_grid(wrs, ctx, n_in, n_out, groups, rows, x_dtype):
+    # small and large grids, x whole in LDS or in pieces
+    note(f"linear_mx4 {rows} x {n_in} -> {n_out} x {groups} {x_dtype}")
+    run(wrs, ctx, x_dtype, rows, n_in, n_out, groups=groups, seed=6)
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
 @pytest.mark.parametrize("rows", [5, 150])
 def test_large_product(wrs, ctx, rows, x_dtype):
     note(f"linear_mx4 {rows} x 1280 -> 5120 {x_dtype}")

@@ -26,31 +26,22 @@ constexpr int kParts<float> = 3;
 template <>
 constexpr int kParts<_Float16> = 2;
 
-// x = the sum of its parts (the top half of their f32 patterns), exactly: each takes the
-// next 8 significant bits. An infinity or NaN is its first part alone.
+// x = the sum of its parts, the top halves of the words of p, exactly: each takes the next 8
+// significant bits. An infinity is its first part alone; a NaN stays one.
 template <int P>
 __device__ inline void split_top(float x, uint32_t (&p)[P]) {
-  const uint32_t b = __builtin_bit_cast(uint32_t, x);
-  p[0] = b & kTop;
-  if constexpr (P > 1) {
-    const bool odd = (b & 0x7F800000u) == 0x7F800000u;
-    if (odd && (b & 0x007FFFFFu)) p[0] |= 0x00400000u;
-    float rest = x - __builtin_bit_cast(float, p[0]);
+  p[0] = __builtin_bit_cast(uint32_t, x);
 #pragma unroll
-    for (int i = 1; i < P; ++i) {
-      p[i] = odd ? 0u : __builtin_bit_cast(uint32_t, rest) & kTop;
-      rest -= __builtin_bit_cast(float, p[i]);
-    }
+  for (int i = 1; i < P; ++i) {
+    float rest = x - __builtin_bit_cast(float, p[i - 1] & kTop);
+    if (i == 1 && __builtin_fabsf(x) == __builtin_inff()) rest = 0.f;
+    x = rest;
+    p[i] = __builtin_bit_cast(uint32_t, rest);
   }
 }
-
-// 8 values of type T as f32.
-template <typename T>
-__device__ inline void load8(const T* p, float (&x)[8]) {
-  typedef T t8 __attribute__((ext_vector_type(8), aligned(16)));
-  const t8 v = *reinterpret_cast<const t8*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(v[i]);
+// The top halves of two words.
+__device__ inline uint32_t pack_top(uint32_t lo, uint32_t hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
 __device__ inline float scale_of(int byte) {
@@ -66,13 +57,37 @@ __device__ inline bf16x8 widen8(uint32_t w, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-constexpr int kRowsWaves = 8;
-constexpr int kRowsBatch = 8;  // steps whose codes a wave has in flight
+constexpr int kRawBuffer = 0x00020000;  // buffer resource word 3: raw, 32-bit data format
+constexpr uint32_t kPast = 0xFFFF0000u;  // an offset past every buffer
 
-template <typename XT, int kCT, typename OT>
-__global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(Mx4LinearArgs a, int ks, int chunk) {
+constexpr int kRowsWaves = 8;
+constexpr int kGroup = 8;       // blocks of a row that a wave takes at a time: 128 bytes of codes
+constexpr int kCodeBytes = 16 * kGroup * 16;            // of a tile's group
+constexpr int kStage = kCodeBytes + 16 * kGroup + 128;  // LDS of a wave: codes, scales, pad
+
+__device__ inline void wave_sync() {
+  // LDS operations of one wave complete in order: only the compiler must keep it.
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// K15 (mx4_rows): up to 16 rows of x, bound by the stream of codes. A wave multiplies tiles of
+//   16 features; `ks` waves share a tile and take its groups of 8 blocks in turn, `chunk` groups
+//   at a time for a workgroup. Codes come in whole 128-byte pieces of rows (a lane's operand is
+//   16 bytes of its own row: loaded so, with a byte of scale each, 36 MB took 15.4 us, in
+//   whole pieces and without scales 9.9), wait in registers, and change places in the wave's
+//   own LDS. x is staged in LDS once for the workgroup.
+// kMany: grids of more than one workgroup per CU keep their registers to what two need;
+// others have x in flight at once (5 rows 5120 -> 1280: 11.3 us with 2 groups a thread).
+template <typename XT, int kCT, int kBatch, bool kMany>
+__global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4LinearArgs a, int ks,
+                                                                           int chunk,
+                                                                           uint32_t wide_inv,
+                                                                           int out_dt) {
   constexpr bool kBoth = sizeof(XT) == 1;  // x is MXFP4 too
   constexpr int kP = kBoth ? 1 : kParts<XT>;
+  constexpr int kXBatch = kMany ? 2 : 4;  // groups of 8 values of x in flight per thread
   constexpr int kPitch = 16 * kCT + 1;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -82,12 +97,33 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(Mx4LinearArgs a, int
   const int grp = blockIdx.y;
   const int first = blockIdx.x * tiles * 16;  // the workgroup's first feature
   const int nb = a.n_in / kMx4Block, bytes = a.n_in / 2;
-  const int64_t row = min(first + 16 * (wave / ks) + c, a.n_out - 1);
-  const uint8_t* const wp = a.w[grp] + row * bytes;
-  const uint8_t* const sp = a.w_scales[grp] + row * nb;
-  const int64_t xrow = min(c, a.n_tokens - 1);  // kBoth
-  const uint8_t* const xp = static_cast<const uint8_t*>(a.x) + xrow * bytes;
-  const uint8_t* const xsp = a.x_scales + xrow * nb;
+  const int n_wg = min(16 * tiles, a.n_out - first);  // features of the workgroup
+  // Rows past the last feature and blocks past the last one read as zero.
+  const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w[grp] + static_cast<int64_t>(first) * bytes), 0, n_wg * bytes,
+      kRawBuffer);
+  const __amdgpu_buffer_rsrc_t srs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w_scales[grp] + static_cast<int64_t>(first) * nb), 0, n_wg * nb,
+      kRawBuffer);
+  char* const mine = lds + wave * kStage;           // this wave's codes, then scales
+  char* const xl = lds + kRowsWaves * kStage;       // x of the chunk
+  const int tile_row = 16 * (wave / ks);
+
+  // Load h of a group: lane j takes 16 bytes of row 8 h + (j / 8 ^ h), block (j ^ j / 8) % 8,
+  // and puts them at place 64 h + j, so that 16 rows read at one block meet distinct banks.
+  const int lr = lane >> 3, lb = (lane ^ lr) & 7;
+  const uint32_t wo0 = (tile_row + lr) * bytes + 16 * lb;
+  const uint32_t wo1 = (tile_row + 8 + (lr ^ 1)) * bytes + 16 * lb;
+  const uint32_t so = (tile_row + (lane >> 2)) * nb + 2 * (lane & 3);
+  // Where this lane's operand of block b of a group lies (block 4 e + g in step e).
+  const int cr = (c & 7) ^ (c >> 3), at = 1024 * (c >> 3) + 128 * cr;
+  const int place[2] = {at + 16 * (g ^ cr), at + 16 * ((g + 4) ^ cr)};
+  static_assert(kGroup == 8, "a group is two steps of four blocks");
+
+  const int pitch = 2 * (kMx4Block * kGroup * chunk + 8);  // bytes of a staged column
+  int col[kCT];  // this lane's staged columns (past the last one, that one again: not stored)
+#pragma unroll
+  for (int i = 0; i < kCT; ++i) col[i] = min(16 * i + c, kP * a.n_tokens - 1) * pitch + 64 * g;
 
   f32x4 acc[2][kCT];
 #pragma unroll
@@ -95,83 +131,129 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(Mx4LinearArgs a, int
 #pragma unroll
     for (int i = 0; i < kCT; ++i) acc[e][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  const int pitch = 2 * (kMx4Block * chunk + 8);  // bytes of a staged column
-  for (int b0 = 0; b0 < nb; b0 += chunk) {
-    const int nbc = min(chunk, nb - b0);
-    const int steps = (nbc + 4 * ks - 1) / (4 * ks);
-    u32x4 cw[kRowsBatch], xw[kBoth ? kRowsBatch : 1];
-    int sw[kRowsBatch], xs[kBoth ? kRowsBatch : 1];
-    // Blocks past the last one read as zero: the last one's codes, times 2^-127 and x's 0.
-    auto load = [&](int s0) __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < kRowsBatch; ++u) {
-        const int at = b0 + 4 * ((s0 + u) * ks + kw) + g, b = min(at, nb - 1);
-        cw[u] = *reinterpret_cast<const u32x4*>(wp + 16 * b);
-        sw[u] = sp[b];
-        if constexpr (kBoth) {
-          xw[u] = *reinterpret_cast<const u32x4*>(xp + 16 * b);
-          xs[u] = at < nb ? xsp[b] : 0;
-        }
-        if (at >= nb) sw[u] = 0;
-      }
+  u32x4 cw[kBatch][2];
+  uint16_t sw[kBatch];
+  for (int g0 = 0; kGroup * g0 < nb; g0 += chunk) {
+    const int nbc = min(kGroup * chunk, nb - kGroup * g0);  // blocks of the chunk
+    const int n = ((nbc + kGroup - 1) / kGroup - kw + ks - 1) / ks;  // this wave's groups
+    auto load = [&](int u, int i) __attribute__((always_inline)) {
+      int b = kGroup * (g0 + kw + ks * i);  // the group's first block
+      // Formed anew for each load: kept as running offsets they cost 18 registers a group.
+      asm("" : "+s"(b));
+      const bool in = i < n && b + lb < nb;
+      cw[u][0] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, in ? wo0 + 16 * b : kPast, 0, 0));
+      cw[u][1] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, in ? wo1 + 16 * b : kPast, 0, 0));
+      sw[u] = __builtin_amdgcn_raw_buffer_load_b16(
+          srs, i < n && b + 2 * (lane & 3) < nb ? so + b : kPast, 0, 0);
     };
-    load(0);
-    if constexpr (!kBoth) {
-      // x's columns of the chunk: part p of row t is column p * n_tokens + t.
-      const int wide = 4 * chunk;  // groups of 8 values a row
-      if (b0) __syncthreads();
-      for (int e = tid; e < (16 * kCT - kP * a.n_tokens) * wide; e += 64 * kRowsWaves)
-        *reinterpret_cast<u32x4*>(lds + (kP * a.n_tokens + e / wide) * pitch + 16 * (e % wide)) =
-            u32x4{0, 0, 0, 0};
-      for (int e = tid; e < a.n_tokens * wide; e += 64 * kRowsWaves) {
-        const int t = e / wide, k = e % wide;
-        u32x4 w[kP];
+    if constexpr (kBoth) {
+      // Codes of block b, row t at (16 b + t) * 16, scales behind them.
 #pragma unroll
-        for (int p = 0; p < kP; ++p) w[p] = u32x4{0, 0, 0, 0};
-        if (k < 4 * nbc) {
-          float x[8];
-          load8<XT>(static_cast<const XT*>(a.x) + t * a.x_rs + kMx4Block * b0 + 8 * k, x);
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            uint32_t lo[kP], hi[kP];
-            split_top<kP>(x[i], lo);
-            split_top<kP>(x[i + 1], hi);
-#pragma unroll
-            for (int p = 0; p < kP; ++p) w[p][i >> 1] = (lo[p] >> 16) | hi[p];
-          }
+      for (int u = 0; u < kBatch; ++u) load(u, u);
+      if (g0) __syncthreads();
+      for (int e = tid; e < 16 * kGroup * chunk; e += 64 * kRowsWaves) {
+        const int b = e >> 4, t = e & 15, at_b = kGroup * g0 + b;
+        u32x4 v = {0, 0, 0, 0};
+        uint8_t sc = 0;
+        if (t < a.n_tokens && b < nbc) {
+          v = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.x) +
+                                              static_cast<int64_t>(t) * bytes + 16 * at_b);
+          sc = a.x_scales[t * nb + at_b];
         }
-#pragma unroll
-        for (int p = 0; p < kP; ++p)
-          *reinterpret_cast<u32x4*>(lds + (p * a.n_tokens + t) * pitch + 16 * k) = w[p];
+        *reinterpret_cast<u32x4*>(xl + 16 * e) = v;
+        xl[256 * kGroup * chunk + e] = sc;
       }
-      __syncthreads();
+    } else {
+      // x's columns: part p of row t is column p * n_tokens + t. The first rows' loads go
+      // ahead of the codes', which then load under the conversion.
+      const int wide = 4 * kGroup * chunk;  // groups of 8 values a row
+      const int groups = a.n_tokens * wide;
+      typedef XT x8 __attribute__((ext_vector_type(8), aligned(16)));
+      x8 xv[kXBatch];
+      auto load_x = [&](int e0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kXBatch; ++i) {
+          const int e = e0 + 64 * kRowsWaves * i + tid;
+          const int t = __umulhi(e, wide_inv), k = e - t * wide;
+          const bool in = e < groups && k < 4 * nbc;
+          const int64_t x_at = in ? t * a.x_rs + kMx4Block * kGroup * g0 + 8 * k : 0;
+          xv[i] = *reinterpret_cast<const x8*>(static_cast<const XT*>(a.x) + x_at);
+        }
+      };
+      load_x(0);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) load(u, u);
+      if (g0) __syncthreads();
+      for (int e0 = 0; e0 < groups; e0 += 64 * kRowsWaves * kXBatch) {
+        if (e0) load_x(e0);
+#pragma unroll
+        for (int i = 0; i < kXBatch; ++i) {
+          const int e = e0 + 64 * kRowsWaves * i + tid;
+          if (e >= groups) break;
+          const int t = __umulhi(e, wide_inv), k = e - t * wide;
+          const bool in = k < 4 * nbc;
+          u32x4 w[kP];
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            uint32_t lo[kP], hi[kP];
+            split_top<kP>(in ? static_cast<float>(xv[i][j]) : 0.f, lo);
+            split_top<kP>(in ? static_cast<float>(xv[i][j + 1]) : 0.f, hi);
+#pragma unroll
+            for (int p = 0; p < kP; ++p) w[p][j >> 1] = pack_top(lo[p], hi[p]);
+          }
+#pragma unroll
+          for (int p = 0; p < kP; ++p)
+            *reinterpret_cast<u32x4*>(xl + (p * a.n_tokens + t) * pitch + 16 * k) = w[p];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     }
-    for (int s0 = 0; s0 < steps; s0 += kRowsBatch) {
-      if (s0) load(s0);
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
 #pragma unroll
-      for (int u = 0; u < kRowsBatch; ++u) {
-        if (s0 + u >= steps) break;
-        if constexpr (kBoth) {
-          i32x8 wa = {}, xa = {};
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u;
+        wave_sync();  // the last group's operands are read
+        *reinterpret_cast<u32x4*>(mine + 16 * lane) = cw[u][0];
+        *reinterpret_cast<u32x4*>(mine + 1024 + 16 * lane) = cw[u][1];
+        *reinterpret_cast<uint16_t*>(mine + kCodeBytes + 2 * lane) = sw[u];
+        wave_sync();
+        load(u, i + kBatch);
+        int b = kGroup * (kw + ks * i);  // in the chunk
+        asm("" : "+s"(b));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            wa[j] = static_cast<int>(cw[u][j]);
-            xa[j] = static_cast<int>(xw[u][j]);
+        for (int e = 0; e < 2; ++e) {
+          if (i >= n) continue;
+          const u32x4 w = *reinterpret_cast<const u32x4*>(mine + place[e]);
+          const int sc = *reinterpret_cast<const uint8_t*>(mine + kCodeBytes + 8 * c + 4 * e + g);
+          if constexpr (kBoth) {
+            const int xb = 16 * (b + 4 * e + g) + c;
+            const u32x4 x = *reinterpret_cast<const u32x4*>(xl + 16 * xb);
+            const int xs = *reinterpret_cast<const uint8_t*>(xl + 256 * kGroup * chunk + xb);
+            i32x8 wa = {}, xa = {};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              wa[j] = static_cast<int>(w[j]);
+              xa[j] = static_cast<int>(x[j]);
+            }
+            acc[e][0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xa, acc[e][0], 4, 4,
+                                                                         0, sc, 0, xs);
+          } else {
+            const char* const xc = xl + 64 * (b + 4 * e);
+            const float scale = scale_of(sc);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bf16x8 wv = widen8(w[j], scale);
+#pragma unroll
+              for (int t = 0; t < kCT; ++t)
+                acc[j & 1][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    wv, *reinterpret_cast<const bf16x8*>(xc + col[t] + 16 * j), acc[j & 1][t], 0,
+                    0, 0);
+            }
           }
-          acc[u & 1][0] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              wa, xa, acc[u & 1][0], 4, 4, 0, sw[u], 0, xs[u]);
-        } else {
-          const char* const xl = lds + c * pitch + 64 * (4 * ((s0 + u) * ks + kw) + g);
-          const float scale = scale_of(sw[u]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bf16x8 wv = widen8(cw[u][j], scale);
-#pragma unroll
-            for (int i = 0; i < kCT; ++i)
-              acc[j & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  wv, *reinterpret_cast<const bf16x8*>(xl + 16 * i * pitch + 16 * j),
-                  acc[j & 1][i], 0, 0, 0);
-          }
+          __builtin_amdgcn_sched_barrier(0);  // one step's operands in registers at a time
         }
       }
     }
@@ -195,8 +277,13 @@ __global__ __launch_bounds__(64 * kRowsWaves) void mx4_rows(Mx4LinearArgs a, int
         y += red[(16 * ((rr >> 4) * ks + k) + (rr & 15)) * kPitch + p * a.n_tokens + t];
     if (a.bias[grp]) y += a.bias[grp][r];
     if (a.act == kActGelu) y = gelu_tanh(y);
-    static_cast<OT*>(a.out[grp])[t * a.out_rs + (r >> 6) * a.out_hs + (r & 63)] =
-        static_cast<OT>(y);
+    const int64_t o = t * a.out_rs + (r >> 6) * a.out_hs + (r & 63);
+    if (out_dt == kF32)
+      static_cast<float*>(a.out[grp])[o] = y;
+    else if (out_dt == kF16)
+      static_cast<_Float16*>(a.out[grp])[o] = static_cast<_Float16>(y);
+    else
+      static_cast<__bf16*>(a.out[grp])[o] = static_cast<__bf16>(y);
   }
 }
 
@@ -258,31 +345,38 @@ __global__ __launch_bounds__(256) void linear_mx4_tile(Mx4LinearArgs a) {
     }
 }
 
-// Few rows: how many waves share a tile's columns, and the blocks staged at a time.
+// Few rows: the waves that share a tile, and the groups staged at a time.
 struct RowsShape {
   int ks, chunk;
+  bool many;  // more than one workgroup per CU
   size_t lds;
 };
-template <int kCT>
-RowsShape rows_shape(const Mx4LinearArgs& a, bool both) {
-  const int nb = a.n_in / kMx4Block;
+RowsShape rows_shape(const Mx4LinearArgs& a, int ct, int cols) {
+  const int groups = (a.n_in / kMx4Block + kGroup - 1) / kGroup;
   const int64_t tiles = (a.n_out + 15ll) / 16 * a.n_groups;
-  int ks = kRowsWaves;
-  while (ks > 1 && (tiles * ks > 2048 || 4 * (ks / 2) >= nb)) ks /= 2;
-  const int unit = 4 * ks, all = (nb + unit - 1) / unit * unit;
-  const int fit = ((80 * 1024) / (32 * kCT) - 8) / kMx4Block / unit * unit;
-  RowsShape r{ks, std::min(all, std::max(unit, fit)), 0};
-  r.lds = sizeof(float) * 16 * kRowsWaves * (16 * kCT + 1);
-  if (!both) r.lds = std::max<size_t>(r.lds, 32ull * kCT * (kMx4Block * r.chunk + 8));
+  const size_t pad = 16 * cols, per = cols ? 2 * kMx4Block * kGroup * cols : 17 * 16 * kGroup;
+  int ks = kRowsWaves, fit = 0;
+  bool many = false;
+  for (;; ks /= 2) {
+    // x whole where a CU has one workgroup, else what leaves room for a second (more
+    // columns than a tile's want it whole all the same: 8 f32 rows 1280 -> 51866 23.9 us in two
+    // pieces, 20.6 whole).
+    many = tiles * ks > 256 * kRowsWaves;
+    const size_t room = (many && ct == 1 ? 78 : 156) * 1024 - kRowsWaves * kStage;
+    fit = static_cast<int>((room - pad) / per) / ks * ks;
+    if (ks == 1 || (fit && tiles * ks <= 2048 && ks / 2 < groups)) break;
+  }
+  RowsShape r{ks, std::min((groups + ks - 1) / ks * ks, std::max(ks, fit)), many, 0};
+  r.lds = std::max<size_t>(sizeof(float) * 16 * kRowsWaves * (16 * ct + 1),
+                           kRowsWaves * kStage + per * r.chunk + pad);
   return r;
 }
 
-template <typename XT, int kCT, typename OT>
-hipError_t launch_rows(const Mx4LinearArgs& a, hipStream_t s) {
-  constexpr size_t kMost = 128 * 1024;
-  const RowsShape r = rows_shape<kCT>(a, sizeof(XT) == 1);
+template <typename XT, int kCT, int kBatch, bool kMany>
+hipError_t launch_rows(const Mx4LinearArgs& a, const RowsShape& r, DType out_dt, hipStream_t s) {
+  constexpr size_t kMost = 160 * 1024;
   if (r.lds > kMost) return hipErrorInvalidConfiguration;
-  const void* fn = reinterpret_cast<const void*>(&mx4_rows<XT, kCT, OT>);
+  const void* fn = reinterpret_cast<const void*>(&mx4_rows<XT, kCT, kBatch, kMany>);
   static std::atomic<uint64_t> attr_set{0};  // one bit per device
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
@@ -295,21 +389,31 @@ hipError_t launch_rows(const Mx4LinearArgs& a, hipStream_t s) {
   }
   const int wide = 16 * (kRowsWaves / r.ks);
   const dim3 grid((a.n_out + wide - 1) / wide, a.n_groups);
-  hipLaunchKernelGGL((mx4_rows<XT, kCT, OT>), grid, dim3(64 * kRowsWaves), r.lds, s, a, r.ks,
-                     r.chunk);
+  const uint32_t inv = static_cast<uint32_t>((1ull << 32) / (4 * kGroup * r.chunk) + 1);
+  hipLaunchKernelGGL((mx4_rows<XT, kCT, kBatch, kMany>), grid, dim3(64 * kRowsWaves), r.lds, s, a, r.ks,
+                     r.chunk, inv, static_cast<int>(out_dt));
   return hipGetLastError();
 }
 
-template <typename XT, typename OT>
-hipError_t launch_rows_of(const Mx4LinearArgs& a, hipStream_t s) {
+template <typename XT, int kCT>
+hipError_t launch_rows_ct(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
+  const RowsShape r = rows_shape(a, kCT, sizeof(XT) == 1 ? 0 : kParts<XT> * a.n_tokens);
+  const int groups = r.chunk / r.ks;
+  if (r.many) return launch_rows<XT, kCT, kCT == 1 ? 5 : 3, true>(a, r, out_dt, s);
+  if (groups <= 1) return launch_rows<XT, kCT, 1, false>(a, r, out_dt, s);
+  return launch_rows<XT, kCT, 3, false>(a, r, out_dt, s);
+}
+
+template <typename XT>
+hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   if constexpr (sizeof(XT) == 1) {
-    return launch_rows<XT, 1, OT>(a, s);
+    return launch_rows_ct<XT, 1>(a, out_dt, s);
   } else {
     const int cols = kParts<XT> * a.n_tokens;
-    if (cols <= 16) return launch_rows<XT, 1, OT>(a, s);
+    if (cols <= 16) return launch_rows_ct<XT, 1>(a, out_dt, s);
     if constexpr (kParts<XT> >= 2)
-      if (cols <= 32) return launch_rows<XT, 2, OT>(a, s);
-    if constexpr (kParts<XT> >= 3) return launch_rows<XT, 3, OT>(a, s);
+      if (cols <= 32) return launch_rows_ct<XT, 2>(a, out_dt, s);
+    if constexpr (kParts<XT> >= 3) return launch_rows_ct<XT, 3>(a, out_dt, s);
     return hipErrorInvalidValue;
   }
 }
@@ -319,25 +423,15 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, hipStream_t s) {
 hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s) {
   if (a.n_tokens <= 0 || a.n_out <= 0 || a.n_groups <= 0) return hipSuccess;
   const dim3 grid((a.n_tokens + kTile - 1) / kTile, (a.n_out + kTile - 1) / kTile, a.n_groups);
-#define WRS_MX4_ROWS(XT)                                                                     \
-  switch (out_dt) {                                                                          \
-    case kF32: return launch_rows_of<XT, float>(a, s);                                       \
-    case kF16: return launch_rows_of<XT, _Float16>(a, s);                                    \
-    case kBF16: return launch_rows_of<XT, __bf16>(a, s);                                     \
-    default: return hipErrorInvalidValue;                                                    \
-  }
   if (a.n_tokens <= kMx4Rows) {
-    if (a.x_scales) {
-      WRS_MX4_ROWS(uint8_t)
-    }
+    if (a.x_scales) return launch_rows_of<uint8_t>(a, out_dt, s);
     switch (x_dt) {
-      case kF32: WRS_MX4_ROWS(float)
-      case kF16: WRS_MX4_ROWS(_Float16)
-      case kBF16: WRS_MX4_ROWS(__bf16)
+      case kF32: return launch_rows_of<float>(a, out_dt, s);
+      case kF16: return launch_rows_of<_Float16>(a, out_dt, s);
+      case kBF16: return launch_rows_of<__bf16>(a, out_dt, s);
       default: return hipErrorInvalidValue;
     }
   }
-#undef WRS_MX4_ROWS
 #define WRS_MX4_OUT(XT)                                                                      \
   switch (out_dt) {                                                                          \
     case kF32:                                                                               \
