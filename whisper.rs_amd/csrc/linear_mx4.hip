@@ -287,6 +287,280 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
   }
 }
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// 2 codes (byte k of w) times a scale as packed 16-bit values.
+template <typename E, int k>
+__device__ inline uint32_t widen2(uint32_t w, float scale) {
+  if constexpr (__is_same(E, __bf16))
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, k));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, k));
+}
+template <typename E>
+__device__ inline u32x4 widen8_as(uint32_t w, float scale) {
+  return u32x4{widen2<E, 0>(w, scale), widen2<E, 1>(w, scale), widen2<E, 2>(w, scale),
+               widen2<E, 3>(w, scale)};
+}
+template <typename E>
+__device__ inline f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (__is_same(E, __bf16))
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// GELU of the projections, x / (1 + exp(-2 u)): 0.5 x (1 + tanh u) without the tanh.
+__device__ inline float gelu_exp(float x) {
+  const float u = 0.7978846f * x * __builtin_fmaf(0.044715f * x, x, 1.f);
+  const float e = __builtin_amdgcn_exp2f(u * -2.88539008f);  // -2 log2(e)
+  return x * __builtin_amdgcn_rcpf(1.f + e);
+}
+
+// Tile of a workgroup: BF features x BT rows of x, waves of WF x WT, kD stages in registers.
+template <int BF_, int BT_, int WF_, int WT_, int D_>
+struct Tile {
+  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, D = D_;
+  static constexpr int kWaves = (BF / WF) * (BT / WT), kThreads = 64 * kWaves;
+};
+constexpr int kK = 64;           // columns per stage
+constexpr int kRow = 2 * kK;     // bytes of a staged row
+constexpr int kOutPitch = 68;    // floats of an output row in LDS
+
+// 16-byte chunk c of staged row r sits at c ^ (r / 2): 16 rows read at one chunk hit
+// distinct banks.
+__device__ inline int chunk_at(int r, int c) { return r * kRow + 16 * (c ^ ((r >> 1) & 7)); }
+
+template <typename T, int P>
+constexpr size_t tile_lds() {
+  const size_t stage = 2ull * (T::BF + P * T::BT) * kRow;
+  const size_t out = sizeof(float) * T::kWaves * 32 * kOutPitch;
+  return stage > out ? stage : out;
+}
+
+// One tile with operands of type E, x in P parts. Returns (to every thread) whether a scale of
+// the tile's weights lies outside what E holds exactly.
+template <typename T, typename XT, typename E, int P>
+__device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
+                                    f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+  constexpr int kF = T::WF / 32, kT = T::WT / 32;
+  constexpr int kWn = (2 * T::BF + T::kThreads - 1) / T::kThreads;  // blocks of W a thread stages
+  constexpr int kXn = T::BT * (kK / 8) / T::kThreads;              // groups of 8 values of x
+  static_assert(kXn >= 1 && T::BT * (kK / 8) % T::kThreads == 0, "whole groups");
+  constexpr int kWBytes = T::BF * kRow, kXBytes = T::BT * kRow;
+  constexpr int kStageBytes = kWBytes + P * kXBytes;
+  typedef XT x8 __attribute__((ext_vector_type(8), aligned(16)));
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, hl = lane >> 5;
+  const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
+  const int nb = a.n_in / kMx4Block, bytes = a.n_in / 2, stages = a.n_in / kK;
+
+  const int n_f = min(T::BF, a.n_out - f0), n_t = min(T::BT, a.n_tokens - t0);
+  const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w[grp] + static_cast<int64_t>(f0) * bytes), 0, n_f * bytes,
+      kRawBuffer);
+  const __amdgpu_buffer_rsrc_t srs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w_scales[grp] + static_cast<int64_t>(f0) * nb), 0, n_f * nb,
+      kRawBuffer);
+  // Rows of x: pointers of this thread's groups (rows past the last one: that one again,
+  // not stored).
+  const XT* xp[kXn];
+#pragma unroll
+  for (int i = 0; i < kXn; ++i) {
+    const int e = tid + T::kThreads * i, row = min(e >> 3, n_t - 1);
+    xp[i] = static_cast<const XT*>(a.x) + (t0 + row) * a.x_rs + 8 * (e & 7);
+  }
+
+  u32x4 cw[T::D][kWn];
+  uint8_t sw[T::D][kWn];
+  x8 xv[T::D][kXn];
+  auto load = [&](int d, int s) __attribute__((always_inline)) {
+    asm("" : "+s"(s));  // offsets are formed per stage, not kept per load
+#pragma unroll
+    for (int i = 0; i < kWn; ++i) {
+      const int e = tid + T::kThreads * i;  // block e & 1 of row e / 2
+      const bool in = s < stages && (2 * T::BF % T::kThreads == 0 || e < 2 * T::BF);
+      cw[d][i] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                     wrs, in ? (e >> 1) * bytes + 16 * (e & 1) + 32 * s : kPast, 0, 0));
+      sw[d][i] = __builtin_amdgcn_raw_buffer_load_b8(
+          srs, in ? (e >> 1) * nb + (e & 1) + 2 * s : kPast, 0, 0);
+    }
+    const int at = kK * min(s, stages - 1);
+#pragma unroll
+    for (int i = 0; i < kXn; ++i) xv[d][i] = *reinterpret_cast<const x8*>(xp[i] + at);
+  };
+  bool odd = false;
+  auto store = [&](int d, char* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kWn; ++i) {
+      const int e = tid + T::kThreads * i;
+      if (2 * T::BF % T::kThreads != 0 && e >= 2 * T::BF) break;
+      // f16 holds 6 * 2^13 and 0.5 * 2^-23.
+      if constexpr (__is_same(E, _Float16))
+        odd |= (e >> 1) < n_f && static_cast<unsigned>(sw[d][i] - 104) > 36u;
+      const float scale = scale_of(sw[d][i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<u32x4*>(buf + chunk_at(e >> 1, 4 * (e & 1) + j)) =
+            widen8_as<E>(cw[d][i][j], scale);
+    }
+#pragma unroll
+    for (int i = 0; i < kXn; ++i) {
+      const int e = tid + T::kThreads * i;
+      char* const at = buf + kWBytes + chunk_at(e >> 3, e & 7);
+      if constexpr (P == 1 && sizeof(XT) == 2) {
+        *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, xv[d][i]);
+      } else {
+        u32x4 w[P];
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          uint32_t lo[P], hi[P];
+          split_top<P>(static_cast<float>(xv[d][i][j]), lo);
+          split_top<P>(static_cast<float>(xv[d][i][j + 1]), hi);
+#pragma unroll
+          for (int p = 0; p < P; ++p) w[p][j >> 1] = pack_top(lo[p], hi[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(at + p * kXBytes) = w[p];
+      }
+    }
+  };
+  auto multiply = [&](const char* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < kK / 16; ++k) {
+      u32x4 wv[kF], xw[P][kT];
+#pragma unroll
+      for (int i = 0; i < kF; ++i)
+        wv[i] = *reinterpret_cast<const u32x4*>(buf + chunk_at(wf + 32 * i + r32, 2 * k + hl));
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < kT; ++i)
+          xw[p][i] = *reinterpret_cast<const u32x4*>(buf + kWBytes + p * kXBytes +
+                                                     chunk_at(wt + 32 * i + r32, 2 * k + hl));
+#pragma unroll
+      for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+        for (int i = 0; i < kF; ++i)
+#pragma unroll
+          for (int t = 0; t < kT; ++t) acc[i][t] = mfma32<E>(wv[i], xw[p][t], acc[i][t]);
+    }
+  };
+
+#pragma unroll
+  for (int i = 0; i < kF; ++i)
+#pragma unroll
+    for (int t = 0; t < kT; ++t) acc[i][t] = f32x16{};
+#pragma unroll
+  for (int d = 0; d < T::D; ++d) load(d, d);
+  store(0, lds);
+  load(0, T::D);
+  __syncthreads();
+  for (int s0 = 0; s0 < stages; s0 += T::D) {
+#pragma unroll
+    for (int d = 0; d < T::D; ++d) {
+      const int s = s0 + d;
+      if (T::D > 1 && s >= stages) break;
+      constexpr int kNext = T::D;
+      const int n = (d + 1) % kNext;
+      if (s + 1 < stages) {
+        store(n, lds + ((s + 1) & 1) * kStageBytes);
+        load(n, s + 1 + T::D);
+      }
+      multiply(lds + (s & 1) * kStageBytes);
+      __syncthreads();
+    }
+  }
+  return __syncthreads_or(odd);
+}
+
+// The tile's outputs: each wave passes 32 rows x 64 features at a time through its own LDS, so
+// that rows are stored in whole pieces (16 bytes a lane straight from the MFMA layout go to
+// 32 rows each).
+template <typename T, typename OT>
+__device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
+                                  bool whole, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+  constexpr int kF = T::WF / 32, kT = T::WT / 32, kFe = kF > 1 ? 2 : 1;  // feature blocks a pass
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, hl = lane >> 5;
+  const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
+  float* const mine = reinterpret_cast<float*>(lds) + wave * 32 * kOutPitch;
+  constexpr int kLanes = 4 * kFe;  // lanes of a row, 8 features each
+  const int lr = lane / kLanes, lf = 8 * (lane % kLanes);
+  const float* const bias = a.bias[grp];
+#pragma unroll
+  for (int i = 0; i < kF; i += kFe) {
+    const int r = f0 + wf + 32 * i + lf;  // this lane's first feature
+    float b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = bias && r + e < a.n_out ? bias[r + e] : 0.f;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      wave_sync();
+#pragma unroll
+      for (int f = 0; f < kFe; ++f)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<f32x4*>(mine + r32 * kOutPitch + 32 * f + 2 * e + 4 * hl) =
+              f32x4{acc[i + f][t][e], acc[i + f][t][e + 1], acc[i + f][t][e + 2],
+                    acc[i + f][t][e + 3]};
+      wave_sync();
+#pragma unroll
+      for (int j = 0; j < 32; j += 64 / kLanes) {
+        const int row = t0 + wt + 32 * t + j + lr;
+        const f32x4 y0 = *reinterpret_cast<const f32x4*>(mine + (j + lr) * kOutPitch + lf);
+        const f32x4 y1 = *reinterpret_cast<const f32x4*>(mine + (j + lr) * kOutPitch + lf + 4);
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y[e] = (e < 4 ? y0[e & 3] : y1[e & 3]) + b[e];
+          if (a.act == kActGelu) y[e] = gelu_exp(y[e]);
+        }
+        if (row >= a.n_tokens || r >= a.n_out) continue;
+        OT* const op = static_cast<OT*>(a.out[grp]) + row * a.out_rs + (r >> 6) * a.out_hs + (r & 63);
+        if (whole && r + 8 <= a.n_out) {
+          typedef OT o8 __attribute__((ext_vector_type(8), aligned(16)));
+          o8 o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = static_cast<OT>(y[e]);
+          *reinterpret_cast<o8*>(op) = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (r + e < a.n_out) op[e] = static_cast<OT>(y[e]);
+        }
+      }
+    }
+  }
+}
+
+// K16 (mx4_tile): many rows of x. W is widened to 16-bit operands on its way into LDS, one block
+//   of 32 a thread and stage, x comes along in one part (f16, bf16) or three bf16 ones (f32), and
+//   both feed 32x32x16 MFMAs. f16 x takes f16 weights, exact for scales of 2^-23 to 2^13; a tile
+//   that meets another scale is formed again from bf16 parts, which hold any.
+template <typename T, typename XT, typename OT>
+__global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int lid = xcd_remap(blockIdx.x, gridDim.x);
+  const int f0 = (lid % n_f) * T::BF, t0 = (lid / n_f) * T::BT, grp = blockIdx.y;
+  f32x16 acc[T::WF / 32][T::WT / 32];
+  if constexpr (__is_same(XT, _Float16)) {
+    if (tile_product<T, XT, _Float16, 1>(a, grp, f0, t0, lds, acc))
+      tile_product<T, XT, __bf16, kParts<XT>>(a, grp, f0, t0, lds, acc);
+  } else {
+    tile_product<T, XT, __bf16, kParts<XT>>(a, grp, f0, t0, lds, acc);
+  }
+  tile_store<T, OT>(a, grp, f0, t0, lds, whole, acc);
+}
+
 constexpr int kTile = 64;
 
 __device__ inline float value_of(uint32_t code, int scale) {
@@ -345,6 +619,28 @@ __global__ __launch_bounds__(256) void linear_mx4_tile(Mx4LinearArgs a) {
     }
 }
 
+// Whether output chunks of 8 features can be stored whole.
+bool whole_chunks(const Mx4LinearArgs& a, DType out_dt) {
+  const int64_t per = out_dt == kF32 ? 4 : 8;
+  bool ok = a.out_rs % per == 0 && a.out_hs % per == 0;
+  for (int g = 0; g < a.n_groups; ++g)
+    ok = ok && (reinterpret_cast<uintptr_t>(a.out[g]) & 15) == 0;
+  return ok;
+}
+
+// Dynamic LDS beyond 64 KB has to be asked for, once per kernel and device.
+template <typename F>
+hipError_t allow_lds(F fn, size_t bytes, std::atomic<uint64_t>& set) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  if (dev < 64 && (set.load(std::memory_order_acquire) & (uint64_t{1} << dev))) return hipSuccess;
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == hipSuccess && dev < 64) set.fetch_or(uint64_t{1} << dev, std::memory_order_acq_rel);
+  return e;
+}
+
 // Few rows: the waves that share a tile, and the groups staged at a time.
 struct RowsShape {
   int ks, chunk;
@@ -376,17 +672,9 @@ template <typename XT, int kCT, int kBatch, bool kMany>
 hipError_t launch_rows(const Mx4LinearArgs& a, const RowsShape& r, DType out_dt, hipStream_t s) {
   constexpr size_t kMost = 160 * 1024;
   if (r.lds > kMost) return hipErrorInvalidConfiguration;
-  const void* fn = reinterpret_cast<const void*>(&mx4_rows<XT, kCT, kBatch, kMany>);
-  static std::atomic<uint64_t> attr_set{0};  // one bit per device
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
+  static std::atomic<uint64_t> set{0};
+  const hipError_t e = allow_lds(&mx4_rows<XT, kCT, kBatch, kMany>, kMost, set);
   if (e != hipSuccess) return e;
-  if (dev >= 64 || !(attr_set.load(std::memory_order_acquire) & (uint64_t{1} << dev))) {
-    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize,
-                            static_cast<int>(kMost));
-    if (e != hipSuccess) return e;
-    if (dev < 64) attr_set.fetch_or(uint64_t{1} << dev, std::memory_order_acq_rel);
-  }
   const int wide = 16 * (kRowsWaves / r.ks);
   const dim3 grid((a.n_out + wide - 1) / wide, a.n_groups);
   const uint32_t inv = static_cast<uint32_t>((1ull << 32) / (4 * kGroup * r.chunk) + 1);
@@ -418,6 +706,38 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   }
 }
 
+template <typename T, typename XT, typename OT>
+hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
+  // f16 x may fall back to two parts.
+  constexpr size_t kLds = tile_lds<T, kParts<XT>>();
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+  static std::atomic<uint64_t> set{0};
+  const hipError_t e = allow_lds(&mx4_tile<T, XT, OT>, kLds, set);
+  if (e != hipSuccess) return e;
+  const int n_f = (a.n_out + T::BF - 1) / T::BF;
+  const int64_t wgs = static_cast<int64_t>(n_f) * ((a.n_tokens + T::BT - 1) / T::BT);
+  if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((mx4_tile<T, XT, OT>), dim3(static_cast<unsigned>(wgs), a.n_groups),
+                     dim3(T::kThreads), kLds, s, a, n_f, whole_chunks(a, out_dt) ? 1 : 0);
+  return hipGetLastError();
+}
+
+template <typename XT, typename OT>
+hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
+  using Small = Tile<64, 64, 32, 32, 2>;
+  using Mid = Tile<128, 128, 64, 64, 1>;
+  auto wgs = [&](int f, int t) {
+    return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups;
+  };
+  if constexpr (sizeof(XT) == 2) {
+    // Two parts of f16 x (scales out of range) take the smaller stages of a 256 x 128 tile.
+    using Large = Tile<256, 128, 64, 64, 1>;
+    if (wgs(256, 128) >= 256) return launch_tile<Large, XT, OT>(a, out_dt, s);
+  }
+  if (wgs(128, 128) >= 192) return launch_tile<Mid, XT, OT>(a, out_dt, s);
+  return launch_tile<Small, XT, OT>(a, out_dt, s);
+}
+
 }  // namespace
 
 hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s) {
@@ -445,16 +765,24 @@ hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, h
       break;                                                                                 \
     default: return hipErrorInvalidValue;                                                    \
   }
+#define WRS_MX4_TILES(XT)                                                                    \
+  switch (out_dt) {                                                                          \
+    case kF32: return launch_tiles<XT, float>(a, out_dt, s);                                 \
+    case kF16: return launch_tiles<XT, _Float16>(a, out_dt, s);                              \
+    case kBF16: return launch_tiles<XT, __bf16>(a, out_dt, s);                               \
+    default: return hipErrorInvalidValue;                                                    \
+  }
   if (a.x_scales) {
     WRS_MX4_OUT(uint8_t)
   } else {
     switch (x_dt) {
-      case kF32: WRS_MX4_OUT(float) break;
-      case kF16: WRS_MX4_OUT(_Float16) break;
-      case kBF16: WRS_MX4_OUT(__bf16) break;
+      case kF32: WRS_MX4_TILES(float)
+      case kF16: WRS_MX4_TILES(_Float16)
+      case kBF16: WRS_MX4_TILES(__bf16)
       default: return hipErrorInvalidValue;
     }
   }
+#undef WRS_MX4_TILES
 #undef WRS_MX4_OUT
   return hipGetLastError();
 }
