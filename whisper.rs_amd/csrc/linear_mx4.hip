@@ -322,10 +322,11 @@ __device__ inline float gelu_exp(float x) {
   return x * __builtin_amdgcn_rcpf(1.f + e);
 }
 
-// Tile of a workgroup: BF features x BT rows of x, waves of WF x WT, kD stages in registers.
-template <int BF_, int BT_, int WF_, int WT_, int D_>
+// Tile of a workgroup: BF features x BT rows of x, waves of WF x WT; x is loaded kDx stages
+// ahead.
+template <int BF_, int BT_, int WF_, int WT_, int Dx_>
 struct Tile {
-  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, D = D_;
+  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, kDx = Dx_;
   static constexpr int kWaves = (BF / WF) * (BT / WT), kThreads = 64 * kWaves;
 };
 constexpr int kK = 64;           // columns per stage
@@ -338,22 +339,24 @@ __device__ inline int chunk_at(int r, int c) { return r * kRow + 16 * (c ^ ((r >
 
 template <typename T, int P>
 constexpr size_t tile_lds() {
-  const size_t stage = 2ull * (T::BF + P * T::BT) * kRow;
+  const size_t stage = 2ull * P * T::BT * kRow;
   const size_t out = sizeof(float) * T::kWaves * 32 * kOutPitch;
   return stage > out ? stage : out;
 }
 
-// One tile with operands of type E, x in P parts. Returns (to every thread) whether a scale of
-// the tile's weights lies outside what E holds exactly.
+// Adds one tile's products with operands of type E to acc. P: the parts of x that a stage
+// holds, all of them, or with P == 1 < kParts part `part`. Returns (to every thread) whether a
+// scale of the tile's weights lies outside what E holds exactly.
+//   W goes from memory to MFMA operands in registers: lane (r, h) of a 32-row block takes block
+//   h of row r, and step j of a stage multiplies values 8 j.. of both blocks, so x's operand is
+//   chunk 4 h + j of its staged row.
 template <typename T, typename XT, typename E, int P>
 __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
-                                    f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+                                    int part, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
-  constexpr int kWn = (2 * T::BF + T::kThreads - 1) / T::kThreads;  // blocks of W a thread stages
-  constexpr int kXn = T::BT * (kK / 8) / T::kThreads;              // groups of 8 values of x
+  constexpr int kXn = T::BT * (kK / 8) / T::kThreads;  // groups of 8 values of x a thread stages
   static_assert(kXn >= 1 && T::BT * (kK / 8) % T::kThreads == 0, "whole groups");
-  constexpr int kWBytes = T::BF * kRow, kXBytes = T::BT * kRow;
-  constexpr int kStageBytes = kWBytes + P * kXBytes;
+  constexpr int kXBytes = T::BT * kRow, kStageBytes = P * kXBytes;
   typedef XT x8 __attribute__((ext_vector_type(8), aligned(16)));
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -361,6 +364,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
   const int nb = a.n_in / kMx4Block, bytes = a.n_in / 2, stages = a.n_in / kK;
 
+  // Rows past the last feature read as zero.
   const int n_f = min(T::BF, a.n_out - f0), n_t = min(T::BT, a.n_tokens - t0);
   const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(a.w[grp] + static_cast<int64_t>(f0) * bytes), 0, n_f * bytes,
@@ -377,74 +381,76 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     xp[i] = static_cast<const XT*>(a.x) + (t0 + row) * a.x_rs + 8 * (e & 7);
   }
 
-  u32x4 cw[T::D][kWn];
-  uint8_t sw[T::D][kWn];
-  x8 xv[T::D][kXn];
-  auto load = [&](int d, int s) __attribute__((always_inline)) {
+  u32x4 cw[2][kF];
+  uint8_t sw[2][kF];
+  x8 xv[T::kDx][kXn];
+  auto load_w = [&](int d, int s) __attribute__((always_inline)) {
     asm("" : "+s"(s));  // offsets are formed per stage, not kept per load
 #pragma unroll
-    for (int i = 0; i < kWn; ++i) {
-      const int e = tid + T::kThreads * i;  // block e & 1 of row e / 2
-      const bool in = s < stages && (2 * T::BF % T::kThreads == 0 || e < 2 * T::BF);
+    for (int i = 0; i < kF; ++i) {
+      const int row = wf + 32 * i + r32;
+      const bool in = s < stages;
       cw[d][i] = __builtin_bit_cast(
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                     wrs, in ? (e >> 1) * bytes + 16 * (e & 1) + 32 * s : kPast, 0, 0));
+                     wrs, in ? row * bytes + 16 * hl + 32 * s : kPast, 0, 0));
       sw[d][i] = __builtin_amdgcn_raw_buffer_load_b8(
-          srs, in ? (e >> 1) * nb + (e & 1) + 2 * s : kPast, 0, 0);
+          srs, in ? row * nb + hl + 2 * s : kPast, 0, 0);
     }
+  };
+  auto load_x = [&](int d, int s) __attribute__((always_inline)) {
     const int at = kK * min(s, stages - 1);
 #pragma unroll
     for (int i = 0; i < kXn; ++i) xv[d][i] = *reinterpret_cast<const x8*>(xp[i] + at);
   };
-  bool odd = false;
-  auto store = [&](int d, char* buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kWn; ++i) {
-      const int e = tid + T::kThreads * i;
-      if (2 * T::BF % T::kThreads != 0 && e >= 2 * T::BF) break;
-      // f16 holds 6 * 2^13 and 0.5 * 2^-23.
-      if constexpr (__is_same(E, _Float16))
-        odd |= (e >> 1) < n_f && static_cast<unsigned>(sw[d][i] - 104) > 36u;
-      const float scale = scale_of(sw[d][i]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<u32x4*>(buf + chunk_at(e >> 1, 4 * (e & 1) + j)) =
-            widen8_as<E>(cw[d][i][j], scale);
-    }
+  auto store_x = [&](int d, char* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kXn; ++i) {
       const int e = tid + T::kThreads * i;
-      char* const at = buf + kWBytes + chunk_at(e >> 3, e & 7);
-      if constexpr (P == 1 && sizeof(XT) == 2) {
+      char* const at = buf + chunk_at(e >> 3, e & 7);
+      if constexpr (P == 1 && __is_same(XT, E)) {
         *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, xv[d][i]);
       } else {
-        u32x4 w[P];
+        constexpr int kAll = kParts<XT>;
+        u32x4 w[kAll];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-          uint32_t lo[P], hi[P];
-          split_top<P>(static_cast<float>(xv[d][i][j]), lo);
-          split_top<P>(static_cast<float>(xv[d][i][j + 1]), hi);
+          uint32_t lo[kAll], hi[kAll];
+          split_top<kAll>(static_cast<float>(xv[d][i][j]), lo);
+          split_top<kAll>(static_cast<float>(xv[d][i][j + 1]), hi);
 #pragma unroll
-          for (int p = 0; p < P; ++p) w[p][j >> 1] = pack_top(lo[p], hi[p]);
+          for (int p = 0; p < kAll; ++p) w[p][j >> 1] = pack_top(lo[p], hi[p]);
         }
+        if constexpr (P == kAll) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(at + p * kXBytes) = w[p];
+          for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(at + p * kXBytes) = w[p];
+        } else {
+          static_assert(P == 1 && kAll == 2, "one of two parts");
+          *reinterpret_cast<u32x4*>(at) = part ? w[1] : w[0];
+        }
       }
     }
   };
-  auto multiply = [&](const char* buf) __attribute__((always_inline)) {
+  bool odd = false;
+  auto multiply = [&](int d, const char* buf) __attribute__((always_inline)) {
+    float scale[kF];
 #pragma unroll
-    for (int k = 0; k < kK / 16; ++k) {
+    for (int i = 0; i < kF; ++i) {
+      // f16 holds 6 * 2^13 and 0.5 * 2^-23.
+      if constexpr (__is_same(E, _Float16))
+        odd |= wf + 32 * i + r32 < n_f && static_cast<unsigned>(sw[d][i] - 104) > 36u;
+      scale[i] = scale_of(sw[d][i]);
+    }
+#pragma unroll
+    for (int j = 0; j < kK / 16; ++j) {
       u32x4 wv[kF], xw[P][kT];
-#pragma unroll
-      for (int i = 0; i < kF; ++i)
-        wv[i] = *reinterpret_cast<const u32x4*>(buf + chunk_at(wf + 32 * i + r32, 2 * k + hl));
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int i = 0; i < kT; ++i)
-          xw[p][i] = *reinterpret_cast<const u32x4*>(buf + kWBytes + p * kXBytes +
-                                                     chunk_at(wt + 32 * i + r32, 2 * k + hl));
+          xw[p][i] = *reinterpret_cast<const u32x4*>(buf + p * kXBytes +
+                                                     chunk_at(wt + 32 * i + r32, 4 * hl + j));
+#pragma unroll
+      for (int i = 0; i < kF; ++i) wv[i] = widen8_as<E>(cw[d][i][j], scale[i]);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
@@ -454,27 +460,22 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     }
   };
 
+  load_x(0, 0);
+  load_w(0, 0);
+  load_w(1, 1);
 #pragma unroll
-  for (int i = 0; i < kF; ++i)
-#pragma unroll
-    for (int t = 0; t < kT; ++t) acc[i][t] = f32x16{};
-#pragma unroll
-  for (int d = 0; d < T::D; ++d) load(d, d);
-  store(0, lds);
-  load(0, T::D);
+  for (int d = 1; d < T::kDx; ++d) load_x(d, d);
+  store_x(0, lds);
+  load_x(0, T::kDx);
   __syncthreads();
-  for (int s0 = 0; s0 < stages; s0 += T::D) {
+  for (int s0 = 0; s0 < stages; s0 += 2) {
 #pragma unroll
-    for (int d = 0; d < T::D; ++d) {
-      const int s = s0 + d;
-      if (T::D > 1 && s >= stages) break;
-      constexpr int kNext = T::D;
-      const int n = (d + 1) % kNext;
-      if (s + 1 < stages) {
-        store(n, lds + ((s + 1) & 1) * kStageBytes);
-        load(n, s + 1 + T::D);
-      }
-      multiply(lds + (s & 1) * kStageBytes);
+    for (int d = 0; d < 2; ++d) {
+      const int s = s0 + d, n = (d + 1) % T::kDx;
+      if (s + 1 < stages) store_x(n, lds + (1 - d) * kStageBytes);
+      load_x(n, s + 1 + T::kDx);
+      if (s < stages) multiply(d, lds + d * kStageBytes);
+      load_w(d, s + 2);
       __syncthreads();
     }
   }
@@ -542,21 +543,32 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
   }
 }
 
-// K16 (mx4_tile): many rows of x. W is widened to 16-bit operands on its way into LDS, one block
-//   of 32 a thread and stage, x comes along in one part (f16, bf16) or three bf16 ones (f32), and
-//   both feed 32x32x16 MFMAs. f16 x takes f16 weights, exact for scales of 2^-23 to 2^13; a tile
-//   that meets another scale is formed again from bf16 parts, which hold any.
+// K16 (mx4_tile): many rows of x. W is widened to 16-bit operands in registers, x passes through
+//   LDS in one part (f16, bf16) or three bf16 ones (f32), and both feed 32x32x16 MFMAs. f16 x
+//   takes f16 weights, exact for scales of 2^-23 to 2^13; a tile that meets another scale is
+//   formed again from bf16 operands, which hold any, one part of x after the other.
 template <typename T, typename XT, typename OT>
 __global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
   const int f0 = (lid % n_f) * T::BF, t0 = (lid / n_f) * T::BT, grp = blockIdx.y;
   f32x16 acc[T::WF / 32][T::WT / 32];
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < T::WF / 32; ++i)
+#pragma unroll
+      for (int t = 0; t < T::WT / 32; ++t) acc[i][t] = f32x16{};
+  };
+  clear();
   if constexpr (__is_same(XT, _Float16)) {
-    if (tile_product<T, XT, _Float16, 1>(a, grp, f0, t0, lds, acc))
-      tile_product<T, XT, __bf16, kParts<XT>>(a, grp, f0, t0, lds, acc);
+    if (tile_product<T, XT, _Float16, 1>(a, grp, f0, t0, lds, 0, acc)) {
+      clear();
+#pragma unroll 1
+      for (int part = 1; part >= 0; --part)
+        tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, part, acc);
+    }
   } else {
-    tile_product<T, XT, __bf16, kParts<XT>>(a, grp, f0, t0, lds, acc);
+    tile_product<T, XT, __bf16, kParts<XT>>(a, grp, f0, t0, lds, 0, acc);
   }
   tile_store<T, OT>(a, grp, f0, t0, lds, whole, acc);
 }
@@ -708,8 +720,7 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 template <typename T, typename XT, typename OT>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
-  // f16 x may fall back to two parts.
-  constexpr size_t kLds = tile_lds<T, kParts<XT>>();
+  constexpr size_t kLds = tile_lds<T, sizeof(XT) == 2 ? 1 : kParts<XT>>();
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> set{0};
   const hipError_t e = allow_lds(&mx4_tile<T, XT, OT>, kLds, set);
@@ -730,9 +741,8 @@ hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
     return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups;
   };
   if constexpr (sizeof(XT) == 2) {
-    // Two parts of f16 x (scales out of range) take the smaller stages of a 256 x 128 tile.
-    using Large = Tile<256, 128, 64, 64, 1>;
-    if (wgs(256, 128) >= 256) return launch_tile<Large, XT, OT>(a, out_dt, s);
+    using Large = Tile<256, 256, 64, 128, 1>;
+    if (wgs(256, 256) >= 192) return launch_tile<Large, XT, OT>(a, out_dt, s);
   }
   if (wgs(128, 128) >= 192) return launch_tile<Mid, XT, OT>(a, out_dt, s);
   return launch_tile<Small, XT, OT>(a, out_dt, s);
