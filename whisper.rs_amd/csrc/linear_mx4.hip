@@ -7,6 +7,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
+#include <type_traits>
 
 namespace wrs {
 namespace {
@@ -323,11 +325,12 @@ __device__ inline float gelu_exp(float x) {
 }
 
 // Tile of a workgroup: BF features x BT rows of x, waves of WF x WT; x is loaded kDx stages
-// ahead.
-template <int BF_, int BT_, int WF_, int WT_, int Dx_>
+// ahead, and KG groups of waves take the stages in turn.
+template <int BF_, int BT_, int WF_, int WT_, int Dx_, int KG_>
 struct Tile {
-  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, kDx = Dx_;
-  static constexpr int kWaves = (BF / WF) * (BT / WT), kThreads = 64 * kWaves;
+  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, kDx = Dx_, KG = KG_;
+  static constexpr int kWaves = (BF / WF) * (BT / WT);  // of a group
+  static constexpr int kGroupThreads = 64 * kWaves, kThreads = kGroupThreads * KG;
 };
 constexpr int kK = 64;           // columns per stage
 constexpr int kRow = 2 * kK;     // bytes of a staged row
@@ -339,14 +342,20 @@ __device__ inline int chunk_at(int r, int c) { return r * kRow + 16 * (c ^ ((r >
 
 template <typename T, int P>
 constexpr size_t tile_lds() {
-  const size_t stage = 2ull * P * T::BT * kRow;
+  const size_t stage = 2ull * P * T::BT * kRow * T::KG;
   const size_t out = sizeof(float) * T::kWaves * 32 * kOutPitch;
-  return stage > out ? stage : out;
+  const size_t join = sizeof(float) * T::BF * T::BT * (T::KG - 1);
+  return stage > out ? (stage > join ? stage : join) : (out > join ? out : join);
 }
 
-// Adds one tile's products with operands of type E to acc. P: the parts of x that a stage
-// holds, all of them, or with P == 1 < kParts part `part`. Returns (to every thread) whether a
-// scale of the tile's weights lies outside what E holds exactly.
+// f32 x as two f16 parts of x * 2^7: 2^-23 of a value and 2^-25 at least. That is 2^-22 of the
+// row's largest value where it lies in [2^-10, 511].
+constexpr float kXUp = 128.f, kXLeast = 0x1p-10f, kXMost = 511.f;
+
+// Adds one tile's products with operands of type E to acc. x goes in P parts: one of its own
+// type, two of f16 (f32 x, E f16: results times kXUp), or with bf16 E part `part` of kParts.
+// Returns (to every thread) whether E cannot hold the tile's operands: a scale of its weights,
+// or a row of f32 x.
 //   W goes from memory to MFMA operands in registers: lane (r, h) of a 32-row block takes block
 //   h of row r, and step j of a stage multiplies values 8 j.. of both blocks, so x's operand is
 //   chunk 4 h + j of its staged row.
@@ -354,12 +363,17 @@ template <typename T, typename XT, typename E, int P>
 __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
                                     int part, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
-  constexpr int kXn = T::BT * (kK / 8) / T::kThreads;  // groups of 8 values of x a thread stages
-  static_assert(kXn >= 1 && T::BT * (kK / 8) % T::kThreads == 0, "whole groups");
+  constexpr int kXn = T::BT * (kK / 8) / T::kGroupThreads;  // groups of 8 values a thread stages
+  static_assert(kXn >= 1 && T::BT * (kK / 8) % T::kGroupThreads == 0, "whole groups");
   constexpr int kXBytes = T::BT * kRow, kStageBytes = P * kXBytes;
+  constexpr bool kHalves = P == 2;  // f32 x in two f16 parts
+  static_assert(!kHalves || (__is_same(XT, float) && __is_same(E, _Float16)), "");
   typedef XT x8 __attribute__((ext_vector_type(8), aligned(16)));
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int lane = threadIdx.x & 63;
+  const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / T::kGroupThreads);
+  const int tid = threadIdx.x - kg * T::kGroupThreads;  // in the group
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  lds += kg * 2 * kStageBytes;
   const int r32 = lane & 31, hl = lane >> 5;
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
   const int nb = a.n_in / kMx4Block, bytes = a.n_in / 2, stages = a.n_in / kK;
@@ -377,14 +391,19 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   const XT* xp[kXn];
 #pragma unroll
   for (int i = 0; i < kXn; ++i) {
-    const int e = tid + T::kThreads * i, row = min(e >> 3, n_t - 1);
+    const int e = tid + T::kGroupThreads * i, row = min(e >> 3, n_t - 1);
     xp[i] = static_cast<const XT*>(a.x) + (t0 + row) * a.x_rs + 8 * (e & 7);
   }
 
   u32x4 cw[2][kF];
   uint8_t sw[2][kF];
   x8 xv[T::kDx][kXn];
-  auto load_w = [&](int d, int s) __attribute__((always_inline)) {
+  float most[kXn];  // largest magnitudes of this thread's rows of x
+#pragma unroll
+  for (int i = 0; i < kXn; ++i) most[i] = 0.f;
+  // Stage i of the group is stage i * KG + kg of the tile.
+  auto load_w = [&](int d, int i_s) __attribute__((always_inline)) {
+    int s = i_s * T::KG + kg;
     asm("" : "+s"(s));  // offsets are formed per stage, not kept per load
 #pragma unroll
     for (int i = 0; i < kF; ++i) {
@@ -397,36 +416,51 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
           srs, in ? row * nb + hl + 2 * s : kPast, 0, 0);
     }
   };
-  auto load_x = [&](int d, int s) __attribute__((always_inline)) {
-    const int at = kK * min(s, stages - 1);
+  auto load_x = [&](int d, int i_s) __attribute__((always_inline)) {
+    const int at = kK * min(i_s * T::KG + kg, stages - 1);
 #pragma unroll
     for (int i = 0; i < kXn; ++i) xv[d][i] = *reinterpret_cast<const x8*>(xp[i] + at);
   };
   auto store_x = [&](int d, char* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kXn; ++i) {
-      const int e = tid + T::kThreads * i;
+      const int e = tid + T::kGroupThreads * i;
       char* const at = buf + chunk_at(e >> 3, e & 7);
-      if constexpr (P == 1 && __is_same(XT, E)) {
-        *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, xv[d][i]);
+      const x8& x = xv[d][i];
+      if constexpr (kHalves) {
+        u32x4 h, l;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          most[i] = fmaxf(most[i], fmaxf(__builtin_fabsf(x[j]), __builtin_fabsf(x[j + 1])));
+          f16x2 hi = {static_cast<_Float16>(__builtin_fmaf(x[j], kXUp, 0.f)),
+                      static_cast<_Float16>(__builtin_fmaf(x[j + 1], kXUp, 0.f))};
+          uint32_t w = __builtin_bit_cast(uint32_t, hi);
+          asm("" : "+v"(w));  // formed once, not again where it is taken off
+          hi = __builtin_bit_cast(f16x2, w);
+          const f16x2 lo = {
+              static_cast<_Float16>(__builtin_fmaf(x[j], kXUp, -static_cast<float>(hi[0]))),
+              static_cast<_Float16>(__builtin_fmaf(x[j + 1], kXUp, -static_cast<float>(hi[1])))};
+          h[j >> 1] = w;
+          l[j >> 1] = __builtin_bit_cast(uint32_t, lo);
+        }
+        *reinterpret_cast<u32x4*>(at) = h;
+        *reinterpret_cast<u32x4*>(at + kXBytes) = l;
+      } else if constexpr (__is_same(XT, E)) {
+        *reinterpret_cast<u32x4*>(at) = __builtin_bit_cast(u32x4, x);
       } else {
         constexpr int kAll = kParts<XT>;
-        u32x4 w[kAll];
+        u32x4 w;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
           uint32_t lo[kAll], hi[kAll];
-          split_top<kAll>(static_cast<float>(xv[d][i][j]), lo);
-          split_top<kAll>(static_cast<float>(xv[d][i][j + 1]), hi);
+          split_top<kAll>(static_cast<float>(x[j]), lo);
+          split_top<kAll>(static_cast<float>(x[j + 1]), hi);
+          uint32_t v = pack_top(lo[0], hi[0]);
 #pragma unroll
-          for (int p = 0; p < kAll; ++p) w[p][j >> 1] = pack_top(lo[p], hi[p]);
+          for (int p = 1; p < kAll; ++p) v = part == p ? pack_top(lo[p], hi[p]) : v;
+          w[j >> 1] = v;
         }
-        if constexpr (P == kAll) {
-#pragma unroll
-          for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(at + p * kXBytes) = w[p];
-        } else {
-          static_assert(P == 1 && kAll == 2, "one of two parts");
-          *reinterpret_cast<u32x4*>(at) = part ? w[1] : w[0];
-        }
+        *reinterpret_cast<u32x4*>(at) = w;
       }
     }
   };
@@ -468,15 +502,43 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   store_x(0, lds);
   load_x(0, T::kDx);
   __syncthreads();
-  for (int s0 = 0; s0 < stages; s0 += 2) {
+  const int turns = (stages + T::KG - 1) / T::KG;  // of every group, the last ones may be empty
+  for (int s0 = 0; s0 < turns; s0 += 2) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
       const int s = s0 + d, n = (d + 1) % T::kDx;
-      if (s + 1 < stages) store_x(n, lds + (1 - d) * kStageBytes);
+      if (s + 1 < turns) store_x(n, lds + (1 - d) * kStageBytes);
       load_x(n, s + 1 + T::kDx);
-      if (s < stages) multiply(d, lds + d * kStageBytes);
+      if (s * T::KG + kg < stages) multiply(d, lds + d * kStageBytes);
       load_w(d, s + 2);
       __syncthreads();
+    }
+  }
+  if constexpr (kHalves) {
+    // 8 neighbouring lanes staged a row. Rows past the last one repeat it.
+#pragma unroll
+    for (int i = 0; i < kXn; ++i) {
+      float m = most[i];
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+      if constexpr (T::KG > 1) {
+        // The groups staged other columns of the same rows.
+        float* const all = reinterpret_cast<float*>(lds - kg * 2 * kStageBytes);
+        const int row = (tid + T::kGroupThreads * i) >> 3;
+        if (i == 0) __syncthreads();
+        if ((tid & 7) == 0) all[kg * T::BT + row] = m;
+      }
+      if constexpr (T::KG == 1) odd |= m != 0.f && !(m >= kXLeast && m <= kXMost);
+    }
+    if constexpr (T::KG > 1) {
+      __syncthreads();
+      const float* const all = reinterpret_cast<const float*>(lds - kg * 2 * kStageBytes);
+      if (threadIdx.x < T::BT) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < T::KG; ++i) m = fmaxf(m, all[i * T::BT + threadIdx.x]);
+        odd |= m != 0.f && !(m >= kXLeast && m <= kXMost);
+      }
     }
   }
   return __syncthreads_or(odd);
@@ -487,10 +549,36 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 // 32 rows each).
 template <typename T, typename OT>
 __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
-                                  bool whole, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+                                  bool whole, float down,
+                                  f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32, kFe = kF > 1 ? 2 : 1;  // feature blocks a pass
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if constexpr (T::KG > 1) {
+    // The groups' sums join the first group's, in order.
+    f32x4* const join = reinterpret_cast<f32x4*>(lds);
+    constexpr int kQuads = kF * kT * 4;
+    if (wave >= T::kWaves) {
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        const f32x16& x = acc[q / 4 / kT][q / 4 % kT];
+        join[((wave - T::kWaves) * kQuads + q) * 64 + lane] =
+            f32x4{x[4 * (q & 3)], x[4 * (q & 3) + 1], x[4 * (q & 3) + 2], x[4 * (q & 3) + 3]};
+      }
+    }
+    __syncthreads();
+    if (wave < T::kWaves) {
+      for (int k = 0; k < T::KG - 1; ++k)
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+          const f32x4 x = join[((k * T::kWaves + wave) * kQuads + q) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[q / 4 / kT][q / 4 % kT][4 * (q & 3) + e] += x[e];
+        }
+    }
+    __syncthreads();
+    if (wave >= T::kWaves) return;
+  }
   const int r32 = lane & 31, hl = lane >> 5;
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
   float* const mine = reinterpret_cast<float*>(lds) + wave * 32 * kOutPitch;
@@ -522,7 +610,7 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          y[e] = (e < 4 ? y0[e & 3] : y1[e & 3]) + b[e];
+          y[e] = __builtin_fmaf(e < 4 ? y0[e & 3] : y1[e & 3], down, b[e]);
           if (a.act == kActGelu) y[e] = gelu_exp(y[e]);
         }
         if (row >= a.n_tokens || r >= a.n_out) continue;
@@ -544,9 +632,10 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
 }
 
 // K16 (mx4_tile): many rows of x. W is widened to 16-bit operands in registers, x passes through
-//   LDS in one part (f16, bf16) or three bf16 ones (f32), and both feed 32x32x16 MFMAs. f16 x
-//   takes f16 weights, exact for scales of 2^-23 to 2^13; a tile that meets another scale is
-//   formed again from bf16 operands, which hold any, one part of x after the other.
+//   LDS in one part (f16, bf16) or two f16 ones (f32), and both feed 32x32x16 MFMAs. f16 holds
+//   weights of scales 2^-23 to 2^13 exactly, and rows of f32 x whose largest value is of
+//   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
+//   one of x's two or three parts after the other.
 template <typename T, typename XT, typename OT>
 __global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -560,17 +649,21 @@ __global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f
       for (int t = 0; t < T::WT / 32; ++t) acc[i][t] = f32x16{};
   };
   clear();
-  if constexpr (__is_same(XT, _Float16)) {
-    if (tile_product<T, XT, _Float16, 1>(a, grp, f0, t0, lds, 0, acc)) {
+  float down = 1.f;
+  if constexpr (__is_same(XT, __bf16)) {
+    tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, 0, acc);
+  } else {
+    constexpr int kP = __is_same(XT, float) ? 2 : 1;
+    if (kP == 2) down = 1.f / kXUp;
+    if (tile_product<T, XT, _Float16, kP>(a, grp, f0, t0, lds, 0, acc)) {
       clear();
+      down = 1.f;
 #pragma unroll 1
-      for (int part = 1; part >= 0; --part)
+      for (int part = kParts<XT> - 1; part >= 0; --part)
         tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, part, acc);
     }
-  } else {
-    tile_product<T, XT, __bf16, kParts<XT>>(a, grp, f0, t0, lds, 0, acc);
   }
-  tile_store<T, OT>(a, grp, f0, t0, lds, whole, acc);
+  tile_store<T, OT>(a, grp, f0, t0, lds, whole, down, acc);
 }
 
 constexpr int kTile = 64;
@@ -720,7 +813,7 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 template <typename T, typename XT, typename OT>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
-  constexpr size_t kLds = tile_lds<T, sizeof(XT) == 2 ? 1 : kParts<XT>>();
+  constexpr size_t kLds = tile_lds<T, sizeof(XT) == 2 ? 1 : 2>();
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> set{0};
   const hipError_t e = allow_lds(&mx4_tile<T, XT, OT>, kLds, set);
@@ -735,16 +828,19 @@ hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 template <typename XT, typename OT>
 hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
-  using Small = Tile<64, 64, 32, 32, 2>;
-  using Mid = Tile<128, 128, 64, 64, 1>;
+  using Small = Tile<64, 32, 32, 32, 1, 4>;
+  using Mid = Tile<64, 64, 32, 32, 1, 2>;
+  using Wide = Tile<128, 128, 64, 64, 1, 1>;
+  using Large = std::conditional_t<sizeof(XT) == 2, Tile<256, 256, 64, 128, 1, 1>,
+                                   Tile<256, 128, 64, 64, 1, 1>>;
   auto wgs = [&](int f, int t) {
     return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups;
   };
-  if constexpr (sizeof(XT) == 2) {
-    using Large = Tile<256, 256, 64, 128, 1>;
-    if (wgs(256, 256) >= 192) return launch_tile<Large, XT, OT>(a, out_dt, s);
-  }
-  if (wgs(128, 128) >= 192) return launch_tile<Mid, XT, OT>(a, out_dt, s);
+  int force = 0;
+  if (const char* e = getenv("MX4_FORCE")) force = atoi(e);
+  if (force == 1 || (!force && wgs(Large::BF, Large::BT) >= 192)) return launch_tile<Large, XT, OT>(a, out_dt, s);
+  if (force == 2 || (!force && wgs(128, 128) >= 192)) return launch_tile<Wide, XT, OT>(a, out_dt, s);
+  if (force == 3 || (!force && wgs(64, 64) >= 256)) return launch_tile<Mid, XT, OT>(a, out_dt, s);
   return launch_tile<Small, XT, OT>(a, out_dt, s);
 }
 
