@@ -341,8 +341,8 @@ constexpr int kOutPitch = 68;    // floats of an output row in LDS
 __device__ inline int chunk_at(int r, int c) { return r * kRow + 16 * (c ^ ((r >> 1) & 7)); }
 
 template <typename T, int P>
-constexpr size_t tile_lds() {
-  const size_t stage = 2ull * P * T::BT * kRow * T::KG;
+constexpr size_t tile_lds() {  // P 0: MXFP4 x, whose scales lie behind its codes
+  const size_t stage = 2ull * (P ? P * kRow : kRow + 8) * T::BT * T::KG;
   const size_t out = sizeof(float) * T::kWaves * 32 * kOutPitch;
   const size_t join = sizeof(float) * T::BF * T::BT * (T::KG - 1);
   return stage > out ? (stage > join ? stage : join) : (out > join ? out : join);
@@ -488,9 +488,9 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-        for (int i = 0; i < kF; ++i)
+        for (int t = 0; t < kT; ++t)
 #pragma unroll
-          for (int t = 0; t < kT; ++t) acc[i][t] = mfma32<E>(wv[i], xw[p][t], acc[i][t]);
+          for (int i = 0; i < kF; ++i) acc[i][t] = mfma32<E>(wv[i], xw[p][t], acc[i][t]);
     }
   };
 
@@ -503,7 +503,22 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   load_x(0, T::kDx);
   __syncthreads();
   const int turns = (stages + T::KG - 1) / T::KG;  // of every group, the last ones may be empty
-  for (int s0 = 0; s0 < turns; s0 += 2) {
+  int s0 = 0;
+  // No branch in this loop: one around the products costs copies of the sums (64 moves per two
+  // stages of a 64 x 128 wave).
+  for (; s0 + 3 < turns; s0 += 2) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const int s = s0 + d, n = (d + 1) % T::kDx;
+      store_x(n, lds + (1 - d) * kStageBytes);
+      load_x(n, s + 1 + T::kDx);
+      __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
+      multiply(d, lds + d * kStageBytes);
+      load_w(d, s + 2);
+      __syncthreads();
+    }
+  }
+  for (; s0 < turns; s0 += 2) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
       const int s = s0 + d, n = (d + 1) % T::kDx;
@@ -542,6 +557,142 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     }
   }
   return __syncthreads_or(odd);
+}
+
+// Four scale bytes from `at` of a row on (an even place): one load where they lie on a word.
+__device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, bool words, uint32_t at,
+                                       bool in, bool in_high) {
+  if (words) return __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at : kPast, 0, 0);
+  const uint32_t lo = static_cast<uint16_t>(
+      __builtin_amdgcn_raw_buffer_load_b16(rs, in ? at : kPast, 0, 0));
+  const uint32_t hi = static_cast<uint16_t>(
+      __builtin_amdgcn_raw_buffer_load_b16(rs, in_high ? at + 2 : kPast, 0, 0));
+  return lo | (hi << 16);
+}
+
+// The same for MXFP4 x: 256 columns a stage, codes as they are into 32x32x64 MFMAs. Lane (r, h)
+// holds blocks 4 h + 0..3 of row r, step q multiplies block 4 h + q, whose scale is byte q of
+// the row's word h.
+template <typename T>
+__device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
+                                        f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+  constexpr int kF = T::WF / 32, kT = T::WT / 32;
+  constexpr int kXn = T::BT * 8 / T::kGroupThreads;  // 16-byte chunks of x a thread stages
+  static_assert(kXn >= 1 && T::BT * 8 % T::kGroupThreads == 0, "whole chunks");
+  static_assert(2 * T::BT <= T::kGroupThreads, "a word of scales a thread");
+  constexpr int kStageBytes = T::BT * kRow + T::BT * 8;
+  constexpr int kBlocks = 8;  // of a stage
+  const int lane = threadIdx.x & 63;
+  const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / T::kGroupThreads);
+  const int tid = threadIdx.x - kg * T::kGroupThreads;  // in the group
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  lds += kg * 2 * kStageBytes;
+  const int r32 = lane & 31, hl = lane >> 5;
+  const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
+  const int nb = a.n_in / kMx4Block, bytes = a.n_in / 2;
+  const int stages = (nb + kBlocks - 1) / kBlocks;
+
+  // Rows past the last and blocks past a row's last read as zero: codes of 0, scale 2^-127.
+  const int n_f = min(T::BF, a.n_out - f0), n_t = min(T::BT, a.n_tokens - t0);
+  const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(a.w[grp] + static_cast<int64_t>(f0) * bytes), 0, n_f * bytes,
+      kRawBuffer);
+  const uint8_t* const sp = a.w_scales[grp] + static_cast<int64_t>(f0) * nb;
+  const __amdgpu_buffer_rsrc_t srs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(sp), 0, n_f * nb, kRawBuffer);
+  const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(static_cast<const uint8_t*>(a.x) + static_cast<int64_t>(t0) * bytes),
+      0, n_t * bytes, kRawBuffer);
+  const uint8_t* const xp = a.x_scales + static_cast<int64_t>(t0) * nb;
+  const __amdgpu_buffer_rsrc_t xsrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(xp), 0, n_t * nb, kRawBuffer);
+  const bool w_words = nb % 4 == 0 && (reinterpret_cast<uintptr_t>(sp) & 3) == 0;
+  const bool x_words = nb % 4 == 0 && (reinterpret_cast<uintptr_t>(xp) & 3) == 0;
+
+  u32x4 cw[2][kF][4], xv[kXn];
+  uint32_t sw[2][kF], xs;
+  auto load_w = [&](int d, int i_s) __attribute__((always_inline)) {
+    int b = kBlocks * (i_s * T::KG + kg);  // the stage's first block
+    asm("" : "+s"(b));  // offsets are formed per stage, not kept per load
+#pragma unroll
+    for (int i = 0; i < kF; ++i) {
+      const int row = wf + 32 * i + r32, at = b + 4 * hl;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        cw[d][i][q] = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                       wrs, at + q < nb ? row * bytes + 16 * (at + q) : kPast, 0, 0));
+      sw[d][i] = load_scales(srs, w_words, row * nb + at, at < nb, at + 2 < nb);
+    }
+  };
+  auto load_x = [&](int i_s) __attribute__((always_inline)) {
+    int b = kBlocks * (i_s * T::KG + kg);
+    asm("" : "+s"(b));
+#pragma unroll
+    for (int i = 0; i < kXn; ++i) {
+      const int e = tid + T::kGroupThreads * i, at = b + (e & 7);
+      xv[i] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                     xrs, at < nb ? (e >> 3) * bytes + 16 * at : kPast, 0, 0));
+    }
+    const int at = b + 4 * (tid & 1);
+    const bool mine = tid < 2 * T::BT;
+    xs = load_scales(xsrs, x_words, (tid >> 1) * nb + at, mine && at < nb, mine && at + 2 < nb);
+  };
+  auto store_x = [&](char* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kXn; ++i) {
+      const int e = tid + T::kGroupThreads * i;
+      *reinterpret_cast<u32x4*>(buf + chunk_at(e >> 3, e & 7)) = xv[i];
+    }
+    if (2 * T::BT == T::kGroupThreads || tid < 2 * T::BT)
+      *reinterpret_cast<uint32_t*>(buf + T::BT * kRow + 4 * tid) = xs;
+  };
+  auto multiply = [&](int d, const char* buf) __attribute__((always_inline)) {
+    int xsc[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t)
+      xsc[t] = *reinterpret_cast<const int*>(buf + T::BT * kRow + 8 * (wt + 32 * t + r32) + 4 * hl);
+#define WRS_MX4_STEP(Q)                                                                         \
+  {                                                                                             \
+    u32x4 xw[kT];                                                                               \
+    _Pragma("unroll") for (int t = 0; t < kT; ++t) xw[t] = *reinterpret_cast<const u32x4*>(     \
+        buf + chunk_at(wt + 32 * t + r32, 4 * hl + Q));                                         \
+    _Pragma("unroll") for (int t = 0; t < kT; ++t)                                              \
+        _Pragma("unroll") for (int i = 0; i < kF; ++i) {                                        \
+      const u32x4 &w = cw[d][i][Q], &x = xw[t];                                                 \
+      const i32x8 wa = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};                \
+      const i32x8 xa = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};                \
+      acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                              \
+          wa, xa, acc[i][t], 4, 4, Q, static_cast<int>(sw[d][i]), Q, xsc[t]);                   \
+    }                                                                                           \
+  }
+    WRS_MX4_STEP(0)
+    WRS_MX4_STEP(1)
+    WRS_MX4_STEP(2)
+    WRS_MX4_STEP(3)
+#undef WRS_MX4_STEP
+  };
+
+  load_x(0);
+  load_w(0, 0);
+  load_w(1, 1);
+  store_x(lds);
+  load_x(1);
+  __syncthreads();
+  // Stages past the last one are zeros.
+  const int turns = (stages + T::KG - 1) / T::KG;
+  for (int s0 = 0; s0 < turns; s0 += 2) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      store_x(lds + (1 - d) * kStageBytes);
+      load_x(s0 + d + 2);
+      __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
+      multiply(d, lds + d * kStageBytes);
+      load_w(d, s0 + d + 2);
+      __syncthreads();
+    }
+  }
 }
 
 // The tile's outputs: each wave passes 32 rows x 64 features at a time through its own LDS, so
@@ -637,7 +788,7 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
 //   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
 //   one of x's two or three parts after the other.
 template <typename T, typename XT, typename OT>
-__global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
+__global__ __launch_bounds__(T::kThreads, 2) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
   const int f0 = (lid % n_f) * T::BF, t0 = (lid / n_f) * T::BT, grp = blockIdx.y;
@@ -650,7 +801,9 @@ __global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f
   };
   clear();
   float down = 1.f;
-  if constexpr (__is_same(XT, __bf16)) {
+  if constexpr (sizeof(XT) == 1) {
+    tile_product_mx4<T>(a, grp, f0, t0, lds, acc);
+  } else if constexpr (__is_same(XT, __bf16)) {
     tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, 0, acc);
   } else {
     constexpr int kP = __is_same(XT, float) ? 2 : 1;
@@ -664,64 +817,6 @@ __global__ __launch_bounds__(T::kThreads) void mx4_tile(Mx4LinearArgs a, int n_f
     }
   }
   tile_store<T, OT>(a, grp, f0, t0, lds, whole, down, acc);
-}
-
-constexpr int kTile = 64;
-
-__device__ inline float value_of(uint32_t code, int scale) {
-  if (scale == 255) return __builtin_nanf("");
-  const uint32_t m = code & 7u;
-  const float y = m < 2 ? 0.5f * m : __builtin_ldexpf(2.f + (m & 1u), static_cast<int>(m >> 1) - 2);
-  return __builtin_ldexpf((code & 8u) ? -y : y, scale - 127);
-}
-
-template <typename XT, typename OT>
-__global__ __launch_bounds__(256) void linear_mx4_tile(Mx4LinearArgs a) {
-  __shared__ float xs[kMx4Block][kTile + 1], ws[kMx4Block][kTile + 1];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int t0 = blockIdx.x * kTile, r0 = blockIdx.y * kTile, g = blockIdx.z;
-  const int blocks = a.n_in / kMx4Block;
-  float acc[4][4] = {};
-  for (int b = 0; b < blocks; ++b) {
-    for (int e = tid; e < kTile * kMx4Block; e += 256) {
-      const int i = e >> 5, k = e & 31, col = b * kMx4Block + k;
-      float xv = 0.f, wv = 0.f;
-      if (t0 + i < a.n_tokens) {
-        if constexpr (sizeof(XT) == 1) {
-          const int64_t row = t0 + i;
-          const uint32_t c = static_cast<const uint8_t*>(a.x)[row * (a.n_in / 2) + col / 2];
-          xv = value_of(c >> (4 * (col & 1)), a.x_scales[row * blocks + b]);
-        } else {
-          xv = static_cast<float>(static_cast<const XT*>(a.x)[(t0 + i) * a.x_rs + col]);
-        }
-      }
-      if (r0 + i < a.n_out) {
-        const int64_t row = r0 + i;
-        const uint32_t c = a.w[g][row * (a.n_in / 2) + col / 2];
-        wv = value_of(c >> (4 * (col & 1)), a.w_scales[g][row * blocks + b]);
-      }
-      xs[k][i] = xv;
-      ws[k][i] = wv;
-    }
-    __syncthreads();
-    for (int k = 0; k < kMx4Block; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + ty + 16 * i, r = r0 + tx + 16 * j;
-      if (t >= a.n_tokens || r >= a.n_out) continue;
-      float y = acc[i][j] + (a.bias[g] ? a.bias[g][r] : 0.f);
-      if (a.act == kActGelu) y = gelu_tanh(y);
-      static_cast<OT*>(a.out[g])[t * a.out_rs + (r >> 6) * a.out_hs + (r & 63)] = static_cast<OT>(y);
-    }
 }
 
 // Whether output chunks of 8 features can be stored whole.
@@ -813,7 +908,7 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 template <typename T, typename XT, typename OT>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
-  constexpr size_t kLds = tile_lds<T, sizeof(XT) == 2 ? 1 : 2>();
+  constexpr size_t kLds = tile_lds<T, sizeof(XT) == 1 ? 0 : sizeof(XT) == 2 ? 1 : 2>();
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> set{0};
   const hipError_t e = allow_lds(&mx4_tile<T, XT, OT>, kLds, set);
@@ -831,7 +926,7 @@ hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   using Small = Tile<64, 32, 32, 32, 1, 4>;
   using Mid = Tile<64, 64, 32, 32, 1, 2>;
   using Wide = Tile<128, 128, 64, 64, 1, 1>;
-  using Large = std::conditional_t<sizeof(XT) == 2, Tile<256, 256, 64, 128, 1, 1>,
+  using Large = std::conditional_t<sizeof(XT) <= 2, Tile<256, 128, 64, 128, 1, 1>,
                                    Tile<256, 128, 64, 64, 1, 1>>;
   auto wgs = [&](int f, int t) {
     return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups;
@@ -848,7 +943,6 @@ hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s) {
   if (a.n_tokens <= 0 || a.n_out <= 0 || a.n_groups <= 0) return hipSuccess;
-  const dim3 grid((a.n_tokens + kTile - 1) / kTile, (a.n_out + kTile - 1) / kTile, a.n_groups);
   if (a.n_tokens <= kMx4Rows) {
     if (a.x_scales) return launch_rows_of<uint8_t>(a, out_dt, s);
     switch (x_dt) {
@@ -858,19 +952,6 @@ hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, h
       default: return hipErrorInvalidValue;
     }
   }
-#define WRS_MX4_OUT(XT)                                                                      \
-  switch (out_dt) {                                                                          \
-    case kF32:                                                                               \
-      hipLaunchKernelGGL((linear_mx4_tile<XT, float>), grid, dim3(256), 0, s, a);            \
-      break;                                                                                 \
-    case kF16:                                                                               \
-      hipLaunchKernelGGL((linear_mx4_tile<XT, _Float16>), grid, dim3(256), 0, s, a);         \
-      break;                                                                                 \
-    case kBF16:                                                                              \
-      hipLaunchKernelGGL((linear_mx4_tile<XT, __bf16>), grid, dim3(256), 0, s, a);           \
-      break;                                                                                 \
-    default: return hipErrorInvalidValue;                                                    \
-  }
 #define WRS_MX4_TILES(XT)                                                                    \
   switch (out_dt) {                                                                          \
     case kF32: return launch_tiles<XT, float>(a, out_dt, s);                                 \
@@ -879,7 +960,7 @@ hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, h
     default: return hipErrorInvalidValue;                                                    \
   }
   if (a.x_scales) {
-    WRS_MX4_OUT(uint8_t)
+    WRS_MX4_TILES(uint8_t)
   } else {
     switch (x_dt) {
       case kF32: WRS_MX4_TILES(float)
@@ -889,7 +970,6 @@ hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, h
     }
   }
 #undef WRS_MX4_TILES
-#undef WRS_MX4_OUT
   return hipGetLastError();
 }
 
