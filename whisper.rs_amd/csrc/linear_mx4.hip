@@ -560,9 +560,10 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 }
 
 // Four scale bytes from `at` of a row on (an even place): one load where they lie on a word.
-__device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, bool words, uint32_t at,
-                                       bool in, bool in_high) {
-  if (words) return __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at : kPast, 0, 0);
+template <bool kWords>
+__device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_t at, bool in,
+                                       bool in_high) {
+  if constexpr (kWords) return __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at : kPast, 0, 0);
   const uint32_t lo = static_cast<uint16_t>(
       __builtin_amdgcn_raw_buffer_load_b16(rs, in ? at : kPast, 0, 0));
   const uint32_t hi = static_cast<uint16_t>(
@@ -573,7 +574,7 @@ __device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, bool wo
 // The same for MXFP4 x: 256 columns a stage, codes as they are into 32x32x64 MFMAs. Lane (r, h)
 // holds blocks 4 h + 0..3 of row r, step q multiplies block 4 h + q, whose scale is byte q of
 // the row's word h.
-template <typename T>
+template <typename T, bool kWords>
 __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
                                         f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
@@ -597,32 +598,34 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(a.w[grp] + static_cast<int64_t>(f0) * bytes), 0, n_f * bytes,
       kRawBuffer);
-  const uint8_t* const sp = a.w_scales[grp] + static_cast<int64_t>(f0) * nb;
   const __amdgpu_buffer_rsrc_t srs = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(sp), 0, n_f * nb, kRawBuffer);
+      const_cast<uint8_t*>(a.w_scales[grp] + static_cast<int64_t>(f0) * nb), 0, n_f * nb,
+      kRawBuffer);
   const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(static_cast<const uint8_t*>(a.x) + static_cast<int64_t>(t0) * bytes),
       0, n_t * bytes, kRawBuffer);
-  const uint8_t* const xp = a.x_scales + static_cast<int64_t>(t0) * nb;
   const __amdgpu_buffer_rsrc_t xsrs = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(xp), 0, n_t * nb, kRawBuffer);
-  const bool w_words = nb % 4 == 0 && (reinterpret_cast<uintptr_t>(sp) & 3) == 0;
-  const bool x_words = nb % 4 == 0 && (reinterpret_cast<uintptr_t>(xp) & 3) == 0;
-
-  u32x4 cw[2][kF][4], xv[kXn];
+      const_cast<uint8_t*>(a.x_scales + static_cast<int64_t>(t0) * nb), 0, n_t * nb, kRawBuffer);
+  // Codes of W load into the registers whose step has just read them.
+  u32x4 cw[kF][4], xv[kXn];
   uint32_t sw[2][kF], xs;
-  auto load_w = [&](int d, int i_s) __attribute__((always_inline)) {
+  auto load_w = [&](int q, int i_s) __attribute__((always_inline)) {
     int b = kBlocks * (i_s * T::KG + kg);  // the stage's first block
     asm("" : "+s"(b));  // offsets are formed per stage, not kept per load
 #pragma unroll
     for (int i = 0; i < kF; ++i) {
-      const int row = wf + 32 * i + r32, at = b + 4 * hl;
+      const int row = wf + 32 * i + r32, at = b + 4 * hl + q;
+      cw[i][q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                               wrs, at < nb ? row * bytes + 16 * at : kPast, 0, 0));
+    }
+  };
+  auto load_sw = [&](int d, int i_s) __attribute__((always_inline)) {
+    int b = kBlocks * (i_s * T::KG + kg);
+    asm("" : "+s"(b));
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        cw[d][i][q] = __builtin_bit_cast(
-            u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                       wrs, at + q < nb ? row * bytes + 16 * (at + q) : kPast, 0, 0));
-      sw[d][i] = load_scales(srs, w_words, row * nb + at, at < nb, at + 2 < nb);
+    for (int i = 0; i < kF; ++i) {
+      const int row = wf + 32 * i + r32, at = b + 4 * hl;
+      sw[d][i] = load_scales<kWords>(srs, row * nb + at, at < nb, at + 2 < nb);
     }
   };
   auto load_x = [&](int i_s) __attribute__((always_inline)) {
@@ -637,7 +640,7 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
     }
     const int at = b + 4 * (tid & 1);
     const bool mine = tid < 2 * T::BT;
-    xs = load_scales(xsrs, x_words, (tid >> 1) * nb + at, mine && at < nb, mine && at + 2 < nb);
+    xs = load_scales<kWords>(xsrs, (tid >> 1) * nb + at, mine && at < nb, mine && at + 2 < nb);
   };
   auto store_x = [&](char* buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -648,7 +651,7 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
     if (2 * T::BT == T::kGroupThreads || tid < 2 * T::BT)
       *reinterpret_cast<uint32_t*>(buf + T::BT * kRow + 4 * tid) = xs;
   };
-  auto multiply = [&](int d, const char* buf) __attribute__((always_inline)) {
+  auto multiply = [&](int d, const char* buf, int next) __attribute__((always_inline)) {
     int xsc[kT];
 #pragma unroll
     for (int t = 0; t < kT; ++t)
@@ -660,12 +663,14 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
         buf + chunk_at(wt + 32 * t + r32, 4 * hl + Q));                                         \
     _Pragma("unroll") for (int t = 0; t < kT; ++t)                                              \
         _Pragma("unroll") for (int i = 0; i < kF; ++i) {                                        \
-      const u32x4 &w = cw[d][i][Q], &x = xw[t];                                                 \
+      const u32x4 &w = cw[i][Q], &x = xw[t];                                                    \
       const i32x8 wa = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};                \
       const i32x8 xa = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};                \
       acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                              \
           wa, xa, acc[i][t], 4, 4, Q, static_cast<int>(sw[d][i]), Q, xsc[t]);                   \
     }                                                                                           \
+    load_w(Q, next);                                                                            \
+    __builtin_amdgcn_sched_barrier(0);                                                          \
   }
     WRS_MX4_STEP(0)
     WRS_MX4_STEP(1)
@@ -675,8 +680,10 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   };
 
   load_x(0);
-  load_w(0, 0);
-  load_w(1, 1);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) load_w(q, 0);
+  load_sw(0, 0);
+  load_sw(1, 1);
   store_x(lds);
   load_x(1);
   __syncthreads();
@@ -688,8 +695,8 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
       store_x(lds + (1 - d) * kStageBytes);
       load_x(s0 + d + 2);
       __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
-      multiply(d, lds + d * kStageBytes);
-      load_w(d, s0 + d + 2);
+      multiply(d, lds + d * kStageBytes, s0 + d + 1);
+      load_sw(d, s0 + d + 2);
       __syncthreads();
     }
   }
@@ -787,7 +794,7 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
 //   weights of scales 2^-23 to 2^13 exactly, and rows of f32 x whose largest value is of
 //   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
 //   one of x's two or three parts after the other.
-template <typename T, typename XT, typename OT>
+template <typename T, typename XT, typename OT, bool kWords>
 __global__ __launch_bounds__(T::kThreads, 2) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
@@ -802,7 +809,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void mx4_tile(Mx4LinearArgs a, int 
   clear();
   float down = 1.f;
   if constexpr (sizeof(XT) == 1) {
-    tile_product_mx4<T>(a, grp, f0, t0, lds, acc);
+    tile_product_mx4<T, kWords>(a, grp, f0, t0, lds, acc);
   } else if constexpr (__is_same(XT, __bf16)) {
     tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, 0, acc);
   } else {
@@ -906,17 +913,24 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   }
 }
 
-template <typename T, typename XT, typename OT>
+template <typename T, typename XT, typename OT, bool kWords = true>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
+  if constexpr (sizeof(XT) == 1 && kWords) {
+    // MXFP4 x: four scales a load where the rows' scales lie on words.
+    bool words = a.n_in % (4 * kMx4Block) == 0 && (reinterpret_cast<uintptr_t>(a.x_scales) & 3) == 0;
+    for (int g = 0; g < a.n_groups; ++g)
+      words = words && (reinterpret_cast<uintptr_t>(a.w_scales[g]) & 3) == 0;
+    if (!words) return launch_tile<T, XT, OT, false>(a, out_dt, s);
+  }
   constexpr size_t kLds = tile_lds<T, sizeof(XT) == 1 ? 0 : sizeof(XT) == 2 ? 1 : 2>();
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
   static std::atomic<uint64_t> set{0};
-  const hipError_t e = allow_lds(&mx4_tile<T, XT, OT>, kLds, set);
+  const hipError_t e = allow_lds(&mx4_tile<T, XT, OT, kWords>, kLds, set);
   if (e != hipSuccess) return e;
   const int n_f = (a.n_out + T::BF - 1) / T::BF;
   const int64_t wgs = static_cast<int64_t>(n_f) * ((a.n_tokens + T::BT - 1) / T::BT);
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((mx4_tile<T, XT, OT>), dim3(static_cast<unsigned>(wgs), a.n_groups),
+  hipLaunchKernelGGL((mx4_tile<T, XT, OT, kWords>), dim3(static_cast<unsigned>(wgs), a.n_groups),
                      dim3(T::kThreads), kLds, s, a, n_f, whole_chunks(a, out_dt) ? 1 : 0);
   return hipGetLastError();
 }
