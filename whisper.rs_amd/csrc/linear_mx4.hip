@@ -67,13 +67,6 @@ constexpr int kGroup = 8;       // blocks of a row that a wave takes at a time: 
 constexpr int kCodeBytes = 16 * kGroup * 16;            // of a tile's group
 constexpr int kStage = kCodeBytes + 16 * kGroup + 128;  // LDS of a wave: codes, scales, pad
 
-__device__ inline void wave_sync() {
-  // LDS operations of one wave complete in order: only the compiler must keep it.
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // K15 (mx4_rows): up to 16 rows of x, bound by the stream of codes. A wave multiplies tiles of
 //   16 features; `ks` waves share a tile and take its groups of 8 blocks in turn, `chunk` groups
 //   at a time for a workgroup. Codes come in whole 128-byte pieces of rows (a lane's operand is

@@ -11,30 +11,44 @@
 //   chunks of a block merge through memory (the last workgroup to count in adds
 //   the partials up in chunk order, so results do not depend on which it is).
 //   Only the steps that reach past the cache test the ancestor bits.
-//   The products run on the f32 matrix pipe, f16 planes widened exactly:
-//   S^T = K Q^T with lane (c, g) holding key c's values d = 16 g + 0..15, so that
-//   lane (r, g) gets scores of keys 4 g + 0..3 of row r, which are the B operand of
-//   O^T += V^T P^T as they stand.
-#include "wrs_internal.hpp"
+//   f16 planes run on the f16 matrix pipe with operands in three parts, f32 ones on the
+//   f32 matrix pipe.
+#include "split16.hpp"
 
 #include <algorithm>
+#include <cstdlib>
 
 namespace wrs {
 namespace {
 
+using namespace split16;
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
-constexpr int kStep = 16;       // keys per wave step
-constexpr int kPitch = 66;      // LDS pitch (floats) of a merge row
+constexpr int kStep = 16;       // keys per wave step of the f32 path
+constexpr int kPitch = 68;      // LDS pitch (floats) of a merge row
 constexpr int kCounterStride = 32;  // 128 bytes between merge counters
 constexpr int kMergeLoads = 8;  // partials in flight per thread in the merge
 constexpr int kRawBuffer = 0x00020000;  // buffer resource word 3: raw, 32-bit data format
+
+// Two floats at once, as st_agent and ld_agent (8-byte aligned).
+__device__ inline void st_agent2(float* p, float x, float y) {
+  const uint64_t v = __builtin_bit_cast(uint32_t, x) |
+                     static_cast<uint64_t>(__builtin_bit_cast(uint32_t, y)) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void ld_agent2(const float* p, float& x, float& y) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  x = __builtin_bit_cast(float, static_cast<uint32_t>(v));
+  y = __builtin_bit_cast(float, static_cast<uint32_t>(v >> 32));
+}
 
 // 4 values of a plane row at byte offset `o` (multiple of 4 values), zero past the range.
 template <typename KT>
@@ -46,13 +60,378 @@ __device__ inline f32x4 load4(const __amdgpu_buffer_rsrc_t& rs, uint32_t o) {
         __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rs, o, 0, 0)), f32x4);
 }
 
-template <typename KT, int kRT>
-__global__ __launch_bounds__(64 * kWaves) void tree_attend(TreeArgs a) {
+// What a wave knows of its block and chunk.
+struct Block {
+  int past, nodes;      // keys that every row sees, drafted rows behind them
+  int key0, key1;       // the workgroup's keys
+  int row0;             // its first row within the tree
+  const uint32_t* anc;  // LDS: words of ancestors-or-self per row, and one of zeros
+  __amdgpu_buffer_rsrc_t k, v;  // the chunk's rows of the head's planes, zero at key1
+};
+// Which of the 32 keys from j0 on (j0 + 32 > past) row r of the block sees: keys of the cache, and
+// its ancestors' bits from j0 - past on. Bits past the drafted rows are zero.
+__device__ inline uint32_t sight_of(const Block& b, int r, int j0) {
+  constexpr int kWords = kTreeMaxNodes / 32;
+  const uint32_t* const w = b.anc + r * (kWords + 1);
+  const int n = j0 - b.past;
+  if (n < 0) return (w[0] << -n) | ((1u << -n) - 1u);
+  const int i = min(n >> 5, kWords);
+  return __builtin_amdgcn_alignbit(w[min(i + 1, kWords)], w[i], n & 31);
+}
+
+// Words of ancestors-or-self of `rows` rows from row0 on (zero past the tree's), to be read after a barrier; every
+// thread of the workgroup calls it. Trees of up to 64 nodes stay in one wave's registers, a node
+// a lane, and double their reach a round; larger ones walk in LDS.
+template <int kWaves>
+__device__ inline void find_ancestors(const int* parents, int nodes, int row0, int rows, int* par,
+                                      uint32_t* anc) {
+  constexpr int kWords = kTreeMaxNodes / 32;
+  const int tid = threadIdx.x;
+  auto parent = [&](int i) {
+    const int p = parents[i];
+    return static_cast<unsigned>(p) < static_cast<unsigned>(i) ? p : -1;
+  };
+  constexpr int kPitch = kWords + 1;
+  if (nodes <= 64) {
+    if (tid >= 64) return;
+    int up = tid < nodes ? parent(tid) : -1;  // the first ancestor that seen does not hold
+    uint64_t seen = uint64_t{1} << tid;
+    while (__any(up >= 0)) {
+      const int from = max(up, 0);
+      const uint32_t lo = __shfl(static_cast<uint32_t>(seen), from);
+      const uint32_t hi = __shfl(static_cast<uint32_t>(seen >> 32), from);
+      const int next = __shfl(up, from);
+      if (up >= 0) {
+        seen |= lo | static_cast<uint64_t>(hi) << 32;
+        up = next;
+      }
+    }
+    const int r = tid - row0;
+    if (r >= 0 && r < rows) {
+      const bool in = tid < nodes;
+      anc[r * kPitch] = in ? static_cast<uint32_t>(seen) : 0u;
+      anc[r * kPitch + 1] = in ? static_cast<uint32_t>(seen >> 32) : 0u;
+#pragma unroll
+      for (int w = 2; w < kPitch; ++w) anc[r * kPitch + w] = 0u;
+    }
+    return;
+  }
+  for (int i = tid; i < nodes; i += 64 * kWaves) par[i] = parent(i);
+  for (int i = tid; i < rows * kPitch; i += 64 * kWaves) anc[i] = 0u;
+  __syncthreads();
+  if (tid < rows && row0 + tid < nodes) {
+    // Ancestors come in falling order: a word is whole when the walk leaves it.
+    int n = row0 + tid, w = n >> 5;
+    uint32_t bits = 0;
+    for (; n >= 0; n = par[n]) {
+      if ((n >> 5) != w) {
+        anc[tid * kPitch + w] = bits;
+        bits = 0;
+        w = n >> 5;
+      }
+      bits |= 1u << (n & 31);
+    }
+    anc[tid * kPitch + w] = bits;
+  }
+}
+
+// A wave's running sums: of lane (c, g), rows 16 rt + c.
+template <int kRT>
+struct Sums {
+  f32x4 o[kRT][4];
+  float m[kRT], l[kRT];
+  __device__ inline void clear() {
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m[rt] = -INFINITY;
+      l[rt] = 0.f;
+    }
+  }
+};
+
+// A wave's pieces of kSpan keys (kSpan * wave, + kSpan * kWaves, ..) on the f32 matrix pipe, 16
+// at a time, f16 planes widened exactly: lane (c, g) holds key c's values d = 16 g + 0..15, so that lane (r, g) gets scores of keys
+// 4 g + 0..3 of row r, which are the B operand of O^T += V^T P^T as they stand. o[rt][dt][e] is
+// column 16 g + 4 e + dt. q: d = 16 g + 0..15 of row c, times scale * log2(e).
+// `sight` runs once the first loads are on their way (it may hold barriers).
+template <typename KT, int kRT, int kSpan, int kWaves, typename F>
+__device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4], int wave, int lane,
+                                  F sight, Sums<kRT>& st) {
+  constexpr uint32_t kRowBytes = 64 * sizeof(KT);
+  const int c = lane & 15, g = lane >> 4;
+  f32x4 kn[4], vn[4];
+  auto load = [&](int j0) __attribute__((always_inline)) {
+    const uint32_t ko = static_cast<uint32_t>(j0 - b.key0 + c) * kRowBytes + 16 * g * sizeof(KT);
+    const uint32_t vo = static_cast<uint32_t>(j0 - b.key0 + 4 * g) * kRowBytes + 4 * c * sizeof(KT);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kn[i] = load4<KT>(b.k, ko + 4 * i * sizeof(KT));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vn[i] = load4<KT>(b.v, vo + i * kRowBytes);
+  };
+  auto after = [&](int j) {
+    j += kStep;
+    return (j - b.key0) % kSpan ? j : j + kSpan * (kWaves - 1);
+  };
+  int j0 = b.key0 + kSpan * wave;
+  if (j0 < b.key1) load(j0);
+  st.clear();
+  sight();
+  for (int next; j0 < b.key1; j0 = next) {
+    next = after(j0);
+    f32x4 kx[4], vx[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kx[i] = kn[i];
+      vx[i] = vn[i];
+    }
+    if (next < b.key1) load(next);
+    // Drafted values that a row does not see have weight 0, and 0 times an infinity or
+    // NaN is NaN: such values leave the product and are added row by row.
+    const bool masked = j0 + kStep > b.past;
+    bool odd = false;
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= !__builtin_isfinite(vx[i][e]);
+      odd = __any(odd);
+    }
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      f32x4 s0 = {}, s1 = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e], qx[rt][i][e], s0, 0, 0, 0);
+          s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e + 1], qx[rt][i][e + 1], s1, 0, 0, 0);
+        }
+      f32x4 s = s0 + s1;
+      int seen = 0xF;  // bit i: the row sees key j0 + 4 g + i
+      if (masked) {
+        seen = static_cast<int>(sight_of(b, 16 * rt + c, j0) >> (4 * g));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(seen >> i & 1)) s[i] = -INFINITY;
+      }
+      const float mx = max_x16_x32(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+      const float m_new = fmaxf(st.m[rt], mx);
+      const float alpha = st.m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[rt] - m_new);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      st.m[rt] = m_new;
+      f32x4 p;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+      st.l[rt] = __builtin_fmaf(st.l[rt], alpha, (p[0] + p[1]) + (p[2] + p[3]));
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) st.o[rt][dt] *= alpha;
+      if (odd) {
+#pragma unroll 1
+        for (int key = 0; key < kStep; ++key) {
+          // Weight and sight of key j0 + key, and its row's values of this lane's columns.
+          const int i = key & 3;
+          const float mine = i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3];
+          const float pk = __shfl(mine, c + 16 * (key >> 2));
+          const bool vis = (__shfl(seen, c + 16 * (key >> 2)) >> i) & 1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x4 vk =
+                load4<KT>(b.v, static_cast<uint32_t>(j0 - b.key0 + key) * kRowBytes +
+                                   (16 * g + 4 * e) * static_cast<uint32_t>(sizeof(KT)));
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+              if (vis && !__builtin_isfinite(vk[dt])) st.o[rt][dt][e] += pk * vk[dt];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          st.o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+              odd && !__builtin_isfinite(vx[i][dt]) ? 0.f : vx[i][dt], p[i], st.o[rt][dt], 0, 0, 0);
+    }
+  }
+}
+
+__device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// Three parts' sums as one, smallest first.
+__device__ inline f32x4 join(const f32x4 (&x)[3]) {
+  f32x4 s = x[2];
+#pragma unroll
+  for (int p = 1; p >= 0; --p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(s[i], kPartUnit, x[p][i]);
+  return s;
+}
+
+// Keys key0 + 32 wave, + 128, .. of an f16 plane on the f16 matrix pipe. Query rows (times a
+// power of two that puts the largest element into [2^14, 2^15)) and weights (in units of 2^-15)
+// are split into three f16 parts, each in a unit 2^-11 of the one before and with sums of its
+// own: all 24 bits down to 2^-28 of the row's largest, smaller ones to 2^-60. K comes from
+// memory in operand layout, V passes through the wave's own swizzled LDS rows and is read
+// transposed; the packed weights are the B operand of O^T += V^T P^T as they stand.
+// o[rt][dt][e] is column 16 dt + 4 g + e. Returns whether a sum came out infinite or NaN: parts
+// of an infinity are not numbers, so such a wave starts again with f32 operands.
+template <int kRT, int kWaves, typename F>
+__device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int wave, int lane,
+                                  char* vw, F sight, Sums<kRT>& st) {
+  constexpr int kN = 32;  // keys per step
+  const int c = lane & 15, g = lane >> 4;
+  u32x4 kx[2][2], vx[4];
+  auto load = [&](int j0) __attribute__((always_inline)) {
+    const uint32_t ko = static_cast<uint32_t>(j0 - b.key0 + c) * 128u + 32u * g;
+    const uint32_t vo = static_cast<uint32_t>(j0 - b.key0) * 128u + 16u * lane;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+        kx[t][kk] = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(b.k, ko + 2048 * t + 16 * kk, 0, 0));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      vx[i] = __builtin_bit_cast(u32x4,
+                                 __builtin_amdgcn_raw_buffer_load_b128(b.v, vo + 1024 * i, 0, 0));
+  };
+  st.clear();
+  int j0 = b.key0 + kN * wave;
+  if (j0 < b.key1) load(j0);
+  sight();
+  u32x4 qf[kRT][3][2];  // d = 16 g + 8 kk + 0..7
+  float down[kRT];
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) amax = fmaxf(amax, __builtin_fabsf(qx[rt][i][e]));
+    amax = max_x16_x32(amax);
+    const int e_max = static_cast<int>((__builtin_bit_cast(uint32_t, amax) >> 23) & 0xFF);
+    const int sh = e_max == 0 ? 0 : clamp_exp(141 - e_max);
+    const float up = pow2(sh);
+    down[rt] = pow2(clamp_exp(-sh));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t w[3];
+      split2(qx[rt][i >> 1][2 * (i & 1)], qx[rt][i >> 1][2 * (i & 1) + 1], up, w);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) qf[rt][p][i >> 2][i & 3] = w[p];
+    }
+  }
+  for (; j0 < b.key1; j0 += kN * kWaves) {
+    u32x4 pf[kRT][3];
+    f32x4 s[kRT][2];
+    float alpha[kRT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 sp[3] = {};
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) sp[p] = mfma16(kx[t][kk], qf[rt][p][kk], sp[p]);
+        s[rt][t] = join(sp);
+      }
+    wave_sync();  // the last step's transposed reads are done
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 8 * i + (lane >> 3);
+      *reinterpret_cast<u32x4*>(vw + row * 128 + (((lane & 7) ^ swz(row)) * 16)) = vx[i];
+    }
+    wave_sync();
+    if (j0 + kN * kWaves < b.key1) load(j0 + kN * kWaves);
+    const bool masked = j0 + kN > b.past;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      // Register i of tile t holds key 16 t + 4 g + i.
+      if (masked) {
+        const uint32_t seen = sight_of(b, 16 * rt + c, j0) >> (4 * g);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(seen >> (16 * t + i) & 1)) s[rt][t][i] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][t][i]);
+      // Maxima are kept in the units of the parts' sums: times down, a power of two, exact.
+      const float m_new = fmaxf(st.m[rt], max_x16_x32(mx));
+      alpha[rt] = st.m[rt] == -INFINITY
+                      ? 0.f
+                      : __builtin_amdgcn_exp2f((st.m[rt] - m_new) * down[rt]);
+      st.m[rt] = m_new;
+      const float md = m_new == -INFINITY ? 0.f : m_new * down[rt];
+      float ls = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], down[rt], -md));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i + 1], down[rt], -md));
+          ls += p0 + p1;
+          uint32_t w[3];
+          split2(p0, p1, kWeightUp, w);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) pf[rt][p][2 * t + (i >> 1)] = w[p];
+        }
+      st.l[rt] = __builtin_fmaf(st.l[rt], alpha[rt], ls);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      u32x2 t[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 16 * e + 4 * g + (c >> 2);
+        t[e] = read_tr(vw + row * 128 + (((2 * dt + ((c & 3) >> 1)) ^ swz(row)) * 16) + 8 * (c & 1));
+      }
+      const u32x4 va = {t[0].x, t[0].y, t[1].x, t[1].y};
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt) {
+        // The step's sums join at once: kept apart over the steps they took 32 registers more a
+        // tile, and as many multiplications by alpha.
+        f32x4 x[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) x[p] = mfma16(va, pf[rt][p], f32x4{0.f, 0.f, 0.f, 0.f});
+        const f32x4 y = join(x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[rt][dt][e] = __builtin_fmaf(st.o[rt][dt][e], alpha[rt], y[e]);
+      }
+    }
+  }
+  bool odd = false;
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt) {
+    odd |= !__builtin_isfinite(st.l[rt]);
+    st.m[rt] *= down[rt];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      st.o[rt][dt] *= 1.f / kWeightUp;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= !__builtin_isfinite(st.o[rt][dt][e]);
+    }
+  }
+  return __any(odd);
+}
+
+template <typename KT, int kRT, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
   constexpr int kRows = 16 * kRT;
+  constexpr bool kHalf = sizeof(KT) == 2;
+  __shared__ __attribute__((aligned(128))) char vs[kHalf ? kWaves : 1][32 * 128];
   __shared__ float mo[kWaves][kRows * kPitch];  // a wave's O rows
   __shared__ float ml[kWaves][2][kRows];        // and their max and sum
   __shared__ int par[kTreeMaxNodes];
-  __shared__ uint32_t anc[kRows][kTreeMaxNodes / 32];  // ancestors-or-self of the block's rows
+  __shared__ uint32_t anc[kRows][kTreeMaxNodes / 32 + 1];  // ancestors-or-self of the block's rows
   __shared__ int last_flag;
 
   // The workgroups of one head's chunk, which read the same rows, share an XCD's L2.
@@ -78,10 +457,11 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attend(TreeArgs a) {
   constexpr uint32_t kRowBytes = 64 * sizeof(KT);
   const int64_t plane = a.off[t] + h * a.kv_hs + static_cast<int64_t>(key0) * 64;
   const uint32_t range = static_cast<uint32_t>(key1 - key0) * kRowBytes;
-  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<KT*>(static_cast<const KT*>(a.k) + plane), 0, range, kRawBuffer);
-  const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<KT*>(static_cast<const KT*>(a.v) + plane), 0, range, kRawBuffer);
+  const Block b = {past, nodes, key0, key1, row0, &anc[0][0],
+                   __builtin_amdgcn_make_buffer_rsrc(
+                       const_cast<KT*>(static_cast<const KT*>(a.k) + plane), 0, range, kRawBuffer),
+                   __builtin_amdgcn_make_buffer_rsrc(
+                       const_cast<KT*>(static_cast<const KT*>(a.v) + plane), 0, range, kRawBuffer)};
 
   // Query rows: d = 16 g + 0..15 of row c of each tile, times scale * log2(e).
   f32x4 qx[kRT][4];
@@ -98,212 +478,122 @@ __global__ __launch_bounds__(64 * kWaves) void tree_attend(TreeArgs a) {
     }
   }
 
-  const bool tail = key1 > past;  // the chunk holds drafted rows
-  if (tail) {
-    for (int i = tid; i < nodes; i += 64 * kWaves) {
-      const int p = a.parents[q_row + i];
-      par[i] = static_cast<unsigned>(p) < static_cast<unsigned>(i) ? p : -1;
+  Sums<kRT> st;
+  bool f32_order = true;  // which column o[rt][dt][e] is
+  auto sight = [&]() __attribute__((always_inline)) {
+    if (key1 > past) {  // the chunk holds drafted rows
+      find_ancestors<kWaves>(a.parents + q_row, nodes, row0, kRows, par, &anc[0][0]);
+      __syncthreads();
     }
-    for (int i = tid; i < kRows * (kTreeMaxNodes / 32); i += 64 * kWaves) anc[0][i] = 0u;
-    __syncthreads();
-    if (tid < kRows && row0 + tid < nodes) {
-      // Ancestors come in falling order: a word is whole when the walk leaves it.
-      int n = row0 + tid, w = n >> 5;
-      uint32_t bits = 0;
-      for (; n >= 0; n = par[n]) {
-        if ((n >> 5) != w) {
-          anc[tid][w] = bits;
-          bits = 0;
-          w = n >> 5;
-        }
-        bits |= 1u << (n & 31);
-      }
-      anc[tid][w] = bits;
-    }
-    __syncthreads();
-  }
-
-  f32x4 o[kRT][4];
-  float m[kRT], l[kRT];
-#pragma unroll
-  for (int rt = 0; rt < kRT; ++rt) {
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    m[rt] = -INFINITY;
-    l[rt] = 0.f;
-  }
-  for (int j0 = key0 + kStep * wave; j0 < key1; j0 += kStep * kWaves) {
-    f32x4 kx[4], vx[4];
-    const uint32_t ko = static_cast<uint32_t>(j0 - key0 + c) * kRowBytes + 16 * g * sizeof(KT);
-    const uint32_t vo = static_cast<uint32_t>(j0 - key0 + 4 * g) * kRowBytes + 4 * c * sizeof(KT);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) kx[i] = load4<KT>(krs, ko + 4 * i * sizeof(KT));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vx[i] = load4<KT>(vrs, vo + i * kRowBytes);
-    // Drafted values that a row does not see have weight 0, and 0 times an infinity or
-    // NaN is NaN: such values leave the product and are added row by row.
-    const bool masked = j0 + kStep > past;
-    bool odd = false;
-    if (masked) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= !__builtin_isfinite(vx[i][e]);
-      odd = __any(odd);
-    }
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      f32x4 s0 = {}, s1 = {};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e], qx[rt][i][e], s0, 0, 0, 0);
-          s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e + 1], qx[rt][i][e + 1], s1, 0, 0, 0);
-        }
-      f32x4 s = s0 + s1;
-      uint32_t seen = 0xF;  // bit i: the row sees key j0 + 4 g + i
-      if (masked) {
-        seen = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = j0 + 4 * g + i - past;
-          const bool vis =
-              n < 0 || (n < nodes && ((anc[16 * rt + c][(n & (kTreeMaxNodes - 1)) >> 5] >> (n & 31)) & 1));
-          seen |= vis ? 1u << i : 0u;
-          if (!vis) s[i] = -INFINITY;
-        }
-      }
-      const float mx = max_x16_x32(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-      const float m_new = fmaxf(m[rt], mx);
-      const float alpha = m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[rt] - m_new);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      m[rt] = m_new;
-      f32x4 p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
-      l[rt] = __builtin_fmaf(l[rt], alpha, (p[0] + p[1]) + (p[2] + p[3]));
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) o[rt][dt] *= alpha;
-      if (!odd) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int dt = 0; dt < 4; ++dt)
-            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[i][dt], p[i], o[rt][dt], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int dt = 0; dt < 4; ++dt)
-            o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                __builtin_isfinite(vx[i][dt]) ? vx[i][dt] : 0.f, p[i], o[rt][dt], 0, 0, 0);
-          for (int kg = 0; kg < 4; ++kg) {
-            // Weight and sight of key j0 + 4 kg + i, and its row's values of this lane's
-            // columns (lane group g holds d = 16 g + 4 e + dt at o[dt][e]).
-            const float pk = __shfl(p[i], c + 16 * kg);
-            const bool vis = (__shfl(static_cast<int>(seen), c + 16 * kg) >> i) & 1;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const f32x4 vk = load4<KT>(
-                  vrs, static_cast<uint32_t>(j0 - key0 + 4 * kg + i) * kRowBytes +
-                           (16 * g + 4 * e) * static_cast<uint32_t>(sizeof(KT)));
-#pragma unroll
-              for (int dt = 0; dt < 4; ++dt)
-                if (vis && !__builtin_isfinite(vk[dt])) o[rt][dt][e] += pk * vk[dt];
-            }
-          }
-        }
-      }
-    }
+  };
+  if constexpr (kHalf) {
+    f32_order = attend_f16<kRT, kWaves>(b, qx, wave, lane, vs[wave], sight, st);
+    if (f32_order) attend_f32<KT, kRT, 32, kWaves>(b, qx, wave, lane, [] {}, st);
+  } else {
+    attend_f32<KT, kRT, kStep, kWaves>(b, qx, wave, lane, sight, st);
   }
 
   // The waves' rows meet in LDS.
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt) {
-    l[rt] = sum_x16_x32(l[rt]);
+    st.l[rt] = sum_x16_x32(st.l[rt]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = 16 * g + 4 * e;
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt) mo[wave][(16 * rt + c) * kPitch + d + dt] = o[rt][dt][e];
-    }
+      for (int dt = 0; dt < 4; ++dt)
+        mo[wave][(16 * rt + c) * kPitch + (f32_order ? 16 * g + 4 * e + dt : 16 * dt + 4 * g + e)] =
+            st.o[rt][dt][e];
     if (g == 0) {
-      ml[wave][0][16 * rt + c] = m[rt];
-      ml[wave][1][16 * rt + c] = l[rt];
+      ml[wave][0][16 * rt + c] = st.m[rt];
+      ml[wave][1][16 * rt + c] = st.l[rt];
     }
   }
   __syncthreads();
-  const int rows = min(kRows, nodes - row0);
-  float* const part =
-      a.part + (static_cast<int64_t>(a.wg0[t] + h * n_split * n_blk + blk) * kRows) * kTreePart;
-  const int64_t part_step = static_cast<int64_t>(n_blk) * kRows * kTreePart;  // to the next chunk
-  for (int e = tid; e < rows * 64; e += 64 * kWaves) {
-    const int r = e >> 6, d = e & 63;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
+  // Thread (r, kCols columns from d0 on) adds the waves up, and the last of a block's chunks
+  // to count in adds the chunks, in their order (exp2 domain).
+  constexpr int kCols = kRows / kWaves;
+  const int r = tid / (64 / kCols), d0 = kCols * (tid % (64 / kCols));
+  const bool mine = row0 + r < nodes;
+  auto store = [&](float L, const float (&acc)[kCols]) {
+    float* const op = a.o + (q_row + row0 + r) * a.o_rs + h * 64 + d0;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w][0][r]);
+    for (int e = 0; e < kCols; e += 2)
+      *reinterpret_cast<f32x2u*>(op + e) = f32x2{acc[e] * inv, acc[e + 1] * inv};
+  };
+  float M = -INFINITY, L = 0.f, acc[kCols] = {};
+  {
+    float mw[kWaves], lw[kWaves];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float mw = ml[w][0][r];
-      const float x = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-      L = __builtin_fmaf(ml[w][1][r], x, L);
-      acc = __builtin_fmaf(mo[w][r * kPitch + d], x, acc);
+      mw[w] = ml[w][0][r];
+      lw[w] = ml[w][1][r];
+      M = fmaxf(M, mw[w]);
     }
-    if (n_split == 1) {
-      a.o[(q_row + row0 + r) * a.o_rs + h * 64 + d] = L == 0.f ? 0.f : acc / L;
-    } else {
-      float* const p = part + split * part_step + r * kTreePart;
-      st_agent(p + 2 + d, acc);
-      if (d == 0) {
-        st_agent(p, M);
-        st_agent(p + 1, L);
-      }
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float x = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M);
+      L = __builtin_fmaf(lw[w], x, L);
+#pragma unroll
+      for (int e = 0; e < kCols; ++e)
+        acc[e] = __builtin_fmaf(mo[w][r * kPitch + d0 + e], x, acc[e]);
     }
   }
-  if (n_split == 1) return;
+  if (n_split == 1) {
+    if (mine) store(L, acc);
+    return;
+  }
+  const int at = a.wg0[t] + h * n_split * n_blk + blk;  // the block's first chunk
+  float* const part =
+      a.part + (static_cast<int64_t>(at) * kRows + r) * kTreePart;
+  const int64_t part_step = static_cast<int64_t>(n_blk) * kRows * kTreePart;  // to the next chunk
+  if (mine) {
+    float* const p = part + split * part_step;
+    if (d0 == 0) st_agent2(p, M, L);
+#pragma unroll
+    for (int e = 0; e < kCols; e += 2) st_agent2(p + 2 + d0 + e, acc[e], acc[e + 1]);
+  }
   // Every wave's stores are performed before the chunk counts in.
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  unsigned* const counter =
-      a.counters + static_cast<int64_t>(a.wg0[t] + h * n_split * n_blk + blk) * kCounterStride;
+  unsigned* const counter = a.counters + static_cast<int64_t>(at) * kCounterStride;
   if (tid == 0)
     last_flag = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                 static_cast<unsigned>(n_split - 1);
   __syncthreads();
   if (!last_flag) return;
-  for (int e = tid; e < rows * 64; e += 64 * kWaves) {
-    const int r = e >> 6, d = e & 63;
-    float M = -INFINITY, L = 0.f, acc = 0.f;
-    for (int s0 = 0; s0 < n_split; s0 += kMergeLoads) {
-      float ms[kMergeLoads], ls[kMergeLoads], as[kMergeLoads];
+  M = -INFINITY;
+  L = 0.f;
 #pragma unroll
-      for (int j = 0; j < kMergeLoads; ++j) {
-        ms[j] = -INFINITY;
-        ls[j] = as[j] = 0.f;
-        if (s0 + j < n_split) {
-          const float* p = part + (s0 + j) * part_step + r * kTreePart;
-          ms[j] = ld_agent(p);
-          ls[j] = ld_agent(p + 1);
-          as[j] = ld_agent(p + 2 + d);
-        }
-      }
-      float Mb = M;
+  for (int e = 0; e < kCols; ++e) acc[e] = 0.f;
+  for (int s0 = 0; mine && s0 < n_split; s0 += kMergeLoads) {
+    float ms[kMergeLoads], ls[kMergeLoads], as[kMergeLoads][kCols];
 #pragma unroll
-      for (int j = 0; j < kMergeLoads; ++j) Mb = fmaxf(Mb, ms[j]);
-      const float x = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mb);
-      L *= x;
-      acc *= x;
+    for (int j = 0; j < kMergeLoads; ++j) {
+      // Chunks past the last one: that one again, without weight.
+      const float* p = part + min(s0 + j, n_split - 1) * part_step;
+      ld_agent2(p, ms[j], ls[j]);
 #pragma unroll
-      for (int j = 0; j < kMergeLoads; ++j) {
-        const float w = ms[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[j] - Mb);
-        L = __builtin_fmaf(ls[j], w, L);
-        acc = __builtin_fmaf(as[j], w, acc);
-      }
-      M = Mb;
+      for (int e = 0; e < kCols; e += 2) ld_agent2(p + 2 + d0 + e, as[j][e], as[j][e + 1]);
     }
-    a.o[(q_row + row0 + r) * a.o_rs + h * 64 + d] = L == 0.f ? 0.f : acc / L;
+    float Mb = M;
+#pragma unroll
+    for (int j = 0; j < kMergeLoads; ++j) Mb = fmaxf(Mb, ms[j]);
+    const float x = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mb);
+    L *= x;
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) acc[e] *= x;
+#pragma unroll
+    for (int j = 0; j < kMergeLoads; ++j) {
+      if (s0 + j >= n_split) break;
+      const float w = ms[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[j] - Mb);
+      L = __builtin_fmaf(ls[j], w, L);
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(as[j][e], w, acc[e]);
+    }
+    M = Mb;
   }
+  if (mine) store(L, acc);
   if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -338,9 +628,12 @@ int64_t tree_plan(TreeArgs& a, bool split) {
     }
     return n;
   };
-  constexpr int kLeast = 2 * kStep * kWaves;  // keys worth a workgroup
+  int kLeast = 256;  // keys worth a workgroup
+  if (const char* e = getenv("TREE_LEAST")) kLeast = atoi(e);
+  int kWgs = kTreeMaxWgs * 3 / 4;
+  if (const char* e = getenv("TREE_WGS")) kWgs = atoi(e);
   if (split && blocks < kTreeMaxWgs / 2 && longest > kLeast) {
-    int64_t chunk = std::max<int64_t>(kLeast, (work + kTreeMaxWgs * 3 / 4 - 1) / (kTreeMaxWgs * 3 / 4));
+    int64_t chunk = std::max<int64_t>(kLeast, (work + kWgs - 1) / kWgs);
     for (chunk = (chunk + kLeast - 1) / kLeast * kLeast; chunk < longest; chunk += kLeast) {
       const int64_t n = lay(static_cast<int>(chunk));
       if (n <= kTreeMaxWgs) return n;
@@ -352,15 +645,21 @@ int64_t tree_plan(TreeArgs& a, bool split) {
 hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStream_t s) {
   if (wgs <= 0) return hipSuccess;
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-  const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kWaves);
+  int waves = 4;
+  if (const char* e = getenv("TREE_WAVES")) waves = atoi(e);
+  const dim3 grid(static_cast<unsigned>(wgs)), block(64 * waves);
   const bool few = block_rows(a) == 16;
-#define WRS_TREE(KT, RT) hipLaunchKernelGGL((tree_attend<KT, RT>), grid, block, 0, s, a)
+#define WRS_TREE(KT, RT)                                                    \
+  if (waves == 8)                                                           \
+    hipLaunchKernelGGL((tree_attend<KT, RT, 8>), grid, block, 0, s, a);     \
+  else                                                                      \
+    hipLaunchKernelGGL((tree_attend<KT, RT, 4>), grid, block, 0, s, a)
   switch (dt) {
     case kF16:
-      if (few) WRS_TREE(_Float16, 1); else WRS_TREE(_Float16, 2);
+      if (few) { WRS_TREE(_Float16, 1); } else { WRS_TREE(_Float16, 2); }
       break;
     case kF32:
-      if (few) WRS_TREE(float, 1); else WRS_TREE(float, 2);
+      if (few) { WRS_TREE(float, 1); } else { WRS_TREE(float, 2); }
       break;
     default: return hipErrorInvalidValue;
   }

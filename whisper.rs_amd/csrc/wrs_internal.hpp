@@ -53,6 +53,14 @@ __device__ inline float ld_agent(const float* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// Orders a wave's own LDS writes and reads: its LDS operations complete in order, only the
+// compiler must keep it.
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // x op x[lane ^ 32] and x op x[lane ^ 16] with the gfx950 lane-swap VALU
 // instructions (no LDS round trip). Issued as inline asm on two distinct
 // registers: the swap writes both operands.
