@@ -16,7 +16,6 @@
 #include "split16.hpp"
 
 #include <algorithm>
-#include <cstdlib>
 
 namespace wrs {
 namespace {
@@ -31,6 +30,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kWaves = 4;
 constexpr int kStep = 16;       // keys per wave step of the f32 path
 constexpr int kPitch = 68;      // LDS pitch (floats) of a merge row
 constexpr int kCounterStride = 32;  // 128 bytes between merge counters
@@ -68,70 +68,97 @@ struct Block {
   const uint32_t* anc;  // LDS: words of ancestors-or-self per row, and one of zeros
   __amdgpu_buffer_rsrc_t k, v;  // the chunk's rows of the head's planes, zero at key1
 };
-// Which of the 32 keys from j0 on (j0 + 32 > past) row r of the block sees: keys of the cache, and
-// its ancestors' bits from j0 - past on. Bits past the drafted rows are zero.
-__device__ inline uint32_t sight_of(const Block& b, int r, int j0) {
-  constexpr int kWords = kTreeMaxNodes / 32;
-  const uint32_t* const w = b.anc + r * (kWords + 1);
+// Which drafted rows the rows of a block see: ancestors-or-self of row c of each tile. Trees of
+// up to 64 nodes are worked out by every wave for itself, in registers; larger ones in LDS.
+template <int kRT>
+struct Sight {
+  uint64_t seen[kRT];
+  bool small;
+};
+constexpr int kWords = kTreeMaxNodes / 32;
+constexpr int kAncPitch = kWords + 1;  // a row's words, and one of zeros
+
+// Which of the 32 keys from j0 on (j0 + 32 > past) row r = 16 rt + c of the block sees: keys of
+// the cache, and its ancestors' bits from j0 - past on. Bits past the drafted rows are zero.
+template <int kRT>
+__device__ inline uint32_t sight_of(const Block& b, const Sight<kRT>& s, int rt, int c, int j0) {
   const int n = j0 - b.past;
+  if (s.small) {
+    if (n < 0) return (static_cast<uint32_t>(s.seen[rt]) << -n) | ((1u << -n) - 1u);
+    return n < 64 ? static_cast<uint32_t>(s.seen[rt] >> n) : 0u;
+  }
+  const uint32_t* const w = b.anc + (16 * rt + c) * kAncPitch;
   if (n < 0) return (w[0] << -n) | ((1u << -n) - 1u);
   const int i = min(n >> 5, kWords);
   return __builtin_amdgcn_alignbit(w[min(i + 1, kWords)], w[i], n & 31);
 }
 
-// Words of ancestors-or-self of `rows` rows from row0 on (zero past the tree's), to be read after a barrier; every
-// thread of the workgroup calls it. Trees of up to 64 nodes stay in one wave's registers, a node
-// a lane, and double their reach a round; larger ones walk in LDS.
-template <int kWaves>
-__device__ inline void find_ancestors(const int* parents, int nodes, int row0, int rows, int* par,
-                                      uint32_t* anc) {
-  constexpr int kWords = kTreeMaxNodes / 32;
-  const int tid = threadIdx.x;
-  auto parent = [&](int i) {
-    const int p = parents[i];
-    return static_cast<unsigned>(p) < static_cast<unsigned>(i) ? p : -1;
-  };
-  constexpr int kPitch = kWords + 1;
-  if (nodes <= 64) {
-    if (tid >= 64) return;
-    int up = tid < nodes ? parent(tid) : -1;  // the first ancestor that seen does not hold
-    uint64_t seen = uint64_t{1} << tid;
-    while (__any(up >= 0)) {
-      const int from = max(up, 0);
-      const uint32_t lo = __shfl(static_cast<uint32_t>(seen), from);
-      const uint32_t hi = __shfl(static_cast<uint32_t>(seen >> 32), from);
-      const int next = __shfl(up, from);
-      if (up >= 0) {
-        seen |= lo | static_cast<uint64_t>(hi) << 32;
-        up = next;
-      }
+// A row's parent, or -1: the last cached token. Whatever the array holds, parents lie below.
+__device__ inline int valid_parent(int p, int i) {
+  return static_cast<unsigned>(p) < static_cast<unsigned>(i) ? p : -1;
+}
+// Up to 64 nodes, one a lane: their ancestors' reach doubles every round. p: the node's parent.
+template <int kRT>
+__device__ inline void find_sight(int p, int nodes, int row0, int lane, Sight<kRT>& s) {
+  int up = lane < nodes ? valid_parent(p, lane) : -1;  // the first ancestor that seen lacks
+  uint64_t seen = uint64_t{1} << lane;
+  while (__any(up >= 0)) {
+    const int from = max(up, 0);
+    const uint32_t lo = __shfl(static_cast<uint32_t>(seen), from);
+    const uint32_t hi = __shfl(static_cast<uint32_t>(seen >> 32), from);
+    const int next = __shfl(up, from);
+    if (up >= 0) {
+      seen |= lo | static_cast<uint64_t>(hi) << 32;
+      up = next;
     }
-    const int r = tid - row0;
-    if (r >= 0 && r < rows) {
-      const bool in = tid < nodes;
-      anc[r * kPitch] = in ? static_cast<uint32_t>(seen) : 0u;
-      anc[r * kPitch + 1] = in ? static_cast<uint32_t>(seen >> 32) : 0u;
-#pragma unroll
-      for (int w = 2; w < kPitch; ++w) anc[r * kPitch + w] = 0u;
-    }
-    return;
   }
-  for (int i = tid; i < nodes; i += 64 * kWaves) par[i] = parent(i);
-  for (int i = tid; i < rows * kPitch; i += 64 * kWaves) anc[i] = 0u;
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt) {
+    const int r = row0 + 16 * rt + (lane & 15);
+    const uint32_t lo = __shfl(static_cast<uint32_t>(seen), r & 63);
+    const uint32_t hi = __shfl(static_cast<uint32_t>(seen >> 32), r & 63);
+    s.seen[rt] = r < nodes ? lo | static_cast<uint64_t>(hi) << 32 : 0;
+  }
+}
+// More nodes: words of `rows` rows from row0 on in LDS (zero past the tree's), to be read after a
+// barrier; every thread of the workgroup calls it. Every node's next four ancestors lie
+// together, so that a chain of 256 is walked in 64 reads (one by one: 13 us of 31).
+__device__ inline void find_ancestors(const int* parents, int nodes, int row0, int rows,
+                                      uint64_t* up, uint32_t* anc) {
+  constexpr uint32_t kNone = 0xFFFFu;
+  static_assert(kTreeMaxNodes <= 64 * kWaves, "a node a thread");
+  const int tid = threadIdx.x;
+  uint32_t* const pair = reinterpret_cast<uint32_t*>(up) + 2 * kTreeMaxNodes;
+  const uint32_t p1 = tid < nodes ? valid_parent(parents[tid], tid) & kNone : kNone;
+  if (tid < nodes) pair[tid] = p1;
+  for (int i = tid; i < rows * kAncPitch; i += 64 * kWaves) anc[i] = 0u;
+  __syncthreads();
+  const uint32_t two = p1 | (p1 == kNone ? kNone : pair[p1]) << 16;
+  __syncthreads();
+  if (tid < nodes) pair[tid] = two;
+  __syncthreads();
+  const uint32_t p2 = two >> 16;
+  if (tid < nodes)
+    up[tid] = two | static_cast<uint64_t>(p2 == kNone ? ~0u : pair[p2]) << 32;
   __syncthreads();
   if (tid < rows && row0 + tid < nodes) {
     // Ancestors come in falling order: a word is whole when the walk leaves it.
-    int n = row0 + tid, w = n >> 5;
-    uint32_t bits = 0;
-    for (; n >= 0; n = par[n]) {
-      if ((n >> 5) != w) {
-        anc[tid * kPitch + w] = bits;
-        bits = 0;
-        w = n >> 5;
+    uint32_t n = row0 + tid, w = n >> 5, bits = 1u << (n & 31);
+    while (n != kNone) {
+      const uint64_t next = up[n];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        n = static_cast<uint32_t>(next >> (16 * i)) & kNone;
+        if (n == kNone) break;
+        if ((n >> 5) != w) {
+          anc[tid * kAncPitch + w] = bits;
+          bits = 0;
+          w = n >> 5;
+        }
+        bits |= 1u << (n & 31);
       }
-      bits |= 1u << (n & 31);
     }
-    anc[tid * kPitch + w] = bits;
+    anc[tid * kAncPitch + w] = bits;
   }
 }
 
@@ -156,9 +183,9 @@ struct Sums {
 // 4 g + 0..3 of row r, which are the B operand of O^T += V^T P^T as they stand. o[rt][dt][e] is
 // column 16 g + 4 e + dt. q: d = 16 g + 0..15 of row c, times scale * log2(e).
 // `sight` runs once the first loads are on their way (it may hold barriers).
-template <typename KT, int kRT, int kSpan, int kWaves, typename F>
+template <typename KT, int kRT, int kSpan, typename F>
 __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4], int wave, int lane,
-                                  F sight, Sums<kRT>& st) {
+                                  F sight, const Sight<kRT>& seen_by, Sums<kRT>& st) {
   constexpr uint32_t kRowBytes = 64 * sizeof(KT);
   const int c = lane & 15, g = lane >> 4;
   f32x4 kn[4], vn[4];
@@ -211,7 +238,7 @@ __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4], int
       f32x4 s = s0 + s1;
       int seen = 0xF;  // bit i: the row sees key j0 + 4 g + i
       if (masked) {
-        seen = static_cast<int>(sight_of(b, 16 * rt + c, j0) >> (4 * g));
+        seen = static_cast<int>(sight_of(b, seen_by, rt, c, j0) >> (4 * g));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (!(seen >> i & 1)) s[i] = -INFINITY;
@@ -278,9 +305,10 @@ __device__ inline f32x4 join(const f32x4 (&x)[3]) {
 // transposed; the packed weights are the B operand of O^T += V^T P^T as they stand.
 // o[rt][dt][e] is column 16 dt + 4 g + e. Returns whether a sum came out infinite or NaN: parts
 // of an infinity are not numbers, so such a wave starts again with f32 operands.
-template <int kRT, int kWaves, typename F>
+template <int kRT, typename F>
 __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int wave, int lane,
-                                  char* vw, F sight, Sums<kRT>& st) {
+                                  char* vw, F sight, const Sight<kRT>& seen_by,
+                                  Sums<kRT>& st) {
   constexpr int kN = 32;  // keys per step
   const int c = lane & 15, g = lane >> 4;
   u32x4 kx[2][2], vx[4];
@@ -301,7 +329,6 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
   st.clear();
   int j0 = b.key0 + kN * wave;
   if (j0 < b.key1) load(j0);
-  sight();
   u32x4 qf[kRT][3][2];  // d = 16 g + 8 kk + 0..7
   float down[kRT];
 #pragma unroll
@@ -324,6 +351,7 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
       for (int p = 0; p < 3; ++p) qf[rt][p][i >> 2][i & 3] = w[p];
     }
   }
+  sight();
   for (; j0 < b.key1; j0 += kN * kWaves) {
     u32x4 pf[kRT][3];
     f32x4 s[kRT][2];
@@ -352,7 +380,7 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
     for (int rt = 0; rt < kRT; ++rt) {
       // Register i of tile t holds key 16 t + 4 g + i.
       if (masked) {
-        const uint32_t seen = sight_of(b, 16 * rt + c, j0) >> (4 * g);
+        const uint32_t seen = sight_of(b, seen_by, rt, c, j0) >> (4 * g);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -423,28 +451,42 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
   return __any(odd);
 }
 
-template <typename KT, int kRT, int kWaves>
+// x / n, with the remainder; inv: 2^32 / n rounded up (for n 1: 2^32 - 1).
+__device__ inline int divide(int x, int n, uint32_t inv, int& rest) {
+  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), inv));
+  rest = x - q * n;
+  if (rest < 0) {
+    --q;
+    rest += n;
+  }
+  if (rest >= n) {
+    ++q;
+    rest -= n;
+  }
+  return q;
+}
+
+template <typename KT, int kRT>
 __global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
   constexpr int kRows = 16 * kRT;
   constexpr bool kHalf = sizeof(KT) == 2;
   __shared__ __attribute__((aligned(128))) char vs[kHalf ? kWaves : 1][32 * 128];
-  __shared__ float mo[kWaves][kRows * kPitch];  // a wave's O rows
+  __shared__ __attribute__((aligned(16))) float mo[kWaves][kRows * kPitch];  // a wave's O rows
   __shared__ float ml[kWaves][2][kRows];        // and their max and sum
-  __shared__ int par[kTreeMaxNodes];
-  __shared__ uint32_t anc[kRows][kTreeMaxNodes / 32 + 1];  // ancestors-or-self of the block's rows
+  __shared__ uint64_t up[kTreeMaxNodes + kTreeMaxNodes / 2];  // of a large tree: ancestors, pairs
+  __shared__ uint32_t anc[kRows][kAncPitch];  // ancestors-or-self of the block's rows
   __shared__ int last_flag;
 
-  // The workgroups of one head's chunk, which read the same rows, share an XCD's L2.
+  // The workgroups of one head's chunk, which read the same rows, share an XCD's L2 (a tree's row
+  // of the grid is a multiple of the XCDs).
+  const int t = blockIdx.y;
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
-  int t = 0;
-  for (int step = kTreeMaxTrees / 2; step; step >>= 1)
-    if (t + step < a.n_trees && a.wg0[t + step] <= lid) t += step;
+  if (lid >= a.n_wgs[t]) return;
   const int past = a.past[t], nodes = a.nodes[t], total = past + nodes;
-  const int n_blk = (nodes + kRows - 1) / kRows;
-  const int n_split = (total + a.chunk - 1) / a.chunk;
-  const int local = lid - a.wg0[t];
-  const int blk = local % n_blk, hs = local / n_blk;
-  const int split = hs % n_split, h = hs / n_split;
+  const int n_blk = a.n_blk[t], n_split = a.n_split[t];
+  int blk, split;
+  const int hs = divide(lid, n_blk, a.blk_inv[t], blk);
+  const int h = divide(hs, n_split, a.split_inv[t], split);
   const int row0 = blk * kRows;
   const int key0 = split * a.chunk, key1 = min(key0 + a.chunk, total);
 
@@ -463,6 +505,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
                    __builtin_amdgcn_make_buffer_rsrc(
                        const_cast<KT*>(static_cast<const KT*>(a.v) + plane), 0, range, kRawBuffer)};
 
+  const int parent = key1 > past && nodes <= 64 && lane < nodes ? a.parents[q_row + lane] : -1;
   // Query rows: d = 16 g + 0..15 of row c of each tile, times scale * log2(e).
   f32x4 qx[kRT][4];
 #pragma unroll
@@ -478,31 +521,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
     }
   }
 
-  Sums<kRT> st;
-  bool f32_order = true;  // which column o[rt][dt][e] is
+  Sight<kRT> seen_by;
+  seen_by.small = nodes <= 64;
+  const bool drafted = key1 > past;  // the chunk holds drafted rows
   auto sight = [&]() __attribute__((always_inline)) {
-    if (key1 > past) {  // the chunk holds drafted rows
-      find_ancestors<kWaves>(a.parents + q_row, nodes, row0, kRows, par, &anc[0][0]);
+    if (!drafted) return;
+    if (seen_by.small) {
+      find_sight<kRT>(parent, nodes, row0, lane, seen_by);
+    } else {
+      find_ancestors(a.parents + q_row, nodes, row0, kRows, up, &anc[0][0]);
       __syncthreads();
     }
   };
+  Sums<kRT> st;
+  bool f32_order = true;  // which column o[rt][dt][e] is
   if constexpr (kHalf) {
-    f32_order = attend_f16<kRT, kWaves>(b, qx, wave, lane, vs[wave], sight, st);
-    if (f32_order) attend_f32<KT, kRT, 32, kWaves>(b, qx, wave, lane, [] {}, st);
+    f32_order = attend_f16<kRT>(b, qx, wave, lane, vs[wave], sight, seen_by, st);
+    if (f32_order) attend_f32<KT, kRT, 32>(b, qx, wave, lane, [] {}, seen_by, st);
   } else {
-    attend_f32<KT, kRT, kStep, kWaves>(b, qx, wave, lane, sight, st);
+    attend_f32<KT, kRT, kStep>(b, qx, wave, lane, sight, seen_by, st);
   }
 
   // The waves' rows meet in LDS.
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt) {
     st.l[rt] = sum_x16_x32(st.l[rt]);
+    float* const row = &mo[wave][(16 * rt + c) * kPitch];
+    const f32x4(&o)[4] = st.o[rt];
+    if (f32_order) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<f32x4*>(row + 16 * g + 4 * e) =
+            f32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
+    } else {
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-        mo[wave][(16 * rt + c) * kPitch + (f32_order ? 16 * g + 4 * e + dt : 16 * dt + 4 * g + e)] =
-            st.o[rt][dt][e];
+      for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4*>(row + 16 * dt + 4 * g) = o[dt];
+    }
     if (g == 0) {
       ml[wave][0][16 * rt + c] = st.m[rt];
       ml[wave][1][16 * rt + c] = st.l[rt];
@@ -543,7 +597,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
     if (mine) store(L, acc);
     return;
   }
-  const int at = a.wg0[t] + h * n_split * n_blk + blk;  // the block's first chunk
+  const int at = a.wg0[t] + (h * n_split) * n_blk + blk;  // the block's first chunk
   float* const part =
       a.part + (static_cast<int64_t>(at) * kRows + r) * kTreePart;
   const int64_t part_step = static_cast<int64_t>(n_blk) * kRows * kTreePart;  // to the next chunk
@@ -597,63 +651,80 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
   if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-int block_rows(const TreeArgs& a) {
+// Rows of a block: 16, so that a tree's blocks run on CUs of their own, or 32, which read a cache
+// half as often, where three blocks or more would read one past what the caches hold. us, 16 / 32
+// rows, 20 heads: 26 nodes over 223 keys 6.4/8.5, 64 over 1500 12.9/15.3, 32 over 8000 (41 MB)
+// 20.8/32.2, 64 over 20000 (102 MB) 53.1/54.6, 32 over 40000 (205 MB) 59.2/65.4, 64 over 40000
+// 89.2/84.1, 64 over 65471 (335 MB) 138/122.
+constexpr int64_t kWideBytes = 128ll << 20;
+int block_rows(const TreeArgs& a, DType dt) {
   int most = 0;
-  for (int t = 0; t < a.n_trees; ++t) most = std::max(most, a.nodes[t]);
-  return most <= 16 ? 16 : kTreeMaxRows;
+  int64_t bytes = 0;
+  for (int t = 0; t < a.n_trees; ++t) {
+    most = std::max(most, a.nodes[t]);
+    bytes += static_cast<int64_t>(a.past[t] + a.nodes[t]) * a.n_heads * 64 * 2 * (dt == kF16 ? 2 : 4);
+  }
+  return most > 32 && bytes >= kWideBytes ? kTreeMaxRows : 16;
 }
 
 }  // namespace
 
-int64_t tree_plan(TreeArgs& a, bool split) {
-  const int rows = block_rows(a);
+int64_t tree_plan(TreeArgs& a, DType dt, bool split) {
+  const int rows = block_rows(a, dt);
   int64_t blocks = 0, work = 0;
   int longest = 1;
   for (int t = 0; t < a.n_trees; ++t) {
-    const int64_t b = static_cast<int64_t>((a.nodes[t] + rows - 1) / rows) * a.n_heads;
+    a.n_blk[t] = (a.nodes[t] + rows - 1) / rows;
+    const int64_t b = static_cast<int64_t>(a.n_blk[t]) * a.n_heads;
     const int total = a.past[t] + a.nodes[t];
     blocks += b;
     work += b * total;
     longest = std::max(longest, total);
   }
-  // Workgroups of a launch: the first tree's start and the sum of all.
-  auto lay = [&](int chunk) {
-    int64_t n = 0;
-    a.chunk = chunk;
-    for (int t = 0; t < a.n_trees; ++t) {
-      a.wg0[t] = static_cast<int>(std::min<int64_t>(n, 0x7fffffff));
-      const int total = a.past[t] + a.nodes[t];
-      n += static_cast<int64_t>((a.nodes[t] + rows - 1) / rows) * a.n_heads *
-           ((static_cast<int64_t>(total) + chunk - 1) / chunk);
-    }
-    return n;
+  auto inverse = [](int n) {
+    return static_cast<uint32_t>(std::min<uint64_t>(((uint64_t{1} << 32) + n - 1) / n, 0xffffffffu));
   };
-  int kLeast = 256;  // keys worth a workgroup
-  if (const char* e = getenv("TREE_LEAST")) kLeast = atoi(e);
-  int kWgs = kTreeMaxWgs * 3 / 4;
-  if (const char* e = getenv("TREE_WGS")) kWgs = atoi(e);
-  if (split && blocks < kTreeMaxWgs / 2 && longest > kLeast) {
-    int64_t chunk = std::max<int64_t>(kLeast, (work + kWgs - 1) / kWgs);
-    for (chunk = (chunk + kLeast - 1) / kLeast * kLeast; chunk < longest; chunk += kLeast) {
-      const int64_t n = lay(static_cast<int>(chunk));
-      if (n <= kTreeMaxWgs) return n;
+  // Chunks of so many keys; returns the sum of all trees' workgroups and the grid's width.
+  int64_t widest = 0;
+  auto lay = [&](int64_t chunk) {
+    int64_t sum = 0;
+    widest = 0;
+    a.chunk = static_cast<int>(chunk);
+    for (int t = 0; t < a.n_trees; ++t) {
+      a.n_split[t] = static_cast<int>((a.past[t] + a.nodes[t] + chunk - 1) / chunk);
+      a.blk_inv[t] = inverse(a.n_blk[t]);
+      a.split_inv[t] = inverse(a.n_split[t]);
+      a.wg0[t] = static_cast<int>(std::min<int64_t>(sum, 0x7fffffff));
+      const int64_t n = static_cast<int64_t>(a.n_blk[t]) * a.n_heads * a.n_split[t];
+      a.n_wgs[t] = static_cast<int>(std::min<int64_t>(n, 0x7fffffff));
+      sum += n;
+      widest = std::max(widest, n);
     }
+    widest = (widest + 7) / 8 * 8;
+    return sum;
+  };
+  // A split costs ~1.5 us: caches of fewer keys than `whole` are not worth it, nor chunks of fewer
+  // than `least`. us, whole / split, 12 heads, 4 trees of 13: f16 430 keys 7.7/8.6 (20 heads, 1500
+  // keys 9.9/8.9), f32 430 keys 10.4/8.9 (249 keys 8.3/8.4). Two workgroups a CU in all, which run
+  // at once (f16, 16 nodes over 65471 keys: 90 us with one, 73 with two, 76 with three; 64 nodes
+  // 122, and 130 with eight workgroups more).
+  const int whole = dt == kF16 ? 512 : 320, least = dt == kF16 ? 256 : 128;
+  constexpr int kWgs = 512;
+  if (split && blocks < kTreeMaxWgs / 2 && longest > whole) {
+    int64_t chunk = std::max<int64_t>(least, (work + kWgs - 1) / kWgs);
+    for (chunk = (chunk + 127) / 128 * 128; chunk < longest; chunk += 128)
+      if (lay(chunk) <= kWgs) return widest;
   }
-  return lay(longest);
+  lay(longest);
+  return widest;
 }
 
 hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStream_t s) {
   if (wgs <= 0) return hipSuccess;
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-  int waves = 4;
-  if (const char* e = getenv("TREE_WAVES")) waves = atoi(e);
-  const dim3 grid(static_cast<unsigned>(wgs)), block(64 * waves);
-  const bool few = block_rows(a) == 16;
-#define WRS_TREE(KT, RT)                                                    \
-  if (waves == 8)                                                           \
-    hipLaunchKernelGGL((tree_attend<KT, RT, 8>), grid, block, 0, s, a);     \
-  else                                                                      \
-    hipLaunchKernelGGL((tree_attend<KT, RT, 4>), grid, block, 0, s, a)
+  const dim3 grid(static_cast<unsigned>(wgs), a.n_trees), block(64 * kWaves);
+  const bool few = block_rows(a, dt) == 16;
+#define WRS_TREE(KT, RT) hipLaunchKernelGGL((tree_attend<KT, RT>), grid, block, 0, s, a)
   switch (dt) {
     case kF16:
       if (few) { WRS_TREE(_Float16, 1); } else { WRS_TREE(_Float16, 2); }

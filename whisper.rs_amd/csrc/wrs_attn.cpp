@@ -1629,8 +1629,9 @@ int wrs_attn_tree_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t* 
     if (rc) return rc;
     a.part = c->tree_part;
     a.counters = c->tree_counters;
-    const int64_t wgs = wrs::tree_plan(a, c->tree_counters != nullptr);
-    WRS_HIP(c, wrs::launch_tree_attend(a, kv->f32() ? wrs::kF32 : wrs::kF16, wgs, c->stream));
+    const wrs::DType dt = kv->f32() ? wrs::kF32 : wrs::kF16;
+    const int64_t wgs = wrs::tree_plan(a, dt, c->tree_counters != nullptr);
+    WRS_HIP(c, wrs::launch_tree_attend(a, dt, wgs, c->stream));
   }
   return WRS_OK;
 }

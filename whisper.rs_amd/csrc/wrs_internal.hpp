@@ -227,7 +227,7 @@ constexpr size_t kRowsMaxKeys = (size_t{1} << 24) - 4095;
 // and v (f16 or f32; head h at + h*kv_hs, key j at + j*64): its `past` keys, and of
 // the drafted rows behind them each row and its ancestors. parents[row0 + i] is
 // row i's parent if it is in [0, i), otherwise the row hangs from the last cached
-// token. tree_plan fills chunk and wg0 and returns the launch's workgroups; with
+// token. tree_plan lays out the launch and returns the workgroups of a tree's row of it; with
 // `split` it may deal a block's keys over several, which then need part
 // (kTreePartFloats) and counters (kTreeCounterWords, zero between launches).
 constexpr int kTreeMaxTrees = 64;   // per launch
@@ -251,9 +251,12 @@ struct TreeArgs {
   int64_t off[kTreeMaxTrees];
   int64_t row0[kTreeMaxTrees];
   int past[kTreeMaxTrees], nodes[kTreeMaxTrees];  // nodes >= 1
-  int wg0[kTreeMaxTrees];
+  // By tree_plan: a tree's workgroups and where they start among all trees', its blocks of rows
+  // and chunks of keys, with 2^32 over each.
+  int n_wgs[kTreeMaxTrees], wg0[kTreeMaxTrees], n_blk[kTreeMaxTrees], n_split[kTreeMaxTrees];
+  uint32_t blk_inv[kTreeMaxTrees], split_inv[kTreeMaxTrees];
 };
-int64_t tree_plan(TreeArgs& a, bool split);
+int64_t tree_plan(TreeArgs& a, DType dt, bool split);
 hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStream_t s);
 
 // Measurement: a streaming read of `bytes` (multiple of 16, 16-byte aligned)
