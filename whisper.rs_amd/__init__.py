@@ -22,6 +22,7 @@ There is no CPU fallback: without the built library every call raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import threading
 
@@ -178,11 +179,17 @@ def mha_with_cache(q, k, v, n_tokens, total_tokens, t_past, n_heads, d_model, ou
 _DT = {"torch.float32": WRS_F32, "torch.float16": WRS_F16, "torch.bfloat16": WRS_BF16}
 
 
+_codes = {}  # torch.dtype -> code, filled as dtypes come by
+
+
 def _dtype_code(t):
-    try:
-        return _DT[str(t.dtype)]
-    except KeyError:
-        raise TypeError(f"unsupported dtype {t.dtype}") from None
+    code = _codes.get(t.dtype)
+    if code is None:
+        try:
+            code = _codes[t.dtype] = _DT[str(t.dtype)]
+        except KeyError:
+            raise TypeError(f"unsupported dtype {t.dtype}") from None
+    return code
 
 
 def token_major(t_rows: int, d_model: int, d_head: int, row_stride: int | None = None) -> Layout:
@@ -305,17 +312,26 @@ def linear_fused(x, ws, biases, outs, *, ln=None, act=None, out_row_stride=None,
 def _on_device(ctx, what, *tensors):
     """Every tensor lies on the context's GPU."""
     for t in tensors:
-        if not t.is_cuda or t.get_device() != ctx.device:
+        if t.get_device() != ctx.device:  # -1: not on a GPU
             raise TypeError(f"{what}: tensors must be on cuda:{ctx.device}, got {t.device}")
 
 
 def _rows(t, what):
     """(rows, columns, row stride) of a 2-D tensor with adjacent columns."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise TypeError(f"{what}: rows of adjacent values expected, got {tuple(t.shape)} "
-                        f"with strides {t.stride()}")
-    n, d = t.shape
-    return n, d, (t.stride(0) if n > 1 else d)
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1):
+        raise TypeError(f"{what}: rows of adjacent values expected, got {tuple(shape)} "
+                        f"with strides {strides}")
+    n, d = shape
+    return n, d, (strides[0] if n > 1 else d)
+
+
+def _sizes(values):
+    """A size_t array of a sequence of counts (negative ones are refused)."""
+    n = len(values)
+    if n <= 16 and (not n or min(values) >= 0):
+        return (ctypes.c_size_t * n)(*values) if n else None
+    return (ctypes.c_size_t * n).from_buffer(array.array("Q", values))
 
 
 class Mx4:
@@ -586,15 +602,15 @@ class KvArena:
         no, do, o_rs = _rows(out, "tree_self")
         trees = len(slots)
         assert d == do == self.d_model and n == no and trees == len(counts)
-        for t, want in ((q, "float32"), (out, "float32"), (parents, "int32")):
-            if str(t.dtype) != "torch." + want:
-                raise TypeError(f"tree_self: {want} expected, got {t.dtype}")
+        if _dtype_code(q) != WRS_F32 or _dtype_code(out) != WRS_F32:
+            raise TypeError(f"tree_self: float32 rows expected, got {q.dtype} and {out.dtype}")
+        if parents.element_size() != 4 or parents.is_floating_point() or parents.is_complex():
+            raise TypeError(f"tree_self: int32 parents expected, got {parents.dtype}")
         if sum(counts) != n or not parents.is_contiguous():
             raise AssertionError("tree_self: one row and one parent per drafted token")
         _on_device(self.ctx, "tree_self", q, out, parents)
-        arr = ctypes.c_size_t * trees
-        self._c(self._lib.wrs_attn_tree_self(self.ctx.handle, self.handle, layer, arr(*slots),
-                                             arr(*counts), trees, parents.data_ptr(),
+        self._c(self._lib.wrs_attn_tree_self(self.ctx.handle, self.handle, layer, _sizes(slots),
+                                             _sizes(counts), trees, parents.data_ptr(),
                                              parents.numel(), q.data_ptr(), q_rs, out.data_ptr(),
                                              o_rs), "tree_self")
 
@@ -605,10 +621,8 @@ class KvArena:
         :meth:`advance` then takes them into the history."""
         n = len(slots)
         assert n == len(counts)
-        arr = ctypes.c_size_t * n
-        self._c(self._lib.wrs_kv_keep_rows(self.handle, arr(*slots), arr(*counts), n,
-                                           (ctypes.c_size_t * len(rows))(*rows), len(rows)),
-                "keep_rows")
+        self._c(self._lib.wrs_kv_keep_rows(self.handle, _sizes(slots), _sizes(counts), n,
+                                           _sizes(rows), len(rows)), "keep_rows")
 
     def prefill_cross(self, layer, q, out, lse=None):
         """Cross-attention of prompt rows (decoder.rs:698-708). With ``lse`` (a

@@ -117,24 +117,29 @@ __global__ __launch_bounds__(256) void kv_copy_planes(const _Float16* k_src, _Fl
 // and in order this is safe: sources rise and are at or above their destinations, so no
 // pass writes a row that a later one reads.
 constexpr int kKeepWaves = 4;
-__global__ __launch_bounds__(64 * kKeepWaves) void kv_keep_rows(KeepArgs a) {
-  const int64_t planes = static_cast<int64_t>(a.n_layers) * a.n_heads * 2;
-  const int64_t p = static_cast<int64_t>(blockIdx.x) * kKeepWaves + (threadIdx.x >> 6);
-  if (p >= planes) return;  // whole wave
+template <int kSlots, int kMoves>
+__global__ __launch_bounds__(64 * kKeepWaves) void kv_keep_rows(KeepArgs<kSlots, kMoves> a) {
+  const int p = blockIdx.x * kKeepWaves + (threadIdx.x >> 6), h = p >> 1;
+  if (h >= a.n_heads) return;  // whole wave
   const int u = blockIdx.y, lane = threadIdx.x & 63;
-  const int64_t lh = p >> 1;
-  const int h = static_cast<int>(lh % a.n_heads);
-  const int64_t layer = lh / a.n_heads;
   u32x4* const base = static_cast<u32x4*>((p & 1) ? a.v : a.k) + a.off[u] +
-                      layer * a.layer_stride + h * a.plane_stride +
+                      blockIdx.z * a.layer_stride + h * a.plane_stride +
                       static_cast<int64_t>(a.past[u]) * a.units;
-  const int i0 = a.first[u], i1 = a.first[u + 1];
-  const int per = 64 / a.units, sub = lane / a.units, c = lane % a.units;
-  for (int i = i0; i < i1; i += per) {
-    const int j = i + sub;
+  const int n = a.count[u], first = a.first[u], dst0 = a.dst0[u];
+  const int shift = a.units == 8 ? 3 : 4;  // 16-byte units of a row: f16 8, f32 16
+  const int per = 64 >> shift, sub = lane >> shift, c = lane & (a.units - 1);
+  for (int i = 0; i < n; i += per) {
+    // The pass's sources (8 of f16 rows, 4 of f32 ones) come with the arguments, in one piece.
+    const uint32_t* const src_words = a.src + ((first + i) & ~7) / 2;
+    uint32_t w[4] = {src_words[0], src_words[1], src_words[2], src_words[3]};
+    asm("" : "+s"(w[0]), "+s"(w[1]), "+s"(w[2]), "+s"(w[3]));  // not a load per lane
+    const int at = (i & 7) + sub;
+    const uint32_t pair = at < 4 ? (at < 2 ? w[0] : w[1]) : (at < 6 ? w[2] : w[3]);
+    const int src = at & 1 ? pair >> 16 : pair & 0xFFFFu;
     u32x4 x = {0, 0, 0, 0};
-    if (j < i1) x = base[static_cast<int64_t>(a.src[j]) * a.units + c];
-    if (j < i1) base[static_cast<int64_t>(a.dst0[u] + j - i0) * a.units + c] = x;
+    const bool in = i + sub < n;
+    if (in) x = base[static_cast<int64_t>(src) * a.units + c];
+    if (in) base[static_cast<int64_t>(dst0 + i + sub) * a.units + c] = x;
   }
 }
 
@@ -216,14 +221,15 @@ hipError_t launch_kv_copy_planes(const _Float16* k_src, _Float16* k_dst, const _
   return hipGetLastError();
 }
 
-hipError_t launch_kv_keep_rows(const KeepArgs& a, hipStream_t s) {
+template <int kSlots, int kMoves>
+hipError_t launch_kv_keep_rows(const KeepArgs<kSlots, kMoves>& a, hipStream_t s) {
   if (a.n_slots <= 0 || a.n_layers <= 0 || a.n_heads <= 0) return hipSuccess;
-  const int64_t planes = static_cast<int64_t>(a.n_layers) * a.n_heads * 2;
-  const int64_t blocks = (planes + kKeepWaves - 1) / kKeepWaves;
-  if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(kv_keep_rows, dim3(static_cast<unsigned>(blocks), a.n_slots),
-                     dim3(64 * kKeepWaves), 0, s, a);
+  if (a.n_layers > 65535 || a.n_heads > (1 << 29)) return hipErrorInvalidConfiguration;
+  const dim3 grid((2 * a.n_heads + kKeepWaves - 1) / kKeepWaves, a.n_slots, a.n_layers);
+  hipLaunchKernelGGL((kv_keep_rows<kSlots, kMoves>), grid, dim3(64 * kKeepWaves), 0, s, a);
   return hipGetLastError();
 }
+template hipError_t launch_kv_keep_rows(const KeepArgs<kKeepSlots, kKeepMoves>&, hipStream_t);
+template hipError_t launch_kv_keep_rows(const KeepArgs<kKeepFewSlots, kKeepFewMoves>&, hipStream_t);
 
 }  // namespace wrs

@@ -16,46 +16,8 @@
 namespace wrs {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
-
-constexpr int kLane = 8;  // values per lane
-
-template <typename T>
-__device__ inline f32x8 load8(const T* p);
-template <>
-__device__ inline f32x8 load8<float>(const float* p) {
-  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-  return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
-template <>
-__device__ inline f32x8 load8<_Float16>(const _Float16* p) {
-  return __builtin_convertvector(*reinterpret_cast<const f16x8*>(p), f32x8);
-}
-template <>
-__device__ inline f32x8 load8<__bf16>(const __bf16* p) {
-  return __builtin_convertvector(*reinterpret_cast<const bf16x8*>(p), f32x8);
-}
-
-template <typename T>
-__device__ inline void store8(T* p, const f32x8& x);
-template <>
-__device__ inline void store8<float>(float* p, const f32x8& x) {
-  reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-  reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
-}
-template <>
-__device__ inline void store8<_Float16>(_Float16* p, const f32x8& x) {
-  *reinterpret_cast<f16x8*>(p) = __builtin_convertvector(x, f16x8);
-}
-template <>
-__device__ inline void store8<__bf16>(__bf16* p, const f32x8& x) {
-  *reinterpret_cast<bf16x8*>(p) = __builtin_convertvector(x, bf16x8);
-}
+constexpr int kLane = 8;   // values per lane and group
+constexpr int kTurns = 4;  // groups a lane has in flight, 256 lanes apart
 
 template <int CTRL>
 __device__ inline uint32_t dpp(uint32_t x) {
@@ -63,13 +25,24 @@ __device__ inline uint32_t dpp(uint32_t x) {
       __builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xF, 0xF, false));
 }
 
-// x * 2^e, e in [-127, 127], exactly rounded also where 2^e or the result is subnormal.
-__device__ inline float scaled(float x, int e) { return __builtin_ldexpf(x, e); }
+template <typename T>
+struct Lane {  // 8 values, loaded and stored 16 bytes at a time
+  typedef T t8 __attribute__((ext_vector_type(8), aligned(16)));
+};
 
 // e2m1 code of |y| < 8: how many of the midpoints lie below it (at one, the even code).
 __device__ inline uint32_t code_of(float y) {
   return (y > 0.25f) + (y >= 0.75f) + (y > 1.25f) + (y >= 1.75f) + (y > 2.5f) + (y >= 3.5f) +
          (y > 5.f);
+}
+__device__ inline float scale_of(int byte) {
+  return __builtin_bit_cast(float, static_cast<uint32_t>(byte) << 23);
+}
+// Two values over a scale as codes, in byte k of w: v_cvt_scalef32_pk_fp4 rounds to nearest, ties
+// to the even code, and saturates.
+template <int k>
+__device__ inline uint32_t encode2(uint32_t w, float a, float b, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, a, b, scale, k);
 }
 
 // Group `t` of 8 values of packed rows is values 8 t.. of x; of strided ones (kPacked
@@ -78,60 +51,106 @@ template <typename T, bool kPacked>
 __global__ __launch_bounds__(256) void mx4_quantize(const T* x, int64_t x_rs, int64_t groups,
                                                     uint32_t per_row, uint32_t* codes,
                                                     uint8_t* scales) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (t >= groups) return;  // groups are a multiple of 4: whole blocks
-  const T* p = x + t * kLane;
-  if constexpr (!kPacked) {
-    const int64_t row = t / per_row;
-    p = x + row * x_rs + (t - row * per_row) * kLane;
-  }
-  const f32x8 v = load8<T>(p);
-  const u32x8 bits = __builtin_bit_cast(u32x8, v);
-  uint32_t top = 0;
+  typedef typename Lane<T>::t8 t8;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (256 * kTurns) + threadIdx.x;
+  t8 v[kTurns];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, bits[i] & 0x7FFFFFFFu);
-  top = max(top, dpp<0xB1>(top));  // xor 1
-  top = max(top, dpp<0x4E>(top));  // xor 2
-  const bool bad = top >= 0x7F800000u;
-  // floor(log2) of a normal number is its exponent field - 127; below the normal ones
-  // the scale is 2^-127 anyway.
-  const int e = max(static_cast<int>(top >> 23) - 127 - 2, -127);
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t c = code_of(__builtin_fabsf(scaled(v[i], -e))) |
-                       ((bits[i] >> 28) & 8u);
-    w |= c << (4 * i);
+  for (int u = 0; u < kTurns; ++u) {
+    const int64_t t = min(t0 + 256 * u, groups - 1);
+    const T* p = x + t * kLane;
+    if constexpr (!kPacked) {
+      const int64_t row = t / per_row;
+      p = x + row * x_rs + (t - row * per_row) * kLane;
+    }
+    v[u] = *reinterpret_cast<const t8*>(p);
   }
-  codes[t] = bad ? 0u : w;
-  if ((t & 3) == 0) scales[t >> 2] = static_cast<uint8_t>(bad ? 255 : e + 127);
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int64_t t = t0 + 256 * u;
+    if (t >= groups) return;  // groups are a multiple of 4: whole blocks
+    float f[kLane];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) {
+      f[i] = static_cast<float>(v[u][i]);
+      top = max(top, __builtin_bit_cast(uint32_t, f[i]) & 0x7FFFFFFFu);
+    }
+    top = max(top, dpp<0xB1>(top));  // xor 1
+    top = max(top, dpp<0x4E>(top));  // xor 2
+    const bool bad = top >= 0x7F800000u;
+    // floor(log2) of a normal number is its exponent field - 127; below the normal ones
+    // the scale is 2^-127 anyway.
+    const int e = max(static_cast<int>(top >> 23) - 127 - 2, -127);
+    uint32_t w = 0;
+    if (e > -126) {
+      const float scale = scale_of(e + 127);
+      w = encode2<0>(w, f[0], f[1], scale);
+      w = encode2<1>(w, f[2], f[3], scale);
+      w = encode2<2>(w, f[4], f[5], scale);
+      w = encode2<3>(w, f[6], f[7], scale);
+    } else {  // values next to or below the normal numbers: exact without them
+#pragma unroll
+      for (int i = 0; i < kLane; ++i)
+        w |= (code_of(__builtin_fabsf(__builtin_ldexpf(f[i], -e))) |
+              ((__builtin_bit_cast(uint32_t, f[i]) >> 28) & 8u)) << (4 * i);
+    }
+    codes[t] = bad ? 0u : w;
+    if ((t & 3) == 0) scales[t >> 2] = static_cast<uint8_t>(bad ? 255 : e + 127);
+  }
+}
+
+// 2 values of byte k of w, times a scale, as T.
+template <typename T, int k>
+__device__ inline void decode2(uint32_t w, float scale, T& a, T& b) {
+  if constexpr (sizeof(T) == 4) {
+    const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, k);
+    a = v[0];
+    b = v[1];
+  } else if constexpr (__is_same(T, _Float16)) {
+    const auto v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, k);
+    a = v[0];
+    b = v[1];
+  } else {
+    const auto v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, k);
+    a = v[0];
+    b = v[1];
+  }
 }
 
 template <typename T, bool kPacked>
 __global__ __launch_bounds__(256) void mx4_dequantize(const uint32_t* codes, const uint8_t* scales,
                                                       int64_t groups, uint32_t per_row, T* out,
                                                       int64_t out_rs) {
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (t >= groups) return;
-  T* p = out + t * kLane;
-  if constexpr (!kPacked) {
-    const int64_t row = t / per_row;
-    p = out + row * out_rs + (t - row * per_row) * kLane;
-  }
-  const uint32_t w = codes[t];
-  const int s = scales[t >> 2];
-  f32x8 v;
+  typedef typename Lane<T>::t8 t8;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (256 * kTurns) + threadIdx.x;
+  uint32_t w[kTurns];
+  int s[kTurns];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t c = w >> (4 * i);
-    // Codes 2..7 are (2 + bit 0) * 2^(code / 2 - 2), 0 and 1 are halves of themselves.
-    const uint32_t m = c & 7u;
-    const float y = m < 2 ? 0.5f * m : __builtin_ldexpf(2.f + (m & 1u), static_cast<int>(m >> 1) - 2);
-    v[i] = s == 255 ? __builtin_nanf("")
-                    : scaled(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) |
-                                                           ((c & 8u) << 28)), s - 127);
+  for (int u = 0; u < kTurns; ++u) {
+    const int64_t t = min(t0 + 256 * u, groups - 1);
+    w[u] = codes[t];
+    s[u] = scales[t >> 2];
   }
-  store8<T>(p, v);
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int64_t t = t0 + 256 * u;
+    if (t >= groups) return;
+    T* p = out + t * kLane;
+    if constexpr (!kPacked) {
+      const int64_t row = t / per_row;
+      p = out + row * out_rs + (t - row * per_row) * kLane;
+    }
+    const float scale = scale_of(s[u]);
+    T y[kLane];
+    decode2<T, 0>(w[u], scale, y[0], y[1]);
+    decode2<T, 1>(w[u], scale, y[2], y[3]);
+    decode2<T, 2>(w[u], scale, y[4], y[5]);
+    decode2<T, 3>(w[u], scale, y[6], y[7]);
+    t8 v;
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) v[i] = y[i];
+    *reinterpret_cast<t8*>(p) = v;
+  }
 }
 
 }  // namespace
@@ -140,7 +159,7 @@ hipError_t launch_mx4_quantize(DType x_dt, const void* x, int64_t x_rs, int64_t 
                                uint8_t* codes, uint8_t* scales, hipStream_t s) {
   const int64_t groups = n_rows * (n_cols / kLane);
   if (groups <= 0) return hipSuccess;
-  const int64_t blocks = (groups + 255) / 256;
+  const int64_t blocks = (groups + 256 * kTurns - 1) / (256 * kTurns);
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
   const bool packed = x_rs == n_cols || n_rows == 1;
@@ -168,7 +187,7 @@ hipError_t launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, in
                                  hipStream_t s) {
   const int64_t groups = n_rows * (n_cols / kLane);
   if (groups <= 0) return hipSuccess;
-  const int64_t blocks = (groups + 255) / 256;
+  const int64_t blocks = (groups + 256 * kTurns - 1) / (256 * kTurns);
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(blocks));
   const bool packed = out_rs == n_cols || n_rows == 1;

@@ -958,6 +958,58 @@ int exact_arena(wrs_attn_ctx* c, wrs_kv* kv, const float* q, float* out, void* k
   return WRS_OK;
 }
 
+// Launches of wrs_kv_keep_rows, its arguments checked.
+template <int kSlots, int kMoves>
+int keep_rows(wrs_attn_ctx* c, wrs_kv* kv, const size_t* slots, const size_t* counts,
+              size_t n_slots, const size_t* rows) {
+  const size_t units = 4 * kv->esize();  // 16-byte units of a row of 64
+  wrs::KeepArgs<kSlots, kMoves> a;
+  a.k = kv->k_self;
+  a.v = kv->v_self;
+  a.layer_stride = static_cast<int64_t>(kv->n_slots * kv->n_heads * kv->max_ctx * units);
+  a.plane_stride = static_cast<int64_t>(kv->max_ctx * units);
+  a.n_layers = static_cast<int>(kv->n_layers);
+  a.n_heads = static_cast<int>(kv->n_heads);
+  a.units = static_cast<int>(units);
+  a.n_slots = 0;
+  size_t used = 0, at = 0;
+  auto flush = [&]() {
+    const hipError_t e = wrs::launch_kv_keep_rows(a, c->stream);
+    a.n_slots = 0;
+    used = 0;
+    return e;
+  };
+  for (size_t i = 0; i < n_slots; at += counts[i++]) {
+    // Rows already in place are the first ones; the others go in order, as many to a
+    // launch as its arguments hold.
+    size_t j = 0;
+    while (j < counts[i] && rows[at + j] == j) ++j;
+    while (j < counts[i]) {
+      if (a.n_slots == kSlots || used == static_cast<size_t>(kMoves)) {
+        WRS_HIP(c, flush());
+        continue;
+      }
+      const size_t n = std::min(counts[i] - j, kMoves - used);
+      const int u = a.n_slots++;
+      a.off[u] = static_cast<int64_t>(kv->self_off(0, slots[i]) / 64 * units);
+      a.past[u] = static_cast<int>(kv->len[slots[i]]);
+      a.dst0[u] = static_cast<int>(j);
+      a.first[u] = static_cast<int>(used);
+      a.count[u] = static_cast<int>(n);
+      for (size_t x = 0; x < align_up(n, 8); x += 2) {
+        const size_t lo = x < n ? rows[at + j + x] : 0, hi = x + 1 < n ? rows[at + j + x + 1] : 0;
+        a.src[(used + x) / 2] = static_cast<uint32_t>(lo | hi << 16);
+      }
+      used += align_up(n, 8);
+      j += n;
+      // A slot's next rows wait for these: they go in a launch of their own.
+      if (j < counts[i]) WRS_HIP(c, flush());
+    }
+  }
+  WRS_HIP(c, flush());
+  return WRS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1217,48 +1269,12 @@ int wrs_kv_keep_rows(wrs_kv* kv, const size_t* slots, const size_t* counts, size
   }
   if (at != n_rows) return fail(c, WRS_EINVAL, "keep_rows: more rows than the slots' counts");
   DeviceGuard g(c->device);
-  const size_t units = 4 * kv->esize();  // 16-byte units of a row of 64
-  wrs::KeepArgs a;
-  a.k = kv->k_self;
-  a.v = kv->v_self;
-  a.layer_stride = static_cast<int64_t>(kv->n_slots * kv->n_heads * kv->max_ctx * units);
-  a.plane_stride = static_cast<int64_t>(kv->max_ctx * units);
-  a.n_layers = static_cast<int>(kv->n_layers);
-  a.n_heads = static_cast<int>(kv->n_heads);
-  a.units = static_cast<int>(units);
-  a.n_slots = 0;
-  a.first[0] = 0;
-  auto flush = [&]() {
-    const hipError_t e = wrs::launch_kv_keep_rows(a, c->stream);
-    a.n_slots = 0;
-    return e;
-  };
-  at = 0;
-  for (size_t i = 0; i < n_slots; at += counts[i++]) {
-    // Rows already in place are the first ones; the others go in order, as many to a
-    // launch as its arguments hold.
-    size_t j = 0;
-    while (j < counts[i] && rows[at + j] == j) ++j;
-    while (j < counts[i]) {
-      const size_t used = a.n_slots ? a.first[a.n_slots] : 0;
-      if (a.n_slots == wrs::kKeepSlots || used == static_cast<size_t>(wrs::kKeepMoves)) {
-        WRS_HIP(c, flush());
-        continue;
-      }
-      const size_t n = std::min(counts[i] - j, wrs::kKeepMoves - used);
-      const int u = a.n_slots++;
-      a.off[u] = static_cast<int64_t>(kv->self_off(0, slots[i]) / 64 * units);
-      a.past[u] = static_cast<int>(kv->len[slots[i]]);
-      a.dst0[u] = static_cast<int>(j);
-      for (size_t x = 0; x < n; ++x) a.src[used + x] = static_cast<uint16_t>(rows[at + j + x]);
-      a.first[u + 1] = static_cast<uint16_t>(used + n);
-      j += n;
-      // A slot's next rows wait for these: they go in a launch of their own.
-      if (j < counts[i]) WRS_HIP(c, flush());
-    }
-  }
-  WRS_HIP(c, flush());
-  return WRS_OK;
+  size_t moved = 0;  // rows of the fullest slot that change places
+  for (size_t i = 0; i < n_slots; ++i) moved = std::max(moved, counts[i]);
+  if (n_slots <= static_cast<size_t>(wrs::kKeepFewSlots) &&
+      n_slots * align_up(moved, 8) <= static_cast<size_t>(wrs::kKeepFewMoves))
+    return keep_rows<wrs::kKeepFewSlots, wrs::kKeepFewMoves>(c, kv, slots, counts, n_slots, rows);
+  return keep_rows<wrs::kKeepSlots, wrs::kKeepMoves>(c, kv, slots, counts, n_slots, rows);
 }
 
 int wrs_kv_set_cross(wrs_kv* kv, size_t layer, const float* k, const float* v, size_t n_audio,

@@ -432,21 +432,24 @@ hipError_t launch_kv_copy_planes(const _Float16* k_src, _Float16* k_dst, const _
                                  _Float16* v_dst, int64_t layer_stride, int64_t plane_stride,
                                  int n_layers, int n_heads, int len, hipStream_t s);
 // Rows of a plane that come together: of slot u, at element off[u] of k and v, rows
-// past[u] + src[i] move to past[u] + dst0[u] + i - first[u], for i in [first[u],
-// first[u + 1]) in order; src rises and is at least its destination. Plane (l, h) at +
+// past[u] + src[first[u] + i] move to past[u] + dst0[u] + i, for i < count[u] in order; src rises and is at least its destination. Plane (l, h) at +
 // l*layer_stride + h*plane_stride, rows of `units` 16-byte units.
+// Arguments are copied per launch and read by every workgroup: those of few slots are small.
 constexpr int kKeepSlots = 64;   // per launch
-constexpr int kKeepMoves = 768;  // per launch, of all slots
+constexpr int kKeepMoves = 768;  // per launch, of all slots, eight to a line of a slot
+constexpr int kKeepFewSlots = 16, kKeepFewMoves = 128;
+template <int kSlots, int kMoves>
 struct KeepArgs {
   void* k;
   void* v;
   int64_t layer_stride, plane_stride;  // in 16-byte units, as off
   int n_layers, n_heads, n_slots, units;
-  int64_t off[kKeepSlots];
-  int past[kKeepSlots], dst0[kKeepSlots];
-  uint16_t first[kKeepSlots + 1];
-  uint16_t src[kKeepMoves];
+  int64_t off[kSlots];
+  int past[kSlots], dst0[kSlots];
+  int first[kSlots], count[kSlots];  // first: a multiple of 8
+  uint32_t src[kMoves / 2];          // two to a word
 };
-hipError_t launch_kv_keep_rows(const KeepArgs& a, hipStream_t s);
+template <int kSlots, int kMoves>
+hipError_t launch_kv_keep_rows(const KeepArgs<kSlots, kMoves>& a, hipStream_t s);
 
 }  // namespace wrs
