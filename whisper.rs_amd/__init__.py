@@ -604,7 +604,7 @@ class KvArena:
         assert d == do == self.d_model and n == no and trees == len(counts)
         if _dtype_code(q) != WRS_F32 or _dtype_code(out) != WRS_F32:
             raise TypeError(f"tree_self: float32 rows expected, got {q.dtype} and {out.dtype}")
-        if parents.element_size() != 4 or parents.is_floating_point() or parents.is_complex():
+        if str(parents.dtype) != "torch.int32":
             raise TypeError(f"tree_self: int32 parents expected, got {parents.dtype}")
         if sum(counts) != n or not parents.is_contiguous():
             raise AssertionError("tree_self: one row and one parent per drafted token")

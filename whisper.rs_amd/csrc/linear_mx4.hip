@@ -7,7 +7,6 @@
 
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 #include <type_traits>
 
 namespace wrs {
@@ -930,19 +929,27 @@ hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 template <typename XT, typename OT>
 hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
+  // The largest tile that fills the chip: larger ones read x and W less often, but a CU without
+  // a workgroup does nothing. Both sides of each step, us (f16 x; f32 and MXFP4 x change sides
+  // at the same places):
+  //   Large, 180 workgroups (1500 rows, 3 x 1280 -> 1280): 29.7, Wide 30.3; 120 (3000 rows
+  //   5120 -> 1280): 78.8, Wide 60.3.
+  //   Wide, 144 (1500 rows 384 -> 1536): 11.0, Mid 12.4; 120 (1500 rows 1280 -> 1280): 18.6, Mid
+  //   16.2.
+  //   Mid, 180 (130 rows, 3 x 1280 -> 1280): 10.4, Small 11.6; 100 (300 rows 1280 -> 1280): 9.3,
+  //   Small 8.0.
   using Small = Tile<64, 32, 32, 32, 1, 4>;
   using Mid = Tile<64, 64, 32, 32, 1, 2>;
   using Wide = Tile<128, 128, 64, 64, 1, 1>;
   using Large = std::conditional_t<sizeof(XT) <= 2, Tile<256, 128, 64, 128, 1, 1>,
                                    Tile<256, 128, 64, 64, 1, 1>>;
-  auto wgs = [&](int f, int t) {
-    return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups;
+  auto fills = [&](int f, int t, int least) {
+    return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups >=
+           least;
   };
-  int force = 0;
-  if (const char* e = getenv("MX4_FORCE")) force = atoi(e);
-  if (force == 1 || (!force && wgs(Large::BF, Large::BT) >= 192)) return launch_tile<Large, XT, OT>(a, out_dt, s);
-  if (force == 2 || (!force && wgs(128, 128) >= 192)) return launch_tile<Wide, XT, OT>(a, out_dt, s);
-  if (force == 3 || (!force && wgs(64, 64) >= 256)) return launch_tile<Mid, XT, OT>(a, out_dt, s);
+  if (fills(Large::BF, Large::BT, 160)) return launch_tile<Large, XT, OT>(a, out_dt, s);
+  if (fills(Wide::BF, Wide::BT, 144)) return launch_tile<Wide, XT, OT>(a, out_dt, s);
+  if (fills(Mid::BF, Mid::BT, 180)) return launch_tile<Mid, XT, OT>(a, out_dt, s);
   return launch_tile<Small, XT, OT>(a, out_dt, s);
 }
 
