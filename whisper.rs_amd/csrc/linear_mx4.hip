@@ -60,6 +60,7 @@ __device__ inline bf16x8 widen8(uint32_t w, float scale) {
 
 constexpr int kRawBuffer = 0x00020000;  // buffer resource word 3: raw, 32-bit data format
 constexpr uint32_t kPast = 0xFFFF0000u;  // an offset past every buffer
+constexpr uint32_t kPastRows = 0x80000000u;  // so with offsets of rows (below 2^28) added
 
 constexpr int kRowsWaves = 8;
 constexpr int kGroup = 8;       // blocks of a row that a wave takes at a time: 128 bytes of codes
@@ -316,11 +317,11 @@ __device__ inline float gelu_exp(float x) {
   return x * __builtin_amdgcn_rcpf(1.f + e);
 }
 
-// Tile of a workgroup: BF features x BT rows of x, waves of WF x WT; x is loaded kDx stages
-// ahead, and KG groups of waves take the stages in turn.
-template <int BF_, int BT_, int WF_, int WT_, int Dx_, int KG_>
+// Tile of a workgroup: BF features x BT rows of x, waves of WF x WT; KG groups of waves take the
+// tile's columns in turn.
+template <int BF_, int BT_, int WF_, int WT_, int KG_>
 struct Tile {
-  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, kDx = Dx_, KG = KG_;
+  static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, KG = KG_;
   static constexpr int kWaves = (BF / WF) * (BT / WT);  // of a group
   static constexpr int kGroupThreads = 64 * kWaves, kThreads = kGroupThreads * KG;
 };
@@ -328,13 +329,17 @@ constexpr int kK = 64;           // columns per stage
 constexpr int kRow = 2 * kK;     // bytes of a staged row
 constexpr int kOutPitch = 68;    // floats of an output row in LDS
 
+constexpr int kCodeRow = kK;     // bytes of codes of a row in two stages
+
 // 16-byte chunk c of staged row r sits at c ^ (r / 2): 16 rows read at one chunk hit
-// distinct banks.
+// distinct banks. So for rows of codes of half the length, at c ^ (r / 4).
 __device__ inline int chunk_at(int r, int c) { return r * kRow + 16 * (c ^ ((r >> 1) & 7)); }
+__device__ inline int code_at(int r, int c) { return r * kCodeRow + 16 * (c ^ ((r >> 2) & 3)); }
 
 template <typename T, int P>
 constexpr size_t tile_lds() {  // P 0: MXFP4 x, whose scales lie behind its codes
-  const size_t stage = 2ull * (P ? P * kRow : kRow + 8) * T::BT * T::KG;
+  const size_t stage = (2ull * (P ? P * kRow : kRow + 8) * T::BT +
+                        static_cast<size_t>(T::kWaves) * T::WF * (P ? kCodeRow : kRow)) * T::KG;
   const size_t out = sizeof(float) * T::kWaves * 32 * kOutPitch;
   const size_t join = sizeof(float) * T::BF * T::BT * (T::KG - 1);
   return stage > out ? (stage > join ? stage : join) : (out > join ? out : join);
@@ -344,19 +349,34 @@ constexpr size_t tile_lds() {  // P 0: MXFP4 x, whose scales lie behind its code
 // row's largest value where it lies in [2^-10, 511].
 constexpr float kXUp = 128.f, kXLeast = 0x1p-10f, kXMost = 511.f;
 
+// Four scale bytes from `at` of a row on (an even place): one load where they lie on a word.
+template <bool kWords>
+__device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_t at, bool in,
+                                       bool in_high) {
+  if constexpr (kWords) return __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at : kPast, 0, 0);
+  const uint32_t lo = static_cast<uint16_t>(
+      __builtin_amdgcn_raw_buffer_load_b16(rs, in ? at : kPast, 0, 0));
+  const uint32_t hi = static_cast<uint16_t>(
+      __builtin_amdgcn_raw_buffer_load_b16(rs, in_high ? at + 2 : kPast, 0, 0));
+  return lo | (hi << 16);
+}
+
 // Adds one tile's products with operands of type E to acc. x goes in P parts: one of its own
 // type, two of f16 (f32 x, E f16: results times kXUp), or with bf16 E part `part` of kParts.
 // Returns (to every thread) whether E cannot hold the tile's operands: a scale of its weights,
 // or a row of f32 x.
-//   W goes from memory to MFMA operands in registers: lane (r, h) of a 32-row block takes block
-//   h of row r, and step j of a stage multiplies values 8 j.. of both blocks, so x's operand is
-//   chunk 4 h + j of its staged row.
-template <typename T, typename XT, typename E, int P>
+//   A wave's own rows of W come 64 bytes of codes at a time, 4 lanes a row, and change places in
+//   its own LDS: lanes that load the 16 bytes that they multiply touch a cache line each, and
+//   the line lookups bound the kernel (24000 x 5120 -> 1280 f16: 376 us). Lane (r, h)
+//   of a 32-row block takes block h of a stage of row r, widened in registers, and step j
+//   multiplies values 8 j.. of both blocks, so x's operand is chunk 4 h + j of its staged row.
+template <typename T, typename XT, typename E, int P, bool kWords>
 __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
                                     int part, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
   constexpr int kXn = T::BT * (kK / 8) / T::kGroupThreads;  // groups of 8 values a thread stages
   static_assert(kXn >= 1 && T::BT * (kK / 8) % T::kGroupThreads == 0, "whole groups");
+  constexpr int kWn = T::WF * 4 / 64;  // chunks of codes a lane loads
   constexpr int kXBytes = T::BT * kRow, kStageBytes = P * kXBytes;
   constexpr bool kHalves = P == 2;  // f32 x in two f16 parts
   static_assert(!kHalves || (__is_same(XT, float) && __is_same(E, _Float16)), "");
@@ -365,6 +385,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / T::kGroupThreads);
   const int tid = threadIdx.x - kg * T::kGroupThreads;  // in the group
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* const codes = lds + T::KG * 2 * kStageBytes + (kg * T::kWaves + wave) * T::WF * kCodeRow;
   lds += kg * 2 * kStageBytes;
   const int r32 = lane & 31, hl = lane >> 5;
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
@@ -387,38 +408,46 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     xp[i] = static_cast<const XT*>(a.x) + (t0 + row) * a.x_rs + 8 * (e & 7);
   }
 
-  u32x4 cw[2][kF];
-  uint8_t sw[2][kF];
-  x8 xv[T::kDx][kXn];
+  u32x4 cw[kWn];
+  uint32_t sw[kF], sw_next[kF];  // four scales of each row
+  x8 xv[kXn];
   float most[kXn];  // largest magnitudes of this thread's rows of x
 #pragma unroll
   for (int i = 0; i < kXn; ++i) most[i] = 0.f;
-  // Stage i of the group is stage i * KG + kg of the tile.
-  auto load_w = [&](int d, int i_s) __attribute__((always_inline)) {
-    int s = i_s * T::KG + kg;
-    asm("" : "+s"(s));  // offsets are formed per stage, not kept per load
+  // Pair i of the group, of two stages, is pair i * KG + kg of the tile.
+  const int pairs = (stages + 1) / 2;
+  auto load_w = [&](int i_p) __attribute__((always_inline)) {
+    int p = i_p * T::KG + kg;
+    asm("" : "+s"(p));  // offsets are formed per pair, not kept per load
+    const int at = 4 * p + (lane & 3);
+    const uint32_t o = at < nb ? (wf + (lane >> 2)) * bytes + 16 * at : kPastRows;
 #pragma unroll
-    for (int i = 0; i < kF; ++i) {
-      const int row = wf + 32 * i + r32;
-      const bool in = s < stages;
-      cw[d][i] = __builtin_bit_cast(
-          u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                     wrs, in ? row * bytes + 16 * hl + 32 * s : kPast, 0, 0));
-      sw[d][i] = __builtin_amdgcn_raw_buffer_load_b8(
-          srs, in ? row * nb + hl + 2 * s : kPast, 0, 0);
-    }
-  };
-  auto load_x = [&](int d, int i_s) __attribute__((always_inline)) {
-    const int at = kK * min(i_s * T::KG + kg, stages - 1);
+    for (int i = 0; i < kWn; ++i)
+      cw[i] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, o + i * 16 * bytes, 0, 0));
 #pragma unroll
-    for (int i = 0; i < kXn; ++i) xv[d][i] = *reinterpret_cast<const x8*>(xp[i] + at);
+    for (int i = 0; i < kF; ++i)
+      sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + 4 * p, p < pairs,
+                                       4 * p + 2 < nb);
   };
-  auto store_x = [&](int d, char* buf) __attribute__((always_inline)) {
+  auto put_w = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kWn; ++i)
+      *reinterpret_cast<u32x4*>(codes + code_at((lane >> 2) + 16 * i, lane & 3)) = cw[i];
+#pragma unroll
+    for (int i = 0; i < kF; ++i) sw[i] = sw_next[i];
+  };
+  auto load_x = [&](int i_s) __attribute__((always_inline)) {
+    const int at = kK * min(2 * ((i_s >> 1) * T::KG + kg) + (i_s & 1), stages - 1);
+#pragma unroll
+    for (int i = 0; i < kXn; ++i) xv[i] = *reinterpret_cast<const x8*>(xp[i] + at);
+  };
+  auto store_x = [&](char* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kXn; ++i) {
       const int e = tid + T::kGroupThreads * i;
       char* const at = buf + chunk_at(e >> 3, e & 7);
-      const x8& x = xv[d][i];
+      const x8& x = xv[i];
       if constexpr (kHalves) {
         u32x4 h, l;
 #pragma unroll
@@ -459,12 +488,15 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   bool odd = false;
   auto multiply = [&](int d, const char* buf) __attribute__((always_inline)) {
     float scale[kF];
+    u32x4 c[kF];
 #pragma unroll
     for (int i = 0; i < kF; ++i) {
+      const int byte = (sw[i] >> (16 * d + 8 * hl)) & 255;
       // f16 holds 6 * 2^13 and 0.5 * 2^-23.
       if constexpr (__is_same(E, _Float16))
-        odd |= wf + 32 * i + r32 < n_f && static_cast<unsigned>(sw[d][i] - 104) > 36u;
-      scale[i] = scale_of(sw[d][i]);
+        odd |= wf + 32 * i + r32 < n_f && static_cast<unsigned>(byte - 104) > 36u;
+      scale[i] = scale_of(byte);
+      c[i] = *reinterpret_cast<const u32x4*>(codes + code_at(32 * i + r32, 2 * d + hl));
     }
 #pragma unroll
     for (int j = 0; j < kK / 16; ++j) {
@@ -476,7 +508,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
           xw[p][i] = *reinterpret_cast<const u32x4*>(buf + p * kXBytes +
                                                      chunk_at(wt + 32 * i + r32, 4 * hl + j));
 #pragma unroll
-      for (int i = 0; i < kF; ++i) wv[i] = widen8_as<E>(cw[d][i][j], scale[i]);
+      for (int i = 0; i < kF; ++i) wv[i] = widen8_as<E>(c[i][j], scale[i]);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
@@ -486,41 +518,36 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     }
   };
 
-  load_x(0, 0);
-  load_w(0, 0);
-  load_w(1, 1);
-#pragma unroll
-  for (int d = 1; d < T::kDx; ++d) load_x(d, d);
-  store_x(0, lds);
-  load_x(0, T::kDx);
+  load_x(0);
+  load_w(0);
+  store_x(lds);
+  load_x(1);
   __syncthreads();
-  const int turns = (stages + T::KG - 1) / T::KG;  // of every group, the last ones may be empty
-  int s0 = 0;
+  const int turns = (pairs + T::KG - 1) / T::KG;  // of every group; the last one's may be empty
+  int i_p = 0;
   // No branch in this loop: one around the products costs copies of the sums (64 moves per two
   // stages of a 64 x 128 wave).
-  for (; s0 + 3 < turns; s0 += 2) {
+  for (; i_p + 1 < turns; ++i_p) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
-      const int s = s0 + d, n = (d + 1) % T::kDx;
-      store_x(n, lds + (1 - d) * kStageBytes);
-      load_x(n, s + 1 + T::kDx);
+      store_x(lds + (1 - d) * kStageBytes);
+      load_x(2 * i_p + d + 2);
+      if (d == 0) {
+        put_w();
+        load_w(i_p + 1);
+      }
       __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
       multiply(d, lds + d * kStageBytes);
-      load_w(d, s + 2);
       __syncthreads();
     }
   }
-  for (; s0 < turns; s0 += 2) {
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      const int s = s0 + d, n = (d + 1) % T::kDx;
-      if (s + 1 < turns) store_x(n, lds + (1 - d) * kStageBytes);
-      load_x(n, s + 1 + T::kDx);
-      if (s * T::KG + kg < stages) multiply(d, lds + d * kStageBytes);
-      load_w(d, s + 2);
-      __syncthreads();
-    }
-  }
+  // The second stage, stored here already, is a repeated one where there is none.
+  store_x(lds + kStageBytes);
+  put_w();
+  const int last = 2 * (i_p * T::KG + kg);
+  if (last < stages) multiply(0, lds);
+  __syncthreads();
+  if (last + 1 < stages) multiply(1, lds + kStageBytes);
   if constexpr (kHalves) {
     // 8 neighbouring lanes staged a row. Rows past the last one repeat it.
 #pragma unroll
@@ -532,7 +559,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
         // The groups staged other columns of the same rows.
         float* const all = reinterpret_cast<float*>(lds - kg * 2 * kStageBytes);
         const int row = (tid + T::kGroupThreads * i) >> 3;
-        if (i == 0) __syncthreads();
+        if (i == 0) __syncthreads();  // the last stage is read
         if ((tid & 7) == 0) all[kg * T::BT + row] = m;
       }
       if constexpr (T::KG == 1) odd |= m != 0.f && !(m >= kXLeast && m <= kXMost);
@@ -548,19 +575,17 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
       }
     }
   }
-  return __syncthreads_or(odd);
-}
-
-// Four scale bytes from `at` of a row on (an even place): one load where they lie on a word.
-template <bool kWords>
-__device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_t at, bool in,
-                                       bool in_high) {
-  if constexpr (kWords) return __builtin_amdgcn_raw_buffer_load_b32(rs, in ? at : kPast, 0, 0);
-  const uint32_t lo = static_cast<uint16_t>(
-      __builtin_amdgcn_raw_buffer_load_b16(rs, in ? at : kPast, 0, 0));
-  const uint32_t hi = static_cast<uint16_t>(
-      __builtin_amdgcn_raw_buffer_load_b16(rs, in_high ? at + 2 : kPast, 0, 0));
-  return lo | (hi << 16);
+  // (__syncthreads_or has LDS of its own, which two workgroups of 80 KB do not leave.)
+  uint64_t* const votes = reinterpret_cast<uint64_t*>(lds - kg * 2 * kStageBytes);
+  const uint64_t vote = __ballot(odd);
+  __syncthreads();
+  if (lane == 0) votes[threadIdx.x >> 6] = vote;
+  __syncthreads();
+  uint64_t any = 0;
+#pragma unroll
+  for (int i = 0; i < T::kThreads / 64; ++i) any |= votes[i];
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(any != 0);
 }
 
 // The same for MXFP4 x: 256 columns a stage, codes as they are into 32x32x64 MFMAs. Lane (r, h)
@@ -575,10 +600,12 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   static_assert(2 * T::BT <= T::kGroupThreads, "a word of scales a thread");
   constexpr int kStageBytes = T::BT * kRow + T::BT * 8;
   constexpr int kBlocks = 8;  // of a stage
+  constexpr int kWn = T::WF * 8 / 64;  // chunks of codes of W a lane loads
   const int lane = threadIdx.x & 63;
   const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x / T::kGroupThreads);
   const int tid = threadIdx.x - kg * T::kGroupThreads;  // in the group
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  char* const codes = lds + T::KG * 2 * kStageBytes + (kg * T::kWaves + wave) * T::WF * kRow;
   lds += kg * 2 * kStageBytes;
   const int r32 = lane & 31, hl = lane >> 5;
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
@@ -598,27 +625,27 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
       0, n_t * bytes, kRawBuffer);
   const __amdgpu_buffer_rsrc_t xsrs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(a.x_scales + static_cast<int64_t>(t0) * nb), 0, n_t * nb, kRawBuffer);
-  // Codes of W load into the registers whose step has just read them.
-  u32x4 cw[kF][4], xv[kXn];
-  uint32_t sw[2][kF], xs;
-  auto load_w = [&](int q, int i_s) __attribute__((always_inline)) {
+  u32x4 cw[kWn], xv[kXn];
+  uint32_t sw[kF], sw_next[kF], xs;
+  auto load_w = [&](int i_s) __attribute__((always_inline)) {
     int b = kBlocks * (i_s * T::KG + kg);  // the stage's first block
     asm("" : "+s"(b));  // offsets are formed per stage, not kept per load
+    const int at = b + (lane & 7), sb = b + 4 * hl;
+    const uint32_t o = at < nb ? (wf + (lane >> 3)) * bytes + 16 * at : kPastRows;
 #pragma unroll
-    for (int i = 0; i < kF; ++i) {
-      const int row = wf + 32 * i + r32, at = b + 4 * hl + q;
-      cw[i][q] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                               wrs, at < nb ? row * bytes + 16 * at : kPast, 0, 0));
-    }
+    for (int i = 0; i < kWn; ++i)
+      cw[i] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, o + i * 8 * bytes, 0, 0));
+#pragma unroll
+    for (int i = 0; i < kF; ++i)
+      sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + sb, sb < nb, sb + 2 < nb);
   };
-  auto load_sw = [&](int d, int i_s) __attribute__((always_inline)) {
-    int b = kBlocks * (i_s * T::KG + kg);
-    asm("" : "+s"(b));
+  auto put_w = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kF; ++i) {
-      const int row = wf + 32 * i + r32, at = b + 4 * hl;
-      sw[d][i] = load_scales<kWords>(srs, row * nb + at, at < nb, at + 2 < nb);
-    }
+    for (int i = 0; i < kWn; ++i)
+      *reinterpret_cast<u32x4*>(codes + chunk_at((lane >> 3) + 8 * i, lane & 7)) = cw[i];
+#pragma unroll
+    for (int i = 0; i < kF; ++i) sw[i] = sw_next[i];
   };
   auto load_x = [&](int i_s) __attribute__((always_inline)) {
     int b = kBlocks * (i_s * T::KG + kg);
@@ -643,26 +670,26 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
     if (2 * T::BT == T::kGroupThreads || tid < 2 * T::BT)
       *reinterpret_cast<uint32_t*>(buf + T::BT * kRow + 4 * tid) = xs;
   };
-  auto multiply = [&](int d, const char* buf, int next) __attribute__((always_inline)) {
+  auto multiply = [&](const char* buf) __attribute__((always_inline)) {
     int xsc[kT];
 #pragma unroll
     for (int t = 0; t < kT; ++t)
       xsc[t] = *reinterpret_cast<const int*>(buf + T::BT * kRow + 8 * (wt + 32 * t + r32) + 4 * hl);
 #define WRS_MX4_STEP(Q)                                                                         \
   {                                                                                             \
-    u32x4 xw[kT];                                                                               \
+    u32x4 xw[kT], ww[kF];                                                                       \
+    _Pragma("unroll") for (int i = 0; i < kF; ++i) ww[i] =                                      \
+        *reinterpret_cast<const u32x4*>(codes + chunk_at(32 * i + r32, 4 * hl + Q));            \
     _Pragma("unroll") for (int t = 0; t < kT; ++t) xw[t] = *reinterpret_cast<const u32x4*>(     \
         buf + chunk_at(wt + 32 * t + r32, 4 * hl + Q));                                         \
     _Pragma("unroll") for (int t = 0; t < kT; ++t)                                              \
         _Pragma("unroll") for (int i = 0; i < kF; ++i) {                                        \
-      const u32x4 &w = cw[i][Q], &x = xw[t];                                                    \
+      const u32x4 &w = ww[i], &x = xw[t];                                                       \
       const i32x8 wa = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};                \
       const i32x8 xa = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};                \
       acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                              \
-          wa, xa, acc[i][t], 4, 4, Q, static_cast<int>(sw[d][i]), Q, xsc[t]);                   \
+          wa, xa, acc[i][t], 4, 4, Q, static_cast<int>(sw[i]), Q, xsc[t]);                      \
     }                                                                                           \
-    load_w(Q, next);                                                                            \
-    __builtin_amdgcn_sched_barrier(0);                                                          \
   }
     WRS_MX4_STEP(0)
     WRS_MX4_STEP(1)
@@ -672,31 +699,33 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   };
 
   load_x(0);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) load_w(q, 0);
-  load_sw(0, 0);
-  load_sw(1, 1);
+  load_w(0);
   store_x(lds);
   load_x(1);
   __syncthreads();
   // Stages past the last one are zeros.
   const int turns = (stages + T::KG - 1) / T::KG;
-  for (int s0 = 0; s0 < turns; s0 += 2) {
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      store_x(lds + (1 - d) * kStageBytes);
-      load_x(s0 + d + 2);
-      __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
-      multiply(d, lds + d * kStageBytes, s0 + d + 1);
-      load_sw(d, s0 + d + 2);
-      __syncthreads();
-    }
+  auto stage = [&](int i_s, int d) __attribute__((always_inline)) {
+    store_x(lds + (1 - d) * kStageBytes);
+    load_x(i_s + 2);
+    put_w();
+    load_w(i_s + 1);
+    __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
+    multiply(lds + d * kStageBytes);
+    __syncthreads();
+  };
+  int i_s = 0;
+  for (; i_s + 1 < turns; i_s += 2) {
+    stage(i_s, 0);
+    stage(i_s + 1, 1);
   }
+  if (i_s < turns) stage(i_s, 0);
 }
 
 // The tile's outputs: each wave passes 32 rows x 64 features at a time through its own LDS, so
 // that rows are stored in whole pieces (16 bytes a lane straight from the MFMA layout go to
-// 32 rows each).
+// 32 rows each). Stores pass by the cache that holds W and x: 24000 x 5120 -> 1280 f16 338 -> 323
+// us.
 template <typename T, typename OT>
 __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
                                   bool whole, float down,
@@ -770,7 +799,7 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
           o8 o;
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = static_cast<OT>(y[e]);
-          *reinterpret_cast<o8*>(op) = o;
+          __builtin_nontemporal_store(o, reinterpret_cast<o8*>(op));
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -781,16 +810,23 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
   }
 }
 
+// Tiles of features that go together: the 64 workgroups of an XCD take 8 by 8 tiles and read
+// each stage of W and x from memory once (24000 x 5120 -> 5120 MXFP4: 421 us with all features
+// first, 401 in panels of 4 and of 8, 411 of 16; tiles of shorter rows don't care).
+constexpr int kPanel = 8;
+
 // K16 (mx4_tile): many rows of x. W is widened to 16-bit operands in registers, x passes through
 //   LDS in one part (f16, bf16) or two f16 ones (f32), and both feed 32x32x16 MFMAs. f16 holds
 //   weights of scales 2^-23 to 2^13 exactly, and rows of f32 x whose largest value is of
 //   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
 //   one of x's two or three parts after the other.
 template <typename T, typename XT, typename OT, bool kWords>
-__global__ __launch_bounds__(T::kThreads, 2) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
+__global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
-  const int f0 = (lid % n_f) * T::BF, t0 = (lid / n_f) * T::BT, grp = blockIdx.y;
+  const int n_t = gridDim.x / n_f, panel = lid / (kPanel * n_t);
+  const int wide = min(kPanel, n_f - kPanel * panel), in = lid - kPanel * n_t * panel;
+  const int f0 = (kPanel * panel + in % wide) * T::BF, t0 = in / wide * T::BT, grp = blockIdx.y;
   f32x16 acc[T::WF / 32][T::WT / 32];
   auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -803,16 +839,16 @@ __global__ __launch_bounds__(T::kThreads, 2) void mx4_tile(Mx4LinearArgs a, int 
   if constexpr (sizeof(XT) == 1) {
     tile_product_mx4<T, kWords>(a, grp, f0, t0, lds, acc);
   } else if constexpr (__is_same(XT, __bf16)) {
-    tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, 0, acc);
+    tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, 0, acc);
   } else {
     constexpr int kP = __is_same(XT, float) ? 2 : 1;
     if (kP == 2) down = 1.f / kXUp;
-    if (tile_product<T, XT, _Float16, kP>(a, grp, f0, t0, lds, 0, acc)) {
+    if (tile_product<T, XT, _Float16, kP, kWords>(a, grp, f0, t0, lds, 0, acc)) {
       clear();
       down = 1.f;
 #pragma unroll 1
       for (int part = kParts<XT> - 1; part >= 0; --part)
-        tile_product<T, XT, __bf16, 1>(a, grp, f0, t0, lds, part, acc);
+        tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, part, acc);
     }
   }
   tile_store<T, OT>(a, grp, f0, t0, lds, whole, down, acc);
@@ -907,8 +943,8 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 
 template <typename T, typename XT, typename OT, bool kWords = true>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
-  if constexpr (sizeof(XT) == 1 && kWords) {
-    // MXFP4 x: four scales a load where the rows' scales lie on words.
+  if constexpr (kWords) {
+    // Four scales a load where the rows' scales lie on words.
     bool words = a.n_in % (4 * kMx4Block) == 0 && (reinterpret_cast<uintptr_t>(a.x_scales) & 3) == 0;
     for (int g = 0; g < a.n_groups; ++g)
       words = words && (reinterpret_cast<uintptr_t>(a.w_scales[g]) & 3) == 0;
@@ -938,11 +974,11 @@ hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   //   16.2.
   //   Mid, 180 (130 rows, 3 x 1280 -> 1280): 10.4, Small 11.6; 100 (300 rows 1280 -> 1280): 9.3,
   //   Small 8.0.
-  using Small = Tile<64, 32, 32, 32, 1, 4>;
-  using Mid = Tile<64, 64, 32, 32, 1, 2>;
-  using Wide = Tile<128, 128, 64, 64, 1, 1>;
-  using Large = std::conditional_t<sizeof(XT) <= 2, Tile<256, 128, 64, 128, 1, 1>,
-                                   Tile<256, 128, 64, 64, 1, 1>>;
+  using Small = Tile<64, 32, 32, 32, 4>;
+  using Mid = Tile<64, 64, 32, 32, 2>;
+  using Wide = Tile<128, 128, 64, 64, 1>;
+  using Large = std::conditional_t<sizeof(XT) <= 2, Tile<256, 128, 64, 128, 1>,
+                                   Tile<256, 128, 64, 64, 1>>;
   auto fills = [&](int f, int t, int least) {
     return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups >=
            least;
