@@ -445,7 +445,7 @@ int wrs_mx4_dequantize(wrs_attn_ctx *ctx, const void *codes, size_t codes_len, c
  * out_dtype (WRS_F32, WRS_F16, WRS_BF16). x is f32, f16 or bf16 rows x_row_stride
  * apart (x_scales NULL), or with x_dtype WRS_MX4 packed MXFP4 rows (x_row_stride ==
  * n_in, x_len in values). bias may be NULL, or hold NULL entries. n_in % 64 == 0;
- * any n_out. */
+ * any n_out. Scales here are 2-byte aligned. */
 int wrs_linear_mx4(wrs_attn_ctx *ctx, int x_dtype, const void *x, const void *x_scales,
                    size_t x_len, int64_t x_row_stride, size_t n_groups, const void *const *w,
                    const void *const *w_scales, const float *const *bias, size_t n_tokens,

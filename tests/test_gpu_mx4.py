@@ -3,6 +3,8 @@ definition, and the projections with them (wrs_linear_mx4) against float64 produ
 of the values that the codes stand for."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -447,3 +449,30 @@ def test_refusals(wrs, ctx):
         wrs.linear_mx4(torch.randn((4, 129), device="cuda")[:, :128], [w], None, [out], ctx=ctx)
     with pytest.raises(AssertionError):  # negative stride
         wrs.linear_mx4(x, [w], None, [out], out_row_stride=-4, ctx=ctx)
+
+
+def test_addresses_and_strides_that_are_refused(wrs, ctx):
+    """Scales at odd bytes, rows whose last one lies at 2^64 and beyond (no launch)."""
+    w = wrs.mx4_quantize(torch.randn((4, 128), device="cuda"), ctx=ctx)
+    x = torch.randn((4, 128), device="cuda")
+    out = torch.empty((4, 4), device="cuda")
+    odd = torch.empty(64, device="cuda", dtype=torch.uint8)[1:17].view(4, 4)
+    shifted = wrs.Mx4(w.codes, odd)
+    for rows, weights in ((x, shifted), (shifted, w)):
+        with pytest.raises(RuntimeError):
+            wrs.linear_mx4(rows, [weights], None, [out], ctx=ctx)
+    lib = wrs._lib.lib()
+    p, q, s = (ctypes.c_void_p(t.data_ptr()) for t in (x, w.codes, w.scales))
+    wraps = 6148914691236517208  # three times it is 2^64 + 8
+    for stride in (2**62, wraps):
+        assert lib.wrs_mx4_quantize(ctx.handle, 0, p, 512, stride, 4, 128, q, 256, s, 16) < 0
+        assert lib.wrs_mx4_dequantize(ctx.handle, q, 256, s, 16, 4, 128, 0, p, 512, stride) < 0
+        ws, ss = (ctypes.c_void_p * 1)(q.value), (ctypes.c_void_p * 1)(s.value)
+        o, n = (ctypes.c_void_p * 1)(out.data_ptr()), (ctypes.c_size_t * 1)(16)
+        assert lib.wrs_linear_mx4(ctx.handle, 0, p, None, 512, stride, 1, ws, ss, None, 4, 128, 4,
+                                  0, 0, o, n, 4, 64) < 0
+        assert lib.wrs_linear_mx4(ctx.handle, 0, p, None, 512, 128, 1, ws, ss, None, 4, 128, 4,
+                                  0, 0, o, n, stride, 64) < 0
+        assert lib.wrs_linear_mx4(ctx.handle, 0, p, None, 512, 128, 1, ws, ss, None, 4, 128, 4,
+                                  0, 0, o, n, 4, 64) == 0
+    torch.cuda.synchronize()

@@ -966,14 +966,12 @@ hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 template <typename XT, typename OT>
 hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   // The largest tile that fills the chip: larger ones read x and W less often, but a CU without
-  // a workgroup does nothing. Both sides of each step, us (f16 x; f32 and MXFP4 x change sides
-  // at the same places):
-  //   Large, 180 workgroups (1500 rows, 3 x 1280 -> 1280): 29.7, Wide 30.3; 120 (3000 rows
-  //   5120 -> 1280): 78.8, Wide 60.3.
-  //   Wide, 144 (1500 rows 384 -> 1536): 11.0, Mid 12.4; 120 (1500 rows 1280 -> 1280): 18.6, Mid
-  //   16.2.
-  //   Mid, 180 (130 rows, 3 x 1280 -> 1280): 10.4, Small 11.6; 100 (300 rows 1280 -> 1280): 9.3,
-  //   Small 8.0.
+  // a workgroup does nothing. Both sides of each step by workgroups, us:
+  //   Large, 180 (f32, 1500 rows, 3 x 1280 -> 1280): 46.9, Wide 51.5; 120 (f32, 3000 rows 5120 ->
+  //   1280): 145, Wide 121.
+  //   Wide, 144 (f32, 1500 rows 384 -> 1536): 15.0, Mid 17.8; 120 (f32, 1500 rows 1280 -> 1280):
+  //   32.8, Mid 24.2.
+  //   Mid, 180 (MXFP4, 130 rows, 3 x 1280 -> 1280): 7.6, Small 8.4; 60 (40 rows): 7.0, Small 6.5.
   using Small = Tile<64, 32, 32, 32, 4>;
   using Mid = Tile<64, 64, 32, 32, 2>;
   using Wide = Tile<128, 128, 64, 64, 1>;

@@ -1835,6 +1835,13 @@ bool aligned_out(const void* p, int dt, int64_t rs, int64_t hs) {
   return (reinterpret_cast<uintptr_t>(p) % need) == 0 && rs % 4 == 0 && hs % 4 == 0;
 }
 
+// Whether n_rows rows of n_cols elements, row_stride apart, lie within len (no product is
+// formed that could pass 64 bits).
+bool rows_fit(size_t n_rows, size_t n_cols, int64_t row_stride, size_t len) {
+  if (n_cols > len) return false;
+  return n_rows == 1 || static_cast<size_t>(row_stride) <= (len - n_cols) / (n_rows - 1);
+}
+
 // The checks that quantisation and its inverse share: values of `dtype` in n_rows rows
 // of n_cols, row_stride apart, against packed codes and scales.
 int mx4_rows(wrs_attn_ctx* c, int dtype, const void* values, size_t len, int64_t row_stride,
@@ -1850,7 +1857,7 @@ int mx4_rows(wrs_attn_ctx* c, int dtype, const void* values, size_t len, int64_t
     return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
   if (row_stride < 0 || (n_rows > 1 && row_stride < static_cast<int64_t>(n_cols)))
     return fail(c, WRS_EINVAL, "row stride < n_cols");
-  if (len < (n_rows - 1) * static_cast<size_t>(row_stride) + n_cols)
+  if (!rows_fit(n_rows, n_cols, row_stride, len))
     return fail(c, WRS_EINVAL, "values shorter than n_rows rows of n_cols");
   if (codes_len < n_rows * n_cols / 2 || scales_len < n_rows * (n_cols / wrs::kMx4Block))
     return fail(c, WRS_EINVAL, "codes or scales shorter than the rows");
@@ -2200,18 +2207,27 @@ int wrs_linear_mx4(wrs_attn_ctx* c, int x_dtype, const void* x, const void* x_sc
     return fail(c, WRS_EUNSUPPORTED, "MX4 rows are packed");
   if (n_tokens > 1 && x_row_stride < static_cast<int64_t>(n_in))
     return fail(c, WRS_EINVAL, "x row stride < n_in");
-  if (x_len < (n_tokens - 1) * static_cast<size_t>(x_row_stride) + n_in)
+  if (!rows_fit(n_tokens, n_in, x_row_stride, x_len))
     return fail(c, WRS_EINVAL, "x shorter than n_tokens rows of n_in");
   if ((reinterpret_cast<uintptr_t>(x) & 15) ||
       (n_tokens > 1 && x_row_stride % (x_dtype == WRS_F32 ? 4 : 8)))
     return fail(c, WRS_EUNSUPPORTED, "x rows must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(x_scales) & 1)
+    return fail(c, WRS_EUNSUPPORTED, "scales need 2-byte alignment");
   const size_t max_off = last_out(n_tokens, n_out, out_row_stride, out_head_stride);
   wrs::Mx4LinearArgs a{};
   for (size_t gi = 0; gi < n_groups; ++gi) {
     if (!w[gi] || !w_scales[gi] || !out[gi]) return fail(c, WRS_EINVAL, "null argument");
-    if (out_len[gi] <= max_off) return fail(c, WRS_EINVAL, "out shorter than the written range");
+    // (last_out's own products hold for strides within the length.)
+    if ((n_tokens > 1 && static_cast<size_t>(out_row_stride) > out_len[gi] / (n_tokens - 1)) ||
+        (n_out > 64 &&
+         static_cast<size_t>(out_head_stride) > out_len[gi] / ((n_out - 1) / 64)) ||
+        out_len[gi] <= max_off)
+      return fail(c, WRS_EINVAL, "out shorter than the written range");
     if (reinterpret_cast<uintptr_t>(w[gi]) & 15)
       return fail(c, WRS_EUNSUPPORTED, "codes need 16-byte alignment");
+    if (reinterpret_cast<uintptr_t>(w_scales[gi]) & 1)
+      return fail(c, WRS_EUNSUPPORTED, "scales need 2-byte alignment");
     if ((reinterpret_cast<uintptr_t>(out[gi]) & (out_dtype == WRS_F32 ? 3 : 1)) ||
         (bias && (reinterpret_cast<uintptr_t>(bias[gi]) & 3)))
       return fail(c, WRS_EINVAL, "tensors must be aligned to their elements");
