@@ -11,7 +11,7 @@
 //   chunks of a block merge through memory (the last workgroup to count in adds
 //   the partials up in chunk order, so results do not depend on which it is).
 //   Only the steps that reach past the cache test the ancestor bits.
-//   f16 planes run on the f16 matrix pipe with operands in three parts, f32 ones on the
+//   f16 planes run on the f16 matrix pipe with operands in two parts, f32 ones on the
 //   f32 matrix pipe.
 #include "split16.hpp"
 
@@ -287,20 +287,33 @@ __device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                 __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// Three parts' sums as one, smallest first.
-__device__ inline f32x4 join(const f32x4 (&x)[3]) {
-  f32x4 s = x[2];
+// Two floats, times `scale` at most 2^15, as packed f16 pairs in two parts, the second in a unit
+// 2^-11 of the first.
+constexpr int kParts = 2;
+__device__ inline void split_units(float x0, float x1, float scale, uint32_t (&out)[kParts]) {
+  constexpr float kUp = 1.f / kPartUnit;
+  const f16x2 h = pack2(x0, x1, scale);
+  x0 = __builtin_fmaf(x0, scale, -static_cast<float>(h[0]));  // exact
+  x1 = __builtin_fmaf(x1, scale, -static_cast<float>(h[1]));
+  out[0] = __builtin_bit_cast(uint32_t, h);
+  out[1] = __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(__builtin_fmaf(x0, kUp, 0.f)),
+                                              static_cast<_Float16>(__builtin_fmaf(x1, kUp, 0.f))});
+}
+// The parts' sums as one.
+__device__ inline f32x4 join(const f32x4 (&x)[kParts]) {
+  f32x4 s;
 #pragma unroll
-  for (int p = 1; p >= 0; --p)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(s[i], kPartUnit, x[p][i]);
+  for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(x[1][i], kPartUnit, x[0][i]);
   return s;
 }
 
 // Keys key0 + 32 wave, + 128, .. of an f16 plane on the f16 matrix pipe. Query rows (times a
 // power of two that puts the largest element into [2^14, 2^15)) and weights (in units of 2^-15)
-// are split into three f16 parts, each in a unit 2^-11 of the one before and with sums of its
-// own: all 24 bits down to 2^-28 of the row's largest, smaller ones to 2^-60. K comes from
+// are split into two f16 parts, the second in a unit 2^-11 of the first and with sums of its
+// own: within 2^-22 of themselves down to 2^-28 of the row's largest, smaller ones to 2^-51 of it,
+// next to v_exp_f32's 2^-23 and what f32 sums over a head's 64 columns round off. A third part
+// (all 24 bits) took 110 us instead of 96 at 64 rows x 65471 keys, 20 heads, and the outputs' error
+// was 2.6e-7 with either. K comes from
 // memory in operand layout, V passes through the wave's own swizzled LDS rows and is read
 // transposed; the packed weights are the B operand of O^T += V^T P^T as they stand.
 // o[rt][dt][e] is column 16 dt + 4 g + e. Returns whether a sum came out infinite or NaN: parts
@@ -329,7 +342,7 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
   st.clear();
   int j0 = b.key0 + kN * wave;
   if (j0 < b.key1) load(j0);
-  u32x4 qf[kRT][3][2];  // d = 16 g + 8 kk + 0..7
+  u32x4 qf[kRT][kParts][2];  // d = 16 g + 8 kk + 0..7
   float down[kRT];
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt) {
@@ -345,26 +358,26 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
     down[rt] = pow2(clamp_exp(-sh));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t w[3];
-      split2(qx[rt][i >> 1][2 * (i & 1)], qx[rt][i >> 1][2 * (i & 1) + 1], up, w);
+      uint32_t w[kParts];
+      split_units(qx[rt][i >> 1][2 * (i & 1)], qx[rt][i >> 1][2 * (i & 1) + 1], up, w);
 #pragma unroll
-      for (int p = 0; p < 3; ++p) qf[rt][p][i >> 2][i & 3] = w[p];
+      for (int p = 0; p < kParts; ++p) qf[rt][p][i >> 2][i & 3] = w[p];
     }
   }
   sight();
   for (; j0 < b.key1; j0 += kN * kWaves) {
-    u32x4 pf[kRT][3];
+    u32x4 pf[kRT][kParts];
     f32x4 s[kRT][2];
     float alpha[kRT];
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        f32x4 sp[3] = {};
+        f32x4 sp[kParts] = {};
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-          for (int p = 0; p < 3; ++p) sp[p] = mfma16(kx[t][kk], qf[rt][p][kk], sp[p]);
+          for (int p = 0; p < kParts; ++p) sp[p] = mfma16(kx[t][kk], qf[rt][p][kk], sp[p]);
         s[rt][t] = join(sp);
       }
     wave_sync();  // the last step's transposed reads are done
@@ -407,10 +420,10 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], down[rt], -md));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i + 1], down[rt], -md));
           ls += p0 + p1;
-          uint32_t w[3];
-          split2(p0, p1, kWeightUp, w);
+          uint32_t w[kParts];
+          split_units(p0, p1, kWeightUp, w);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) pf[rt][p][2 * t + (i >> 1)] = w[p];
+          for (int p = 0; p < kParts; ++p) pf[rt][p][2 * t + (i >> 1)] = w[p];
         }
       st.l[rt] = __builtin_fmaf(st.l[rt], alpha[rt], ls);
     }
@@ -427,9 +440,9 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
       for (int rt = 0; rt < kRT; ++rt) {
         // The step's sums join at once: kept apart over the steps they took 32 registers more a
         // tile, and as many multiplications by alpha.
-        f32x4 x[3];
+        f32x4 x[kParts];
 #pragma unroll
-        for (int p = 0; p < 3; ++p) x[p] = mfma16(va, pf[rt][p], f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int p = 0; p < kParts; ++p) x[p] = mfma16(va, pf[rt][p], f32x4{0.f, 0.f, 0.f, 0.f});
         const f32x4 y = join(x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) st.o[rt][dt][e] = __builtin_fmaf(st.o[rt][dt][e], alpha[rt], y[e]);
