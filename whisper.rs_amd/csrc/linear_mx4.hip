@@ -894,10 +894,11 @@ RowsShape rows_shape(const Mx4LinearArgs& a, int ct, int cols) {
     // pieces, 20.6 whole).
     many = tiles * ks > 256 * kRowsWaves;
     const size_t room = (many && ct == 1 ? 78 : 156) * 1024 - kRowsWaves * kStage;
-    fit = static_cast<int>((room - pad) / per) / ks * ks;
+    fit = static_cast<int>((room - pad) / per);
+    if (fit < groups) fit = fit / ks * ks;  // every wave has as many in a piece
     if (ks == 1 || (fit && tiles * ks <= 2048 && ks / 2 < groups)) break;
   }
-  RowsShape r{ks, std::min((groups + ks - 1) / ks * ks, std::max(ks, fit)), many, 0};
+  RowsShape r{ks, std::min(groups, std::max(ks, fit)), many, 0};
   r.lds = std::max<size_t>(sizeof(float) * 16 * kRowsWaves * (16 * ct + 1),
                            kRowsWaves * kStage + per * r.chunk + pad);
   return r;
@@ -921,7 +922,7 @@ hipError_t launch_rows(const Mx4LinearArgs& a, const RowsShape& r, DType out_dt,
 template <typename XT, int kCT>
 hipError_t launch_rows_ct(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   const RowsShape r = rows_shape(a, kCT, sizeof(XT) == 1 ? 0 : kParts<XT> * a.n_tokens);
-  const int groups = r.chunk / r.ks;
+  const int groups = (r.chunk + r.ks - 1) / r.ks;
   if (r.many) return launch_rows<XT, kCT, kCT == 1 ? 5 : 3, true>(a, r, out_dt, s);
   if (groups <= 1) return launch_rows<XT, kCT, 1, false>(a, r, out_dt, s);
   return launch_rows<XT, kCT, 3, false>(a, r, out_dt, s);
