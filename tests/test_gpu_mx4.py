@@ -476,3 +476,62 @@ def test_addresses_and_strides_that_are_refused(wrs, ctx):
         assert lib.wrs_linear_mx4(ctx.handle, 0, p, None, 512, 128, 1, ws, ss, None, 4, 128, 4,
                                   0, 0, o, n, 4, 64) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,n_in,n_out,groups,x_dtype", [
+    (5, 5120, 1280, 1, "f32"), (16, 5120, 1280, 1, "f32"), (7, 4096, 1031, 1, "f16"),
+    (16, 1600, 48, 3, "f32"), (13, 5056, 17, 5, "f32"), (16, 5120, 2048, 1, "bf16"),
+    (16, 65536, 16, 1, "f32"),
+])
+def test_long_rows_whose_columns_split(wrs, ctx, rows, n_in, n_out, groups, x_dtype):
+    """Few rows over few features and many columns; the splits are the same ones each time."""
+    note(f"linear_mx4 {rows} x {n_in} -> {n_out} x {groups} {x_dtype}, split")
+    run(wrs, ctx, x_dtype, rows, n_in, n_out, groups=groups, act="gelu", seed=8)
+    x = torch.randn((rows, n_in), device="cuda").to(DT[x_dtype])
+    ws = [wrs.mx4_quantize(torch.randn((n_out, n_in), device="cuda"), ctx=ctx)
+          for _ in range(groups)]
+    outs = [[torch.empty((rows, n_out), device="cuda") for _ in ws] for _ in range(4)]
+    for o in outs:
+        wrs.linear_mx4(x, ws, None, o, ctx=ctx)
+    torch.cuda.synchronize()
+    for o in outs[1:]:
+        for a, b in zip(outs[0], o):
+            assert torch.equal(a, b)
+
+
+def test_long_rows_captured_before_and_after_the_scratch(wrs):
+    """A context's first call, captured, finds no scratch and sums in one piece; the graphs
+    captured later split, and share scratch and counters with each other and eager calls."""
+    note("linear_mx4 5 x 5120 -> 128, captured before any eager call")
+    c = wrs.Context(0)
+    side = torch.cuda.Stream()
+    rng = np.random.default_rng(15)
+    with torch.cuda.stream(side):
+        c.use_torch_stream()
+        m, w = make(wrs, c, rng, 128, 5120)
+        x = torch.empty((5, 5120), device="cuda")
+        outs = [torch.empty((5, 128), device="cuda") for _ in range(3)]
+        eager = torch.empty((5, 128), device="cuda")
+        side.synchronize()
+        graphs = []
+        for i, o in enumerate(outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                wrs.linear_mx4(x, [m], None, [o], ctx=c)
+            graphs.append(g)
+            if i == 0:
+                wrs.linear_mx4(x, [m], None, [eager], ctx=c)
+                side.synchronize()
+        for _ in range(4):
+            x.copy_(torch.from_numpy(rng.standard_normal((5, 5120)).astype(np.float32)))
+            for o in outs:
+                o.fill_(float("nan"))
+            for g in graphs + graphs[1:]:
+                g.replay()
+            wrs.linear_mx4(x, [m], None, [eager], ctx=c)
+            side.synchronize()
+            y, tol = reference(x.double().cpu().numpy(), w, None, None, "f32")
+            assert np.all(np.abs(host(outs[0]).astype(np.float64) - y) <= tol)
+            assert torch.equal(outs[1], eager) and torch.equal(outs[2], eager)
+            assert np.all(np.abs(host(eager).astype(np.float64) - y) <= tol)
+    c.close()

@@ -63,6 +63,8 @@ constexpr uint32_t kPast = 0xFFFF0000u;  // an offset past every buffer
 constexpr uint32_t kPastRows = 0x80000000u;  // so with offsets of rows (below 2^28) added
 
 constexpr int kRowsWaves = 8;
+constexpr int kMx4MaxSplits = 8;
+constexpr int kMx4CounterStride = 32;  // words between counters: a 128-byte line
 constexpr int kGroup = 8;       // blocks of a row that a wave takes at a time: 128 bytes of codes
 constexpr int kCodeBytes = 16 * kGroup * 16;            // of a tile's group
 constexpr int kStage = kCodeBytes + 16 * kGroup + 128;  // LDS of a wave: codes, scales, pad
@@ -79,6 +81,7 @@ template <typename XT, int kCT, int kBatch, bool kMany>
 __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4LinearArgs a, int ks,
                                                                            int chunk,
                                                                            uint32_t wide_inv,
+                                                                           int per_split,
                                                                            int out_dt) {
   constexpr bool kBoth = sizeof(XT) == 1;  // x is MXFP4 too
   constexpr int kP = kBoth ? 1 : kParts<XT>;
@@ -128,8 +131,9 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
 
   u32x4 cw[kBatch][2];
   uint16_t sw[kBatch];
-  for (int g0 = 0; kGroup * g0 < nb; g0 += chunk) {
-    const int nbc = min(kGroup * chunk, nb - kGroup * g0);  // blocks of the chunk
+  const int first_g = blockIdx.z * per_split, nb1 = min(nb, kGroup * (first_g + per_split));
+  for (int g0 = first_g; kGroup * g0 < nb1; g0 += chunk) {
+    const int nbc = min(kGroup * chunk, nb1 - kGroup * g0);  // blocks of the chunk
     const int n = ((nbc + kGroup - 1) / kGroup - kw + ks - 1) / ks;  // this wave's groups
     auto load = [&](int u, int i) __attribute__((always_inline)) {
       int b = kGroup * (g0 + kw + ks * i);  // the group's first block
@@ -147,7 +151,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
       // Codes of block b, row t at (16 b + t) * 16, scales behind them.
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) load(u, u);
-      if (g0) __syncthreads();
+      if (g0 != first_g) __syncthreads();
       for (int e = tid; e < 16 * kGroup * chunk; e += 64 * kRowsWaves) {
         const int b = e >> 4, t = e & 15, at_b = kGroup * g0 + b;
         u32x4 v = {0, 0, 0, 0};
@@ -180,7 +184,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
       load_x(0);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) load(u, u);
-      if (g0) __syncthreads();
+      if (g0 != first_g) __syncthreads();
       for (int e0 = 0; e0 < groups; e0 += 64 * kRowsWaves * kXBatch) {
         if (e0) load_x(e0);
 #pragma unroll
@@ -262,14 +266,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
     for (int e = 0; e < 4; ++e)
       red[(16 * wave + 4 * g + e) * kPitch + 16 * i + c] = acc[0][i][e] + acc[1][i][e];
   __syncthreads();
-  for (int e = tid; e < 16 * tiles * a.n_tokens; e += 64 * kRowsWaves) {
-    const int t = e / (16 * tiles), rr = e % (16 * tiles), r = first + rr;
-    if (r >= a.n_out) continue;
-    float y = 0.f;
-#pragma unroll
-    for (int p = kP - 1; p >= 0; --p)
-      for (int k = 0; k < ks; ++k)
-        y += red[(16 * ((rr >> 4) * ks + k) + (rr & 15)) * kPitch + p * a.n_tokens + t];
+  auto store = [&](int t, int r, float y) __attribute__((always_inline)) {
     if (a.bias[grp]) y += a.bias[grp][r];
     if (a.act == kActGelu) y = gelu_tanh(y);
     const int64_t o = t * a.out_rs + (r >> 6) * a.out_hs + (r & 63);
@@ -279,7 +276,44 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
       static_cast<_Float16*>(a.out[grp])[o] = static_cast<_Float16>(y);
     else
       static_cast<__bf16*>(a.out[grp])[o] = static_cast<__bf16>(y);
+  };
+  const int splits = gridDim.z, n_e = 16 * tiles * a.n_tokens;
+  const int unit = grp * gridDim.x + blockIdx.x;
+  float* const part = splits > 1 ? a.part + static_cast<int64_t>(unit) * splits * n_e : nullptr;
+  for (int e = tid; e < n_e; e += 64 * kRowsWaves) {
+    const int t = e / (16 * tiles), rr = e % (16 * tiles), r = first + rr;
+    if (r >= a.n_out) continue;
+    float y = 0.f;
+#pragma unroll
+    for (int p = kP - 1; p >= 0; --p)
+      for (int k = 0; k < ks; ++k)
+        y += red[(16 * ((rr >> 4) * ks + k) + (rr & 15)) * kPitch + p * a.n_tokens + t];
+    if (splits == 1)
+      store(t, r, y);
+    else
+      st_agent(part + blockIdx.z * n_e + e, y);
   }
+  if (splits == 1) return;
+  // The workgroup that counts in last adds the splits in their order and re-arms the counter.
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  unsigned* const counter = a.counters + unit * kMx4CounterStride;
+  if (tid == 0)
+    *reinterpret_cast<unsigned*>(lds) =
+        __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (*reinterpret_cast<const unsigned*>(lds) != static_cast<unsigned>(splits - 1)) return;
+  for (int e = tid; e < n_e; e += 64 * kRowsWaves) {
+    const int t = e / (16 * tiles), r = first + e % (16 * tiles);
+    if (r >= a.n_out) continue;
+    float x[kMx4MaxSplits], y = 0.f;
+#pragma unroll
+    for (int s = 0; s < kMx4MaxSplits; ++s) x[s] = s < splits ? ld_agent(part + s * n_e + e) : 0.f;
+#pragma unroll
+    for (int s = 0; s < kMx4MaxSplits; ++s) y += x[s];
+    store(t, r, y);
+  }
+  if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -876,14 +910,28 @@ hipError_t allow_lds(F fn, size_t bytes, std::atomic<uint64_t>& set) {
   return e;
 }
 
+// Long rows of x over few features: a workgroup stages all of x for 16 features, so what bounds
+// the call is that work on a part of the CUs, and its columns split over workgroups. The sums'
+// way through memory costs 1.2 us, which staged columns x groups of `kSplitWork` make up for
+// (us, split / not, 5120 -> 1280: 5 rows f32, 300: 7.3 / 9.9; 16 rows, 960: 8.7 / 16.3; 2 rows,
+// 120: 7.1 / 6.4; 2048 -> 512, 8 rows f32, 192: 6.9 / 5.7; 16, 384: 8.0 / 8.6). Splits of fewer
+// groups are faster down to 3 (16 rows 4096 -> 1024: 8.9 us, of 5 10.7, of 8 10.7).
+constexpr int kSplitLeast = 3, kSplitWork = 200;
+bool rows_split(const Mx4LinearArgs& a, int cols) {
+  const int groups = (a.n_in / kMx4Block + kGroup - 1) / kGroup;
+  return cols * groups >= kSplitWork && groups >= 2 * kSplitLeast &&
+         (a.n_out + 15ll) / 16 * a.n_groups <= 128;
+}
+
 // Few rows: the waves that share a tile, and the groups staged at a time.
 struct RowsShape {
   int ks, chunk;
   bool many;  // more than one workgroup per CU
+  int splits, per_split;  // workgroups that share a row's groups, groups of each
   size_t lds;
 };
 RowsShape rows_shape(const Mx4LinearArgs& a, int ct, int cols) {
-  const int groups = (a.n_in / kMx4Block + kGroup - 1) / kGroup;
+  int groups = (a.n_in / kMx4Block + kGroup - 1) / kGroup;
   const int64_t tiles = (a.n_out + 15ll) / 16 * a.n_groups;
   const size_t pad = 16 * cols, per = cols ? 2 * kMx4Block * kGroup * cols : 17 * 16 * kGroup;
   int ks = kRowsWaves, fit = 0;
@@ -898,7 +946,23 @@ RowsShape rows_shape(const Mx4LinearArgs& a, int ct, int cols) {
     if (fit < groups) fit = fit / ks * ks;  // every wave has as many in a piece
     if (ks == 1 || (fit && tiles * ks <= 2048 && ks / 2 < groups)) break;
   }
-  RowsShape r{ks, std::min(groups, std::max(ks, fit)), many, 0};
+  const int wide = 16 * (kRowsWaves / ks);
+  const int64_t units = (a.n_out + wide - 1ll) / wide * a.n_groups;
+  int splits = 1;
+  if (a.part && rows_split(a, cols))
+    splits = static_cast<int>(std::min<int64_t>(
+        {256 / units, groups / kSplitLeast, kMx4MaxSplits,
+         static_cast<int64_t>(a.part_floats) / (units * wide * a.n_tokens),
+         static_cast<int64_t>(a.counter_words) / kMx4CounterStride >= units ? kMx4MaxSplits : 1}));
+  splits = std::max(splits, 1);
+  const int per_split = (groups + splits - 1) / splits;
+  splits = (groups + per_split - 1) / per_split;
+  if (splits > 1) {
+    groups = per_split;
+    fit = static_cast<int>((156 * 1024 - kRowsWaves * kStage - pad) / per);
+    if (fit < groups) fit = fit / ks * ks;
+  }
+  RowsShape r{ks, std::min(groups, std::max(ks, fit)), many, splits, per_split, 0};
   r.lds = std::max<size_t>(sizeof(float) * 16 * kRowsWaves * (16 * ct + 1),
                            kRowsWaves * kStage + per * r.chunk + pad);
   return r;
@@ -912,10 +976,10 @@ hipError_t launch_rows(const Mx4LinearArgs& a, const RowsShape& r, DType out_dt,
   const hipError_t e = allow_lds(&mx4_rows<XT, kCT, kBatch, kMany>, kMost, set);
   if (e != hipSuccess) return e;
   const int wide = 16 * (kRowsWaves / r.ks);
-  const dim3 grid((a.n_out + wide - 1) / wide, a.n_groups);
+  const dim3 grid((a.n_out + wide - 1) / wide, a.n_groups, r.splits);
   const uint32_t inv = static_cast<uint32_t>((1ull << 32) / (4 * kGroup * r.chunk) + 1);
   hipLaunchKernelGGL((mx4_rows<XT, kCT, kBatch, kMany>), grid, dim3(64 * kRowsWaves), r.lds, s, a, r.ks,
-                     r.chunk, inv, static_cast<int>(out_dt));
+                     r.chunk, inv, r.per_split, static_cast<int>(out_dt));
   return hipGetLastError();
 }
 
@@ -989,6 +1053,12 @@ hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
 }
 
 }  // namespace
+
+bool linear_mx4_splits(const Mx4LinearArgs& a, DType x_dt) {
+  if (a.n_tokens > kMx4Rows || a.x_scales) return false;
+  const int parts = x_dt == kF32 ? kParts<float> : x_dt == kF16 ? kParts<_Float16> : 1;
+  return rows_split(a, parts * a.n_tokens);
+}
 
 hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s) {
   if (a.n_tokens <= 0 || a.n_out <= 0 || a.n_groups <= 0) return hipSuccess;

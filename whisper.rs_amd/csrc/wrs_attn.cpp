@@ -2247,6 +2247,16 @@ int wrs_linear_mx4(wrs_attn_ctx* c, int x_dtype, const void* x, const void* x_sc
   a.out_hs = out_head_stride;
   a.act = activation == WRS_ACT_GELU ? wrs::kActGelu : wrs::kActNone;
   DeviceGuard g(c->device);
+  if (wrs::linear_mx4_splits(a, both ? wrs::kF32 : static_cast<wrs::DType>(x_dtype))) {
+    const int rc = linear_scratch(c);
+    if (rc) return rc;
+    if (c->lin_counters) {  // captured before any scratch: no split
+      a.part = c->lin_part;
+      a.part_floats = c->lin_part_bytes / sizeof(float);
+      a.counters = c->lin_counters;
+      a.counter_words = c->lin_counter_bytes / sizeof(unsigned);
+    }
+  }
   WRS_HIP(c, wrs::launch_linear_mx4(a, both ? wrs::kF32 : static_cast<wrs::DType>(x_dtype),
                                     static_cast<wrs::DType>(out_dtype), c->stream));
   return WRS_OK;

@@ -324,7 +324,14 @@ struct Mx4LinearArgs {
   const uint8_t* w_scales[kMx4Groups];
   const float* bias[kMx4Groups];  // nullable entries
   void* out[kMx4Groups];
+  // Few rows over long ones: room for partial sums, and zeroed counters (nullptr: no split).
+  float* part;
+  size_t part_floats;
+  unsigned* counters;
+  size_t counter_words;
 };
+// Few rows that split over workgroups where they find scratch.
+bool linear_mx4_splits(const Mx4LinearArgs& a, DType x_dt);
 hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s);
 
 // Projections with f16 weights (quant.rs:415-473 semantics):
