@@ -1,8 +1,7 @@
-// Projections with MXFP4 weights.
-//
-// K15 (linear_mx4_tile): out[g](t, r) = act(w[g][r] . x[t] + bias[g][r]), sums in f32. A
-//   workgroup takes 64 rows by 64 features; x and the weights, as the f32 values they
-//   stand for, pass through LDS 32 columns (one scale block) at a time.
+// Projections with MXFP4 weights: out[g](t, r) = act(w[g][r] . x[t] + bias[g][r]), sums in f32.
+// Weights keep their 4 bits up to the MFMA: widened to 16-bit operands in registers, exactly, or
+// with MXFP4 x taken as they are by the scaled MFMAs. Up to 16 rows of x stream the weights
+// (K15), more go by tiles (K16).
 #include "wrs_internal.hpp"
 
 #include <algorithm>
@@ -74,7 +73,11 @@ constexpr int kStage = kCodeBytes + 16 * kGroup + 128;  // LDS of a wave: codes,
 //   at a time for a workgroup. Codes come in whole 128-byte pieces of rows (a lane's operand is
 //   16 bytes of its own row: loaded so, with a byte of scale each, 36 MB took 15.4 us, in
 //   whole pieces and without scales 9.9), wait in registers, and change places in the wave's
-//   own LDS. x is staged in LDS once for the workgroup.
+//   own LDS. x is staged in LDS once for the workgroup, f32 in three bf16 parts (every bit of
+//   it), f16 in two, each with an MFMA column of its own.
+//   5 rows f32 1280 -> 51866 11.8 us, 3.0 TB/s of weights (read alone, the same bytes take 7.9; the
+//   rest is x's way in and the last tiles' sums; f16 weights, K7m, 29); 1280 -> 5120 6.1; 5120 ->
+//   1280 7.3; 3 x 1280 -> 1280 5.1.
 // kMany: grids of more than one workgroup per CU keep their registers to what two need;
 // others have x in flight at once (5 rows 5120 -> 1280: 11.3 us with 2 groups a thread).
 template <typename XT, int kCT, int kBatch, bool kMany>
@@ -854,6 +857,11 @@ constexpr int kPanel = 8;
 //   weights of scales 2^-23 to 2^13 exactly, and rows of f32 x whose largest value is of
 //   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
 //   one of x's two or three parts after the other.
+//   24000 x 5120 -> 1280: f16 302 us, 1040 TFLOP/s (zeros in its place 233: the card's power bounds
+//   it; the library's product of f16 weights 274), bf16 280, f32 693, MXFP4 108, 2.9 PFLOP/s
+//   (zeros a quarter less); 1280 -> 5120 MXFP4 with GELU 156, of which the epilogue's 123 M
+//   outputs are about 60. 130 rows f32, 3 x 1280 -> 1280 13.7 us: ten steps of x's way through
+//   LDS in two parts on one workgroup a CU (f16 10.0, MXFP4 7.6).
 template <typename T, typename XT, typename OT, bool kWords>
 __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];

@@ -8,7 +8,9 @@
 //   2^-127. Four lanes take a block, 8 values each; the largest magnitude is the largest
 //   bit pattern, so the block's maximum needs no floating point and keeps NaN on top.
 // K14 (mx4_dequantize): the values that codes and scales stand for, rounded once to the
-//   output type. Both are bound by memory: one pass, 16-byte accesses.
+//   output type. Both are bound by memory: one pass, 16-byte accesses, four of them in flight a
+//   lane (with one, and codes made by comparisons, 49.7 and 44.0 us). 51866 x 1280 f16 29.4 us
+//   and 25.3 us, 5.7 and 6.6 TB/s; 24000 x 1280 13.0; 1500 x 1280 f32 2.9 and 3.9.
 #include "wrs_internal.hpp"
 
 #include <algorithm>

@@ -6,13 +6,17 @@
 //   over those j only. parents[i] in [0, i) is the row's parent; anything else
 //   makes it a child of the last cached token, so any parents end every walk.
 //   A workgroup of four waves runs one block of 16 kRT rows of one head over one
-//   chunk of the keys; wave w takes the chunk's 16-key steps w, w + 4, ... with an
-//   online softmax of its own, the waves merge their (max, sum, O) in LDS, and the
-//   chunks of a block merge through memory (the last workgroup to count in adds
-//   the partials up in chunk order, so results do not depend on which it is).
+//   chunk of the keys; wave w takes the chunk's steps w, w + 4, ... (of 16 f32 keys or
+//   32 f16 ones) with an online softmax of its own, the waves merge their (max, sum, O)
+//   in LDS, and the chunks of a block merge through memory (the last workgroup to count
+//   in adds the partials up in chunk order, so results do not depend on which it is).
 //   Only the steps that reach past the cache test the ancestor bits.
 //   f16 planes run on the f16 matrix pipe with operands in two parts, f32 ones on the
 //   f32 matrix pipe.
+//   Short caches are bound by latency: 8 nodes over 60 keys, 6 heads 5.0 us, five trees of up to
+//   26 over 223, 20 heads 6.5, four of 13 over 430, 12 heads f32 8.2 (smallest launch 2.3). Long ones by the matrix
+//   pipe and the softmax's arithmetic beside it: 64 nodes x 20 heads over 65471 f16 keys 95 us,
+//   3.5 TB/s of K and V (floor 66), 16 nodes 73 us, 4.6 TB/s.
 #include "split16.hpp"
 
 #include <algorithm>
@@ -665,11 +669,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void tree_attend(TreeArgs a) {
 }
 
 // Rows of a block: 16, so that a tree's blocks run on CUs of their own, or 32, which read a cache
-// half as often, where three blocks or more would read one past what the caches hold. us, 16 / 32
-// rows, 20 heads: 26 nodes over 223 keys 6.4/8.5, 64 over 1500 12.9/15.3, 32 over 8000 (41 MB)
-// 20.8/32.2, 64 over 20000 (102 MB) 53.1/54.6, 32 over 40000 (205 MB) 59.2/65.4, 64 over 40000
-// 89.2/84.1, 64 over 65471 (335 MB) 138/122.
-constexpr int64_t kWideBytes = 128ll << 20;
+// half as often, where an even number of three blocks or more would read one past what the caches
+// hold (the f32 matrix pipe, slower, later). us, 16 / 32 rows, 20 heads: f16 26 nodes over 223 keys
+// 6.3/8.1, 64 over 1500 11.6/16.6, 32 over 8000 (41 MB) 19.5/29.9, 64 over 20000 (102 MB)
+// 47.9/45.9, 32 over 40000 (205 MB) 58.6/64.8, 48 over 40000 70.1/68.8, 64 over 40000 85.0/70.3, 64
+// over 65471 (335 MB) 132/99; f32 64 over 20000 (205 MB) 101/102, 8 trees of 64 over 4000 (333 MB)
+// 162/185, 48 over 40000 146/171, 64 over 40000 (410 MB) 183/172.
 int block_rows(const TreeArgs& a, DType dt) {
   int most = 0;
   int64_t bytes = 0;
@@ -677,7 +682,8 @@ int block_rows(const TreeArgs& a, DType dt) {
     most = std::max(most, a.nodes[t]);
     bytes += static_cast<int64_t>(a.past[t] + a.nodes[t]) * a.n_heads * 64 * 2 * (dt == kF16 ? 2 : 4);
   }
-  return most > 32 && bytes >= kWideBytes ? kTreeMaxRows : 16;
+  const int64_t wide = (dt == kF16 ? 128ll : 384ll) << 20;
+  return most > 32 && (most + 15) / 16 % 2 == 0 && bytes >= wide ? kTreeMaxRows : 16;
 }
 
 }  // namespace
