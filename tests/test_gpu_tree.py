@@ -555,3 +555,23 @@ def test_verification_step_equals_decoding_the_path(wrs, ctx):
     assert np.abs(drafted[path] - np.concatenate(singles)).max() <= bar
     assert np.abs(last[0] - last[1]).max() <= bar
     ar.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("octaves", [14, 20, 26])
+def test_weights_far_below_the_largest(wrs, ctx, dtype, octaves):
+    """One key takes nearly all of the softmax and its value is 0: the outputs are what the
+    weights 2^-octaves of the largest carry."""
+    note(f"tree_self with weights 2^-{octaves} of the largest, {dtype}")
+    dt = getattr(wrs, "WRS_" + dtype.upper())
+    t = Trees(wrs, ctx, dt, 2, [300], [20], "tree", 43)
+    t.q *= 0.25
+    t.q.reshape(20, 2, 64)[:, :, 7] = 8 * octaves * np.log(2)
+    k, v = t.k[0].reshape(-1, 2, 64), t.v[0].reshape(-1, 2, 64)
+    k[:, :, 7], k[77, :, 7] = 0, 1
+    v[77] = 0
+    t.arena.set_len(0, 0)
+    t.arena.append(1, 0, dev(t.k[0]), dev(t.v[0]))
+    t.arena.advance(0, 300)
+    t.check(host(t.run()))
+    t.arena.close()
