@@ -237,7 +237,8 @@ int wrs_kv_advance(wrs_kv *kv, size_t slot, size_t n);
  * Rows behind the kept ones are undefined afterwards; slot lengths are left, so
  * that wrs_kv_advance takes the path in. n_rows is the sum of counts; a row lies
  * within max_ctx and at most 65535 past the length. Every argument is checked
- * before any row moves. No reference counterpart: the reference's cache keeps one
+ * before any row moves; a replayed graph makes the same moves. No reference
+ * counterpart: the reference's cache keeps one
  * candidate per slot. */
 int wrs_kv_keep_rows(wrs_kv *kv, const size_t *slots, const size_t *counts, size_t n_slots,
                      const size_t *rows, size_t n_rows);
@@ -308,7 +309,10 @@ int wrs_attn_prefill_cross(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const fl
  * lie q_row_stride and out_row_stride elements apart, so that q may lie in wider
  * rows. Values of rows that a row does not see never reach it, infinities and NaN
  * among them; a row whose visible scores are all -infinity is zero, and one with
- * a NaN among them NaN. Any arena, up to 2^24 - 4096 keys. No reference counterpart:
+ * a NaN among them NaN. Any arena, up to 2^24 - 4096 keys; f16 arenas take q and the
+ * weights in two f16 parts (2^-22 down to 2^-28 of the row's largest), f32 ones whole.
+ * Slots, counts and lengths are read when the call is made: a replayed graph keeps
+ * them. No reference counterpart:
  * the reference decodes one token per beam and step. */
 int wrs_attn_tree_self(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const size_t *slots,
                        const size_t *n_nodes, size_t n_trees, const void *parents,
