@@ -535,3 +535,22 @@ def test_long_rows_captured_before_and_after_the_scratch(wrs):
             assert torch.equal(outs[1], eager) and torch.equal(outs[2], eager)
             assert np.all(np.abs(host(eager).astype(np.float64) - y) <= tol)
     c.close()
+
+
+def test_new_rows_for_a_context_on_another_stream(wrs):
+    """A new Mx4's memory may still be written by torch's stream when it is allocated."""
+    note("mx4_quantize into new rows, the context on its own stream")
+    c = wrs.Context(0)
+    x = torch.randn((4096, 4096), device="cuda")
+    want = wrs.Mx4.empty(4096, 4096)
+    torch.cuda.synchronize()
+    wrs.mx4_quantize(x, want, ctx=c)
+    torch.cuda.synchronize()
+    before = torch.empty((4096, 2048), dtype=torch.uint8, device="cuda")
+    for i in range(300):
+        before.fill_(i % 7)
+    del before
+    got = wrs.mx4_quantize(x, ctx=c)
+    torch.cuda.synchronize()
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    c.close()

@@ -56,6 +56,7 @@ class Context:
                                f"{_L.status_string(rc)}")
         self.handle = h
         self.device = int(device)
+        self._stream = None  # the adopted stream's handle (0: the null stream), or its own
 
     def close(self) -> None:
         if getattr(self, "handle", None):
@@ -81,6 +82,7 @@ class Context:
         """Queue work on a hipStream_t handle; 0/None is the null stream."""
         self.check(self._lib.wrs_attn_set_stream(self.handle, stream_handle or None),
                    "wrs_attn_set_stream")
+        self._stream = stream_handle or 0
 
     def use_torch_stream(self) -> None:
         """Queue work on torch's current stream of this device."""
@@ -363,11 +365,17 @@ class Mx4:
 def mx4_quantize(x, out=None, ctx=None):
     """Rows of a float32, float16 or bfloat16 CUDA tensor as MXFP4 (into ``out``, or a
     new :class:`Mx4`): scales 2^(floor(log2(largest of 32)) - 2), nearest codes, ties
-    to the even one (``wrs_mx4_quantize``). Asynchronous on ctx's stream."""
+    to the even one (``wrs_mx4_quantize``). Asynchronous on ctx's stream; a new Mx4 comes
+    from torch's current stream, whose work is waited for if ctx is on another."""
     ctx = ctx or default_context()
     n, d, rs = _rows(x, "mx4_quantize")
     if out is None:
         out = Mx4.empty(n, d, device=x.device)
+        if x.is_cuda:
+            import torch
+            current = torch.cuda.current_stream(x.device)
+            if current.cuda_stream != ctx._stream:
+                current.synchronize()  # its memory may still be in use there
     assert out.shape == (n, d)
     _on_device(ctx, "mx4_quantize", x, out.codes)
     ctx.check(ctx._lib.wrs_mx4_quantize(ctx.handle, _dtype_code(x), x.data_ptr(), _span(x), rs, n,
