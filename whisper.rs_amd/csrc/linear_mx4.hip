@@ -454,19 +454,26 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   for (int i = 0; i < kXn; ++i) most[i] = 0.f;
   // Pair i of the group, of two stages, is pair i * KG + kg of the tile.
   const int pairs = (stages + 1) / 2;
-  auto load_w = [&](int i_p) __attribute__((always_inline)) {
+  // Loads of stage i_s of x and pair i_p of W: number k of kXn + kWn + kF.
+  constexpr int kLoads = kXn + kWn + kF;
+  auto load = [&](int k, int i_s, int i_p) __attribute__((always_inline)) {
+    if (k < kXn) {
+      const int at = kK * min(2 * ((i_s >> 1) * T::KG + kg) + (i_s & 1), stages - 1);
+      xv[k] = *reinterpret_cast<const x8*>(xp[k] + at);
+      return;
+    }
     int p = i_p * T::KG + kg;
     asm("" : "+s"(p));  // offsets are formed per pair, not kept per load
-    const int at = 4 * p + (lane & 3);
-    const uint32_t o = at < nb ? (wf + (lane >> 2)) * bytes + 16 * at : kPastRows;
-#pragma unroll
-    for (int i = 0; i < kWn; ++i)
+    if (k < kXn + kWn) {
+      const int i = k - kXn, at = 4 * p + (lane & 3);
+      const uint32_t o = at < nb ? (wf + (lane >> 2)) * bytes + 16 * at : kPastRows;
       cw[i] = __builtin_bit_cast(
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, o + i * 16 * bytes, 0, 0));
-#pragma unroll
-    for (int i = 0; i < kF; ++i)
+    } else {
+      const int i = k - kXn - kWn;
       sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + 4 * p, p < pairs,
                                        4 * p + 2 < nb);
+    }
   };
   auto put_w = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -474,11 +481,6 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
       *reinterpret_cast<u32x4*>(codes + code_at((lane >> 2) + 16 * i, lane & 3)) = cw[i];
 #pragma unroll
     for (int i = 0; i < kF; ++i) sw[i] = sw_next[i];
-  };
-  auto load_x = [&](int i_s) __attribute__((always_inline)) {
-    const int at = kK * min(2 * ((i_s >> 1) * T::KG + kg) + (i_s & 1), stages - 1);
-#pragma unroll
-    for (int i = 0; i < kXn; ++i) xv[i] = *reinterpret_cast<const x8*>(xp[i] + at);
   };
   auto store_x = [&](char* buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -524,7 +526,10 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     }
   };
   bool odd = false;
-  auto multiply = [&](int d, const char* buf) __attribute__((always_inline)) {
+  // Stage d of a pair: operands of step j + 1 are formed behind the products that use their
+  // registers last, and the first `n` loads of stage i_s and pair i_p go between them.
+  auto multiply = [&](int d, const char* buf, auto n, int i_s, int i_p)
+      __attribute__((always_inline)) {
     float scale[kF];
     u32x4 c[kF];
 #pragma unroll
@@ -536,56 +541,66 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
       scale[i] = scale_of(byte);
       c[i] = *reinterpret_cast<const u32x4*>(codes + code_at(32 * i + r32, 2 * d + hl));
     }
+    u32x4 wv[2][kF], xw[P][kT];
+    auto widen = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < kK / 16; ++j) {
-      u32x4 wv[kF], xw[P][kT];
+      for (int i = 0; i < kF; ++i) wv[j & 1][i] = widen8_as<E>(c[i][j], scale[i]);
+    };
+    auto read_x = [&](int j, int t) __attribute__((always_inline)) {
 #pragma unroll
       for (int p = 0; p < P; ++p)
+        xw[p][t] = *reinterpret_cast<const u32x4*>(buf + p * kXBytes +
+                                                   chunk_at(wt + 32 * t + r32, 4 * hl + j));
+    };
+    constexpr int kSteps = kK / 16, kSlots = kSteps * kT, kNow = decltype(n)::value;
 #pragma unroll
-        for (int i = 0; i < kT; ++i)
-          xw[p][i] = *reinterpret_cast<const u32x4*>(buf + p * kXBytes +
-                                                     chunk_at(wt + 32 * i + r32, 4 * hl + j));
+    for (int t = 0; t < kT; ++t) read_x(0, t);
+    widen(0);
 #pragma unroll
-      for (int i = 0; i < kF; ++i) wv[i] = widen8_as<E>(c[i][j], scale[i]);
+    for (int j = 0; j < kSteps; ++j)
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p)
+      for (int t = 0; t < kT; ++t) {
 #pragma unroll
-        for (int t = 0; t < kT; ++t)
+        for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-          for (int i = 0; i < kF; ++i) acc[i][t] = mfma32<E>(wv[i], xw[p][t], acc[i][t]);
-    }
+          for (int i = 0; i < kF; ++i) acc[i][t] = mfma32<E>(wv[j & 1][i], xw[p][t], acc[i][t]);
+        if (j + 1 < kSteps) {
+          if (t == 0) widen(j + 1);
+          read_x(j + 1, t);
+        }
+#pragma unroll
+        for (int k = 0; k < kNow; ++k)
+          if (k * kSlots / (kNow ? kNow : 1) == j * kT + t) load(k, i_s, i_p);
+        __builtin_amdgcn_sched_barrier(0);
+      }
   };
 
-  load_x(0);
-  load_w(0);
+#pragma unroll
+  for (int k = 0; k < kLoads; ++k) load(k, 0, 0);
   store_x(lds);
-  load_x(1);
+#pragma unroll
+  for (int k = 0; k < kXn; ++k) load(k, 1, 0);
   __syncthreads();
   const int turns = (pairs + T::KG - 1) / T::KG;  // of every group; the last one's may be empty
   int i_p = 0;
   // No branch in this loop: one around the products costs copies of the sums (64 moves per two
   // stages of a 64 x 128 wave).
   for (; i_p + 1 < turns; ++i_p) {
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      store_x(lds + (1 - d) * kStageBytes);
-      load_x(2 * i_p + d + 2);
-      if (d == 0) {
-        put_w();
-        load_w(i_p + 1);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // or the loads sink below the products
-      multiply(d, lds + d * kStageBytes);
-      __syncthreads();
-    }
+    store_x(lds + kStageBytes);
+    put_w();
+    multiply(0, lds, std::integral_constant<int, kLoads>{}, 2 * i_p + 2, i_p + 1);
+    __syncthreads();
+    store_x(lds);
+    multiply(1, lds + kStageBytes, std::integral_constant<int, kXn>{}, 2 * i_p + 3, 0);
+    __syncthreads();
   }
   // The second stage, stored here already, is a repeated one where there is none.
   store_x(lds + kStageBytes);
   put_w();
   const int last = 2 * (i_p * T::KG + kg);
-  if (last < stages) multiply(0, lds);
+  if (last < stages) multiply(0, lds, std::integral_constant<int, 0>{}, 0, 0);
   __syncthreads();
-  if (last + 1 < stages) multiply(1, lds + kStageBytes);
+  if (last + 1 < stages) multiply(1, lds + kStageBytes, std::integral_constant<int, 0>{}, 0, 0);
   if constexpr (kHalves) {
     // 8 neighbouring lanes staged a row. Rows past the last one repeat it.
 #pragma unroll
