@@ -1095,16 +1095,15 @@ template <typename XT, typename OT>
 hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   // The largest tile that fills the chip: larger ones read x and W less often, but a CU without
   // a workgroup does nothing. Both sides of each step by workgroups, us:
-  //   Large, 180 (f32, 1500 rows, 3 x 1280 -> 1280): 46.9, Wide 51.5; 120 (f32, 3000 rows 5120 ->
-  //   1280): 145, Wide 121.
-  //   Wide, 144 (f32, 1500 rows 384 -> 1536): 15.0, Mid 17.8; 120 (f32, 1500 rows 1280 -> 1280):
-  //   32.8, Mid 24.2.
-  //   Mid, 180 (MXFP4, 130 rows, 3 x 1280 -> 1280): 7.6, Small 8.4; 60 (40 rows): 7.0, Small 6.5.
+  //   Large, 180 (f32, 1500 rows, 3 x 1280 -> 1280): 46.6, Wide 49.3; 120 (f32, 3000 rows 5120 ->
+  //   1280): 138, Wide 109.
+  //   Wide, 144 (f32, 1500 rows 384 -> 1536): 14.4, Mid 16.1; 120 (f32, 1500 rows 1280 -> 1280):
+  //   29.4, Mid 21.7.
+  //   Mid, 180 (MXFP4, 130 rows, 3 x 1280 -> 1280): 7.4, Small 8.0; 60 (40 rows): 6.7, Small 6.1.
   using Small = Tile<64, 32, 32, 32, 4>;
   using Mid = Tile<64, 64, 32, 32, 2>;
   using Wide = Tile<128, 128, 64, 64, 1>;
-  using Large = std::conditional_t<sizeof(XT) <= 2, Tile<256, 128, 64, 128, 1>,
-                                   Tile<256, 128, 64, 64, 1>>;
+  using Large = Tile<256, 128, 64, 128, 1>;
   auto fills = [&](int f, int t, int least) {
     return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups >=
            least;
