@@ -873,7 +873,8 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
           const f32x4 y1 = *reinterpret_cast<const f32x4*>(mine + (j + lr) * kOutPitch + lf + 4);
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = __builtin_fmaf(e < 4 ? y0[e & 3] : y1[e & 3], down, b[e]);
+          for (int e = 0; e < 8; ++e)
+            y[e] = __builtin_fmaf(e < 4 ? y0[e & 3] : y1[e & 3], down, b[e]);
           if (act == kActGelu) {
             asm volatile("");  // a branch, not both ways and a choice for each value
 #pragma unroll
@@ -912,13 +913,14 @@ constexpr int kPanel = 8;
 //   weights of scales 2^-23 to 2^13 exactly, and rows of f32 x whose largest value is of
 //   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
 //   one of x's two or three parts after the other.
-//   24000 x 5120 -> 1280: f16 302 us, 1040 TFLOP/s (zeros in its place 233: the card's power bounds
-//   it; the library's product of f16 weights 274), bf16 280, f32 693, MXFP4 108, 2.9 PFLOP/s
-//   (zeros a quarter less); 1280 -> 5120 MXFP4 with GELU 156, of which the epilogue's 123 M
-//   outputs are about 60. 130 rows f32, 3 x 1280 -> 1280 13.7 us: ten steps of x's way through
-//   LDS in two parts on one workgroup a CU (f16 10.0, MXFP4 7.6).
+//   24000 x 5120 -> 1280: f16 291 us, 1080 TFLOP/s, the matrix pipe 57% busy and the card's power
+//   the bound (the library's product of f16 weights 274), bf16 265, f32 586, MXFP4 101, 3.1
+//   PFLOP/s (zeros in its place a quarter less); 1280 -> 5120 MXFP4 with GELU 127, of which the
+//   epilogue's 123 M outputs are about 50. 130 rows f32, 3 x 1280 -> 1280 12.8 us: ten steps of x's
+//   way through LDS in two parts on one workgroup a CU (f16 9.2, MXFP4 7.4).
 template <typename T, typename XT, typename OT, bool kWords>
-__global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4LinearArgs a, int n_f, int whole) {
+__global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4LinearArgs a,
+                                                                           int n_f, int whole) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
   const int n_t = gridDim.x / n_f, panel = lid / (kPanel * n_t);
@@ -1041,8 +1043,8 @@ hipError_t launch_rows(const Mx4LinearArgs& a, const RowsShape& r, DType out_dt,
   const int wide = 16 * (kRowsWaves / r.ks);
   const dim3 grid((a.n_out + wide - 1) / wide, a.n_groups, r.splits);
   const uint32_t inv = static_cast<uint32_t>((1ull << 32) / (4 * kGroup * r.chunk) + 1);
-  hipLaunchKernelGGL((mx4_rows<XT, kCT, kBatch, kMany>), grid, dim3(64 * kRowsWaves), r.lds, s, a, r.ks,
-                     r.chunk, inv, r.per_split, static_cast<int>(out_dt));
+  hipLaunchKernelGGL((mx4_rows<XT, kCT, kBatch, kMany>), grid, dim3(64 * kRowsWaves), r.lds, s, a,
+                     r.ks, r.chunk, inv, r.per_split, static_cast<int>(out_dt));
   return hipGetLastError();
 }
 
@@ -1073,7 +1075,8 @@ template <typename T, typename XT, typename OT, bool kWords = true>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   if constexpr (kWords) {
     // Four scales a load where the rows' scales lie on words.
-    bool words = a.n_in % (4 * kMx4Block) == 0 && (reinterpret_cast<uintptr_t>(a.x_scales) & 3) == 0;
+    bool words =
+        a.n_in % (4 * kMx4Block) == 0 && (reinterpret_cast<uintptr_t>(a.x_scales) & 3) == 0;
     for (int g = 0; g < a.n_groups; ++g)
       words = words && (reinterpret_cast<uintptr_t>(a.w_scales[g]) & 3) == 0;
     if (!words) return launch_tile<T, XT, OT, false>(a, out_dt, s);

@@ -14,9 +14,10 @@
 //   f16 planes run on the f16 matrix pipe with operands in two parts, f32 ones on the
 //   f32 matrix pipe.
 //   Short caches are bound by latency: 8 nodes over 60 keys, 6 heads 5.0 us, five trees of up to
-//   26 over 223, 20 heads 6.5, four of 13 over 430, 12 heads f32 8.2 (smallest launch 2.3). Long ones by the matrix
-//   pipe and the softmax's arithmetic beside it: 64 nodes x 20 heads over 65471 f16 keys 95 us,
-//   3.5 TB/s of K and V (floor 66), 16 nodes 73 us, 4.6 TB/s.
+//   26 over 223, 20 heads 6.2, four of 13 over 430, 12 heads f32 8.2 (smallest launch 2.3).
+//   Long ones by the chain from scores to weights to products, whose vector instructions hold the
+//   SIMDs 39% of the time and whose MFMAs 19%: 64 nodes x 20 heads over 65471 f16 keys 94 us, 3.5
+//   TB/s of K and V (floor 66), 16 nodes 73 us, 4.6 TB/s.
 #include "split16.hpp"
 
 #include <algorithm>
@@ -183,9 +184,9 @@ struct Sums {
 };
 
 // A wave's pieces of kSpan keys (kSpan * wave, + kSpan * kWaves, ..) on the f32 matrix pipe, 16
-// at a time, f16 planes widened exactly: lane (c, g) holds key c's values d = 16 g + 0..15, so that lane (r, g) gets scores of keys
-// 4 g + 0..3 of row r, which are the B operand of O^T += V^T P^T as they stand. o[rt][dt][e] is
-// column 16 g + 4 e + dt. q: d = 16 g + 0..15 of row c, times scale * log2(e).
+// at a time, f16 planes widened exactly: lane (c, g) holds key c's values d = 16 g + 0..15, so
+// that lane (r, g) gets scores of keys 4 g + 0..3 of row r, which are the B operand of
+// O^T += V^T P^T as they stand. o[rt][dt][e] is column 16 g + 4 e + dt. q: d = 16 g + 0..15 of row c, times scale * log2(e).
 // `sight` runs once the first loads are on their way (it may hold barriers).
 template <typename KT, int kRT, int kSpan, typename F>
 __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4], int wave, int lane,
