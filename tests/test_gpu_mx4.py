@@ -554,3 +554,49 @@ def test_new_rows_for_a_context_on_another_stream(wrs):
     torch.cuda.synchronize()
     assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
     c.close()
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
+@pytest.mark.parametrize("n_in", [64, 192, 320, 576])
+@pytest.mark.parametrize("rows,n_out", [(130, 3850), (1500, 1530), (2100, 2500)])
+def test_tiles_of_every_size_at_their_edges(wrs, ctx, rows, n_out, n_in, x_dtype):
+    """Tiles of 64 x 64, 128 x 128 and 256 x 128, whole ones and the last, over few columns."""
+    note(f"linear_mx4 {rows} x {n_in} -> {n_out} {x_dtype}")
+    run(wrs, ctx, x_dtype, rows, n_in, n_out, out="f16" if n_in == 192 else "f32",
+        act="gelu" if n_in == 320 else None, seed=16)
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,n_out", [(130, 3850), (1500, 1530), (2100, 2500)])
+def test_large_tiles_formed_again(wrs, ctx, rows, n_out, x_dtype):
+    """A row of x and a feature's scales that 16-bit operands of a tile cannot hold."""
+    note(f"linear_mx4 {rows} x 256 -> {n_out} {x_dtype}, values out of f16's range")
+    rng = np.random.default_rng(17)
+    w = rng.standard_normal((n_out, 256)) / 16
+    w[77] *= 2.0 ** 40
+    w[-1] *= 2.0 ** -50
+    m = wrs.mx4_quantize(torch.from_numpy(w.astype(np.float32)).cuda(), ctx=ctx)
+    wf = unpack_f64(m.codes.cpu().numpy(), m.scales.cpu().numpy())
+    x = rng.standard_normal((rows, 256)).astype(np.float32)
+    if x_dtype == "f32":
+        x[5] *= 2.0 ** 60
+        x[-1] *= 2.0 ** -70
+    xt = torch.from_numpy(x).cuda().to(DT[x_dtype])
+    out = torch.full((rows, n_out), float("nan"), device="cuda")
+    wrs.linear_mx4(xt, [m], None, [out], ctx=ctx)
+    y, tol = reference(xt.double().cpu().numpy(), wf, None, None, "f32")
+    err = np.abs(host(out).astype(np.float64) - y)
+    assert np.all(err <= tol), (float(err.max()), float((err / tol).max()))
+
+
+def test_rows_between_the_outputs_stay(wrs, ctx):
+    """Whole tiles stored into wider rows write nothing beside them."""
+    note("linear_mx4 2100 x 128 -> 2560 into rows of 2600")
+    m = wrs.mx4_quantize(torch.randn((2560, 128), device="cuda"), ctx=ctx)
+    x = torch.randn((2100, 128), device="cuda").half()
+    wide = torch.full((2101, 2600), 7.0, device="cuda", dtype=torch.float16)
+    flat = torch.empty((2100, 2560), device="cuda", dtype=torch.float16)
+    wrs.linear_mx4(x, [m], None, [wide], out_row_stride=2600, ctx=ctx)
+    wrs.linear_mx4(x, [m], None, [flat], ctx=ctx)
+    assert torch.equal(wide[:2100, :2560], flat)
+    assert bool((wide[:, 2560:] == 7).all()) and bool((wide[2100] == 7).all())
