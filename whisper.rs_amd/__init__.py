@@ -328,12 +328,16 @@ def _rows(t, what):
     return n, d, (strides[0] if n > 1 else d)
 
 
+_size_arrays = [None] + [ctypes.c_size_t * n for n in range(1, 17)]
+
+
 def _sizes(values):
-    """A size_t array of a sequence of counts (negative ones are refused)."""
+    """A size_t array of a sequence of counts (negative ones come out past every range, or
+    are refused here)."""
     n = len(values)
-    if n <= 16 and (not n or min(values) >= 0):
-        return (ctypes.c_size_t * n)(*values) if n else None
-    return (ctypes.c_size_t * n).from_buffer(array.array("Q", values))
+    if n > 16:
+        return (ctypes.c_size_t * n).from_buffer(array.array("Q", values))
+    return _size_arrays[n](*values) if n else None
 
 
 class Mx4:
