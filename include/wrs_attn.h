@@ -99,9 +99,9 @@ const char *wrs_attn_status_string(int status);
  * blocks split over two workgroups through a fixed context buffer (~9 MB on
  * 256 CUs), allocated by the first such call outside capture; during capture
  * before then, the call takes another schedule instead; projections of more
- * than 8 rows over n_in >= 2048 whose tiles cover less than half the CUs, and up
- * to 16 rows over long MXFP4 weights (wrs_linear_mx4), which split k through
- * another fixed buffer (~8 MB on 256 CUs) under the same rule;
+ * than 8 rows over n_in >= 2048 whose tiles cover less than half the CUs, and few
+ * rows over long MXFP4 weights (wrs_linear_mx4), which split k through another
+ * fixed buffer (~8 MB on 256 CUs) under the same rule;
  * and fused norms of decode rows over many features (wrs_linear_fused), likewise
  * (reserving linear_tokens allocates both). Tree attention splits long caches through
  * a third one (~9 MB, which reserving heads with decode rows and keys allocates too)

@@ -600,3 +600,68 @@ def test_rows_between_the_outputs_stay(wrs, ctx):
     wrs.linear_mx4(x, [m], None, [flat], ctx=ctx)
     assert torch.equal(wide[:2100, :2560], flat)
     assert bool((wide[:, 2560:] == 7).all()) and bool((wide[2100] == 7).all())
+
+
+@pytest.mark.parametrize("rows,n_in,n_out,groups,x_dtype", [
+    (17, 5120, 1280, 1, "f32"), (64, 5120, 1280, 1, "f16"), (130, 5120, 1280, 1, "f32"),
+    (33, 2112, 500, 3, "f32"), (90, 4160, 77, 2, "bf16"), (20, 65536, 16, 1, "f32"),
+    (40, 5056, 1, 8, "f16"),
+])
+def test_small_tiles_whose_columns_split(wrs, ctx, rows, n_in, n_out, groups, x_dtype):
+    """Tiles over few features and many columns; the splits are the same ones each time."""
+    note(f"linear_mx4 {rows} x {n_in} -> {n_out} x {groups} {x_dtype}, tiles split")
+    run(wrs, ctx, x_dtype, rows, n_in, n_out, groups=groups, act="gelu", seed=18)
+    x = torch.randn((rows, n_in), device="cuda")
+    if x_dtype == "f32":
+        x[3] *= 2.0 ** 40  # one split's range is another's too: a tile formed again in all
+    x = x.to(DT[x_dtype])
+    ws = [wrs.mx4_quantize(torch.randn((n_out, n_in), device="cuda"), ctx=ctx)
+          for _ in range(groups)]
+    outs = [[torch.empty((rows, n_out), device="cuda") for _ in ws] for _ in range(4)]
+    for o in outs:
+        wrs.linear_mx4(x, ws, None, o, ctx=ctx)
+    torch.cuda.synchronize()
+    for o in outs[1:]:
+        for a, b in zip(outs[0], o):
+            assert torch.equal(a, b)
+    for w, o in zip(ws, outs[0]):
+        y, tol = reference(x.double().cpu().numpy(),
+                           unpack_f64(w.codes.cpu().numpy(), w.scales.cpu().numpy()), None, None,
+                           "f32")
+        assert np.all(np.abs(host(o).astype(np.float64) - y) <= tol)
+
+
+def test_split_tiles_captured(wrs):
+    note("linear_mx4 40 x 5120 -> 192, captured before and after an eager call")
+    c = wrs.Context(0)
+    side = torch.cuda.Stream()
+    rng = np.random.default_rng(19)
+    with torch.cuda.stream(side):
+        c.use_torch_stream()
+        m, w = make(wrs, c, rng, 192, 5120)
+        x = torch.empty((40, 5120), device="cuda")
+        outs = [torch.empty((40, 192), device="cuda") for _ in range(3)]
+        eager = torch.empty((40, 192), device="cuda")
+        side.synchronize()
+        graphs = []
+        for i, o in enumerate(outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                wrs.linear_mx4(x, [m], None, [o], ctx=c)
+            graphs.append(g)
+            if i == 0:
+                wrs.linear_mx4(x, [m], None, [eager], ctx=c)
+                side.synchronize()
+        for _ in range(4):
+            x.copy_(torch.from_numpy(rng.standard_normal((40, 5120)).astype(np.float32)))
+            for o in outs:
+                o.fill_(float("nan"))
+            for g in graphs + graphs[1:]:
+                g.replay()
+            wrs.linear_mx4(x, [m], None, [eager], ctx=c)
+            side.synchronize()
+            y, tol = reference(x.double().cpu().numpy(), w, None, None, "f32")
+            assert np.all(np.abs(host(outs[0]).astype(np.float64) - y) <= tol)
+            assert torch.equal(outs[1], eager) and torch.equal(outs[2], eager)
+            assert np.all(np.abs(host(eager).astype(np.float64) - y) <= tol)
+    c.close()

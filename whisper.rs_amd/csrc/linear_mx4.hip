@@ -362,8 +362,10 @@ struct Tile {
   static constexpr int BF = BF_, BT = BT_, WF = WF_, WT = WT_, KG = KG_;
   static constexpr int kWaves = (BF / WF) * (BT / WT);  // of a group
   static constexpr int kGroupThreads = 64 * kWaves, kThreads = kGroupThreads * KG;
+  static constexpr bool kSplits = KG == 4;  // whose columns may split over workgroups
 };
 constexpr int kK = 64;           // columns per stage
+constexpr int kUnit = 256;       // columns in which a tile's columns split
 constexpr int kRow = 2 * kK;     // bytes of a staged row
 constexpr int kOutPitch = 68;    // floats of an output row in LDS
 
@@ -410,7 +412,8 @@ __device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_
 //   multiplies values 8 j.. of both blocks, so x's operand is chunk 4 h + j of its staged row.
 template <typename T, typename XT, typename E, int P, bool kWords>
 __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
-                                    int part, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+                                    int u0, int u1, int part,
+                                    f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
   constexpr int kXn = T::BT * (kK / 8) / T::kGroupThreads;  // groups of 8 values a thread stages
   static_assert(kXn >= 1 && T::BT * (kK / 8) % T::kGroupThreads == 0, "whole groups");
@@ -452,17 +455,17 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   float most[kXn];  // largest magnitudes of this thread's rows of x
 #pragma unroll
   for (int i = 0; i < kXn; ++i) most[i] = 0.f;
-  // Pair i of the group, of two stages, is pair i * KG + kg of the tile.
-  const int pairs = (stages + 1) / 2;
+  // Pair i of the group, of two stages, is pair i * KG + kg of the tile's.
+  const int pair0 = 2 * u0, pair1 = min((stages + 1) / 2, 2 * u1), stages1 = min(stages, 4 * u1);
   // Loads of stage i_s of x and pair i_p of W: number k of kXn + kWn + kF.
   constexpr int kLoads = kXn + kWn + kF;
   auto load = [&](int k, int i_s, int i_p) __attribute__((always_inline)) {
     if (k < kXn) {
-      const int at = kK * min(2 * ((i_s >> 1) * T::KG + kg) + (i_s & 1), stages - 1);
+      const int at = kK * min(2 * (pair0 + (i_s >> 1) * T::KG + kg) + (i_s & 1), stages - 1);
       xv[k] = *reinterpret_cast<const x8*>(xp[k] + at);
       return;
     }
-    int p = i_p * T::KG + kg;
+    int p = pair0 + i_p * T::KG + kg;
     asm("" : "+s"(p));  // offsets are formed per pair, not kept per load
     if (k < kXn + kWn) {
       const int i = k - kXn, at = 4 * p + (lane & 3);
@@ -471,7 +474,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, o + i * 16 * bytes, 0, 0));
     } else {
       const int i = k - kXn - kWn;
-      sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + 4 * p, p < pairs,
+      sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + 4 * p, 4 * p < nb,
                                        4 * p + 2 < nb);
     }
   };
@@ -581,7 +584,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 #pragma unroll
   for (int k = 0; k < kXn; ++k) load(k, 1, 0);
   __syncthreads();
-  const int turns = (pairs + T::KG - 1) / T::KG;  // of every group; the last one's may be empty
+  const int turns = (pair1 - pair0 + T::KG - 1) / T::KG;  // every group's; the last may be empty
   int i_p = 0;
   // No branch in this loop: one around the products costs copies of the sums (64 moves per two
   // stages of a 64 x 128 wave).
@@ -597,10 +600,10 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   // The second stage, stored here already, is a repeated one where there is none.
   store_x(lds + kStageBytes);
   put_w();
-  const int last = 2 * (i_p * T::KG + kg);
-  if (last < stages) multiply(0, lds, std::integral_constant<int, 0>{}, 0, 0);
+  const int last = 2 * (pair0 + i_p * T::KG + kg);
+  if (last < stages1) multiply(0, lds, std::integral_constant<int, 0>{}, 0, 0);
   __syncthreads();
-  if (last + 1 < stages) multiply(1, lds + kStageBytes, std::integral_constant<int, 0>{}, 0, 0);
+  if (last + 1 < stages1) multiply(1, lds + kStageBytes, std::integral_constant<int, 0>{}, 0, 0);
   if constexpr (kHalves) {
     // 8 neighbouring lanes staged a row. Rows past the last one repeat it.
 #pragma unroll
@@ -646,7 +649,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 // the row's word h.
 template <typename T, bool kWords>
 __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
-                                        f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
+                                        int u0, int u1, f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
   constexpr int kXn = T::BT * 8 / T::kGroupThreads;  // 16-byte chunks of x a thread stages
   static_assert(kXn >= 1 && T::BT * 8 % T::kGroupThreads == 0, "whole chunks");
@@ -663,7 +666,7 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   const int r32 = lane & 31, hl = lane >> 5;
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
   const int nb = a.n_in / kMx4Block, bytes = a.n_in / 2;
-  const int stages = (nb + kBlocks - 1) / kBlocks;
+  const int nb1 = min(nb, kBlocks * u1);  // where the tile's columns end
 
   // Rows past the last and blocks past a row's last read as zero: codes of 0, scale 2^-127.
   const int n_f = min(T::BF, a.n_out - f0), n_t = min(T::BT, a.n_tokens - t0);
@@ -684,25 +687,25 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   // per stage, not kept per load.
   constexpr int kLoads = kWn + kF + kXn + 1;
   auto load = [&](int k, int i_s, int i_x) __attribute__((always_inline)) {
-    int b = kBlocks * (i_s * T::KG + kg), bx = kBlocks * (i_x * T::KG + kg);  // first blocks
+    int b = kBlocks * (u0 + i_s * T::KG + kg), bx = kBlocks * (u0 + i_x * T::KG + kg);
     asm("" : "+s"(b), "+s"(bx));
     if (k < kXn) {
       const int e = tid + T::kGroupThreads * k, at = bx + (e & 7);
       xv[k] = __builtin_bit_cast(
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                     xrs, at < nb ? (e >> 3) * bytes + 16 * at : kPast, 0, 0));
+                     xrs, at < nb1 ? (e >> 3) * bytes + 16 * at : kPast, 0, 0));
     } else if (k == kXn) {
       const int at = bx + 4 * (tid & 1);
       const bool mine = tid < 2 * T::BT;
-      xs = load_scales<kWords>(xsrs, (tid >> 1) * nb + at, mine && at < nb, mine && at + 2 < nb);
+      xs = load_scales<kWords>(xsrs, (tid >> 1) * nb + at, mine && at < nb1, mine && at + 2 < nb1);
     } else if (k <= kXn + kWn) {
       const int i = k - kXn - 1, at = b + (lane & 7);
-      const uint32_t o = at < nb ? (wf + (lane >> 3)) * bytes + 16 * at : kPastRows;
+      const uint32_t o = at < nb1 ? (wf + (lane >> 3)) * bytes + 16 * at : kPastRows;
       cw[i] = __builtin_bit_cast(
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(wrs, o + i * 8 * bytes, 0, 0));
     } else {
       const int i = k - kXn - 1 - kWn, sb = b + 4 * hl;
-      sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + sb, sb < nb, sb + 2 < nb);
+      sw_next[i] = load_scales<kWords>(srs, (wf + 32 * i + r32) * nb + sb, sb < nb1, sb + 2 < nb1);
     }
   };
   auto put_w = [&]() __attribute__((always_inline)) {
@@ -778,7 +781,7 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   for (int k = 0; k <= kXn; ++k) load(k, 0, 1);
   __syncthreads();
   // Stages past the last one are zeros.
-  const int turns = (stages + T::KG - 1) / T::KG;
+  const int turns = (u1 - u0 + T::KG - 1) / T::KG;
   auto stage = [&](int i_s, int d) __attribute__((always_inline)) {
     store_x(lds + (1 - d) * kStageBytes);
     put_w();
@@ -828,6 +831,49 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
     }
     __syncthreads();
     if (wave >= T::kWaves) return;
+  }
+  if constexpr (T::kSplits) {
+    const int splits = gridDim.z;
+    if (splits > 1) {
+      // A wave's sums meet those of the same wave of the other splits, in their order: the wave that
+      // counts in last adds them and re-arms the counter.
+      static_assert(kF == 1 && kT == 1, "one MFMA tile a wave");
+      const int unit = (grp * gridDim.x + blockIdx.x) * T::kWaves + wave, split = blockIdx.z;
+      float* const part = a.part + static_cast<int64_t>(unit) * splits * 1024 + lane;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        acc[0][0][e] *= down;
+        st_agent(part + split * 1024 + 64 * e, acc[0][0][e]);
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0);
+      asm volatile("" ::: "memory");
+      unsigned* const counter = a.counters + static_cast<int64_t>(unit) * kMx4CounterStride;
+      unsigned before = 0;
+      if (lane == 0)
+        before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("" ::: "memory");
+      if (__builtin_amdgcn_readfirstlane(before) != static_cast<unsigned>(splits - 1)) return;
+      f32x16 sum = {};
+      constexpr int kAtOnce = 4;
+#pragma unroll 1
+      for (int s0 = 0; s0 < splits; s0 += kAtOnce) {
+        float x[kAtOnce][16];
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            x[s][e] = s0 + s < splits ? ld_agent(part + (s0 + s) * 1024 + 64 * e) : 0.f;
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum[e] += x[s][e];
+      }
+      acc[0][0] = sum;
+      down = 1.f;
+      if (lane == 0)
+        __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
   const int r32 = lane & 31, hl = lane >> 5;
   const int wf = (wave % (T::BF / T::WF)) * T::WF, wt = (wave / (T::BF / T::WF)) * T::WT;
@@ -920,12 +966,16 @@ constexpr int kPanel = 8;
 //   way through LDS in two parts on one workgroup a CU (f16 9.2, MXFP4 7.4).
 template <typename T, typename XT, typename OT, bool kWords>
 __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4LinearArgs a,
-                                                                           int n_f, int whole) {
+                                                                           int n_f, int whole,
+                                                                           int per_split) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lid = xcd_remap(blockIdx.x, gridDim.x);
   const int n_t = gridDim.x / n_f, panel = lid / (kPanel * n_t);
   const int wide = min(kPanel, n_f - kPanel * panel), in = lid - kPanel * n_t * panel;
   const int f0 = (kPanel * panel + in % wide) * T::BF, t0 = in / wide * T::BT, grp = blockIdx.y;
+  const int units = (a.n_in + kUnit - 1) / kUnit;
+  const int u0 = T::kSplits ? blockIdx.z * per_split : 0;
+  const int u1 = T::kSplits ? min(units, u0 + per_split) : units;
   f32x16 acc[T::WF / 32][T::WT / 32];
   auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -936,18 +986,18 @@ __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4Li
   clear();
   float down = 1.f;
   if constexpr (sizeof(XT) == 1) {
-    tile_product_mx4<T, kWords>(a, grp, f0, t0, lds, acc);
+    tile_product_mx4<T, kWords>(a, grp, f0, t0, lds, u0, u1, acc);
   } else if constexpr (__is_same(XT, __bf16)) {
-    tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, 0, acc);
+    tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, u0, u1, 0, acc);
   } else {
     constexpr int kP = __is_same(XT, float) ? 2 : 1;
     if (kP == 2) down = 1.f / kXUp;
-    if (tile_product<T, XT, _Float16, kP, kWords>(a, grp, f0, t0, lds, 0, acc)) {
+    if (tile_product<T, XT, _Float16, kP, kWords>(a, grp, f0, t0, lds, u0, u1, 0, acc)) {
       clear();
       down = 1.f;
 #pragma unroll 1
       for (int part = kParts<XT> - 1; part >= 0; --part)
-        tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, part, acc);
+        tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, u0, u1, part, acc);
     }
   }
   tile_store<T, OT>(a, grp, f0, t0, lds, whole, down, acc);
@@ -1071,6 +1121,34 @@ hipError_t launch_rows_of(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   }
 }
 
+using Small = Tile<64, 32, 32, 32, 4>;
+using Mid = Tile<64, 64, 32, 32, 2>;
+using Wide = Tile<128, 128, 64, 64, 1>;
+template <typename T>
+int64_t tile_wgs(const Mx4LinearArgs& a) {
+  return static_cast<int64_t>((a.n_out + T::BF - 1) / T::BF) *
+         ((a.n_tokens + T::BT - 1) / T::BT) * a.n_groups;
+}
+constexpr int kMidLeast = 180;  // workgroups
+
+// Splits of the columns of small tiles that leave CUs idle over long rows, of kUnitsLeast units at
+// least. The sums' way through memory costs ~2 us. us, split / not, 5120 -> 1280 (20 units): f32 17
+// rows 11.7/21.5, 64 12.7/22.1, 130 17.0/22.8; f16 64 10.3/14.0, 130 12.3/14.8; MXFP4 x, whose
+// units are cheap, 64 9.0/9.0. 2048 -> 512 (8 units): f32 40 rows 10.1/11.5, f16 8.0/7.7, MXFP4
+// 7.2/6.4; 1280 -> 1280 (5) in units of two at least: f32 9.9/9.8, f16 8.1/7.0.
+constexpr int kUnitsLeast = 4;
+int tile_splits(const Mx4LinearArgs& a, DType x_dt) {
+  const int64_t wgs = tile_wgs<Small>(a), units = (a.n_in + kUnit - 1) / kUnit;
+  if (a.x_scales || units < (x_dt == kF32 ? 8 : 16) || tile_wgs<Mid>(a) >= kMidLeast) return 1;
+  int64_t n = std::min<int64_t>(
+      {256 / wgs, units / kUnitsLeast, kMx4MaxSplits});
+  if (a.part)
+    n = std::min<int64_t>({n, static_cast<int64_t>(a.part_floats) / (wgs * Small::BF * Small::BT),
+                           static_cast<int64_t>(a.counter_words) /
+                                       (kMx4CounterStride * Small::kWaves) >= wgs ? n : 1});
+  return static_cast<int>(std::max<int64_t>(n, 1));
+}
+
 template <typename T, typename XT, typename OT, bool kWords = true>
 hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   if constexpr (kWords) {
@@ -1089,8 +1167,13 @@ hipError_t launch_tile(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   const int n_f = (a.n_out + T::BF - 1) / T::BF;
   const int64_t wgs = static_cast<int64_t>(n_f) * ((a.n_tokens + T::BT - 1) / T::BT);
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((mx4_tile<T, XT, OT, kWords>), dim3(static_cast<unsigned>(wgs), a.n_groups),
-                     dim3(T::kThreads), kLds, s, a, n_f, whole_chunks(a, out_dt) ? 1 : 0);
+  const int units = (a.n_in + kUnit - 1) / kUnit;
+  int splits = T::kSplits && a.part ? tile_splits(a, sizeof(XT) == 4 ? kF32 : kF16) : 1;
+  const int per_split = (units + splits - 1) / splits;
+  splits = (units + per_split - 1) / per_split;
+  hipLaunchKernelGGL((mx4_tile<T, XT, OT, kWords>),
+                     dim3(static_cast<unsigned>(wgs), a.n_groups, splits), dim3(T::kThreads), kLds,
+                     s, a, n_f, whole_chunks(a, out_dt) ? 1 : 0, per_split);
   return hipGetLastError();
 }
 
@@ -1103,24 +1186,18 @@ hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   //   Wide, 144 (f32, 1500 rows 384 -> 1536): 14.4, Mid 16.1; 120 (f32, 1500 rows 1280 -> 1280):
   //   29.4, Mid 21.7.
   //   Mid, 180 (MXFP4, 130 rows, 3 x 1280 -> 1280): 7.4, Small 8.0; 60 (40 rows): 6.7, Small 6.1.
-  using Small = Tile<64, 32, 32, 32, 4>;
-  using Mid = Tile<64, 64, 32, 32, 2>;
-  using Wide = Tile<128, 128, 64, 64, 1>;
   using Large = Tile<256, 128, 64, 128, 1>;
-  auto fills = [&](int f, int t, int least) {
-    return static_cast<int64_t>((a.n_out + f - 1) / f) * ((a.n_tokens + t - 1) / t) * a.n_groups >=
-           least;
-  };
-  if (fills(Large::BF, Large::BT, 160)) return launch_tile<Large, XT, OT>(a, out_dt, s);
-  if (fills(Wide::BF, Wide::BT, 144)) return launch_tile<Wide, XT, OT>(a, out_dt, s);
-  if (fills(Mid::BF, Mid::BT, 180)) return launch_tile<Mid, XT, OT>(a, out_dt, s);
+  if (tile_wgs<Large>(a) >= 160) return launch_tile<Large, XT, OT>(a, out_dt, s);
+  if (tile_wgs<Wide>(a) >= 144) return launch_tile<Wide, XT, OT>(a, out_dt, s);
+  if (tile_wgs<Mid>(a) >= kMidLeast) return launch_tile<Mid, XT, OT>(a, out_dt, s);
   return launch_tile<Small, XT, OT>(a, out_dt, s);
 }
 
 }  // namespace
 
 bool linear_mx4_splits(const Mx4LinearArgs& a, DType x_dt) {
-  if (a.n_tokens > kMx4Rows || a.x_scales) return false;
+  if (a.n_tokens > kMx4Rows) return tile_splits(a, x_dt) > 1;
+  if (a.x_scales) return false;
   const int parts = x_dt == kF32 ? kParts<float> : x_dt == kF16 ? kParts<_Float16> : 1;
   return rows_split(a, parts * a.n_tokens);
 }
