@@ -853,7 +853,7 @@ __device__ inline void tile_store(const Mx4LinearArgs& a, int grp, int f0, int t
       if (lane == 0)
         before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       asm volatile("" ::: "memory");
-      if (__builtin_amdgcn_readfirstlane(before) != static_cast<unsigned>(splits - 1)) return;
+      if (__builtin_amdgcn_readfirstlane(static_cast<int>(before)) != splits - 1) return;
       f32x16 sum = {};
       constexpr int kAtOnce = 4;
 #pragma unroll 1
@@ -974,7 +974,7 @@ __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4Li
   const int wide = min(kPanel, n_f - kPanel * panel), in = lid - kPanel * n_t * panel;
   const int f0 = (kPanel * panel + in % wide) * T::BF, t0 = in / wide * T::BT, grp = blockIdx.y;
   const int units = (a.n_in + kUnit - 1) / kUnit;
-  const int u0 = T::kSplits ? blockIdx.z * per_split : 0;
+  const int u0 = T::kSplits ? static_cast<int>(blockIdx.z) * per_split : 0;
   const int u1 = T::kSplits ? min(units, u0 + per_split) : units;
   f32x16 acc[T::WF / 32][T::WT / 32];
   auto clear = [&]() __attribute__((always_inline)) {
