@@ -665,3 +665,32 @@ def test_split_tiles_captured(wrs):
             assert torch.equal(outs[1], eager) and torch.equal(outs[2], eager)
             assert np.all(np.abs(host(eager).astype(np.float64) - y) <= tol)
     c.close()
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("octaves", [20, 25])
+@pytest.mark.parametrize("rows,n_out", [(3, 70), (17, 70), (50, 70), (130, 3850), (1500, 1530),
+                                        (2100, 2500)])
+def test_small_x_that_decides(wrs, ctx, rows, n_out, octaves, x_dtype):
+    """The large values of every row of x meet weights of 0 (in blocks with others): the result
+    is the small values' alone, 2^-octaves of them. Two parts of f32 x leave 2^-22 of a value,
+    which reference() counts, or 2^-43."""
+    note(f"linear_mx4 {rows} x 256 -> {n_out} {x_dtype}, x at 2^-{octaves} beside large values")
+    rng = np.random.default_rng(20)
+    w = rng.standard_normal((n_out, 256)) / 16
+    w[:, 64:72] = w[:, 250:] = 0.0
+    m = wrs.mx4_quantize(torch.from_numpy(w.astype(np.float32)).cuda(), ctx=ctx)
+    x = rng.standard_normal((rows, 256)).astype(np.float32)
+    small = np.ones(256, bool)
+    small[64:72] = small[250:] = False
+    x[:, small] *= np.float32(2.0 ** -octaves)
+    x[:, ~small] *= 30
+    xt = torch.from_numpy(x).cuda().to(DT[x_dtype])
+    out = torch.full((rows, n_out), float("nan"), device="cuda")
+    wrs.linear_mx4(xt, [m], None, [out], ctx=ctx)
+    wf = unpack_f64(m.codes.cpu().numpy(), m.scales.cpu().numpy())
+    y, tol = reference(xt.double().cpu().numpy(), wf, None, None, "f32")
+    if x_dtype == "f32":
+        tol = tol + 2.0 ** -43 * np.abs(wf).sum(axis=1)
+    err = np.abs(host(out).astype(np.float64) - y)
+    assert np.all(err <= tol), (float(err.max()), float((err / tol).max()))

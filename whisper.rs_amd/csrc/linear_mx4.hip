@@ -385,9 +385,16 @@ constexpr size_t tile_lds() {  // P 0: MXFP4 x, whose scales lie behind its code
   return stage > out ? (stage > join ? stage : join) : (out > join ? out : join);
 }
 
-// f32 x as two f16 parts of x * 2^7: 2^-23 of a value and 2^-25 at least. That is 2^-22 of the
-// row's largest value where it lies in [2^-10, 511].
+// f32 x as two f16 parts of x * 2^7, the second in a unit 2^-11 of the first: within 2^-22 of a
+// value down to 2^-21, and 2^-43 below. Rows whose largest value lies in [2^-10, 511] take them:
+// there that is 2^-33 of it at most. Both parts meet one sum, so the second one's weights are
+// 2^-11 of the first one's, and f16 holds both of a scale in 2^-20 .. 2^5 (their unit is 2^-8).
+// (With both parts in one unit, 2^-32 was lost of every value: next to large values that meet
+// weights of 0, 10^-6 kept 12 bits.)
 constexpr float kXUp = 128.f, kXLeast = 0x1p-10f, kXMost = 511.f;
+constexpr float kPartUnit = 0x1p-11f;
+constexpr int kWUpLog2 = 8;
+constexpr float kHalvesDown = 1.f / (kXUp * (1 << kWUpLog2));
 
 // Four scale bytes from `at` of a row on (an even place): one load where they lie on a word.
 template <bool kWords>
@@ -402,7 +409,7 @@ __device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_
 }
 
 // Adds one tile's products with operands of type E to acc. x goes in P parts: one of its own
-// type, two of f16 (f32 x, E f16: results times kXUp), or with bf16 E part `part` of kParts.
+// type, two of f16 (f32 x, E f16: results over kHalvesDown), or with bf16 E part `part` of kParts.
 // Returns (to every thread) whether E cannot hold the tile's operands: a scale of its weights,
 // or a row of f32 x.
 //   A wave's own rows of W come 64 bytes of codes at a time, 4 lanes a row, and change places in
@@ -501,9 +508,13 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
           uint32_t w = __builtin_bit_cast(uint32_t, hi);
           asm("" : "+v"(w));  // formed once, not again where it is taken off
           hi = __builtin_bit_cast(f16x2, w);
+          // The difference is exact, and so is its product with the unit's inverse.
+          constexpr float kUp = 1.f / kPartUnit;
           const f16x2 lo = {
-              static_cast<_Float16>(__builtin_fmaf(x[j], kXUp, -static_cast<float>(hi[0]))),
-              static_cast<_Float16>(__builtin_fmaf(x[j + 1], kXUp, -static_cast<float>(hi[1])))};
+              static_cast<_Float16>(
+                  __builtin_fmaf(static_cast<float>(hi[0]), -kUp, x[j] * (kXUp * kUp))),
+              static_cast<_Float16>(
+                  __builtin_fmaf(static_cast<float>(hi[1]), -kUp, x[j + 1] * (kXUp * kUp)))};
           h[j >> 1] = w;
           l[j >> 1] = __builtin_bit_cast(uint32_t, lo);
         }
@@ -538,44 +549,61 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 #pragma unroll
     for (int i = 0; i < kF; ++i) {
       const int byte = (sw[i] >> (16 * d + 8 * hl)) & 255;
-      // f16 holds 6 * 2^13 and 0.5 * 2^-23.
+      // f16 holds 6 * 2^13 and 0.5 * 2^-23, of two parts' weights 0.5 * 2^-12 * kPartUnit.
+      constexpr int kLeast = kHalves ? 127 - 12 - kWUpLog2 : 127 - 23;
+      constexpr int kMost = kHalves ? 127 + 13 - kWUpLog2 : 127 + 13;
       if constexpr (__is_same(E, _Float16))
-        odd |= wf + 32 * i + r32 < n_f && static_cast<unsigned>(byte - 104) > 36u;
-      scale[i] = scale_of(byte);
+        odd |= wf + 32 * i + r32 < n_f &&
+               static_cast<unsigned>(byte - kLeast) > static_cast<unsigned>(kMost - kLeast);
+      scale[i] = scale_of(kHalves ? byte + kWUpLog2 : byte);
       c[i] = *reinterpret_cast<const u32x4*>(codes + code_at(32 * i + r32, 2 * d + hl));
     }
-    u32x4 wv[2][kF], xw[P][kT];
+    // Operands of x are read a step ahead. With two parts, waves of several tiles read them a part
+    // ahead and form the second part's weights in the first one's registers, just before its
+    // products: waves of 64 x 128 spill as it is, and 64 x 64 are no faster the other way (3000
+    // rows 5120 -> 1280: 110 us, 111 to 113).
+    constexpr bool kTight = P > 1 && kT >= 2;
+    constexpr int kAhead = kTight ? 1 : P;  // parts
+    u32x4 wv[2][kF], wl[kF], xw[kAhead][kT];
     auto widen = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kF; ++i) wv[j & 1][i] = widen8_as<E>(c[i][j], scale[i]);
     };
-    auto read_x = [&](int j, int t) __attribute__((always_inline)) {
+    auto lower = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-        xw[p][t] = *reinterpret_cast<const u32x4*>(buf + p * kXBytes +
-                                                   chunk_at(wt + 32 * t + r32, 4 * hl + j));
+      for (int i = 0; i < kF; ++i)
+        wl[i] = __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, wv[j & 1][i]) *
+                                              static_cast<_Float16>(kPartUnit));
     };
-    constexpr int kSteps = kK / 16, kSlots = kSteps * kT, kNow = decltype(n)::value;
+    // Part p of step j, numbered s = j * P + p.
+    auto read_x = [&](int s, int t) __attribute__((always_inline)) {
+      xw[s % kAhead][t] = *reinterpret_cast<const u32x4*>(
+          buf + s % P * kXBytes + chunk_at(wt + 32 * t + r32, 4 * hl + s / P));
+    };
+    constexpr int kSteps = kK / 16 * P, kSlots = kSteps * kT, kNow = decltype(n)::value;
 #pragma unroll
-    for (int t = 0; t < kT; ++t) read_x(0, t);
+    for (int s = 0; s < kAhead; ++s)
+#pragma unroll
+      for (int t = 0; t < kT; ++t) read_x(s, t);
     widen(0);
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j)
+    for (int s = 0; s < kSteps; ++s) {
+      const int j = s / P, p = s % P;
+      if (kTight && p) lower(j);
 #pragma unroll
       for (int t = 0; t < kT; ++t) {
 #pragma unroll
-        for (int p = P - 1; p >= 0; --p)
-#pragma unroll
-          for (int i = 0; i < kF; ++i) acc[i][t] = mfma32<E>(wv[j & 1][i], xw[p][t], acc[i][t]);
-        if (j + 1 < kSteps) {
-          if (t == 0) widen(j + 1);
-          read_x(j + 1, t);
-        }
+        for (int i = 0; i < kF; ++i)
+          acc[i][t] = mfma32<E>(p ? wl[i] : wv[j & 1][i], xw[s % kAhead][t], acc[i][t]);
+        if (!kTight && P > 1 && p == 0 && t == 0) lower(j);
+        if (p == 0 && t == 0 && s + P < kSteps) widen(j + 1);
+        if (s + kAhead < kSteps) read_x(s + kAhead, t);
 #pragma unroll
         for (int k = 0; k < kNow; ++k)
-          if (k * kSlots / (kNow ? kNow : 1) == j * kT + t) load(k, i_s, i_p);
+          if (k * kSlots / (kNow ? kNow : 1) == s * kT + t) load(k, i_s, i_p);
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
   };
 
 #pragma unroll
@@ -956,13 +984,13 @@ constexpr int kPanel = 8;
 
 // K16 (mx4_tile): many rows of x. W is widened to 16-bit operands in registers, x passes through
 //   LDS in one part (f16, bf16) or two f16 ones (f32), and both feed 32x32x16 MFMAs. f16 holds
-//   weights of scales 2^-23 to 2^13 exactly, and rows of f32 x whose largest value is of
-//   ordinary size; a tile that meets others is formed again from bf16 operands, which hold any,
-//   one of x's two or three parts after the other.
+//   weights of scales 2^-23 to 2^13 exactly (beside two parts of x 2^-20 to 2^5), and rows of f32
+//   x whose largest value is of ordinary size; a tile that meets others is formed again from bf16
+//   operands, which hold any, one of x's two or three parts after the other.
 //   24000 x 5120 -> 1280: f16 291 us, 1080 TFLOP/s, the matrix pipe 57% busy and the card's power
-//   the bound (the library's product of f16 weights 274), bf16 265, f32 586, MXFP4 101, 3.1
+//   the bound (the library's product of f16 weights 274), bf16 265, f32 595, MXFP4 101, 3.1
 //   PFLOP/s (zeros in its place a quarter less); 1280 -> 5120 MXFP4 with GELU 127, of which the
-//   epilogue's 123 M outputs are about 50. 130 rows f32, 3 x 1280 -> 1280 12.8 us: ten steps of x's
+//   epilogue's 123 M outputs are about 50. 130 rows f32, 3 x 1280 -> 1280 13.1 us: ten steps of x's
 //   way through LDS in two parts on one workgroup a CU (f16 9.2, MXFP4 7.4).
 template <typename T, typename XT, typename OT, bool kWords>
 __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4LinearArgs a,
@@ -991,7 +1019,7 @@ __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4Li
     tile_product<T, XT, __bf16, 1, kWords>(a, grp, f0, t0, lds, u0, u1, 0, acc);
   } else {
     constexpr int kP = __is_same(XT, float) ? 2 : 1;
-    if (kP == 2) down = 1.f / kXUp;
+    if (kP == 2) down = kHalvesDown;
     if (tile_product<T, XT, _Float16, kP, kWords>(a, grp, f0, t0, lds, u0, u1, 0, acc)) {
       clear();
       down = 1.f;
