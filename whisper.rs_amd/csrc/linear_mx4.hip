@@ -491,6 +491,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
       *reinterpret_cast<u32x4*>(codes + code_at((lane >> 2) + 16 * i, lane & 3)) = cw[i];
 #pragma unroll
     for (int i = 0; i < kF; ++i) sw[i] = sw_next[i];
+    wave_sync();  // other lanes read the codes
   };
   auto store_x = [&](char* buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -617,8 +618,8 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
   // No branch in this loop: one around the products costs copies of the sums (64 moves per two
   // stages of a 64 x 128 wave).
   for (; i_p + 1 < turns; ++i_p) {
-    store_x(lds + kStageBytes);
     put_w();
+    store_x(lds + kStageBytes);
     multiply(0, lds, std::integral_constant<int, kLoads>{}, 2 * i_p + 2, i_p + 1);
     __syncthreads();
     store_x(lds);
@@ -626,8 +627,8 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
     __syncthreads();
   }
   // The second stage, stored here already, is a repeated one where there is none.
-  store_x(lds + kStageBytes);
   put_w();
+  store_x(lds + kStageBytes);
   const int last = 2 * (pair0 + i_p * T::KG + kg);
   if (last < stages1) multiply(0, lds, std::integral_constant<int, 0>{}, 0, 0);
   __syncthreads();
@@ -742,6 +743,7 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
       *reinterpret_cast<u32x4*>(codes + chunk_at((lane >> 3) + 8 * i, lane & 7)) = cw[i];
 #pragma unroll
     for (int i = 0; i < kF; ++i) sw[i] = sw_next[i];
+    wave_sync();  // other lanes read the codes
   };
   auto store_x = [&](char* buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -811,8 +813,8 @@ __device__ inline void tile_product_mx4(const Mx4LinearArgs& a, int grp, int f0,
   // Stages past the last one are zeros.
   const int turns = (u1 - u0 + T::KG - 1) / T::KG;
   auto stage = [&](int i_s, int d) __attribute__((always_inline)) {
-    store_x(lds + (1 - d) * kStageBytes);
     put_w();
+    store_x(lds + (1 - d) * kStageBytes);
     multiply(lds + d * kStageBytes, i_s);
     __syncthreads();
   };
