@@ -694,3 +694,58 @@ def test_small_x_that_decides(wrs, ctx, rows, n_out, octaves, x_dtype):
         tol = tol + 2.0 ** -43 * np.abs(wf).sum(axis=1)
     err = np.abs(host(out).astype(np.float64) - y)
     assert np.all(err <= tol), (float(err.max()), float((err / tol).max()))
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
+@pytest.mark.parametrize("rows,n_out", [(3, 70), (50, 70), (130, 3850), (1500, 1530), (2100, 2500)])
+def test_blocks_of_zeros_leave_the_others_alone(wrs, ctx, rows, n_out, x_dtype):
+    """Padded columns and pruned rows: blocks of zeros, which quantise to the scale 2^-127. The
+    results are bit for bit those of the same zeros under a scale of 1."""
+    note(f"linear_mx4 {rows} x 256 -> {n_out} {x_dtype}, blocks of zeros")
+    rng = np.random.default_rng(21)
+    w = rng.standard_normal((n_out, 256)) / 16
+    w[:, 224:] = 0.0
+    w[5] = w[n_out - 1] = 0.0
+    w[:, 32:64] *= rng.random((n_out, 1)) < 0.5
+    w[9, 64:96] = -0.0
+    m = wrs.mx4_quantize(torch.from_numpy(w.astype(np.float32)).cuda(), ctx=ctx)
+    other = wrs.Mx4(m.codes, torch.where(m.scales == 0, 127, m.scales).to(torch.uint8))
+    assert int((m.scales == 0).sum()) > n_out
+    x = torch.from_numpy(rng.standard_normal((rows, 256)).astype(np.float32)).cuda()
+    if x_dtype == "mx4":
+        x = wrs.mx4_quantize(x, ctx=ctx)
+        xr = unpack_f64(x.codes.cpu().numpy(), x.scales.cpu().numpy())
+    else:
+        x = x.to(DT[x_dtype])
+        xr = x.double().cpu().numpy()
+    outs = [torch.full((rows, n_out), float("nan"), device="cuda") for _ in range(2)]
+    for weights, out in zip((m, other), outs):
+        wrs.linear_mx4(x, [weights], None, [out], ctx=ctx)
+    y, tol = reference(xr, unpack_f64(m.codes.cpu().numpy(), m.scales.cpu().numpy()), None, None,
+                       "f32")
+    for out in outs:
+        assert np.all(np.abs(host(out).astype(np.float64) - y) <= tol)
+    assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("byte", [1, 114, 115, 133, 200, 247, 254, 255])
+@pytest.mark.parametrize("rows", [3, 50])
+def test_zeros_under_any_scale(wrs, ctx, rows, byte, x_dtype):
+    """A block of zeros is 0 under every scale but the NaN, which stays one."""
+    note(f"linear_mx4 {rows} rows {x_dtype}, zeros under the scale byte {byte}")
+    rng = np.random.default_rng(22)
+    w = rng.standard_normal((70, 128)) / 8
+    w[11, 32:64] = 0.0
+    m = wrs.mx4_quantize(torch.from_numpy(w.astype(np.float32)).cuda(), ctx=ctx)
+    m.scales[11, 1] = byte
+    x = torch.from_numpy(rng.standard_normal((rows, 128)).astype(np.float32)).cuda().to(DT[x_dtype])
+    out = torch.full((rows, 70), float("nan"), device="cuda")
+    wrs.linear_mx4(x, [m], None, [out], ctx=ctx)
+    y, tol = reference(x.double().cpu().numpy(),
+                       unpack_f64(m.codes.cpu().numpy(), m.scales.cpu().numpy()), None, None, "f32")
+    got = host(out).astype(np.float64)
+    if byte == 255:
+        assert np.all(np.isnan(got[:, 11]))
+        got[:, 11] = y[:, 11] = tol[:, 11] = 0.0
+    assert np.all(np.abs(got - y) <= tol)

@@ -396,6 +396,32 @@ constexpr float kPartUnit = 0x1p-11f;
 constexpr int kWUpLog2 = 8;
 constexpr float kHalvesDown = 1.f / (kXUp * (1 << kWUpLog2));
 
+// Whether f16 holds every weight under a scale: 6 * 2^13 and 0.5 * 2^-23, of two parts' weights
+// 0.5 * 2^-12 * kPartUnit.
+template <int P>
+__device__ inline bool f16_scale(int byte) {
+  constexpr int kLeast = P == 2 ? 127 - 12 - kWUpLog2 : 127 - 23;
+  constexpr int kMost = P == 2 ? 127 + 13 - kWUpLog2 : 127 + 13;
+  return static_cast<unsigned>(byte - kLeast) <= static_cast<unsigned>(kMost - kLeast);
+}
+
+constexpr int kOddX = 1, kOddW = 2;
+// The workgroup's threads' bits (of 0..3) in one, for every thread; lds: free after a barrier.
+// (__syncthreads_or has LDS of its own, which two workgroups of 80 KB do not leave.)
+template <typename T>
+__device__ inline int any_of(int bits, char* lds) {
+  int* const votes = reinterpret_cast<int*>(lds);
+  const int mine = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) votes[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int i = 0; i < T::kThreads / 64; ++i) any |= votes[i];
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(any);
+}
+
 // Four scale bytes from `at` of a row on (an even place): one load where they lie on a word.
 template <bool kWords>
 __device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_t at, bool in,
@@ -410,15 +436,15 @@ __device__ inline uint32_t load_scales(const __amdgpu_buffer_rsrc_t& rs, uint32_
 
 // Adds one tile's products with operands of type E to acc. x goes in P parts: one of its own
 // type, two of f16 (f32 x, E f16: results over kHalvesDown), or with bf16 E part `part` of kParts.
-// Returns (to every thread) whether E cannot hold the tile's operands: a scale of its weights,
-// or a row of f32 x.
+// Returns (to every thread) whether E cannot hold the tile's operands: kOddX, a row of f32 x, and
+// kOddW, a scale of its weights, which may be that of zeros.
 //   A wave's own rows of W come 64 bytes of codes at a time, 4 lanes a row, and change places in
 //   its own LDS: lanes that load the 16 bytes that they multiply touch a cache line each, and
 //   the line lookups bound the kernel (24000 x 5120 -> 1280 f16: 376 us). Lane (r, h)
 //   of a 32-row block takes block h of a stage of row r, widened in registers, and step j
 //   multiplies values 8 j.. of both blocks, so x's operand is chunk 4 h + j of its staged row.
 template <typename T, typename XT, typename E, int P, bool kWords>
-__device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
+__device__ inline int tile_product(const Mx4LinearArgs& a, int grp, int f0, int t0, char* lds,
                                     int u0, int u1, int part,
                                     f32x16 (&acc)[T::WF / 32][T::WT / 32]) {
   constexpr int kF = T::WF / 32, kT = T::WT / 32;
@@ -540,7 +566,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
       }
     }
   };
-  bool odd = false;
+  bool odd_x = false, odd_w = false;
   // Stage d of a pair: operands of step j + 1 are formed behind the products that use their
   // registers last, and the first `n` loads of stage i_s and pair i_p go between them.
   auto multiply = [&](int d, const char* buf, auto n, int i_s, int i_p)
@@ -550,12 +576,8 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
 #pragma unroll
     for (int i = 0; i < kF; ++i) {
       const int byte = (sw[i] >> (16 * d + 8 * hl)) & 255;
-      // f16 holds 6 * 2^13 and 0.5 * 2^-23, of two parts' weights 0.5 * 2^-12 * kPartUnit.
-      constexpr int kLeast = kHalves ? 127 - 12 - kWUpLog2 : 127 - 23;
-      constexpr int kMost = kHalves ? 127 + 13 - kWUpLog2 : 127 + 13;
       if constexpr (__is_same(E, _Float16))
-        odd |= wf + 32 * i + r32 < n_f &&
-               static_cast<unsigned>(byte - kLeast) > static_cast<unsigned>(kMost - kLeast);
+        odd_w |= wf + 32 * i + r32 < n_f && !f16_scale<P>(byte);
       scale[i] = scale_of(kHalves ? byte + kWUpLog2 : byte);
       c[i] = *reinterpret_cast<const u32x4*>(codes + code_at(32 * i + r32, 2 * d + hl));
     }
@@ -647,7 +669,7 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
         if (i == 0) __syncthreads();  // the last stage is read
         if ((tid & 7) == 0) all[kg * T::BT + row] = m;
       }
-      if constexpr (T::KG == 1) odd |= m != 0.f && !(m >= kXLeast && m <= kXMost);
+      if constexpr (T::KG == 1) odd_x |= m != 0.f && !(m >= kXLeast && m <= kXMost);
     }
     if constexpr (T::KG > 1) {
       __syncthreads();
@@ -656,21 +678,47 @@ __device__ inline bool tile_product(const Mx4LinearArgs& a, int grp, int f0, int
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < T::KG; ++i) m = fmaxf(m, all[i * T::BT + threadIdx.x]);
-        odd |= m != 0.f && !(m >= kXLeast && m <= kXMost);
+        odd_x |= m != 0.f && !(m >= kXLeast && m <= kXMost);
       }
     }
   }
-  // (__syncthreads_or has LDS of its own, which two workgroups of 80 KB do not leave.)
-  uint64_t* const votes = reinterpret_cast<uint64_t*>(lds - kg * 2 * kStageBytes);
-  const uint64_t vote = __ballot(odd);
-  __syncthreads();
-  if (lane == 0) votes[threadIdx.x >> 6] = vote;
-  __syncthreads();
-  uint64_t any = 0;
+  return any_of<T>((odd_x ? kOddX : 0) | (odd_w ? kOddW : 0), lds - kg * 2 * kStageBytes);
+}
+
+// Whether a block of a tile's weights has a scale that f16 does not hold and is not of zeros, whose
+// small scale (2^-127 as quantised) does not matter: padded columns and pruned weights. Asked after
+// the product, for tiles that met such a scale. us, 24000 x 5120 -> 1280 without zeros / with the
+// last block of every row of zeros: f16 268/300, f32 575/604, 130 rows 1280 -> 3 x 1280 8.0/9.7,
+// 13.3/14.8 (formed again in bf16 parts 857, 1690, 22.2, 34.6; with the codes looked at within the
+// product's loop f16 286/285, f32, which then spills 63 registers, 814/814).
+template <typename T, int P>
+__device__ inline bool odd_weights(const Mx4LinearArgs& a, int grp, int f0, int u0, int u1,
+                                   char* lds) {
+  const int nb = a.n_in / kMx4Block, b0 = u0 * (kUnit / kMx4Block);
+  const int pairs = (min(nb, u1 * (kUnit / kMx4Block)) - b0) / 2;  // of blocks, of a row
+  const int n = min(T::BF, a.n_out - f0) * pairs;
+  constexpr int kAtOnce = 4;
+  int odd = 0;
+  for (int e0 = threadIdx.x; e0 < n; e0 += kAtOnce * T::kThreads) {
+    int64_t at[kAtOnce];
+    uint32_t two[kAtOnce];
 #pragma unroll
-  for (int i = 0; i < T::kThreads / 64; ++i) any |= votes[i];
-  __syncthreads();
-  return __builtin_amdgcn_readfirstlane(any != 0);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int e = min(e0 + i * T::kThreads, n - 1), row = e / pairs;
+      at[i] = static_cast<int64_t>(f0 + row) * nb + b0 + 2 * (e - row * pairs);
+      two[i] = *reinterpret_cast<const uint16_t*>(a.w_scales[grp] + at[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int byte = (two[i] >> (8 * k)) & 255;
+        if (f16_scale<P>(byte)) continue;
+        const u32x4 c = *reinterpret_cast<const u32x4*>(a.w[grp] + 16 * (at[i] + k));
+        if (byte > 127 || ((c[0] | c[1] | c[2] | c[3]) & 0x77777777u)) odd = 1;
+      }
+  }
+  return any_of<T>(odd, lds) != 0;
 }
 
 // The same for MXFP4 x: 256 columns a stage, codes as they are into 32x32x64 MFMAs. Lane (r, h)
@@ -1022,7 +1070,9 @@ __global__ __launch_bounds__(T::kThreads, T::KG > 1 ? 4 : 2) void mx4_tile(Mx4Li
   } else {
     constexpr int kP = __is_same(XT, float) ? 2 : 1;
     if (kP == 2) down = kHalvesDown;
-    if (tile_product<T, XT, _Float16, kP, kWords>(a, grp, f0, t0, lds, u0, u1, 0, acc)) {
+    int odd = tile_product<T, XT, _Float16, kP, kWords>(a, grp, f0, t0, lds, u0, u1, 0, acc);
+    if (odd == kOddW) odd = odd_weights<T, kP>(a, grp, f0, u0, u1, lds);
+    if (odd) {
       clear();
       down = 1.f;
 #pragma unroll 1
