@@ -575,3 +575,174 @@ def test_weights_far_below_the_largest(wrs, ctx, dtype, octaves):
     t.arena.advance(0, 300)
     t.check(host(t.run()))
     t.arena.close()
+
+
+def head_f64(q, k, v, parents, past):
+    """tree_f64 of one head, all rows at once: outputs and tolerances [n][64]."""
+    n = len(parents)
+    q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
+    seen = np.ones((n, past + n), bool)
+    seen[:, past:] = ancestors(parents)
+    k, v = k[:past + n], v[:past + n]
+    s = np.where(seen, q @ k.T / 8, -np.inf)
+    mag = np.where(seen, np.abs(q) @ np.abs(k).T / 8, 0.0).max(axis=1)
+    largest = np.where(seen, np.abs(s), 0.0).max(axis=1)
+    p = np.exp(s - s.max(axis=1, keepdims=True))
+    p /= p.sum(axis=1, keepdims=True)
+    rel = (2 * (200 * U32 * mag + 8 * U32 * (1 + largest)) + 2 * seen.sum(axis=1) * U32)
+    return p @ v, rel[:, None] * (p @ np.abs(v)) + 1e-30
+
+
+class LargeTrees:
+    """Caches past the size from which blocks of 32 rows run (128 MB of f16 K and V, 384 of f32,
+    and an even number of three or more blocks of 16 rows in the largest tree), drawn on the GPU;
+    some (slot, head) pairs are checked. From head 10 on the history's values are 2^-14 of the
+    drafted rows', so that the outputs are the drafted rows' and one seen too many or too few
+    stands out (of 40000 equal weights one is 2.5e-5, f32 sums of as many may be off by 5e-3)."""
+
+    heads = 20
+
+    def __init__(self, wrs, ctx, dtype, pasts, counts, seed):
+        size, least = (2, 128 << 20) if dtype == "f16" else (4, 384 << 20)
+        blocks = (max(counts) + 15) // 16
+        assert max(counts) > 32 and blocks % 2 == 0
+        assert sum(p + n for p, n in zip(pasts, counts)) * self.heads * 64 * 2 * size >= least
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        rng = np.random.default_rng(seed)
+        d = self.heads * 64
+        self.pasts, self.counts = pasts, counts
+        self.arena = wrs.KvArena(1, len(pasts), self.heads,
+                                 max(p + n for p, n in zip(pasts, counts)) + 8, 0, ctx=ctx,
+                                 dtype=getattr(wrs, "WRS_" + dtype.upper()))
+        store = torch.float16 if dtype == "f16" else torch.float32
+        self.kv = []
+        for s, (p, n) in enumerate(zip(pasts, counts)):
+            k, v = (torch.randn((p + n, d), generator=gen, device="cuda") for _ in range(2))
+            v[:p, 640:] *= 2.0 ** -14
+            k, v = (x.to(store).float() for x in (k, v))
+            self.kv.append((k, v))
+            self.arena.append(0, s, k, v)
+            self.arena.advance(s, pasts[s])
+        self.q = torch.randn((sum(counts), d), generator=gen, device="cuda")
+        self.new_trees(rng)
+        torch.cuda.synchronize()
+
+    def new_trees(self, rng):
+        self.parents = [make_parents(rng, n, rng.choice(["tree", "tree", "chain", "star"]))
+                        for n in self.counts]
+
+    def device_parents(self):
+        return torch.from_numpy(np.concatenate(self.parents).astype(np.int32)).cuda()
+
+    def run(self, out=None, parents=None):
+        out = torch.full_like(self.q, float("nan")) if out is None else out
+        parents = self.device_parents() if parents is None else parents
+        self.arena.tree_self(0, list(range(len(self.counts))), self.counts, parents, self.q, out)
+        return out
+
+    def check(self, out, pairs, rows=None):
+        starts = np.concatenate([[0], np.cumsum(self.counts)])
+        for s, h in pairs:
+            at = slice(64 * h, 64 * h + 64)
+            r = slice(int(starts[s]), int(starts[s + 1]))
+            k, v = (x[:, at].cpu().numpy() for x in self.kv[s])
+            ref, tol = head_f64(self.q[r, at].cpu().numpy(), k, v, self.parents[s], self.pasts[s])
+            err = np.abs(host(out[r, at]).astype(np.float64) - ref)
+            if rows is not None:
+                err, tol = err[rows], tol[rows]
+            assert np.all(err <= tol), (s, h, float((err / tol).max()))
+
+
+LARGE = {  # pasts and counts of the slots
+    # one long history: masks in registers, and (250 nodes) walks in LDS
+    "one_64": lambda f32: ([39400 if f32 else 27000], [64]),
+    "one_250": lambda f32: ([39500 if f32 else 26219], [250]),
+    # ragged trees over many short histories
+    "many": lambda f32: ([1000 - 7 * i for i in range(46 if f32 else 32)],
+                         [(64, 17, 40, 1, 50, 33)[i % 6] for i in range(46 if f32 else 32)]),
+    # large trees beside small ones
+    "both": lambda f32: ([30000 if f32 else 20000, 12000, 0], [96, 64, 255]),
+}
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("case", sorted(LARGE))
+def test_large_caches_match_float64(wrs, ctx, case, dtype):
+    note(f"tree_self, blocks of 32 rows, {case} {dtype}")
+    pasts, counts = LARGE[case](dtype == "f32")
+    t = LargeTrees(wrs, ctx, dtype, pasts, counts, 81)
+    first = t.run()
+    some = sorted({0, 1, 2, 3, len(counts) // 2, len(counts) - 1} & set(range(len(counts))))
+    t.check(first, [(s, h) for s in some for h in (0, 7, 12, 19)])
+    assert bool(torch.isfinite(first).all())
+    for _ in range(3):  # and the same bits each time
+        assert torch.equal(t.run(), first)
+    t.arena.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("nodes", [64, 122])
+def test_large_caches_hide_what_a_row_does_not_see(wrs, ctx, nodes, bad, dtype):
+    """Leaves of either half of a block hold non-finite keys and values; other rows never see
+    them, nor rows behind the tree. A value that rows see is their result."""
+    note(f"tree_self, blocks of 32 rows, {bad} in hidden rows, {nodes} nodes {dtype}")
+    past = 39400 if dtype == "f32" else 26300
+    t = LargeTrees(wrs, ctx, dtype, [past], [nodes], 83)
+    par = np.minimum(make_parents(np.random.default_rng(84), nodes, "tree"), 2)
+    par[nodes - 1] = 40  # a deeper path, through the second half of a block
+    t.parents = [par]
+    leaves = [3, 20, 33, nodes - 2]
+    k, v = (x.clone() for x in t.kv[0])
+    for x in (k, v):
+        x[[past + r for r in leaves]] = bad
+    junk = torch.full((8, t.heads * 64), bad, device="cuda")
+    v[past + 40, 5] = float("inf")  # of head 0, seen by row 40 and the last
+    t.arena.set_len(0, 0)
+    t.arena.append(0, 0, torch.cat([k, junk]), torch.cat([v, junk]))
+    t.arena.advance(0, past)
+    out = t.run()
+    clean = [i for i in range(nodes) if i not in leaves]
+    t.check(out, [(0, 1), (0, 19)], rows=clean)
+    t.check(out, [(0, 0)], rows=[i for i in clean if i not in (40, nodes - 1)])
+    got = host(out)
+    assert np.all(got[[40, nodes - 1], 5] == np.inf)
+    if bad != bad:
+        assert np.all(np.isnan(got[leaves]))
+    t.arena.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("reserved", [True, False])
+def test_large_caches_captured(wrs, reserved, dtype):
+    """Captured with the scratch (chunks) and without (whole), replayed with new trees, eager
+    calls of the same context between the replays."""
+    note(f"tree_self, blocks of 32 rows, captured, reserved {reserved}, {dtype}")
+    c = wrs.Context(0)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        c.use_torch_stream()
+        if reserved:
+            c.reserve(n_heads=20, decode_rows=8, decode_keys=1500)
+        t = LargeTrees(wrs, c, dtype, [27000 if dtype == "f32" else 18000, 13000], [64, 39], 85)
+        par, out = t.device_parents(), torch.full_like(t.q, float("nan"))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            t.run(out=out, parents=par)
+        for seed in range(3):
+            t.new_trees(np.random.default_rng(seed))
+            t.q.copy_(torch.randn(t.q.shape))
+            par.copy_(t.device_parents())
+            out.fill_(float("nan"))
+            g.replay()
+            side.synchronize()
+            some = [(0, 3), (0, 18), (1, 9), (1, 10)]
+            t.check(out, some)
+            eager = t.run()
+            side.synchronize()
+            t.check(eager, some)
+            if reserved:
+                assert torch.equal(eager, out)
+        t.arena.close()
+    c.close()
