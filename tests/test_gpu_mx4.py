@@ -749,3 +749,35 @@ def test_zeros_under_any_scale(wrs, ctx, rows, byte, x_dtype):
         assert np.all(np.isnan(got[:, 11]))
         got[:, 11] = y[:, 11] = tol[:, 11] = 0.0
     assert np.all(np.abs(got - y) <= tol)
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
+@pytest.mark.parametrize("rows,n_in,n_out,groups", [
+    (5, 64, 512, 1), (16, 256, 512, 1), (5, 1280, 5120, 1), (8, 1280, 51866, 1),  # the stream
+    (16, 1600, 48, 3), (5, 5120, 1280, 1), (16, 5120, 1280, 1), (16, 65536, 16, 1),  # split
+    (40, 64, 512, 1), (33, 256, 70, 1), (130, 1280, 1280, 3), (1500, 1280, 1530, 1),  # tiles
+    (2100, 256, 2500, 1), (300, 5120, 5120, 1),
+    (33, 2112, 500, 3), (17, 5120, 1280, 1), (130, 5120, 1280, 1), (20, 65536, 16, 1),  # split
+])
+def test_norm_of_the_error(wrs, ctx, rows, n_in, n_out, groups, x_dtype):
+    """The whole result's error against its norm, which unlike a bound of the absolute sums sees
+    a part of x that is lost. Roundings of random terms add in squares: each of the n f32 sums is
+    off by u / sqrt(3) of what it holds then, sqrt(k / n) of the result after k products, and the
+    operands of each product by 2^-22 / sqrt(3): sqrt(n / 6 + 16 / 3) u, here twice that (one
+    f16 part alone leaves about 2e-4, two bf16 parts 4e-6)."""
+    note(f"linear_mx4 {rows} x {n_in} -> {n_out} x {groups} {x_dtype}, norm of the error")
+    rng = np.random.default_rng(23)
+    x = torch.from_numpy(rng.standard_normal((rows, n_in)).astype(np.float32)).cuda()
+    if x_dtype == "mx4":
+        x = wrs.mx4_quantize(x, ctx=ctx)
+        xr = unpack_f64(x.codes.cpu().numpy(), x.scales.cpu().numpy())
+    else:
+        x = x.to(DT[x_dtype])
+        xr = x.double().cpu().numpy()
+    ws = [make(wrs, ctx, rng, n_out, n_in) for _ in range(groups)]
+    outs = [torch.full((rows, n_out), float("nan"), device="cuda") for _ in ws]
+    wrs.linear_mx4(x, [w for w, _ in ws], None, outs, ctx=ctx)
+    for (_, w), out in zip(ws, outs):
+        y = xr @ w.T
+        off = np.linalg.norm(host(out).astype(np.float64) - y) / np.linalg.norm(y)
+        assert off <= 2 * U32 * np.sqrt(n_in / 6 + 16 / 3), off

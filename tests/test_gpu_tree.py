@@ -746,3 +746,45 @@ def test_large_caches_captured(wrs, reserved, dtype):
                 assert torch.equal(eager, out)
         t.arena.close()
     c.close()
+
+
+def norm_bound(keys):
+    """How far the norm of the outputs' error may be off, of the outputs' norm: roundings of
+    random terms add in squares. A score of size 1 is off by 64 sums and products, the maximum
+    and the exponential, 8 u in all, and so is its weight; a sum over n keys of either sign by
+    sqrt(n / 6) u, one of weights by sqrt(n / 9) u. Twice that (q in one f16 part alone leaves
+    about 1e-4)."""
+    return 2 * U32 * np.sqrt(64 + keys / 6 + keys / 9)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("case", [i for i, c in enumerate(CASES) if max(c[1]) >= 100])
+def test_norm_of_the_error(wrs, ctx, case, dtype):
+    heads, pasts, counts, shape = CASES[case]
+    note(f"tree_self {dtype}, norm of the error, heads={heads} pasts={pasts} counts={counts}")
+    t = Trees(wrs, ctx, getattr(wrs, "WRS_" + dtype.upper()), heads, pasts, counts, shape,
+              200 + case)
+    got, row = host(t.run()).astype(np.float64), 0
+    for s, (p, n) in enumerate(zip(pasts, counts)):
+        ref, _ = tree_f64(t.q[row:row + n], t.k[s], t.v[s], t.parents[s], p, heads)
+        off = np.linalg.norm(got[row:row + n] - ref) / np.linalg.norm(ref)
+        assert off <= norm_bound(p + n), (s, off)
+        row += n
+    t.arena.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("case", sorted(LARGE))
+def test_norm_of_the_error_of_large_caches(wrs, ctx, case, dtype):
+    note(f"tree_self, blocks of 32 rows, norm of the error, {case} {dtype}")
+    pasts, counts = LARGE[case](dtype == "f32")
+    t = LargeTrees(wrs, ctx, dtype, pasts, counts, 87)
+    out, starts = t.run(), np.concatenate([[0], np.cumsum(counts)])
+    for s in sorted({0, 1, len(counts) - 1} & set(range(len(counts)))):
+        for h in (1, 9):
+            at, r = slice(64 * h, 64 * h + 64), slice(int(starts[s]), int(starts[s + 1]))
+            k, v = (x[:, at].cpu().numpy() for x in t.kv[s])
+            ref, _ = head_f64(t.q[r, at].cpu().numpy(), k, v, t.parents[s], pasts[s])
+            off = np.linalg.norm(host(out[r, at]) - ref) / np.linalg.norm(ref)
+            assert off <= norm_bound(pasts[s] + counts[s]), (s, h, off)
+    t.arena.close()
