@@ -104,7 +104,7 @@ const char *wrs_attn_status_string(int status);
  * fixed buffer (~8 MB on 256 CUs) under the same rule;
  * and fused norms of decode rows over many features (wrs_linear_fused), likewise
  * (reserving linear_tokens allocates both). Tree attention splits long caches through
- * a third one (~9 MB, which reserving heads with decode rows and keys allocates too)
+ * a third one (~4 MB, which reserving heads with decode rows and keys allocates too)
  * and, captured before it exists, runs unsplit. Switching streams
  * (wrs_attn_set_stream) drains the old stream unless either stream is
  * recording a graph. Zero fields are ignored; reserving never shrinks.

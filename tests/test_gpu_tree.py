@@ -788,3 +788,18 @@ def test_norm_of_the_error_of_large_caches(wrs, ctx, case, dtype):
             off = np.linalg.norm(host(out[r, at]) - ref) / np.linalg.norm(ref)
             assert off <= norm_bound(pasts[s] + counts[s]), (s, h, off)
     t.arena.close()
+
+
+def test_reserved_scratch_is_what_trees_can_use(wrs):
+    """Reserving decode rows gives a context the scratch of split caches: partial rows of as many
+    workgroups as a launch splits into (512 of 32 rows of 66 floats, 4.3 MB), no more."""
+    note("reserve of eight contexts (no launch)")
+    made = [wrs.Context(0) for _ in range(8)]
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info(0)[0]
+    for c in made:
+        c.reserve(n_heads=1, decode_rows=1, decode_keys=64)
+    taken = before - torch.cuda.mem_get_info(0)[0]
+    for c in made:
+        c.close()
+    assert taken <= 8 * 7 * 2 ** 20, taken / 8

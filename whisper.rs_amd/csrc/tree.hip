@@ -729,11 +729,10 @@ int64_t tree_plan(TreeArgs& a, DType dt, bool split) {
   // at once (f16, 16 nodes over 65471 keys: 90 us with one, 73 with two, 76 with three; 64 nodes
   // 122, and 130 with eight workgroups more).
   const int whole = dt == kF16 ? 512 : 320, least = dt == kF16 ? 256 : 128;
-  constexpr int kWgs = 512;
-  if (split && blocks < kTreeMaxWgs / 2 && longest > whole) {
-    int64_t chunk = std::max<int64_t>(least, (work + kWgs - 1) / kWgs);
+  if (split && blocks < kTreeMaxWgs && longest > whole) {
+    int64_t chunk = std::max<int64_t>(least, (work + kTreeMaxWgs - 1) / kTreeMaxWgs);
     for (chunk = (chunk + 127) / 128 * 128; chunk < longest; chunk += 128)
-      if (lay(chunk) <= kWgs) return widest;
+      if (lay(chunk) <= kTreeMaxWgs) return widest;
   }
   lay(longest);
   return widest;

@@ -233,7 +233,7 @@ constexpr size_t kRowsMaxKeys = (size_t{1} << 24) - 4095;
 constexpr int kTreeMaxTrees = 64;   // per launch
 constexpr int kTreeMaxNodes = 256;  // of one tree
 constexpr int kTreeMaxRows = 32;    // query rows of a workgroup, at most
-constexpr int kTreeMaxWgs = 1024;   // workgroups of a launch that splits keys
+constexpr int kTreeMaxWgs = 512;    // workgroups of a launch that splits keys: two a CU
 constexpr int kTreePart = 66;       // floats of a partial row: max, sum, 64 sums
 constexpr size_t kTreePartFloats = size_t{kTreeMaxWgs} * kTreeMaxRows * kTreePart;
 constexpr size_t kTreeCounterWords = size_t{kTreeMaxWgs} * 32;
