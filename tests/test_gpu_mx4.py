@@ -781,3 +781,30 @@ def test_norm_of_the_error(wrs, ctx, rows, n_in, n_out, groups, x_dtype):
         y = xr @ w.T
         off = np.linalg.norm(host(out).astype(np.float64) - y) / np.linalg.norm(y)
         assert off <= 2 * U32 * np.sqrt(n_in / 6 + 16 / 3), off
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 130, 2100])
+def test_gelu_is_one_function_for_any_rows(wrs, ctx, rows, x_dtype):
+    """GELU of numbers that the products give exactly, small results among them, relative to
+    themselves: x / (1 + exp(-2 u)) is off by its exponential's argument, whose constants and
+    four operations round, 6 u of 2 u(x), and by a few roundings of the rest."""
+    note(f"linear_mx4 {rows} rows {x_dtype}, gelu")
+    w = torch.zeros((640, 64), device="cuda")
+    w[:, 3] = torch.arange(640, device="cuda") % 3 - 1.0
+    m = wrs.mx4_quantize(w, ctx=ctx)
+    x = torch.zeros((rows, 64), device="cuda")
+    x[:, 3] = torch.linspace(-6, 6, rows, device="cuda") if rows > 1 else -4.0
+    x = x.bfloat16().float()
+    if x_dtype == "mx4":
+        x = wrs.mx4_quantize(x, ctx=ctx)
+        xr = unpack_f64(x.codes.cpu().numpy(), x.scales.cpu().numpy())
+    else:
+        x = x.to(DT[x_dtype])
+        xr = x.double().cpu().numpy()
+    out = torch.full((rows, 640), float("nan"), device="cuda")
+    wrs.linear_mx4(x, [m], None, [out], act="gelu", ctx=ctx)
+    y = xr @ unpack_f64(m.codes.cpu().numpy(), m.scales.cpu().numpy()).T
+    two_u = 2 * 0.7978846 * np.abs(y) * (1 + 0.044715 * y * y)
+    ref = gelu(y)
+    assert np.all(np.abs(host(out) - ref) <= (6 * two_u + 16) * U32 * np.abs(ref))

@@ -57,6 +57,15 @@ __device__ inline bf16x8 widen8(uint32_t w, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// GELU of the projections, x / (1 + exp(-2 u)): 0.5 x (1 + tanh u) without the tanh, u = 0.7978846
+// (x + 0.044715 x^3). Seven instructions (two more, with u formed first, took 3 us of 165), and
+// small results keep their bits, which 1 + tanh u loses as tanh u nears -1.
+__device__ inline float gelu_exp(float x) {
+  constexpr float kOne = -2.f * 0.7978846f * 1.44269504f, kThree = kOne * 0.044715f;
+  const float e = __builtin_amdgcn_exp2f(x * __builtin_fmaf(x * x, kThree, kOne));
+  return x * __builtin_amdgcn_rcpf(1.f + e);
+}
+
 constexpr int kRawBuffer = 0x00020000;  // buffer resource word 3: raw, 32-bit data format
 constexpr uint32_t kPast = 0xFFFF0000u;  // an offset past every buffer
 constexpr uint32_t kPastRows = 0x80000000u;  // so with offsets of rows (below 2^28) added
@@ -271,7 +280,7 @@ __global__ __launch_bounds__(64 * kRowsWaves, kMany ? 4 : 2) void mx4_rows(Mx4Li
   __syncthreads();
   auto store = [&](int t, int r, float y) __attribute__((always_inline)) {
     if (a.bias[grp]) y += a.bias[grp][r];
-    if (a.act == kActGelu) y = gelu_tanh(y);
+    if (a.act == kActGelu) y = gelu_exp(y);
     const int64_t o = t * a.out_rs + (r >> 6) * a.out_hs + (r & 63);
     if (out_dt == kF32)
       static_cast<float*>(a.out[grp])[o] = y;
@@ -345,14 +354,6 @@ __device__ inline f32x16 mfma32(const u32x4& a, const u32x4& b, const f32x16& c)
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-// GELU of the projections, x / (1 + exp(-2 u)): 0.5 x (1 + tanh u) without the tanh, u = 0.7978846
-// (x + 0.044715 x^3). Seven instructions (two more, with u formed first, took 3 us of 165).
-__device__ inline float gelu_exp(float x) {
-  constexpr float kOne = -2.f * 0.7978846f * 1.44269504f, kThree = kOne * 0.044715f;
-  const float e = __builtin_amdgcn_exp2f(x * __builtin_fmaf(x * x, kThree, kOne));
-  return x * __builtin_amdgcn_rcpf(1.f + e);
 }
 
 // Tile of a workgroup: BF features x BT rows of x, waves of WF x WT; KG groups of waves take the
