@@ -803,3 +803,52 @@ def test_reserved_scratch_is_what_trees_can_use(wrs):
     for c in made:
         c.close()
     assert taken <= 8 * 7 * 2 ** 20, taken / 8
+
+
+def test_drafts_of_several_slots_from_one_projection(wrs, ctx):
+    """One projection makes q, k and v of every drafted row; each slot's rows are appended from
+    it, one call attends them all, and the accepted paths are kept and taken in."""
+    note("linear_mx4, append per slot, tree_self, keep_rows over three slots")
+    heads, pasts, counts = 3, [20, 0, 41], [7, 12, 5]
+    d, slots, total = heads * 64, [2, 0, 1], sum(counts)
+    rng = np.random.default_rng(91)
+    w_qkv = [dev((rng.standard_normal((d, d)) * d ** -0.5).astype(np.float32)).half()
+             for _ in range(3)]
+    b_q, b_v = (dev(rng.standard_normal(d).astype(np.float32)) for _ in range(2))
+    ar = wrs.KvArena(1, 3, heads, 64, 0, ctx=ctx, dtype=wrs.WRS_F32)
+    old = [tuple(dev(rng.standard_normal((p, d)).astype(np.float32)) for _ in range(2))
+           for p in pasts]
+    for s, p, (k, v) in zip(slots, pasts, old):
+        if p:
+            ar.append(0, s, k, v)
+            ar.advance(s, p)
+    x = dev(rng.standard_normal((total, d)).astype(np.float32))
+    q, k, v, att = (torch.full((total, d), float("nan"), device="cuda") for _ in range(4))
+    trees = [make_parents(rng, n, "tree") for n in counts]
+    parents = torch.from_numpy(np.concatenate(trees).astype(np.int32)).cuda()
+
+    w_q, w_k, w_v = (wrs.mx4_quantize(w, ctx=ctx) for w in w_qkv)
+    wrs.linear_mx4(x, [w_q, w_k, w_v], [b_q, None, b_v], [q, k, v], ctx=ctx)
+    r0 = 0
+    for s, n in zip(slots, counts):
+        ar.append(0, s, k[r0:r0 + n], v[r0:r0 + n])
+        r0 += n
+    ar.tree_self(0, slots, counts, parents, q, att)
+    paths = [[0, 3, 6], [], [1, 4]]
+    ar.keep_rows(slots, [len(p) for p in paths], [r for p in paths for r in p])
+    for s, p in zip(slots, paths):
+        ar.advance(s, len(p))
+
+    kh, vh, qh, got, r0 = host(k), host(v), host(q), host(att), 0
+    kp, vp = _planes(wrs, ar, "<f4", (1, 3, heads, 64, 64))
+    for s, p, n, par, path, (k0, v0) in zip(slots, pasts, counts, trees, paths, old):
+        kk, vv = (np.concatenate([host(a), b[r0:r0 + n]]) for a, b in ((k0, kh), (v0, vh)))
+        ref, tol = tree_f64(qh[r0:r0 + n], kk, vv, par, p, heads)
+        assert np.all(np.abs(got[r0:r0 + n] - ref) <= tol)
+        assert ar.slot_len(s) == p + len(path)
+        for plane, rows in ((kp, kk), (vp, vv)):
+            want = np.concatenate([rows[:p], rows[p:][path]]).reshape(-1, heads, 64)
+            kept = plane[0, s].transpose(0, 1)[:p + len(path)].cpu().numpy()
+            assert np.array_equal(kept, want)
+        r0 += n
+    ar.close()
