@@ -99,9 +99,10 @@ const char *wrs_attn_status_string(int status);
  * blocks split over two workgroups through a fixed context buffer (~9 MB on
  * 256 CUs), allocated by the first such call outside capture; during capture
  * before then, the call takes another schedule instead; projections of more
- * than 8 rows over n_in >= 2048 whose tiles cover less than half the CUs, and few
- * rows over long MXFP4 weights (wrs_linear_mx4), which split k through another
- * fixed buffer (~8 MB on 256 CUs) under the same rule;
+ * than 8 rows over n_in >= 2048 whose tiles cover less than half the CUs, and MXFP4
+ * projections (wrs_linear_mx4) of any rows over long columns whose features leave CUs
+ * idle, which split k through another fixed buffer (~8 MB on 256 CUs) under the same
+ * rule;
  * and fused norms of decode rows over many features (wrs_linear_fused), likewise
  * (reserving linear_tokens allocates both). Tree attention splits long caches through
  * a third one (~4 MB, which reserving heads with decode rows and keys allocates too)
@@ -300,8 +301,8 @@ int wrs_attn_prefill_cross(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const fl
 /* Self-attention of drafted tokens: what decoder.rs:613-647 computes for a chain,
  * for trees of drafted continuations, so that one pass over the weights checks
  * several of them. Tree i holds n_nodes[i] rows (0..256) of slots[i] (host arrays;
- * a slot may carry several trees), whose K/V rows wrs_kv_append stored at the
- * slot's length (not advanced). `parents` is a device array of int32, one per row
+ * several trees of a slot share its drafted rows), whose K/V rows wrs_kv_append stored
+ * at the slot's length (not advanced). `parents` is a device array of int32, one per row
  * in the order of q, read when the call runs (a replayed graph takes new trees):
  * row r of a tree hangs from row parents[r] of the same tree if that is in [0, r),
  * from the last cached token otherwise, and attends the slot's slot_len rows, its

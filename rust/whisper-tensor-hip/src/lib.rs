@@ -205,7 +205,6 @@ pub mod ffi {
             n_tokens: usize, n_in: usize, n_out: usize, activation: c_int, out_dtype: c_int,
             out: *const *mut c_void, out_len: *const usize, out_row_stride: i64,
             out_head_stride: i64) -> c_int;
-        // norm.rs:116-143 and gelu.rs:11-23 over device f32 rows
         // MXFP4 rows and the projections with them
         pub fn wrs_mx4_quantize(ctx: *mut WrsCtx, x_dtype: c_int, x: *const c_void, x_len: usize,
             x_row_stride: i64, n_rows: usize, n_cols: usize, codes: *mut c_void,
@@ -219,6 +218,7 @@ pub mod ffi {
             bias: *const *const f32, n_tokens: usize, n_in: usize, n_out: usize,
             activation: c_int, out_dtype: c_int, out: *const *mut c_void,
             out_len: *const usize, out_row_stride: i64, out_head_stride: i64) -> c_int;
+        // norm.rs:116-143 and gelu.rs:11-23 over device f32 rows
         pub fn wrs_layer_norm(ctx: *mut WrsCtx, x: *const f32, x_len: usize,
             gamma: *const f32, beta: *const f32, eps: f32, n_tokens: usize, d_model: usize,
             out_dtype: c_int, out: *mut c_void, out_len: usize) -> c_int;

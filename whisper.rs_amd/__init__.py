@@ -607,7 +607,7 @@ class KvArena:
     def tree_self(self, layer, slots, counts, parents, q, out):
         """Self-attention of drafted trees (``wrs_attn_tree_self``): ``counts[i]`` rows of
         ``slots[i]``, appended and not advanced, each against the slot's history, its
-        ancestors and itself. ``parents`` int32 CUDA tensor, one per row: the parent's
+        ancestors and itself (trees of one slot share its drafted rows). ``parents`` int32 CUDA tensor, one per row: the parent's
         index within the tree, or -1 for a child of the last cached token. ``q`` and
         ``out`` float32 [sum(counts)][d_model], rows of any stride."""
         n, d, q_rs = _rows(q, "tree_self")

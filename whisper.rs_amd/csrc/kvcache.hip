@@ -117,8 +117,8 @@ __global__ __launch_bounds__(256) void kv_copy_planes(const _Float16* k_src, _Fl
 // and in order this is safe: sources rise and are at or above their destinations, so no
 // pass writes a row that a later one reads. Bound by the launch and two round trips to
 // memory: 5 rows of a slot, 20 heads x 32 layers f16 3.3 us, 7 rows of 16 slots, 12 x 12 f32 5.1
-// (smallest launch 2.3). Sources come as packed words by scalar loads: from an array of ints, a load per lane and
-// row, the second took 9.2 us.
+// (smallest launch 2.3). Sources come as packed words by scalar loads: from an array of ints, a
+// load per lane and row, the second took 9.2 us.
 constexpr int kKeepWaves = 4;
 template <int kSlots, int kMoves>
 __global__ __launch_bounds__(64 * kKeepWaves) void kv_keep_rows(KeepArgs<kSlots, kMoves> a) {

@@ -1038,7 +1038,7 @@ constexpr int kPanel = 8;
 //   weights of scales 2^-23 to 2^13 exactly (beside two parts of x 2^-20 to 2^5), and rows of f32
 //   x whose largest value is of ordinary size; a tile that meets others is formed again from bf16
 //   operands, which hold any, one of x's two or three parts after the other.
-//   24000 x 5120 -> 1280: f16 291 us, 1080 TFLOP/s, the matrix pipe 57% busy and the card's power
+//   24000 x 5120 -> 1280: f16 284 us, 1110 TFLOP/s, the matrix pipe 58% busy and the card's power
 //   the bound (the library's product of f16 weights 274), bf16 265, f32 595, MXFP4 101, 3.1
 //   PFLOP/s (zeros in its place a quarter less); 1280 -> 5120 MXFP4 with GELU 127, of which the
 //   epilogue's 123 M outputs are about 50. 130 rows f32, 3 x 1280 -> 1280 13.1 us: ten steps of x's
@@ -1214,8 +1214,8 @@ constexpr int kMidLeast = 180;  // workgroups
 
 // Splits of the columns of small tiles that leave CUs idle over long rows, of kUnitsLeast units at
 // least. The sums' way through memory costs ~2 us. us, split / not, 5120 -> 1280 (20 units): f32 17
-// rows 11.7/21.5, 64 12.7/22.1, 130 17.0/22.8; f16 64 10.3/14.0, 130 12.3/14.8; MXFP4 x, whose
-// units are cheap, 64 9.0/9.0. 2048 -> 512 (8 units): f32 40 rows 10.1/11.5, f16 8.0/7.7, MXFP4
+// rows 11.3/20.7, 64 11.7/21.3, 130 15.7/21.5; f16 64 9.8/13.1, 130 11.1/13.0; MXFP4 x, whose
+// units are cheap, 64 9.0/9.0. 2048 -> 512 (8 units): f32 40 rows 9.4/10.8, f16 8.0/7.7, MXFP4
 // 7.2/6.4; 1280 -> 1280 (5) in units of two at least: f32 9.9/9.8, f16 8.1/7.0.
 constexpr int kUnitsLeast = 4;
 int tile_splits(const Mx4LinearArgs& a, DType x_dt) {
@@ -1262,11 +1262,13 @@ template <typename XT, typename OT>
 hipError_t launch_tiles(const Mx4LinearArgs& a, DType out_dt, hipStream_t s) {
   // The largest tile that fills the chip: larger ones read x and W less often, but a CU without
   // a workgroup does nothing. Both sides of each step by workgroups, us:
-  //   Large, 180 (f32, 1500 rows, 3 x 1280 -> 1280): 46.6, Wide 49.3; 120 (f32, 3000 rows 5120 ->
-  //   1280): 138, Wide 109.
-  //   Wide, 144 (f32, 1500 rows 384 -> 1536): 14.4, Mid 16.1; 120 (f32, 1500 rows 1280 -> 1280):
-  //   29.4, Mid 21.7.
+  //   Large, 180 (f32, 1500 rows, 3 x 1280 -> 1280): 45.6, Wide 50.3; 120 (f32, 3000 rows 5120 ->
+  //   1280): 140, Wide 108.
+  //   Wide, 144 (f32, 1500 rows 384 -> 1536): 13.0, Mid 14.7; 120 (f32, 1500 rows 1280 -> 1280):
+  //   30.6, Mid 21.8.
   //   Mid, 180 (MXFP4, 130 rows, 3 x 1280 -> 1280): 7.4, Small 8.0; 60 (40 rows): 6.7, Small 6.1.
+  // Few rows over a vocabulary's features take large tiles too, mostly empty ones (17 rows 1280 ->
+  // 51866: f32 43.5, Mid 37.6; f16 24.0, Mid 21.7; MXFP4 15.9, Wide 15.3; Mid 17.3).
   using Large = Tile<256, 128, 64, 128, 1>;
   if (tile_wgs<Large>(a) >= 160) return launch_tile<Large, XT, OT>(a, out_dt, s);
   if (tile_wgs<Wide>(a) >= 144) return launch_tile<Wide, XT, OT>(a, out_dt, s);

@@ -186,8 +186,8 @@ struct Sums {
 // A wave's pieces of kSpan keys (kSpan * wave, + kSpan * kWaves, ..) on the f32 matrix pipe, 16
 // at a time, f16 planes widened exactly: lane (c, g) holds key c's values d = 16 g + 0..15, so
 // that lane (r, g) gets scores of keys 4 g + 0..3 of row r, which are the B operand of
-// O^T += V^T P^T as they stand. o[rt][dt][e] is column 16 g + 4 e + dt. q: d = 16 g + 0..15 of row c, times scale * log2(e).
-// `sight` runs once the first loads are on their way (it may hold barriers).
+// O^T += V^T P^T as they stand. o[rt][dt][e] is column 16 g + 4 e + dt. q: d = 16 g + 0..15 of row
+// c, times scale * log2(e). `sight` runs once the first loads are on their way (it may hold barriers).
 template <typename KT, int kRT, int kSpan, typename F>
 __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4], int wave, int lane,
                                   F sight, const Sight<kRT>& seen_by, Sums<kRT>& st) {

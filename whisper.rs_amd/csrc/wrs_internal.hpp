@@ -324,13 +324,13 @@ struct Mx4LinearArgs {
   const uint8_t* w_scales[kMx4Groups];
   const float* bias[kMx4Groups];  // nullable entries
   void* out[kMx4Groups];
-  // Few rows over long ones: room for partial sums, and zeroed counters (nullptr: no split).
+  // Few features over long rows: room for partial sums, and zeroed counters (nullptr: no split).
   float* part;
   size_t part_floats;
   unsigned* counters;
   size_t counter_words;
 };
-// Few rows that split over workgroups where they find scratch.
+// Whether a call's columns split over workgroups where it finds scratch.
 bool linear_mx4_splits(const Mx4LinearArgs& a, DType x_dt);
 hipError_t launch_linear_mx4(const Mx4LinearArgs& a, DType x_dt, DType out_dt, hipStream_t s);
 
@@ -439,8 +439,9 @@ hipError_t launch_kv_copy_planes(const _Float16* k_src, _Float16* k_dst, const _
                                  _Float16* v_dst, int64_t layer_stride, int64_t plane_stride,
                                  int n_layers, int n_heads, int len, hipStream_t s);
 // Rows of a plane that come together: of slot u, at element off[u] of k and v, rows
-// past[u] + src[first[u] + i] move to past[u] + dst0[u] + i, for i < count[u] in order; src rises and is at least its destination. Plane (l, h) at +
-// l*layer_stride + h*plane_stride, rows of `units` 16-byte units.
+// past[u] + src[first[u] + i] move to past[u] + dst0[u] + i, for i < count[u] in order; src rises
+// and is at least its destination. Plane (l, h) at + l*layer_stride + h*plane_stride, rows of
+// `units` 16-byte units.
 // Arguments are copied per launch and read by every workgroup: those of few slots are small.
 constexpr int kKeepSlots = 64;   // per launch
 constexpr int kKeepMoves = 768;  // per launch, of all slots, eight to a line of a slot
