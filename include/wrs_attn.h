@@ -452,9 +452,10 @@ int wrs_mx4_dequantize(wrs_attn_ctx *ctx, const void *codes, size_t codes_len, c
  * apart (x_scales NULL), or with x_dtype WRS_MX4 packed MXFP4 rows (x_row_stride ==
  * n_in, x_len in values). bias may be NULL, or hold NULL entries. n_in % 64 == 0;
  * any n_out. Scales here are 2-byte aligned. f16, bf16 and MXFP4 x enter the products
- * whole, and so does f32 x of up to 16 rows. More f32 rows enter within 2^-22 of a value
- * down to 2^-21 and within 2^-43 below, where the row's largest value lies in
- * [2^-10, 511] and the weights' scales in 2^-20 .. 2^5, and whole otherwise. */
+ * whole, and so does f32 x of up to 16 rows (down to its bit of 2^-133). More f32 rows
+ * enter within 2^-22 of a value down to 2^-21 and within 2^-43 below, where the row's
+ * largest value lies in [2^-10, 511] and the weights' scales in 2^-20 .. 2^5, and like
+ * few rows otherwise. */
 int wrs_linear_mx4(wrs_attn_ctx *ctx, int x_dtype, const void *x, const void *x_scales,
                    size_t x_len, int64_t x_row_stride, size_t n_groups, const void *const *w,
                    const void *const *w_scales, const float *const *bias, size_t n_tokens,

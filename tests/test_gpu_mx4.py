@@ -808,3 +808,49 @@ def test_gelu_is_one_function_for_any_rows(wrs, ctx, rows, x_dtype):
     two_u = 2 * 0.7978846 * np.abs(y) * (1 + 0.044715 * y * y)
     ref = gelu(y)
     assert np.all(np.abs(host(out) - ref) <= (6 * two_u + 16) * U32 * np.abs(ref))
+
+
+@pytest.mark.parametrize("x_dtype", ["f32", "f16", "bf16", "mx4"])
+@pytest.mark.parametrize("rows", [1, 6, 40, 300])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_groups_side_by_side_in_wider_rows(wrs, ctx, rows, pad, x_dtype):
+    """q, k and v as column slices of one tensor, its rows on 16 bytes or not; what lies between
+    them stays."""
+    note(f"linear_mx4 {rows} rows {x_dtype} into slices of rows padded by {pad}")
+    rng = np.random.default_rng(24)
+    d = 192
+    ws = [make(wrs, ctx, rng, d, 128) for _ in range(3)]
+    x = torch.from_numpy(rng.standard_normal((rows, 128)).astype(np.float32)).cuda()
+    if x_dtype == "mx4":
+        x = wrs.mx4_quantize(x, ctx=ctx)
+        xr = unpack_f64(x.codes.cpu().numpy(), x.scales.cpu().numpy())
+    else:
+        x = x.to(DT[x_dtype])
+        xr = x.double().cpu().numpy()
+    for out in ("f32", "f16", "bf16"):
+        wide = torch.full((rows + 1, 3 * d + 3 * pad), 7.0, dtype=DT[out], device="cuda")
+        at = [g * (d + pad) + pad for g in range(3)]
+        wrs.linear_mx4(x, [w for w, _ in ws], None, [wide[:, a:a + d] for a in at],
+                       out_row_stride=wide.shape[1], ctx=ctx)
+        got, rest = host(wide).astype(np.float64), np.ones(wide.shape, bool)
+        for a, (_, w) in zip(at, ws):
+            y, tol = reference(xr, w, None, None, out)
+            assert np.all(np.abs(got[:rows, a:a + d] - y) <= tol)
+            rest[:rows, a:a + d] = False
+        assert np.all(got[rest] == 7.0)
+
+
+@pytest.mark.parametrize("rows", [3, 16, 40, 300])
+@pytest.mark.parametrize("octaves", [100, 115, 130])
+def test_f32_x_next_to_the_smallest(wrs, ctx, rows, octaves):
+    """f32 x goes in bf16 parts where two f16 ones do not hold it; their last bit is 2^-133."""
+    note(f"linear_mx4 {rows} rows f32 at 2^-{octaves}")
+    rng = np.random.default_rng(25)
+    w = rng.standard_normal((70, 128)) * 2.0 ** 60
+    m = wrs.mx4_quantize(torch.from_numpy(w.astype(np.float32)).cuda(), ctx=ctx)
+    wf = unpack_f64(m.codes.cpu().numpy(), m.scales.cpu().numpy())
+    x = torch.from_numpy((rng.standard_normal((rows, 128)) * 2.0 ** -octaves).astype(np.float32))
+    out = torch.full((rows, 70), float("nan"), device="cuda")
+    wrs.linear_mx4(x.cuda(), [m], None, [out], ctx=ctx)
+    y, tol = reference(x.double().numpy(), wf, None, None, "f32")
+    assert np.all(np.abs(host(out) - y) <= tol + 2.0 ** -133 * np.abs(wf).sum(axis=1))

@@ -4,6 +4,8 @@ that each drafted row sees, and a whole verification step of a small decoder wit
 MXFP4 projections against decoding the accepted tokens one by one."""
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -852,3 +854,82 @@ def test_drafts_of_several_slots_from_one_projection(wrs, ctx):
             assert np.array_equal(kept, want)
         r0 += n
     ar.close()
+
+
+def test_keep_rows_captured(wrs):
+    """A replayed graph makes the moves it was captured with, whatever the rows hold by then;
+    eager calls of the same arena run between the replays."""
+    note("keep_rows captured and replayed")
+    c = wrs.Context(0)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        c.use_torch_stream()
+        ar = wrs.KvArena(2, 3, 2, 64, 0, ctx=c)
+        planes = _planes(wrs, ar, "<f2", (2, 3, 2, 64, 64))
+        for s, n in enumerate((5, 0, 30)):
+            ar.advance(s, n)
+        moves = {0: [1, 4, 9], 1: [], 2: [0, 2, 3, 33]}
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            ar.keep_rows(list(moves), [len(r) for r in moves.values()], sum(moves.values(), []))
+        for _ in range(4):
+            for p in planes:
+                p.copy_(torch.randn(p.shape, device="cuda"))
+            want = [p.clone() for p in planes]
+            for p, x in zip(planes, want):
+                for s, past in ((0, 5), (2, 30)):
+                    x[:, s, :, past:past + len(moves[s])] = \
+                        p[:, s][:, :, torch.tensor(moves[s], device="cuda") + past]
+            g.replay()
+            side.synchronize()
+            assert all(torch.equal(p, x) for p, x in zip(planes, want))
+            ar.keep_rows([1], [1], [7])
+            for x in want:
+                x[:, 1, :, 0] = x[:, 1, :, 7]
+            side.synchronize()
+            assert all(torch.equal(p, x) for p, x in zip(planes, want))
+        ar.close()
+    c.close()
+
+
+def test_nothing_kept(wrs, ctx):
+    note("keep_rows of empty paths")
+    ar = wrs.KvArena(1, 2, 2, 32, 0, ctx=ctx)
+    ar.keep_rows([], [], [])
+    ar.keep_rows([0, 1], [0, 0], [])
+    ar.keep_rows([1], [3], [0, 1, 2])  # in place already
+    ar.close()
+
+
+def test_another_context_than_the_arenas(wrs, ctx):
+    """A context of the same device attends an arena that another one made, on its own stream."""
+    note("wrs_attn_tree_self from a second context")
+    t = Trees(wrs, ctx, wrs.WRS_F16, 2, [1400, 70], [20, 9], "tree", 95)
+    q, par = dev(t.q), t.device_parents()
+    out = torch.full_like(q, float("nan"))
+    want = t.run()
+    torch.cuda.synchronize()
+    c = wrs.Context(0)
+    size = lambda *v: (ctypes.c_size_t * len(v))(*v)  # noqa: E731
+    rc = c._lib.wrs_attn_tree_self(c.handle, t.arena.handle, 1, size(0, 1), size(20, 9), 2,
+                                   par.data_ptr(), par.numel(), q.data_ptr(), 128, out.data_ptr(),
+                                   128)
+    assert rc == 0
+    c.synchronize()
+    assert torch.equal(out, want)
+    c.close()
+    t.check(host(out))
+    t.arena.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("past", [60, 3000])
+def test_queries_of_any_size(wrs, ctx, past, dtype):
+    """Rows of q from 2^-60 to 2^8 of the others' size: each row has a scale of its own."""
+    note(f"tree_self over {past} keys, rows of q of very different size, {dtype}")
+    t = Trees(wrs, ctx, getattr(wrs, "WRS_" + dtype.upper()), 2, [past], [33], "tree", 97)
+    t.q *= np.exp2(np.linspace(-60, 8, 33)).astype(np.float32)[:, None]
+    t.q[7] = 0.0
+    t.check(host(t.run()))
+    t.arena.close()

@@ -26,8 +26,9 @@ constexpr int kParts<float> = 3;
 template <>
 constexpr int kParts<_Float16> = 2;
 
-// x = the sum of its parts, the top halves of the words of p, exactly: each takes the next 8
-// significant bits. An infinity is its first part alone; a NaN stays one.
+// x = the sum of its parts, the top halves of the words of p, exactly down to bf16's last bit,
+// 2^-133: each takes the next 8 significant bits. An infinity is its first part alone; a NaN stays
+// one.
 template <int P>
 __device__ inline void split_top(float x, uint32_t (&p)[P]) {
   p[0] = __builtin_bit_cast(uint32_t, x);
