@@ -40,6 +40,7 @@ extern "C" {
 #define WRS_F16 1
 #define WRS_BF16 2
 #define WRS_MX4 3 /* packed MXFP4 rows: input of wrs_linear_mx4 only */
+#define WRS_I8 4  /* 8-bit codes with a scale for each row of a head: KV arenas only */
 
 typedef struct wrs_attn_ctx wrs_attn_ctx;
 typedef struct wrs_kv wrs_kv;
@@ -193,17 +194,28 @@ int wrs_attn_prefill(wrs_attn_ctx *ctx, int q_dtype, const void *q, const wrs_la
  * WRS_EUNSUPPORTED, and the attention calls size their score scratch (9
  * bytes per row, head and key; calls of up to 8 rows for the arena's longest
  * rows) on the first eager call; only those over more than 512 keys use it, and
- * such a first call under stream capture fails with WRS_ECAPTURE. */
+ * such a first call under stream capture fails with WRS_ECAPTURE.
+ * Or 8-bit codes (WRS_I8; no reference counterpart), for long sessions: a row of
+ * a head is 64 whole numbers times a power of two, the least that leaves none past
+ * 127, so 65 bytes against 128 or 256; a value is off by at most 2/255 of its row's
+ * largest (of each head), and rows with an infinity or NaN read as NaN. A row has a
+ * scale to itself, so storing, moving, cutting and sliding rows never rounds
+ * another one, and rows that were read back store as the same codes. Attention runs on
+ * the codes (q split in two f16 parts, weights in two bf16 parts: 2^-22 and 2^-18), the
+ * cross calls with any 16-byte aligned q and any rows as on f16 arenas; a row of q
+ * with an infinity or NaN gives NaN. Planes hold up to 2^24 - 4096 rows.
+ * wrs_attn_decode_cross_noalloc, the _lse pair, wrs_attn_capture_cross_heads and
+ * wrs_attn_tree_self return WRS_EUNSUPPORTED on them. */
 
 /* DecoderKvCache::new (decoder.rs:148-157) with the arena capacity fixed;
  * f16 planes. */
 int wrs_kv_create(wrs_attn_ctx *ctx, size_t n_layers, size_t n_slots, size_t n_heads,
                   size_t max_ctx, size_t n_audio_max, wrs_kv **out);
-/* The same with the plane element type: WRS_F16 or WRS_F32 (the reference
- * cache's Vec<f32>, decoder.rs:131-157). */
+/* The same with the plane element type: WRS_F16, WRS_F32 (the reference
+ * cache's Vec<f32>, decoder.rs:131-157) or WRS_I8. */
 int wrs_kv_create_dtype(wrs_attn_ctx *ctx, size_t n_layers, size_t n_slots, size_t n_heads,
                         size_t max_ctx, size_t n_audio_max, int dtype, wrs_kv **out);
-/* Plane element type of an arena (WRS_F16 or WRS_F32). No reference
+/* Plane element type of an arena (WRS_F16, WRS_F32 or WRS_I8). No reference
  * counterpart: the reference cache has one type. */
 int wrs_kv_dtype(wrs_kv *kv, int *dtype);
 void wrs_kv_destroy(wrs_kv *kv);
@@ -230,6 +242,21 @@ int wrs_kv_slide_to_fit(wrs_kv *kv, size_t slot, size_t n_new, size_t max_ctx, s
  * host or device source pointers. */
 int wrs_kv_append(wrs_kv *kv, size_t layer, size_t slot, const float *k_rows,
                   const float *v_rows, size_t n, int src_on_host);
+/* The same append for several slots in one launch, from device rows of any stride (a
+ * step's beams, in place in a fused projection's output): counts[i] rows of slots[i] (host
+ * arrays; each slot once), packed in that order, land at the slot's current length. k_len and
+ * v_len are the buffers' lengths in elements. Everything is checked before a row is
+ * written; slots and lengths are read when the call is made, so a replayed graph keeps
+ * them. */
+int wrs_kv_append_rows(wrs_kv *kv, size_t layer, const size_t *slots, const size_t *counts,
+                       size_t n_slots, const float *k_rows, size_t k_len, int64_t k_row_stride,
+                       const float *v_rows, size_t v_len, int64_t v_row_stride);
+/* The stored values of counts[i] rows of slots[i] from row first[i] on (within max_ctx; rows
+ * never stored read as anything), as f32 rows on the device: the inverse of the append, to keep
+ * a session elsewhere. Slots may repeat. No reference counterpart: its cache is host memory. */
+int wrs_kv_read_rows(wrs_kv *kv, size_t layer, const size_t *slots, const size_t *first,
+                     const size_t *counts, size_t n_slots, float *k_rows, size_t k_len,
+                     int64_t k_row_stride, float *v_rows, size_t v_len, int64_t v_row_stride);
 int wrs_kv_advance(wrs_kv *kv, size_t slot, size_t n);
 /* The rows of an accepted path of a drafted tree (wrs_attn_tree_self) come
  * together behind their slot's history: for every layer and head, K and V, row
@@ -247,6 +274,11 @@ int wrs_kv_keep_rows(wrs_kv *kv, const size_t *slots, const size_t *counts, size
  * K and V of one layer, into the head planes (converted to f16, or copied). */
 int wrs_kv_set_cross(wrs_kv *kv, size_t layer, const float *k, const float *v, size_t n_audio,
                      int src_on_host);
+/* The stored values of n cross rows from row `first` on (within the layer's n_audio), as
+ * wrs_kv_read_rows gives self rows. */
+int wrs_kv_read_cross(wrs_kv *kv, size_t layer, size_t first, size_t n, float *k_rows,
+                      size_t k_len, int64_t k_row_stride, float *v_rows, size_t v_len,
+                      int64_t v_row_stride);
 /* n_audio of one layer's stored cross K/V (DecoderKvCache keeps cross K/V per
  * layer, decoder.rs:136-139); 0 after wrs_kv_invalidate_cross. */
 int wrs_kv_cross_len(wrs_kv *kv, size_t layer, size_t *n_audio);
@@ -319,6 +351,23 @@ int wrs_attn_tree_self(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const size_t
                        const size_t *n_nodes, size_t n_trees, const void *parents,
                        size_t parents_len, const float *q, int64_t q_row_stride, float *out,
                        int64_t out_row_stride);
+/* Self-attention of long sessions: counts[i] rows of slots[i] (host arrays), appended and not
+ * advanced, one token each or whole texts. Row j of a slot stands at position p = slot_len + j
+ * and sees the keys up to its own that are among the first `sinks` or among the last `window`
+ * (p - window < key <= p; window >= 1, SIZE_MAX: every key). Keys that no row of a block sees are
+ * not read. Rows of q and out ([sum of counts][d_model] f32, device) lie q_row_stride and
+ * out_row_stride elements apart; q_len and out_len are the buffers' lengths in elements. Values of
+ * keys that a row does not see never reach it, infinities and NaN among them; a row whose visible
+ * scores are all -infinity is zero, and one with a NaN among them NaN. Any arena, up to
+ * 2^24 - 4096 keys; f16 arenas take q and the weights in two f16 parts (2^-22 down to 2^-28 of the
+ * row's largest), f32 ones whole, 8-bit ones as above. Slots, counts and lengths are read
+ * when the call is made: a replayed graph keeps them. Long keys of few rows split over
+ * workgroups through the buffer of tree attention. No reference counterpart: its decoder
+ * sees the whole cache and drops the oldest tokens (decoder.rs:248-263). */
+int wrs_attn_window_self(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const size_t *slots,
+                         const size_t *counts, size_t n_slots, size_t window, size_t sinks,
+                         const float *q, size_t q_len, int64_t q_row_stride, float *out,
+                         size_t out_len, int64_t out_row_stride);
 /* wrs_attn_prefill_cross (the multi_head_attention call of decoder.rs:698-708)
  * that also writes each row's softmax statistics for
  * wrs_attn_capture_cross_heads_lse: lse is an f32
@@ -461,6 +510,30 @@ int wrs_linear_mx4(wrs_attn_ctx *ctx, int x_dtype, const void *x, const void *x_
                    const void *const *w_scales, const float *const *bias, size_t n_tokens,
                    size_t n_in, size_t n_out, int activation, int out_dtype, void *const *out,
                    const size_t *out_len, int64_t out_row_stride, int64_t out_head_stride);
+
+/* ---- scores of tokens (asynchronous) -------------------------------------
+ * What a sampler and a scorer take from a step's or a transcript's logits, in one pass over them
+ * (the reference's host loops over each row: log-softmax, average log probability, beam candidates).
+ * Row r of logits (n_vocab entries in dtype WRS_F32, WRS_F16 or WRS_BF16, row_stride elements
+ * apart) at `temperature` T: lp_j = x_j / T - ln sum_i exp(x_i / T), over the entries whose byte in
+ * `allowed` is not zero (device bytes, rows allowed_row_stride apart or 0: one row for all;
+ * NULL: every entry). Writes, each if it is not NULL:
+ *   logprobs[r]: lp of tokens[r] (device int32; both or neither), -infinity for an entry that is
+ *     hidden or no entry at all;
+ *   entropy[r]: -sum_j exp(lp_j) lp_j, in nats;
+ *   top_ids, top_logprobs [n_rows][top_k] (int32 and f32; top_k <= 32 and <= n_vocab): the
+ *     likeliest entries above -infinity, the lowest index first among equals; where there are
+ *     fewer, -1 and -infinity.
+ * A row without such an entry has log probabilities of -infinity and entropy 0; one with a NaN or
+ * +infinity among its allowed entries gives NaN and ids of -1. A log probability near 0 keeps f32's
+ * relative precision. Up to 2^22 entries a row. logits_len and allowed_len are the buffers' lengths
+ * in elements. Few rows (and those past 65536 entries) split over workgroups through the buffer of
+ * tree attention; captured before it exists, they run unsplit (past 65536 entries: WRS_ECAPTURE). */
+int wrs_token_logprobs(wrs_attn_ctx *ctx, int dtype, const void *logits, size_t logits_len,
+                       int64_t row_stride, size_t n_rows, size_t n_vocab, const void *allowed,
+                       size_t allowed_len, int64_t allowed_row_stride, float temperature,
+                       const void *tokens, float *logprobs, float *entropy, size_t top_k,
+                       void *top_ids, float *top_logprobs);
 
 /* WhisperDecoder::precompute_cross_attn (crates/whisper/src/decoder.rs:423-447)
  * straight into the arena: for every layer l, K = enc . w_k[l]^T and

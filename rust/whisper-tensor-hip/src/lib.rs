@@ -77,6 +77,7 @@ pub mod ffi {
     pub const WRS_F16: c_int = 1;
     pub const WRS_BF16: c_int = 2;
     pub const WRS_MX4: c_int = 3;
+    pub const WRS_I8: c_int = 4;
 
     pub const WRS_ACT_NONE: c_int = 0;
     pub const WRS_ACT_GELU: c_int = 1;
@@ -142,12 +143,22 @@ pub mod ffi {
             pos: *mut usize) -> c_int;
         pub fn wrs_kv_append(kv: *mut WrsKv, layer: usize, slot: usize, k_rows: *const f32,
             v_rows: *const f32, n: usize, src_on_host: c_int) -> c_int;
+        pub fn wrs_kv_append_rows(kv: *mut WrsKv, layer: usize, slots: *const usize,
+            counts: *const usize, n_slots: usize, k_rows: *const f32, k_len: usize,
+            k_row_stride: i64, v_rows: *const f32, v_len: usize, v_row_stride: i64) -> c_int;
+        pub fn wrs_kv_read_rows(kv: *mut WrsKv, layer: usize, slots: *const usize,
+            first: *const usize, counts: *const usize, n_slots: usize, k_rows: *mut f32,
+            k_len: usize, k_row_stride: i64, v_rows: *mut f32, v_len: usize,
+            v_row_stride: i64) -> c_int;
         pub fn wrs_kv_advance(kv: *mut WrsKv, slot: usize, n: usize) -> c_int;
         // drafted trees (no reference counterpart): an accepted path's rows
         pub fn wrs_kv_keep_rows(kv: *mut WrsKv, slots: *const usize, counts: *const usize,
             n_slots: usize, rows: *const usize, n_rows: usize) -> c_int;
         pub fn wrs_kv_set_cross(kv: *mut WrsKv, layer: usize, k: *const f32, v: *const f32,
             n_audio: usize, src_on_host: c_int) -> c_int;
+        pub fn wrs_kv_read_cross(kv: *mut WrsKv, layer: usize, first: usize, n: usize,
+            k_rows: *mut f32, k_len: usize, k_row_stride: i64, v_rows: *mut f32, v_len: usize,
+            v_row_stride: i64) -> c_int;
         pub fn wrs_kv_cross_len(kv: *mut WrsKv, layer: usize, n_audio: *mut usize) -> c_int;
         pub fn wrs_kv_self_planes(kv: *mut WrsKv, k: *mut *mut c_void, v: *mut *mut c_void,
             slot_stride_elems: *mut usize) -> c_int;
@@ -172,6 +183,11 @@ pub mod ffi {
             slots: *const usize, n_nodes: *const usize, n_trees: usize, parents: *const c_void,
             parents_len: usize, q: *const f32, q_row_stride: i64, out: *mut f32,
             out_row_stride: i64) -> c_int;
+        // long sessions: a sliding window and the first tokens (no reference counterpart)
+        pub fn wrs_attn_window_self(ctx: *mut WrsCtx, kv: *mut WrsKv, layer: usize,
+            slots: *const usize, counts: *const usize, n_slots: usize, window: usize,
+            sinks: usize, q: *const f32, q_len: usize, q_row_stride: i64, out: *mut f32,
+            out_len: usize, out_row_stride: i64) -> c_int;
         // prefill_cross, also writing the rows' softmax statistics for the one-pass capture
         pub fn wrs_attn_prefill_cross_lse(ctx: *mut WrsCtx, kv: *mut WrsKv, layer: usize,
             q: *const f32, n_tokens: usize, out: *mut f32, lse: *mut f32) -> c_int;
@@ -223,6 +239,12 @@ pub mod ffi {
             gamma: *const f32, beta: *const f32, eps: f32, n_tokens: usize, d_model: usize,
             out_dtype: c_int, out: *mut c_void, out_len: usize) -> c_int;
         pub fn wrs_gelu_inplace(ctx: *mut WrsCtx, data: *mut f32, n: usize) -> c_int;
+        // scores of tokens; allowed: device bytes, tokens and top_ids: device int32
+        pub fn wrs_token_logprobs(ctx: *mut WrsCtx, dtype: c_int, logits: *const c_void,
+            logits_len: usize, row_stride: i64, n_rows: usize, n_vocab: usize,
+            allowed: *const c_void, allowed_len: usize, allowed_row_stride: i64,
+            temperature: f32, tokens: *const c_void, logprobs: *mut f32, entropy: *mut f32,
+            top_k: usize, top_ids: *mut c_void, top_logprobs: *mut f32) -> c_int;
         // decoder.rs:423-447 precompute_cross_attn, every layer into the arena
         pub fn wrs_kv_set_cross_proj(kv: *mut WrsKv, x_dtype: c_int, enc: *const c_void,
             enc_len: usize, enc_row_stride: i64, n_audio: usize, w_k: *const *const c_void,
@@ -348,7 +370,8 @@ impl<'c> KvArena<'c> {
     }
 
     /// The same with f32 planes (`ffi::WRS_F32`): the reference cache's own
-    /// values, attention with the reference's arithmetic.
+    /// values, attention with the reference's arithmetic; or 8-bit codes
+    /// (`ffi::WRS_I8`), half of f16's bytes.
     pub fn new_with_dtype(ctx: &'c AttnCtx, n_layers: usize, n_slots: usize, n_heads: usize,
                           max_ctx: usize, n_audio_max: usize, dtype: c_int) -> Self {
         let mut kv = std::ptr::null_mut();

@@ -14,6 +14,9 @@ Host-side mirror of the reference's attention interface over the C ABI of
   ``prefill`` and the ``KvArena`` (DecoderKvCache, decoder.rs:131-264) with
   its ``decode_self`` / ``decode_cross`` / ``prefill_self`` / ``prefill_cross``
   and the DTW alignment-head capture ``capture_cross_heads``;
+* long sessions: arenas of 8-bit codes (``KvArena(..., dtype=WRS_I8)``) with
+  ``KvArena.append_rows`` / ``read_rows`` / ``read_cross``, and ``KvArena.window_self``,
+  whose rows see a sliding window and the first tokens; ``token_logprobs`` scores tokens;
 * drafted tokens: ``KvArena.tree_self`` checks trees of them in one pass and
   ``KvArena.keep_rows`` keeps the accepted path; MXFP4 weights: ``mx4_quantize``,
   ``mx4_dequantize`` and ``linear_mx4`` on :class:`Mx4` rows.
@@ -29,8 +32,8 @@ import threading
 import numpy as np
 
 from . import _lib as _L
-from ._lib import (WRS_BF16, WRS_EINVAL, WRS_F16, WRS_F32, WRS_MX4, WRS_OK, ExtensionMissing,
-                   Layout, header_symbols)
+from ._lib import (WRS_BF16, WRS_EINVAL, WRS_F16, WRS_F32, WRS_I8, WRS_MX4, WRS_OK,
+                   ExtensionMissing, Layout, header_symbols)
 
 Q_TILE = 128  # crates/tensor/src/ops/attention.rs:13 (reference tile constants)
 KV_TILE = 128  # crates/tensor/src/ops/attention.rs:26
@@ -40,7 +43,7 @@ __all__ = [
     "multi_head_attention", "single_token_mha_d64", "mha_with_cache", "prefill",
     "token_major", "default_context", "header_symbols", "Q_TILE", "KV_TILE", "linear",
     "linear_group", "linear_fused", "layer_norm", "gelu_inplace", "Mx4", "mx4_quantize",
-    "mx4_dequantize", "linear_mx4",
+    "mx4_dequantize", "linear_mx4", "token_logprobs",
 ]
 
 
@@ -443,6 +446,51 @@ def linear_mx4(x, ws, biases, outs, *, act=None, out_row_stride=None, out_head_s
         (ctypes.c_size_t * n)(*[_span(t) for t in outs]), rs, out_head_stride), "linear_mx4")
 
 
+def token_logprobs(logits, tokens=None, logprobs=None, *, entropy=None, top_ids=None,
+                   top_logprobs=None, allowed=None, temperature=1.0, ctx=None):
+    """Log probabilities of given tokens, with entropy and the likeliest alternatives, in one pass
+    over the logits (``wrs_token_logprobs``).
+
+    ``logits`` [n][n_vocab] float32, float16 or bfloat16 rows of any stride. Every output is
+    given by the caller or left out: ``logprobs`` float32 [n] of ``tokens`` int32 [n];
+    ``entropy`` float32 [n], in nats; ``top_ids`` int32 and ``top_logprobs`` float32 [n][k], k <= 32,
+    likeliest first, the lowest index first among equals. ``allowed`` bool or uint8 [n][n_vocab] or
+    [1][n_vocab] (one row for all) hides the entries where it is zero; ``temperature`` divides the
+    logits. A token that is hidden or no entry has -inf."""
+    ctx = ctx or default_context()
+    n, v, rs = _rows(logits, "token_logprobs")
+    _on_device(ctx, "token_logprobs", logits)
+    k = 0
+    for t, dtype, dims, name in ((tokens, "int32", 1, "tokens"), (logprobs, "float32", 1, "logprobs"),
+                                 (entropy, "float32", 1, "entropy"),
+                                 (top_ids, "int32", 2, "top_ids"),
+                                 (top_logprobs, "float32", 2, "top_logprobs")):
+        if t is None:
+            continue
+        if str(t.dtype) != "torch." + dtype or not t.is_contiguous():
+            raise TypeError(f"token_logprobs: contiguous {dtype} {name} expected, got {t.dtype}")
+        assert t.dim() == dims and t.shape[0] == n
+        _on_device(ctx, "token_logprobs", t)
+        if dims == 2:
+            assert k in (0, t.shape[1]) and t.shape[1] > 0
+            k = t.shape[1]
+    ok_p, ok_len, ok_rs = None, 0, 0
+    if allowed is not None:
+        if str(allowed.dtype) not in ("torch.bool", "torch.uint8"):
+            raise TypeError(f"token_logprobs: bool or uint8 allowed expected, got {allowed.dtype}")
+        rows, width, ok_rs = _rows(allowed, "token_logprobs")
+        assert width == v and rows in (1, n)
+        _on_device(ctx, "token_logprobs", allowed)
+        ok_p, ok_len = allowed.data_ptr(), _span(allowed)
+        if rows == 1:
+            ok_rs = 0
+    ptr = [None if t is None else t.data_ptr()
+           for t in (tokens, logprobs, entropy, top_ids, top_logprobs)]
+    ctx.check(ctx._lib.wrs_token_logprobs(
+        ctx.handle, _dtype_code(logits), logits.data_ptr(), _span(logits), rs, n, v, ok_p, ok_len,
+        ok_rs, float(temperature), ptr[0], ptr[1], ptr[2], k, ptr[3], ptr[4]), "token_logprobs")
+
+
 def layer_norm(x, gamma, beta, eps, out, ctx=None):
     """layer_norm (crates/tensor/src/ops/norm.rs:116-143) over the rows of the
     float32 CUDA tensor x ([num_tokens][d_model]); out float32/float16/bfloat16."""
@@ -472,8 +520,9 @@ class KvArena:
 
     def __init__(self, n_layers, n_slots, n_heads, max_ctx, n_audio_max, ctx=None,
                  dtype=WRS_F16):
-        """dtype WRS_F16 (default) or WRS_F32: the plane element type (WRS_F32
-        keeps the reference cache's f32 values and runs its arithmetic)."""
+        """dtype WRS_F16 (default), WRS_F32 or WRS_I8: the plane element type (WRS_F32
+        keeps the reference cache's f32 values and runs its arithmetic; WRS_I8 keeps 8-bit
+        codes with a power of two for each row of a head, half of f16's bytes)."""
         self.ctx = ctx or default_context()
         self._lib = self.ctx._lib
         h = ctypes.c_void_p()
@@ -488,7 +537,7 @@ class KvArena:
         self.d_model = n_heads * 64
 
     def plane_dtype(self) -> int:
-        """Plane element type as the library reports it (WRS_F16 or WRS_F32)."""
+        """Plane element type as the library reports it (WRS_F16, WRS_F32 or WRS_I8)."""
         d = ctypes.c_int()
         self._c(self._lib.wrs_kv_dtype(self.handle, ctypes.byref(d)), "dtype")
         return d.value
@@ -553,6 +602,42 @@ class KvArena:
         assert nk == nv and nk % self.d_model == 0 and host == host2
         self._c(self._lib.wrs_kv_append(self.handle, layer, slot, pk, pv, nk // self.d_model,
                                         host), "append")
+
+    def _device_rows(self, what, *tensors):
+        """(rows, [pointer, span, stride of each]) of float32 rows of d_model."""
+        count, args = None, []
+        for t in tensors:
+            n, d, rs = _rows(t, what)
+            if _dtype_code(t) != WRS_F32:
+                raise TypeError(f"{what}: float32 rows expected, got {t.dtype}")
+            assert d == self.d_model and count in (None, n)
+            count = n
+            args += [t.data_ptr(), _span(t), rs]
+        _on_device(self.ctx, what, *tensors)
+        return count, args
+
+    def append_rows(self, layer, slots, counts, k, v):
+        """Appends ``counts[i]`` rows of ``slots[i]`` (each slot once) in one launch
+        (``wrs_kv_append_rows``): ``k`` and ``v`` float32 CUDA tensors [sum(counts)][d_model],
+        rows of any stride. :meth:`advance` takes them into the history."""
+        n, args = self._device_rows("append_rows", k, v)
+        assert len(slots) == len(counts) and sum(counts) == n
+        self._c(self._lib.wrs_kv_append_rows(self.handle, layer, _sizes(slots), _sizes(counts),
+                                             len(slots), *args), "append_rows")
+
+    def read_rows(self, layer, slots, first, counts, k, v):
+        """The stored values of ``counts[i]`` rows of ``slots[i]`` from row ``first[i]`` on, into
+        the rows of ``k`` and ``v`` (``wrs_kv_read_rows``)."""
+        n, args = self._device_rows("read_rows", k, v)
+        assert len(slots) == len(counts) == len(first) and sum(counts) == n
+        self._c(self._lib.wrs_kv_read_rows(self.handle, layer, _sizes(slots), _sizes(first),
+                                           _sizes(counts), len(slots), *args), "read_rows")
+
+    def read_cross(self, layer, first, k, v):
+        """The stored values of cross rows from ``first`` on, into the rows of ``k`` and ``v``
+        (``wrs_kv_read_cross``)."""
+        n, args = self._device_rows("read_cross", k, v)
+        self._c(self._lib.wrs_kv_read_cross(self.handle, layer, first, n, *args), "read_cross")
 
     def advance(self, slot, n):
         self._c(self._lib.wrs_kv_advance(self.handle, slot, n), "advance")
@@ -625,6 +710,19 @@ class KvArena:
                                              _sizes(counts), trees, parents.data_ptr(),
                                              parents.numel(), q.data_ptr(), q_rs, out.data_ptr(),
                                              o_rs), "tree_self")
+
+    def window_self(self, layer, slots, counts, window, sinks, q, out):
+        """Self-attention of ``counts[i]`` rows of ``slots[i]``, appended and not advanced, each
+        against the last ``window`` keys up to its own (None: all) and the first ``sinks``
+        (``wrs_attn_window_self``). ``q`` and ``out`` float32 [sum(counts)][d_model], rows of any
+        stride."""
+        n, args = self._device_rows("window_self", q, out)
+        assert len(slots) == len(counts) and sum(counts) == n
+        window = 2 ** 64 - 1 if window is None else window
+        assert window > 0 and sinks >= 0
+        self._c(self._lib.wrs_attn_window_self(self.ctx.handle, self.handle, layer, _sizes(slots),
+                                               _sizes(counts), len(slots), window, sinks, *args),
+                "window_self")
 
     def keep_rows(self, slots, counts, rows):
         """Moves the rows of an accepted path together (``wrs_kv_keep_rows``): for every

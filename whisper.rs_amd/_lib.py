@@ -31,6 +31,7 @@ WRS_F32 = 0
 WRS_F16 = 1
 WRS_BF16 = 2
 WRS_MX4 = 3
+WRS_I8 = 4
 
 
 class Reserve(ctypes.Structure):
@@ -89,6 +90,12 @@ _SIGNATURES = {
     "wrs_kv_set_len": (_int, [_vp, _sz, _sz]),
     "wrs_kv_slide_to_fit": (_int, [_vp, _sz, _sz, _sz, _szp]),
     "wrs_kv_append": (_int, [_vp, _sz, _sz, _vp, _vp, _sz, _int]),
+    "wrs_kv_append_rows": (_int, [_vp, _sz, _szp, _szp, _sz, _vp, _sz, ctypes.c_int64, _vp, _sz,
+                                  ctypes.c_int64]),
+    "wrs_kv_read_rows": (_int, [_vp, _sz, _szp, _szp, _szp, _sz, _vp, _sz, ctypes.c_int64, _vp,
+                                _sz, ctypes.c_int64]),
+    "wrs_kv_read_cross": (_int, [_vp, _sz, _sz, _sz, _vp, _sz, ctypes.c_int64, _vp, _sz,
+                                 ctypes.c_int64]),
     "wrs_kv_advance": (_int, [_vp, _sz, _sz]),
     "wrs_kv_keep_rows": (_int, [_vp, _szp, _szp, _sz, _szp, _sz]),
     "wrs_kv_set_cross": (_int, [_vp, _sz, _vp, _vp, _sz, _int]),
@@ -101,6 +108,8 @@ _SIGNATURES = {
     "wrs_attn_prefill_self": (_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp]),
     "wrs_attn_tree_self": (_int, [_vp, _vp, _sz, _szp, _szp, _sz, _vp, _sz, _vp, ctypes.c_int64,
                                   _vp, ctypes.c_int64]),
+    "wrs_attn_window_self": (_int, [_vp, _vp, _sz, _szp, _szp, _sz, _sz, _sz, _vp, _sz,
+                                    ctypes.c_int64, _vp, _sz, ctypes.c_int64]),
     "wrs_attn_prefill_cross": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
     "wrs_attn_prefill_cross_lse": (_int, [_vp, _vp, _sz, _vp, _sz, _vp, _vp]),
     "wrs_linear": (_int, [_vp, _int, _vp, _sz, ctypes.c_int64, _vp, _vp, _sz, _sz, _sz, _int,
@@ -117,6 +126,8 @@ _SIGNATURES = {
     "wrs_linear_mx4": (_int, [_vp, _int, _vp, _vp, _sz, ctypes.c_int64, _sz, ctypes.POINTER(_vp),
                               ctypes.POINTER(_vp), ctypes.POINTER(_vp), _sz, _sz, _sz, _int, _int,
                               ctypes.POINTER(_vp), _szp, ctypes.c_int64, ctypes.c_int64]),
+    "wrs_token_logprobs": (_int, [_vp, _int, _vp, _sz, ctypes.c_int64, _sz, _sz, _vp, _sz,
+                                  ctypes.c_int64, ctypes.c_float, _vp, _vp, _vp, _sz, _vp, _vp]),
     "wrs_layer_norm": (_int, [_vp, _vp, _sz, _vp, _vp, ctypes.c_float, _sz, _sz, _int, _vp, _sz]),
     "wrs_gelu_inplace": (_int, [_vp, _vp, _sz]),
     "wrs_kv_set_cross_proj": (_int, [_vp, _int, _vp, _sz, ctypes.c_int64, _sz,

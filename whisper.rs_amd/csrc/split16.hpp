@@ -10,6 +10,9 @@ namespace split16 {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr float kWeightUp = 0x1p15f;  // softmax weights, at most 1, are split in units of its inverse
@@ -64,6 +67,30 @@ __device__ inline void split2(float x0, float x1, float scale, uint32_t (&out)[3
   out[0] = __builtin_bit_cast(uint32_t, h);
   out[1] = __builtin_bit_cast(uint32_t, m);
   out[2] = __builtin_bit_cast(uint32_t, l);
+}
+
+__device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// Two floats, times `scale` at most 2^15, as packed f16 pairs in two parts, the second in a unit
+// 2^-11 of the first.
+constexpr int kParts = 2;
+__device__ inline void split_units(float x0, float x1, float scale, uint32_t (&out)[kParts]) {
+  constexpr float kUp = 1.f / kPartUnit;
+  const f16x2 h = pack2(x0, x1, scale);
+  x0 = __builtin_fmaf(x0, scale, -static_cast<float>(h[0]));  // exact
+  x1 = __builtin_fmaf(x1, scale, -static_cast<float>(h[1]));
+  out[0] = __builtin_bit_cast(uint32_t, h);
+  out[1] = __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(__builtin_fmaf(x0, kUp, 0.f)),
+                                              static_cast<_Float16>(__builtin_fmaf(x1, kUp, 0.f))});
+}
+// The parts' sums as one.
+__device__ inline f32x4 join(const f32x4 (&x)[kParts]) {
+  f32x4 s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(x[1][i], kPartUnit, x[0][i]);
+  return s;
 }
 
 }  // namespace split16

@@ -42,19 +42,6 @@ constexpr int kCounterStride = 32;  // 128 bytes between merge counters
 constexpr int kMergeLoads = 8;  // partials in flight per thread in the merge
 constexpr int kRawBuffer = 0x00020000;  // buffer resource word 3: raw, 32-bit data format
 
-// Two floats at once, as st_agent and ld_agent (8-byte aligned).
-__device__ inline void st_agent2(float* p, float x, float y) {
-  const uint64_t v = __builtin_bit_cast(uint32_t, x) |
-                     static_cast<uint64_t>(__builtin_bit_cast(uint32_t, y)) << 32;
-  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ inline void ld_agent2(const float* p, float& x, float& y) {
-  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
-  x = __builtin_bit_cast(float, static_cast<uint32_t>(v));
-  y = __builtin_bit_cast(float, static_cast<uint32_t>(v >> 32));
-}
-
 // 4 values of a plane row at byte offset `o` (multiple of 4 values), zero past the range.
 template <typename KT>
 __device__ inline f32x4 load4(const __amdgpu_buffer_rsrc_t& rs, uint32_t o) {
@@ -288,30 +275,6 @@ __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4], int
   }
 }
 
-__device__ inline f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-// Two floats, times `scale` at most 2^15, as packed f16 pairs in two parts, the second in a unit
-// 2^-11 of the first.
-constexpr int kParts = 2;
-__device__ inline void split_units(float x0, float x1, float scale, uint32_t (&out)[kParts]) {
-  constexpr float kUp = 1.f / kPartUnit;
-  const f16x2 h = pack2(x0, x1, scale);
-  x0 = __builtin_fmaf(x0, scale, -static_cast<float>(h[0]));  // exact
-  x1 = __builtin_fmaf(x1, scale, -static_cast<float>(h[1]));
-  out[0] = __builtin_bit_cast(uint32_t, h);
-  out[1] = __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(__builtin_fmaf(x0, kUp, 0.f)),
-                                              static_cast<_Float16>(__builtin_fmaf(x1, kUp, 0.f))});
-}
-// The parts' sums as one.
-__device__ inline f32x4 join(const f32x4 (&x)[kParts]) {
-  f32x4 s;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(x[1][i], kPartUnit, x[0][i]);
-  return s;
-}
-
 // Keys key0 + 32 wave, + 128, .. of an f16 plane on the f16 matrix pipe. Query rows (times a
 // power of two that puts the largest element into [2^14, 2^15)) and weights (in units of 2^-15)
 // are split into two f16 parts, the second in a unit 2^-11 of the first and with sums of its
@@ -467,21 +430,6 @@ __device__ inline bool attend_f16(const Block& b, const f32x4 (&qx)[kRT][4], int
     }
   }
   return __any(odd);
-}
-
-// x / n, with the remainder; inv: 2^32 / n rounded up (for n 1: 2^32 - 1).
-__device__ inline int divide(int x, int n, uint32_t inv, int& rest) {
-  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), inv));
-  rest = x - q * n;
-  if (rest < 0) {
-    --q;
-    rest += n;
-  }
-  if (rest >= n) {
-    ++q;
-    rest -= n;
-  }
-  return q;
 }
 
 template <typename KT, int kRT>
@@ -701,9 +649,6 @@ int64_t tree_plan(TreeArgs& a, DType dt, bool split) {
     work += b * total;
     longest = std::max(longest, total);
   }
-  auto inverse = [](int n) {
-    return static_cast<uint32_t>(std::min<uint64_t>(((uint64_t{1} << 32) + n - 1) / n, 0xffffffffu));
-  };
   // Chunks of so many keys; returns the sum of all trees' workgroups and the grid's width.
   int64_t widest = 0;
   auto lay = [&](int64_t chunk) {

@@ -74,12 +74,14 @@ struct wrs_attn_ctx {
   size_t split_part_bytes = 0;
   unsigned* split_counters = nullptr;
   size_t split_counter_bytes = 0;
-  // Tree attention whose keys split over workgroups: partials and merge counters
-  // (kept zero between launches), of one size from the first such call on.
+  // Tree and window attention whose keys split over workgroups, and scored rows that do: partials
+  // and merge counters (kept zero between launches), of one size from the first such call on.
   float* tree_part = nullptr;
   size_t tree_part_bytes = 0;
   unsigned* tree_counters = nullptr;
   size_t tree_counter_bytes = 0;
+  float* cross_rows = nullptr;  // 8-bit arenas: projected cross K and V of a layer, before rounding
+  size_t cross_rows_bytes = 0;
   // Prefill schedule overrides (wrs_attn_set_schedule).
   int prefill_queries = 0;
   int f32_split = -1;
@@ -90,17 +92,23 @@ struct wrs_attn_ctx {
 
 struct wrs_kv {
   wrs_attn_ctx* ctx = nullptr;
-  int dtype = WRS_F16;  // element type of every plane: WRS_F16 or WRS_F32
+  int dtype = WRS_F16;  // element type of every plane: WRS_F16, WRS_F32 or WRS_I8
   size_t n_layers = 0, n_slots = 0, n_heads = 0, max_ctx = 0, n_audio_max = 0;
   void* k_self = nullptr;  // [layer][slot][head][max_ctx][64]
   void* v_self = nullptr;
   void* k_cross = nullptr;  // [layer][head][n_audio_max][64]
   void* v_cross = nullptr;
+  // 8-bit arenas: a scale byte a row, [..][head][scale_rows()].
+  uint8_t *k_self_scale = nullptr, *v_self_scale = nullptr;
+  uint8_t *k_cross_scale = nullptr, *v_cross_scale = nullptr;
   std::vector<size_t> len;        // per slot: rows stored (reference t_past)
   std::vector<size_t> cross_len;  // per layer: n_audio of the stored cross K/V
 
   bool f32() const { return dtype == WRS_F32; }
-  size_t esize() const { return f32() ? 4 : 2; }
+  bool i8() const { return dtype == WRS_I8; }
+  size_t esize() const { return f32() ? 4 : i8() ? 1 : 2; }
+  wrs::DType plane_type() const { return f32() ? wrs::kF32 : i8() ? wrs::kI8 : wrs::kF16; }
+  static size_t scale_rows(size_t rows) { return (rows + 63) / 64 * 64; }
   size_t d_model() const { return n_heads * 64; }
   size_t plane() const { return max_ctx * 64; }
   size_t self_off(size_t layer, size_t slot) const {
@@ -109,13 +117,20 @@ struct wrs_kv {
   size_t cross_off(size_t layer) const { return layer * n_heads * n_audio_max * 64; }
   // Element `off` of a plane set, typed. words() views any plane set as
   // 16-bit words (an f32 row of 64 is two f16-sized rows), so the row moves
-  // of kv_slide / kv_copy_planes serve both element types.
+  // of kv_slide / kv_copy_planes serve both element types (8-bit planes have moves of their own).
   static uint16_t* u16(void* p, size_t off = 0) { return static_cast<uint16_t*>(p) + off; }
   static float* f32p(void* p, size_t off = 0) { return static_cast<float*>(p) + off; }
   _Float16* words(void* p, size_t off = 0) const {
     return static_cast<_Float16*>(p) + off * (esize() / 2);
   }
   size_t word_scale() const { return esize() / 2; }
+  // A slot's planes of an 8-bit arena.
+  wrs::Kv8Planes planes8(size_t slot) const {
+    const size_t p = slot * n_heads, rows = p * max_ctx * 64, scales = p * scale_rows(max_ctx);
+    return {static_cast<uint8_t*>(k_self) + rows, static_cast<uint8_t*>(v_self) + rows,
+            k_self_scale + scales, v_self_scale + scales, static_cast<int64_t>(n_slots * n_heads),
+            static_cast<int64_t>(max_ctx), static_cast<int64_t>(scale_rows(max_ctx))};
+  }
 };
 
 namespace {
@@ -599,6 +614,7 @@ void wrs_attn_destroy(wrs_attn_ctx* c) {
   if (c->ln_rows) (void)hipFree(c->ln_rows);
   if (c->exact_scores) (void)hipFree(c->exact_scores);
   if (c->exact_counters) (void)hipFree(c->exact_counters);
+  if (c->cross_rows) (void)hipFree(c->cross_rows);
   if (c->tree_part) (void)hipFree(c->tree_part);
   if (c->tree_counters) (void)hipFree(c->tree_counters);
   if (c->split_part) (void)hipFree(c->split_part);
@@ -881,10 +897,49 @@ int wrs_attn_prefill(wrs_attn_ctx* c, int q_dtype, const void* q, const wrs_layo
 
 namespace {
 
+void free_planes(wrs_kv* kv) {
+  for (void* p : {kv->k_self, kv->v_self, kv->k_cross, kv->v_cross,
+                  static_cast<void*>(kv->k_self_scale), static_cast<void*>(kv->v_self_scale),
+                  static_cast<void*>(kv->k_cross_scale), static_cast<void*>(kv->v_cross_scale)})
+    if (p) (void)hipFree(p);
+}
+
+// Rows of the arena's self or cross planes, no slot's yet, and one slot's (first plane `plane`).
+wrs::KvSlotRows slot_rows(const wrs_kv* kv, bool cross) {
+  wrs::KvSlotRows a;
+  a.k = cross ? kv->k_cross : kv->k_self;
+  a.v = cross ? kv->v_cross : kv->v_self;
+  a.k_scale = cross ? kv->k_cross_scale : kv->k_self_scale;
+  a.v_scale = cross ? kv->v_cross_scale : kv->v_self_scale;
+  const size_t rows = cross ? kv->n_audio_max : kv->max_ctx;
+  a.plane_rows = static_cast<int64_t>(rows);
+  a.scale_rows = static_cast<int64_t>(wrs_kv::scale_rows(rows));
+  a.n_heads = static_cast<int>(kv->n_heads);
+  a.heads_inv = wrs::inverse(a.n_heads);
+  a.n_slots = 0;
+  return a;
+}
+void add_rows(wrs::KvSlotRows& a, size_t plane, size_t row0, size_t pos, size_t count) {
+  const int u = a.n_slots++;
+  a.plane[u] = static_cast<int64_t>(plane);
+  a.row0[u] = static_cast<int64_t>(row0);
+  a.pos[u] = static_cast<int>(pos);
+  a.count[u] = static_cast<int>(count);
+}
+
 // Rows [pos, pos + n) of every head plane of K and V (element `off` on), from n
 // f32 rows of d_model each: converted to f16, or copied for f32 arenas.
 int write_rows(wrs_attn_ctx* c, wrs_kv* kv, const float* k_src, const float* v_src, size_t n,
                void* k, void* v, size_t off, size_t plane, size_t pos) {
+  if (kv->i8()) {
+    wrs::KvSlotRows a = slot_rows(kv, k == kv->k_cross);
+    a.k_rows = const_cast<float*>(k_src);
+    a.v_rows = const_cast<float*>(v_src);
+    a.k_rs = a.v_rs = static_cast<int64_t>(kv->d_model());
+    add_rows(a, off / plane, 0, pos, n);
+    WRS_HIP(c, wrs::launch_kv_slot_rows(a, wrs::kI8, true, c->stream));
+    return WRS_OK;
+  }
   const wrs::KvRows rows{k_src, v_src, kv->words(k, off), kv->words(v, off)};
   WRS_HIP(c, wrs::launch_kv_write_rows(rows, kv->f32(), static_cast<int64_t>(kv->d_model()),
                                        static_cast<int>(n), static_cast<int>(kv->n_heads),
@@ -974,7 +1029,8 @@ int keep_rows(wrs_attn_ctx* c, wrs_kv* kv, const size_t* slots, const size_t* co
   a.n_slots = 0;
   size_t used = 0, at = 0;
   auto flush = [&]() {
-    const hipError_t e = wrs::launch_kv_keep_rows(a, c->stream);
+    const hipError_t e = kv->i8() ? wrs::launch_kv8_keep_rows(a, kv->planes8(0), c->stream)
+                                  : wrs::launch_kv_keep_rows(a, c->stream);
     a.n_slots = 0;
     used = 0;
     return e;
@@ -1021,10 +1077,12 @@ int wrs_kv_create_dtype(wrs_attn_ctx* c, size_t n_layers, size_t n_slots, size_t
   if (n_layers == 0 || n_heads == 0 || max_ctx == 0 || !fits_int(max_ctx) ||
       !fits_int(n_audio_max) || !fits_int(n_slots))
     return fail(c, WRS_EINVAL, "wrs_kv_create: bad geometry");
-  if (dtype != WRS_F16 && dtype != WRS_F32)
-    return fail(c, WRS_EINVAL, "wrs_kv_create: arena dtype must be WRS_F16 or WRS_F32");
+  if (dtype != WRS_F16 && dtype != WRS_F32 && dtype != WRS_I8)
+    return fail(c, WRS_EINVAL, "wrs_kv_create: arena dtype must be WRS_F16, WRS_F32 or WRS_I8");
   if (dtype == WRS_F32 && !fits_int(2 * max_ctx))  // row moves count f16-sized rows
     return fail(c, WRS_EINVAL, "wrs_kv_create: bad geometry");
+  if (dtype == WRS_I8 && (max_ctx >= wrs::kRowsMaxKeys || n_audio_max >= wrs::kRowsMaxKeys))
+    return fail(c, WRS_EUNSUPPORTED, "wrs_kv_create: planes too long for 8-bit codes");
   std::lock_guard<std::mutex> lk(c->mu);
   DeviceGuard g(c->device);
   auto* kv = new (std::nothrow) wrs_kv();
@@ -1049,9 +1107,16 @@ int wrs_kv_create_dtype(wrs_attn_ctx* c, size_t n_layers, size_t n_slots, size_t
     ok = ok && hipMalloc(&kv->k_cross, cross_bytes) == hipSuccess;
     ok = ok && hipMalloc(&kv->v_cross, cross_bytes) == hipSuccess;
   }
+  if (kv->i8()) {
+    const size_t self = n_layers * n_slots * n_heads * wrs_kv::scale_rows(max_ctx);
+    const size_t cross = n_layers * n_heads * wrs_kv::scale_rows(n_audio_max);
+    for (uint8_t** p : {&kv->k_self_scale, &kv->v_self_scale})
+      ok = ok && (!self || hipMalloc(reinterpret_cast<void**>(p), self) == hipSuccess);
+    for (uint8_t** p : {&kv->k_cross_scale, &kv->v_cross_scale})
+      ok = ok && (!cross || hipMalloc(reinterpret_cast<void**>(p), cross) == hipSuccess);
+  }
   if (!ok) {
-    for (void* p : {(void*)kv->k_self, (void*)kv->v_self, (void*)kv->k_cross, (void*)kv->v_cross})
-      if (p) (void)hipFree(p);
+    free_planes(kv);
     delete kv;
     return fail(c, WRS_ENOMEM, "wrs_kv_create: hipMalloc failed");
   }
@@ -1076,8 +1141,7 @@ void wrs_kv_destroy(wrs_kv* kv) {
   std::lock_guard<std::mutex> lk(c->mu);
   DeviceGuard g(c->device);
   (void)hipStreamSynchronize(c->stream);
-  for (void* p : {(void*)kv->k_self, (void*)kv->v_self, (void*)kv->k_cross, (void*)kv->v_cross})
-    if (p) (void)hipFree(p);
+  free_planes(kv);
   delete kv;
 }
 
@@ -1112,9 +1176,13 @@ int wrs_kv_ensure_slots(wrs_kv* kv, size_t n_slots) {
   DeviceGuard g(c->device);
   const size_t slot_bytes = kv->n_heads * kv->plane() * kv->esize();
   const size_t bytes = kv->n_layers * n_slots * slot_bytes;
-  void *nk = nullptr, *nv = nullptr;
-  if (hipMalloc(&nk, bytes) != hipSuccess || hipMalloc(&nv, bytes) != hipSuccess) {
-    if (nk) (void)hipFree(nk);
+  void *nk = nullptr, *nv = nullptr, *nks = nullptr, *nvs = nullptr;
+  const size_t slot_scales = kv->i8() ? kv->n_heads * wrs_kv::scale_rows(kv->max_ctx) : 0;
+  const size_t scales = kv->n_layers * n_slots * slot_scales;
+  if (hipMalloc(&nk, bytes) != hipSuccess || hipMalloc(&nv, bytes) != hipSuccess ||
+      (scales && (hipMalloc(&nks, scales) != hipSuccess || hipMalloc(&nvs, scales) != hipSuccess))) {
+    for (void* p : {nk, nv, nks, nvs})
+      if (p) (void)hipFree(p);
     return fail(c, WRS_ENOMEM, "wrs_kv_ensure_slots: hipMalloc failed");
   }
   if (kv->n_slots) {
@@ -1123,12 +1191,22 @@ int wrs_kv_ensure_slots(wrs_kv* kv, size_t n_slots) {
                                 hipMemcpyDeviceToDevice, c->stream));
     WRS_HIP(c, hipMemcpy2DAsync(nv, n_slots * slot_bytes, kv->v_self, w, w, kv->n_layers,
                                 hipMemcpyDeviceToDevice, c->stream));
+    if (scales) {
+      const size_t ws = kv->n_slots * slot_scales;
+      WRS_HIP(c, hipMemcpy2DAsync(nks, n_slots * slot_scales, kv->k_self_scale, ws, ws,
+                                  kv->n_layers, hipMemcpyDeviceToDevice, c->stream));
+      WRS_HIP(c, hipMemcpy2DAsync(nvs, n_slots * slot_scales, kv->v_self_scale, ws, ws,
+                                  kv->n_layers, hipMemcpyDeviceToDevice, c->stream));
+    }
     WRS_HIP(c, hipStreamSynchronize(c->stream));
-    (void)hipFree(kv->k_self);
-    (void)hipFree(kv->v_self);
+    for (void* p : {kv->k_self, kv->v_self, static_cast<void*>(kv->k_self_scale),
+                    static_cast<void*>(kv->v_self_scale)})
+      if (p) (void)hipFree(p);
   }
   kv->k_self = nk;
   kv->v_self = nv;
+  kv->k_self_scale = static_cast<uint8_t*>(nks);
+  kv->v_self_scale = static_cast<uint8_t*>(nvs);
   kv->n_slots = n_slots;
   kv->len.resize(n_slots, 0);
   return WRS_OK;
@@ -1141,6 +1219,13 @@ int wrs_kv_copy_slot(wrs_kv* kv, size_t dst, size_t src) {
   if (dst >= kv->n_slots || src >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
   if (dst == src) return WRS_OK;
   DeviceGuard g(c->device);
+  if (kv->i8()) {
+    WRS_HIP(c, wrs::launch_kv8_copy(kv->planes8(dst), kv->planes8(src),
+                                    static_cast<int>(kv->n_layers), static_cast<int>(kv->n_heads),
+                                    static_cast<int>(kv->len[src]), c->stream));
+    kv->len[dst] = kv->len[src];
+    return WRS_OK;
+  }
   // Strides and row counts in f16-sized rows (twice the rows for f32 planes).
   const size_t w = kv->word_scale();
   const int64_t layer_stride =
@@ -1183,6 +1268,14 @@ int wrs_kv_slide_to_fit(wrs_kv* kv, size_t slot, size_t n_new, size_t max_ctx, s
   if (t_past + n_new > max_ctx) {  // decoder.rs:250-261
     const size_t drop = std::min(t_past + n_new - max_ctx, t_past);
     DeviceGuard g(c->device);
+    if (kv->i8()) {
+      WRS_HIP(c, wrs::launch_kv8_slide(kv->planes8(slot), static_cast<int>(kv->n_layers),
+                                       static_cast<int>(kv->n_heads), static_cast<int>(t_past),
+                                       static_cast<int>(drop), c->stream));
+      kv->len[slot] = t_past - drop;
+      if (pos) *pos = t_past - drop;
+      return WRS_OK;
+    }
     // In f16-sized rows: an f32 row moves as two.
     const size_t w = kv->word_scale();
     const int64_t layer_stride =
@@ -1225,6 +1318,143 @@ int wrs_kv_append(wrs_kv* kv, size_t layer, size_t slot, const float* k_rows,
                   kv->plane(), pos);
   if (rc) return rc;
   if (src_on_host) WRS_HIP(c, hipStreamSynchronize(c->stream));
+  return WRS_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Whether n_rows rows of n_cols elements, row_stride apart, lie within len (no product is
+// formed that could pass 64 bits).
+bool rows_fit(size_t n_rows, size_t n_cols, int64_t row_stride, size_t len) {
+  if (n_cols > len) return false;
+  return n_rows == 1 || static_cast<size_t>(row_stride) <= (len - n_cols) / (n_rows - 1);
+}
+
+// Rows of d_model f32 in device memory, as a call's argument.
+int check_rows(wrs_attn_ctx* c, const wrs_kv* kv, size_t n, const float* p, size_t len, int64_t rs) {
+  const int64_t dm = static_cast<int64_t>(kv->d_model());
+  if (!p) return fail(c, WRS_EINVAL, "null rows");
+  if (reinterpret_cast<uintptr_t>(p) & 3)
+    return fail(c, WRS_EINVAL, "tensors must be aligned to their elements");
+  if (n > 1 && rs < dm) return fail(c, WRS_EINVAL, "row stride below d_model");
+  if (!rows_fit(n, kv->d_model(), rs, len))
+    return fail(c, WRS_EINVAL, "buffer shorter than its rows of d_model");
+  return WRS_OK;
+}
+
+// Rows of several slots into the arena (first: nullptr, at the slots' lengths) or out of it, their
+// arguments checked; kRowSlots of them to a launch.
+int move_slot_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* first,
+                   const size_t* counts, size_t n_slots, float* k, int64_t k_rs, float* v,
+                   int64_t v_rs) {
+  wrs_attn_ctx* c = kv->ctx;
+  DeviceGuard g(c->device);
+  wrs::KvSlotRows a = slot_rows(kv, false);
+  a.k_rows = k;
+  a.v_rows = v;
+  a.k_rs = k_rs;
+  a.v_rs = v_rs;
+  size_t row = 0;
+  for (size_t i = 0; i < n_slots; ++i) {
+    if (counts[i])
+      add_rows(a, (layer * kv->n_slots + slots[i]) * kv->n_heads, row,
+               first ? first[i] : kv->len[slots[i]], counts[i]);
+    row += counts[i];
+    if (a.n_slots == wrs::kRowSlots || i + 1 == n_slots) {
+      WRS_HIP(c, wrs::launch_kv_slot_rows(a, kv->plane_type(), !first, c->stream));
+      a.n_slots = 0;
+    }
+  }
+  return WRS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wrs_kv_append_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* counts,
+                       size_t n_slots, const float* k_rows, size_t k_len, int64_t k_row_stride,
+                       const float* v_rows, size_t v_len, int64_t v_row_stride) {
+  if (!kv) return WRS_EINVAL;
+  wrs_attn_ctx* c = kv->ctx;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (layer >= kv->n_layers) return fail(c, WRS_ERANGE, "layer out of range");
+  if (n_slots == 0) return WRS_OK;
+  if (!slots || !counts) return fail(c, WRS_EINVAL, "null argument");
+  size_t rows = 0;
+  try {
+    std::vector<bool> seen(kv->n_slots, false);
+    for (size_t i = 0; i < n_slots; ++i) {
+      if (slots[i] >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
+      if (seen[slots[i]]) return fail(c, WRS_EINVAL, "append_rows: the same slot twice");
+      seen[slots[i]] = true;
+      if (counts[i] > kv->max_ctx - kv->len[slots[i]])
+        return fail(c, WRS_ERANGE, "append past the arena's max_ctx");
+      rows += counts[i];
+    }
+  } catch (const std::bad_alloc&) {
+    return fail(c, WRS_ENOMEM, "out of host memory");
+  }
+  if (rows == 0) return WRS_OK;
+  if (!fits_int(rows)) return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+  int rc = check_rows(c, kv, rows, k_rows, k_len, k_row_stride);
+  if (rc) return rc;
+  rc = check_rows(c, kv, rows, v_rows, v_len, v_row_stride);
+  if (rc) return rc;
+  return move_slot_rows(kv, layer, slots, nullptr, counts, n_slots, const_cast<float*>(k_rows),
+                        k_row_stride, const_cast<float*>(v_rows), v_row_stride);
+}
+
+int wrs_kv_read_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* first,
+                     const size_t* counts, size_t n_slots, float* k_rows, size_t k_len,
+                     int64_t k_row_stride, float* v_rows, size_t v_len, int64_t v_row_stride) {
+  if (!kv) return WRS_EINVAL;
+  wrs_attn_ctx* c = kv->ctx;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (layer >= kv->n_layers) return fail(c, WRS_ERANGE, "layer out of range");
+  if (n_slots == 0) return WRS_OK;
+  if (!slots || !first || !counts) return fail(c, WRS_EINVAL, "null argument");
+  size_t rows = 0;
+  for (size_t i = 0; i < n_slots; ++i) {
+    if (slots[i] >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
+    if (first[i] > kv->max_ctx || counts[i] > kv->max_ctx - first[i])
+      return fail(c, WRS_ERANGE, "rows past the arena's max_ctx");
+    rows += counts[i];
+  }
+  if (rows == 0) return WRS_OK;
+  if (!fits_int(rows)) return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+  int rc = check_rows(c, kv, rows, k_rows, k_len, k_row_stride);
+  if (rc) return rc;
+  rc = check_rows(c, kv, rows, v_rows, v_len, v_row_stride);
+  if (rc) return rc;
+  return move_slot_rows(kv, layer, slots, first, counts, n_slots, k_rows, k_row_stride, v_rows,
+                        v_row_stride);
+}
+
+int wrs_kv_read_cross(wrs_kv* kv, size_t layer, size_t first, size_t n, float* k_rows,
+                      size_t k_len, int64_t k_row_stride, float* v_rows, size_t v_len,
+                      int64_t v_row_stride) {
+  if (!kv) return WRS_EINVAL;
+  wrs_attn_ctx* c = kv->ctx;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (layer >= kv->n_layers) return fail(c, WRS_ERANGE, "layer out of range");
+  if (first > kv->cross_len[layer] || n > kv->cross_len[layer] - first)
+    return fail(c, WRS_ERANGE, "rows past the layer's cross K/V");
+  if (n == 0) return WRS_OK;
+  int rc = check_rows(c, kv, n, k_rows, k_len, k_row_stride);
+  if (rc) return rc;
+  rc = check_rows(c, kv, n, v_rows, v_len, v_row_stride);
+  if (rc) return rc;
+  DeviceGuard g(c->device);
+  wrs::KvSlotRows a = slot_rows(kv, true);
+  a.k_rows = k_rows;
+  a.v_rows = v_rows;
+  a.k_rs = k_row_stride;
+  a.v_rs = v_row_stride;
+  add_rows(a, layer * kv->n_heads, 0, first, n);
+  WRS_HIP(c, wrs::launch_kv_slot_rows(a, kv->plane_type(), false, c->stream));
   return WRS_OK;
 }
 
@@ -1331,6 +1561,80 @@ int wrs_kv_cross_planes(wrs_kv* kv, void** k, void** v) {
   return WRS_OK;
 }
 
+}  // extern "C"
+
+namespace {
+
+// Attention of rows that see a window and the first keys, on K19: n_seqs sequences of count(i) rows
+// whose first plane is plane(i) and whose history is past(i) (window_plan's terms). At most
+// kRowsMaxKeys keys each, checked before.
+template <typename P, typename L, typename C>
+int window_rows(wrs_attn_ctx* c, const wrs_kv* kv, bool cross, bool causal, size_t window,
+                size_t sinks, size_t n_seqs, P plane, L past, C count, const float* q, int64_t q_rs,
+                float* out, int64_t o_rs) {
+  wrs::WindowArgs a;
+  a.q = q;
+  a.o = out;
+  a.k = cross ? kv->k_cross : kv->k_self;
+  a.v = cross ? kv->v_cross : kv->v_self;
+  a.k_scale = cross ? kv->k_cross_scale : kv->k_self_scale;
+  a.v_scale = cross ? kv->v_cross_scale : kv->v_self_scale;
+  a.q_rs = q_rs;
+  a.o_rs = o_rs;
+  const size_t rows = cross ? kv->n_audio_max : kv->max_ctx;
+  a.plane_rows = static_cast<int64_t>(rows);
+  a.scale_rows = static_cast<int64_t>(wrs_kv::scale_rows(rows));
+  a.n_heads = static_cast<int>(kv->n_heads);
+  a.window = static_cast<int>(std::min<size_t>(window, size_t{1} << 24));
+  a.sinks = static_cast<int>(std::min<size_t>(sinks, size_t{1} << 24));
+  a.causal = causal ? 1 : 0;
+  a.scale_log2 = 0.125f * 1.4426950408889634f;
+  const wrs::DType dt = kv->plane_type();
+  size_t row = 0;
+  for (size_t i = 0; i < n_seqs;) {
+    a.n_seqs = 0;
+    for (; i < n_seqs && a.n_seqs < wrs::kWindowMaxSeqs; ++i) {
+      if (count(i) == 0) continue;
+      const int t = a.n_seqs++;
+      a.plane[t] = static_cast<int64_t>(plane(i));
+      a.row0[t] = static_cast<int64_t>(row);
+      a.past[t] = static_cast<int>(past(i));
+      a.rows[t] = static_cast<int>(count(i));
+      row += count(i);
+    }
+    if (a.n_seqs == 0) break;
+    const int rc = tree_scratch(c);
+    if (rc) return rc;
+    a.part = c->tree_part;
+    a.counters = c->tree_counters;
+    const int64_t wgs = wrs::window_plan(a, dt, c->tree_counters != nullptr);
+    WRS_HIP(c, wrs::launch_window_attend(a, dt, wgs, c->stream));
+  }
+  return WRS_OK;
+}
+
+// Rows of a slot's cache with every key up to their own, rows of cross-attention with every key:
+// an 8-bit arena's attention. q and out: packed rows.
+int self_rows_i8(wrs_attn_ctx* c, const wrs_kv* kv, size_t layer, const size_t* slots, size_t n_slots,
+                 size_t count, const float* q, float* out) {
+  const int64_t dm = static_cast<int64_t>(kv->d_model());
+  return window_rows(
+      c, kv, false, true, SIZE_MAX, 0, n_slots,
+      [&](size_t i) { return (layer * kv->n_slots + slots[i]) * kv->n_heads; },
+      [&](size_t i) { return kv->len[slots[i]]; }, [&](size_t) { return count; }, q, dm, out, dm);
+}
+int cross_rows_i8(wrs_attn_ctx* c, const wrs_kv* kv, size_t layer, const float* q, size_t n,
+                  float* out) {
+  const int64_t dm = static_cast<int64_t>(kv->d_model());
+  return window_rows(
+      c, kv, true, false, SIZE_MAX, 0, 1, [&](size_t) { return layer * kv->n_heads; },
+      [&](size_t) { return kv->cross_len[layer]; }, [&](size_t) { return n; }, q, dm, out, dm);
+}
+
+}  // namespace
+
+extern "C" {
+
 int wrs_attn_decode_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t* slots,
                          size_t n, const float* q, float* out) {
   if (!c || !kv) return WRS_EINVAL;
@@ -1340,6 +1644,13 @@ int wrs_attn_decode_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t
   if (!slots || !q || !out) return fail(c, WRS_EINVAL, "null argument");
   DeviceGuard g(c->device);
   const int64_t dm = static_cast<int64_t>(kv->d_model());
+  if (kv->i8()) {
+    for (size_t i = 0; i < n; ++i) {
+      if (slots[i] >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
+      if (kv->len[slots[i]] + 1 > kv->max_ctx) return fail(c, WRS_ERANGE, "slot is full");
+    }
+    return self_rows_i8(c, kv, layer, slots, n, 1, q, out);
+  }
   for (size_t i0 = 0; i0 < n; i0 += wrs::kMaxDecodeGroups) {
     const size_t m = std::min<size_t>(wrs::kMaxDecodeGroups, n - i0);
     std::vector<int64_t> goff(m);
@@ -1383,6 +1694,10 @@ int decode_cross_impl(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const float* q,
     WRS_HIP(c, wrs::launch_fill_zero_rows(out, 0, 0, dm, 1, 1, static_cast<int>(n_beams),
                                           static_cast<int>(dm), c->stream));
     return WRS_OK;
+  }
+  if (kv->i8()) {
+    if (!fits_int(n_beams)) return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+    return cross_rows_i8(c, kv, layer, q, n_beams, out);
   }
   if (kv->f32()) {
     // f32 arena: every beam row on the exact kernel (attention.rs:246-434,
@@ -1462,6 +1777,7 @@ int cross_rows_impl(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const float* q, s
                                           static_cast<int>(dm), c->stream));
     return WRS_OK;
   }
+  if (kv->i8()) return cross_rows_i8(c, kv, layer, q, n, out);
   if (kv->f32()) {
     // f32 arena: the prompt rows as flash_attention_2 takes them
     // (attention.rs:79-105): one row on the exact single-token kernel, more on
@@ -1530,7 +1846,8 @@ int wrs_attn_decode_cross_noalloc(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, con
                                   size_t n_beams, float* out) {
   if (!c || !kv) return WRS_EINVAL;
   std::lock_guard<std::mutex> lk(c->mu);
-  if (kv->f32()) return fail(c, WRS_EUNSUPPORTED, "allocation-free decode needs an f16 arena");
+  if (kv->f32() || kv->i8())
+    return fail(c, WRS_EUNSUPPORTED, "allocation-free decode needs an f16 arena");
   int rc = WRS_OK;
   unsigned char* fixed = noalloc_slot_ptr(c, &rc);
   if (!fixed) return rc;
@@ -1548,6 +1865,10 @@ int wrs_attn_prefill_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, size_t slot
   if (t_past + n_tokens > kv->max_ctx) return fail(c, WRS_ERANGE, "rows past max_ctx");
   DeviceGuard g(c->device);
   const int64_t dm = static_cast<int64_t>(kv->d_model());
+  if (kv->i8()) {
+    if (!q || !out) return fail(c, WRS_EINVAL, "null tensor pointer");
+    return self_rows_i8(c, kv, layer, &slot, 1, n_tokens, q, out);
+  }
   if (kv->f32()) {
     // f32 arena: mha_with_cache's multi-token path (decoder.rs:857-892) on the
     // exact kernel; prompt row i sees t_past + 1 + i keys.
@@ -1592,6 +1913,7 @@ int wrs_attn_tree_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t* 
   std::lock_guard<std::mutex> lk(c->mu);
   if (layer >= kv->n_layers) return fail(c, WRS_ERANGE, "layer out of range");
   if (kv->ctx->device != c->device) return fail(c, WRS_EINVAL, "arena of another device");
+  if (kv->i8()) return fail(c, WRS_EUNSUPPORTED, "tree attention needs an f16 or f32 arena");
   if (n_trees == 0) return WRS_OK;
   if (!slots || !n_nodes) return fail(c, WRS_EINVAL, "null argument");
   size_t rows = 0;
@@ -1652,6 +1974,41 @@ int wrs_attn_tree_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t* 
   return WRS_OK;
 }
 
+int wrs_attn_window_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t* slots,
+                         const size_t* counts, size_t n_slots, size_t window, size_t sinks,
+                         const float* q, size_t q_len, int64_t q_row_stride, float* out,
+                         size_t out_len, int64_t out_row_stride) {
+  if (!c || !kv) return WRS_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (layer >= kv->n_layers) return fail(c, WRS_ERANGE, "layer out of range");
+  if (kv->ctx->device != c->device) return fail(c, WRS_EINVAL, "arena of another device");
+  if (window == 0) return fail(c, WRS_EINVAL, "a window holds at least the row's own key");
+  if (n_slots == 0) return WRS_OK;
+  if (!slots || !counts) return fail(c, WRS_EINVAL, "null argument");
+  size_t rows = 0;
+  for (size_t i = 0; i < n_slots; ++i) {
+    if (slots[i] >= kv->n_slots) return fail(c, WRS_ERANGE, "slot out of range");
+    // The rows are appended, not yet advanced.
+    if (counts[i] > kv->max_ctx - kv->len[slots[i]])
+      return fail(c, WRS_ERANGE, "rows past max_ctx");
+    if (kv->len[slots[i]] + counts[i] >= wrs::kRowsMaxKeys)
+      return fail(c, WRS_EUNSUPPORTED, "cache too long for window attention");
+    rows += counts[i];
+  }
+  if (rows == 0) return WRS_OK;
+  if (!fits_int(rows)) return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+  int rc = check_rows(c, kv, rows, q, q_len, q_row_stride);
+  if (rc) return rc;
+  rc = check_rows(c, kv, rows, out, out_len, out_row_stride);
+  if (rc) return rc;
+  DeviceGuard g(c->device);
+  return window_rows(
+      c, kv, false, true, window, sinks, n_slots,
+      [&](size_t i) { return (layer * kv->n_slots + slots[i]) * kv->n_heads; },
+      [&](size_t i) { return kv->len[slots[i]]; }, [&](size_t i) { return counts[i]; }, q,
+      q_row_stride, out, out_row_stride);
+}
+
 int wrs_attn_prefill_cross(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const float* q,
                            size_t n_tokens, float* out) {
   if (!c || !kv) return WRS_EINVAL;
@@ -1664,6 +2021,7 @@ int wrs_attn_prefill_cross_lse(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const 
   if (!c || !kv) return WRS_EINVAL;
   std::lock_guard<std::mutex> lk(c->mu);
   if (!lse && n_tokens) return fail(c, WRS_EINVAL, "null lse");
+  if (kv->i8()) return fail(c, WRS_EUNSUPPORTED, "row statistics need an f16 arena");
   return cross_rows_impl(c, kv, layer, q, n_tokens, out, lse);
 }
 
@@ -1685,6 +2043,7 @@ int capture_impl(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const float* q, size
     if (heads[p] >= kv->n_heads) return fail(c, WRS_EINVAL, "head index >= n_heads");
     if (slots[p] >= n_selected) return fail(c, WRS_EINVAL, "slot index >= n_selected");
   }
+  if (kv->i8()) return fail(c, WRS_EUNSUPPORTED, "alignment heads need an f16 or f32 arena");
   const size_t n_audio = kv->cross_len[layer];
   // decoder.rs:812 / :822: out holds (row_offset + n_tokens) rows of
   // n_selected * n_audio weights.
@@ -1833,13 +2192,6 @@ int linear_prepare(wrs_attn_ctx* c, int x_dtype, const void* x, int64_t x_rs, si
 bool aligned_out(const void* p, int dt, int64_t rs, int64_t hs) {
   const uintptr_t need = dt == WRS_F32 ? 16 : 8;
   return (reinterpret_cast<uintptr_t>(p) % need) == 0 && rs % 4 == 0 && hs % 4 == 0;
-}
-
-// Whether n_rows rows of n_cols elements, row_stride apart, lie within len (no product is
-// formed that could pass 64 bits).
-bool rows_fit(size_t n_rows, size_t n_cols, int64_t row_stride, size_t len) {
-  if (n_cols > len) return false;
-  return n_rows == 1 || static_cast<size_t>(row_stride) <= (len - n_cols) / (n_rows - 1);
 }
 
 // The checks that quantisation and its inverse share: values of `dtype` in n_rows rows
@@ -2119,6 +2471,31 @@ int wrs_kv_set_cross_proj(wrs_kv* kv, int x_dtype, const void* enc, size_t enc_l
     const size_t dm = kv->d_model();
     int rc = linear_prepare(c, x_dtype, enc, enc_row_stride, n_audio, dm, dm, a);
     if (rc) return rc;
+    if (kv->i8()) {
+      // A layer at a time: projected as f32 rows, then rounded into its planes.
+      const size_t half = align_up(n_audio * dm * sizeof(float), 256);
+      rc = grow(c, reinterpret_cast<void**>(&c->cross_rows), &c->cross_rows_bytes, 2 * half, false);
+      if (rc) return rc;
+      float* const k = c->cross_rows;
+      float* const v = k + half / sizeof(float);
+      a.out_rs = static_cast<int64_t>(dm);
+      a.out_hs = 64;
+      a.n_groups = 2;
+      for (size_t l = 0; l < kv->n_layers; ++l) {
+        a.w[0] = static_cast<const _Float16*>(w_k[l]);
+        a.bias[0] = nullptr;
+        a.out[0] = k;
+        a.w[1] = static_cast<const _Float16*>(w_v[l]);
+        a.bias[1] = b_v ? b_v[l] : nullptr;
+        a.out[1] = v;
+        WRS_HIP(c, wrs::launch_linear_f16w(a, wrs::kF32, c->stream));
+        rc = write_rows(c, kv, k, v, n_audio, kv->k_cross, kv->v_cross, kv->cross_off(l),
+                        kv->n_audio_max * 64, 0);
+        if (rc) return rc;
+      }
+      for (size_t l = 0; l < kv->n_layers; ++l) kv->cross_len[l] = n_audio;
+      return WRS_OK;
+    }
     a.out_rs = 64;  // [head][n_audio_max][64] planes
     a.out_hs = static_cast<int64_t>(kv->n_audio_max * 64);
     // decoder.rs:433-442: K without bias, V with cross_attn_v_b; every layer's
@@ -2140,6 +2517,90 @@ int wrs_kv_set_cross_proj(wrs_kv* kv, int x_dtype, const void* enc, size_t enc_l
     }
   }
   for (size_t l = 0; l < kv->n_layers; ++l) kv->cross_len[l] = n_audio;
+  return WRS_OK;
+}
+
+int wrs_token_logprobs(wrs_attn_ctx* c, int dtype, const void* logits, size_t logits_len,
+                       int64_t row_stride, size_t n_rows, size_t n_vocab, const void* allowed,
+                       size_t allowed_len, int64_t allowed_row_stride, float temperature,
+                       const void* tokens, float* logprobs, float* entropy, size_t top_k,
+                       void* top_ids, float* top_logprobs) {
+  if (!c) return WRS_EINVAL;
+  std::lock_guard<std::mutex> lk(c->mu);
+  if (dtype != WRS_F32 && dtype != WRS_F16 && dtype != WRS_BF16)
+    return fail(c, WRS_EUNSUPPORTED, "logits must be f32, f16 or bf16");
+  if (n_rows == 0) return WRS_OK;
+  if (!logits) return fail(c, WRS_EINVAL, "null logits");
+  if (n_vocab == 0) return fail(c, WRS_EINVAL, "rows of no entries");
+  if (n_vocab > (size_t{1} << 22))
+    return fail(c, WRS_EUNSUPPORTED, "more than 2^22 entries in a row");
+  if (!fits_int(n_rows)) return fail(c, WRS_EINVAL, "dimension exceeds 2^31");
+  if (!(temperature > 0.f) || !std::isfinite(temperature) ||
+      !std::isfinite(1.4426950408889634f / temperature))
+    return fail(c, WRS_EINVAL, "temperature must be positive and finite, and so its inverse");
+  if (top_k > static_cast<size_t>(wrs::kScoreMostTop) || top_k > n_vocab)
+    return fail(c, WRS_EUNSUPPORTED, "at most 32 alternatives, and no more than entries");
+  if ((tokens == nullptr) != (logprobs == nullptr))
+    return fail(c, WRS_EINVAL, "tokens and logprobs come together");
+  if (top_k ? !top_ids && !top_logprobs : top_ids || top_logprobs)
+    return fail(c, WRS_EINVAL, "alternatives need a top_k and a place");
+  if (!logprobs && !entropy && !top_k) return fail(c, WRS_EINVAL, "nothing to compute");
+  const size_t size = dtype == WRS_F32 ? 4 : 2;
+  uintptr_t words = 0;
+  for (const void* p : {tokens, static_cast<const void*>(logprobs), static_cast<const void*>(entropy),
+                        static_cast<const void*>(top_ids), static_cast<const void*>(top_logprobs)})
+    words |= reinterpret_cast<uintptr_t>(p);
+  if (reinterpret_cast<uintptr_t>(logits) % size || words & 3)
+    return fail(c, WRS_EINVAL, "tensors must be aligned to their elements");
+  if (n_rows > 1 && row_stride < static_cast<int64_t>(n_vocab))
+    return fail(c, WRS_EINVAL, "row stride below n_vocab");
+  if (!rows_fit(n_rows, n_vocab, row_stride, logits_len))
+    return fail(c, WRS_EINVAL, "logits shorter than their rows");
+  if (allowed) {
+    if (n_rows > 1 && allowed_row_stride != 0 && allowed_row_stride < static_cast<int64_t>(n_vocab))
+      return fail(c, WRS_EINVAL, "allowed rows are n_vocab apart or more, or one for all (0)");
+    if (!rows_fit(n_rows, n_vocab, allowed_row_stride, allowed_len))
+      return fail(c, WRS_EINVAL, "allowed shorter than its rows");
+  }
+  DeviceGuard g(c->device);
+  int rc = tree_scratch(c);
+  if (rc) return rc;
+  wrs::ScoreArgs a{};
+  a.row_stride = row_stride;
+  a.allowed_stride = allowed_row_stride;
+  a.n_vocab = static_cast<int>(n_vocab);
+  a.top_k = static_cast<int>(top_k);
+  a.temperature = temperature;
+  a.scale_log2 = 1.4426950408889634f / temperature;
+  a.entropy = entropy;
+  a.part = c->tree_part;
+  a.counters = c->tree_counters;
+  a.n_rows = static_cast<int64_t>(n_rows);
+  wrs::score_plan(a, c->tree_counters != nullptr);
+  size_t most = n_rows;
+  if (a.n_chunks > 1) {
+    if (!c->tree_counters)
+      return fail(c, WRS_ECAPTURE, "rows past 65536 entries need scratch: call wrs_attn_reserve "
+                                   "(n_heads, decode_rows, decode_keys) or score once first");
+    // What the scratch takes at once.
+    most = std::min<size_t>(wrs::kTreePartFloats / wrs::kScorePart / a.n_chunks,
+                            wrs::kTreeCounterWords / 32);
+  }
+  for (size_t r = 0; r < n_rows; r += most) {
+    a.logits = static_cast<const char*>(logits) + r * static_cast<size_t>(row_stride) * size;
+    a.allowed = allowed ? static_cast<const uint8_t*>(allowed) +
+                              r * static_cast<size_t>(allowed_row_stride)
+                        : nullptr;
+    a.n_rows = static_cast<int64_t>(std::min(most, n_rows - r));
+    a.tokens = tokens ? static_cast<const int*>(tokens) + r : nullptr;
+    a.logprobs = logprobs ? logprobs + r : nullptr;
+    a.entropy = entropy ? entropy + r : nullptr;
+    a.top_ids = top_ids ? static_cast<int*>(top_ids) + r * top_k : nullptr;
+    a.top_logprobs = top_logprobs ? top_logprobs + r * top_k : nullptr;
+    WRS_HIP(c, wrs::launch_score_rows(
+                   a, dtype == WRS_F32 ? wrs::kF32 : dtype == WRS_F16 ? wrs::kF16 : wrs::kBF16,
+                   c->stream));
+  }
   return WRS_OK;
 }
 

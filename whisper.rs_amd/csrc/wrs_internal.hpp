@@ -13,7 +13,7 @@
 
 namespace wrs {
 
-enum DType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+enum DType : int { kF32 = 0, kF16 = 1, kBF16 = 2, kI8 = 4 };
 
 // Activation applied by a projection's epilogue, in f32 before the output
 // rounding (the reference runs gelu_inplace on the f32 projection output).
@@ -51,6 +51,38 @@ __device__ inline void st_agent(float* p, float v) {
 }
 __device__ inline float ld_agent(const float* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Two floats at once, as st_agent and ld_agent (8-byte aligned).
+__device__ inline void st_agent2(float* p, float x, float y) {
+  const uint64_t v = __builtin_bit_cast(uint32_t, x) |
+                     static_cast<uint64_t>(__builtin_bit_cast(uint32_t, y)) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline void ld_agent2(const float* p, float& x, float& y) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  x = __builtin_bit_cast(float, static_cast<uint32_t>(v));
+  y = __builtin_bit_cast(float, static_cast<uint32_t>(v >> 32));
+}
+
+// x / n, with the remainder; inv: inverse(n).
+inline uint32_t inverse(int n) {  // 2^32 / n rounded up, for n 1: 2^32 - 1
+  const uint64_t i = ((uint64_t{1} << 32) + n - 1) / n;
+  return i > 0xffffffffu ? 0xffffffffu : static_cast<uint32_t>(i);
+}
+__device__ inline int divide(int x, int n, uint32_t inv, int& rest) {
+  int q = static_cast<int>(__umulhi(static_cast<uint32_t>(x), inv));
+  rest = x - q * n;
+  if (rest < 0) {
+    --q;
+    rest += n;
+  }
+  if (rest >= n) {
+    ++q;
+    rest -= n;
+  }
+  return q;
 }
 
 // Orders a wave's own LDS writes and reads: its LDS operations complete in order, only the
@@ -259,6 +291,61 @@ struct TreeArgs {
 int64_t tree_plan(TreeArgs& a, DType dt, bool split);
 hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStream_t s);
 
+// Attention of rows that see a sliding window and the first keys: sequence t's rows[t] query rows
+// (row row0[t] + i, head h at q + row*q_rs + h*64, any dword) against planes plane[t] + h of k and v
+// (plane_rows rows of 64 f16, f32, or 8-bit codes with scale_rows scales). With `causal` row i stands
+// at position past[t] + i, otherwise every row at past[t] - 1, and sees the keys j up to it with
+// j > position - window or j < sinks. past + rows < 2^24 - 4095 and window <= 2^24. window_plan lays
+// out the launch as tree_plan does, with the same scratch.
+constexpr int kWindowMaxSeqs = 64;  // per launch
+struct WindowArgs {
+  const float* q;
+  float* o;  // row r at o + r*o_rs
+  const void *k, *v;
+  const uint8_t *k_scale, *v_scale;  // 8-bit planes only
+  int64_t q_rs, o_rs, plane_rows, scale_rows;
+  int n_heads, n_seqs, chunk, window, sinks, causal;
+  float scale_log2;  // (1/8) * log2(e)
+  float* part;
+  unsigned* counters;
+  int64_t plane[kWindowMaxSeqs], row0[kWindowMaxSeqs];
+  int past[kWindowMaxSeqs], rows[kWindowMaxSeqs];  // rows >= 1; past >= 1 where not causal
+  // By window_plan, as TreeArgs has them; chunk counts steps.
+  int n_wgs[kWindowMaxSeqs], wg0[kWindowMaxSeqs], n_blk[kWindowMaxSeqs], n_split[kWindowMaxSeqs];
+  uint32_t blk_inv[kWindowMaxSeqs], split_inv[kWindowMaxSeqs];
+};
+int64_t window_plan(WindowArgs& a, DType dt, bool split);
+hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipStream_t s);
+
+// Log probabilities of given tokens, entropies and the top_k likeliest entries of rows of logits
+// (f32, f16 or bf16, row r at r*row_stride) over the entries whose allowed byte is not zero (nullptr:
+// all; row r at r*allowed_stride). tokens, logprobs, entropy, top_ids and top_logprobs may be null.
+// score_plan deals the rows: n_chunks workgroups each, which need part (kScorePart floats a
+// workgroup) and counters (a line of 32 words a row, zero between launches) where it is more than one;
+// without `split` only rows past kScoreChunk entries are dealt.
+constexpr int kScoreMostTop = 32;
+constexpr int kScoreChunk = 65536;   // entries of one workgroup, at most
+constexpr int kScoreMaxWgs = 512;    // of a launch that splits rows which fit a workgroup
+constexpr int kScoreMostChunks = 64;  // of a row
+constexpr int kScorePart = 4 + 2 * kScoreMostTop;  // floats: m, s, t, and the best entries' keys
+struct ScoreArgs {
+  const void* logits;
+  int64_t row_stride;
+  const uint8_t* allowed;
+  int64_t allowed_stride;
+  int64_t n_rows;
+  int n_vocab, top_k, chunk, n_chunks;
+  float temperature, scale_log2;  // log2(e) / temperature
+  const int* tokens;
+  float *logprobs, *entropy;
+  int* top_ids;
+  float* top_logprobs;
+  float* part;
+  unsigned* counters;
+};
+void score_plan(ScoreArgs& a, bool split);
+hipError_t launch_score_rows(const ScoreArgs& a, DType dt, hipStream_t s);
+
 // Measurement: a streaming read of `bytes` (multiple of 16, 16-byte aligned)
 // with the split-K decode's grid shape (512 threads x 64 bytes per
 // workgroup); sink receives stream_read_blocks(bytes) floats.
@@ -459,5 +546,36 @@ struct KeepArgs {
 };
 template <int kSlots, int kMoves>
 hipError_t launch_kv_keep_rows(const KeepArgs<kSlots, kMoves>& a, hipStream_t s);
+
+// Rows of several slots into the planes (f16, f32, or 8-bit codes with scales), or back out as
+// f32: count[u] rows from row row0[u] of k_rows and v_rows (k_rs and v_rs apart, head h at + h*64)
+// against rows pos[u].. of planes plane[u] + h, each plane_rows rows of 64 (and scale_rows scales).
+constexpr int kRowSlots = 64;  // per launch
+struct KvSlotRows {
+  float *k_rows, *v_rows;  // only read where rows are stored
+  int64_t k_rs, v_rs;
+  void *k, *v;
+  uint8_t *k_scale, *v_scale;  // 8-bit planes only
+  int64_t plane_rows, scale_rows;
+  int n_heads, n_slots;
+  uint32_t heads_inv;  // 2^32 / n_heads, as divide() takes it
+  int64_t plane[kRowSlots], row0[kRowSlots];
+  int pos[kRowSlots], count[kRowSlots];
+};
+hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStream_t s);
+// The planes of an 8-bit arena's slot: plane (l, h) is plane l*layer + h, of `rows` rows of codes
+// and `scale_rows` scales.
+struct Kv8Planes {
+  uint8_t *k, *v, *k_scale, *v_scale;
+  int64_t layer, rows, scale_rows;
+};
+hipError_t launch_kv8_copy(const Kv8Planes& to, const Kv8Planes& from, int n_layers, int n_heads,
+                           int len, hipStream_t s);
+hipError_t launch_kv8_slide(const Kv8Planes& a, int n_layers, int n_heads, int len, int drop,
+                            hipStream_t s);
+// launch_kv_keep_rows for an 8-bit arena; p: its planes from plane 0 on (a.off and a.plane_stride
+// give a slot's first plane, both in any one unit).
+template <int kSlots, int kMoves>
+hipError_t launch_kv8_keep_rows(const KeepArgs<kSlots, kMoves>& a, const Kv8Planes& p, hipStream_t s);
 
 }  // namespace wrs
