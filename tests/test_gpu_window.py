@@ -296,19 +296,34 @@ def test_8_bit_rows_of_any_scale_in_one_sum(wrs, ctx):
     sc = torch.where(hidden(100, 4, 10 ** 6, 0), -INF, sc)
     scale = torch.softmax(sc, 1) @ v.abs()
     assert ((got - want).abs() <= scale * 1.2e-4).all()  # 2 dw with S below 12, as above
-    # one key takes the whole weight against huge values elsewhere
-    def far(i, k, v):
+    # one key takes the whole weight against huge values elsewhere, before and behind it
+    for past, at, rows in ((100, 50, 2), (2000, 1900, 1), (2000, 70, 20), (400, 300, 40)):
+        def far(i, k, v):
+            k.zero_()
+            k[:, 0] = -80.0
+            k[at, 0] = 80.0
+            v *= 2.0 ** 40
+            v[at] = v[at] * 2.0 ** -40
+        s = Session(wrs, ctx, "i8", 1, [past], [rows], seed=15, spoil=far)
+        s.q.zero_()
+        s.q[:, 0] = 8.0  # scores 80 and -80: the others weigh e^-160
+        got = s.run(10 ** 6, 0).double()
+        want = stored(s.rows[0][1], "i8")[at]
+        assert (got - want).abs().max().item() <= want.abs().max().item() * 2.0 ** -17
+    # scores that rise from key to key, values that fall
+    def ramp(i, k, v):
         k.zero_()
-        k[:, 0] = -80.0
-        k[50, 0] = 80.0
-        v *= 2.0 ** 40
-        v[50] = v[50] * 2.0 ** -40
-    s = Session(wrs, ctx, "i8", 1, [100], [2], seed=15, spoil=far)
+        k[:, 0] = torch.arange(k.shape[0], device="cuda") * 0.25 - 100.0
+        v *= torch.exp2(100.0 - torch.arange(v.shape[0], device="cuda") * 0.2)[:, None]
+    s = Session(wrs, ctx, "i8", 1, [900], [33], seed=17, spoil=ramp)
     s.q.zero_()
-    s.q[:, 0] = 8.0  # scores 80 and -80: the others weigh e^-160
+    s.q[:, 0] = 4.0
+    want, _ = s.expect(10 ** 6, 0)
     got = s.run(10 ** 6, 0).double()
-    want = stored(s.rows[0][1], "i8")[50]
-    assert (got - want).abs().max().item() <= want.abs().max().item() * 2.0 ** -17
+    k, v = (stored(x, "i8") for x in s.rows[0])
+    sc = torch.where(hidden(900, 33, 10 ** 6, 0), -INF, s.q.double() @ k.T.contiguous() / 8)
+    # scores of up to 66 (S above): 2 dw = 2 (66 (2^-22 + 2^-21 + 2^-23) + 2^-18 + 2^-22)
+    assert ((got - want).abs() <= torch.softmax(sc, 1) @ v.abs() * 1.3e-4).all()
 
 
 def test_wide_range_of_values_f16(wrs, ctx):

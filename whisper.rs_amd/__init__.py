@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import struct
 import threading
 
 import numpy as np
@@ -343,6 +344,34 @@ def _sizes(values):
     return _size_arrays[n](*values) if n else None
 
 
+_packers = {}
+
+
+def _packed(values):
+    """A sequence of counts as size_t values in memory, for a call's duration (made in a third of
+    the time of a ctypes array)."""
+    n = len(values)
+    pack = _packers.get(n)
+    if pack is None:
+        pack = struct.Struct(f"{n}N").pack
+        if n <= 256:
+            _packers[n] = pack
+    try:
+        return pack(*values)
+    except struct.error:
+        raise AssertionError("slots and counts are whole numbers from 0 on") from None
+
+
+_names = {}  # torch.dtype -> its name, filled as dtypes come by
+
+
+def _dtype_name(t):
+    name = _names.get(t.dtype)
+    if name is None:
+        name = _names[t.dtype] = str(t.dtype).rpartition(".")[2]
+    return name
+
+
 class Mx4:
     """Packed MXFP4 rows (OCP Microscaling Formats v1.0): ``codes`` uint8
     [rows][cols / 2], two e2m1 codes to a byte with the even column in the low
@@ -459,36 +488,38 @@ def token_logprobs(logits, tokens=None, logprobs=None, *, entropy=None, top_ids=
     logits. A token that is hidden or no entry has -inf."""
     ctx = ctx or default_context()
     n, v, rs = _rows(logits, "token_logprobs")
-    _on_device(ctx, "token_logprobs", logits)
-    k = 0
-    for t, dtype, dims, name in ((tokens, "int32", 1, "tokens"), (logprobs, "float32", 1, "logprobs"),
-                                 (entropy, "float32", 1, "entropy"),
-                                 (top_ids, "int32", 2, "top_ids"),
-                                 (top_logprobs, "float32", 2, "top_logprobs")):
+    device, k, ptr = ctx.device, 0, []
+    for t, dtype, dims in ((tokens, "int32", 1), (logprobs, "float32", 1), (entropy, "float32", 1),
+                           (top_ids, "int32", 2), (top_logprobs, "float32", 2)):
         if t is None:
+            ptr.append(None)
             continue
-        if str(t.dtype) != "torch." + dtype or not t.is_contiguous():
-            raise TypeError(f"token_logprobs: contiguous {dtype} {name} expected, got {t.dtype}")
-        assert t.dim() == dims and t.shape[0] == n
-        _on_device(ctx, "token_logprobs", t)
+        if _dtype_name(t) != dtype or not t.is_contiguous():
+            raise TypeError(f"token_logprobs: contiguous {dtype} outputs and int32 tokens expected, "
+                            f"got {t.dtype}")
+        shape = t.shape
+        assert len(shape) == dims and shape[0] == n
         if dims == 2:
-            assert k in (0, t.shape[1]) and t.shape[1] > 0
-            k = t.shape[1]
+            assert k in (0, shape[1]) and shape[1] > 0
+            k = shape[1]
+        if t.get_device() != device:
+            _on_device(ctx, "token_logprobs", t)
+        ptr.append(t.data_ptr())
+    _on_device(ctx, "token_logprobs", logits)
     ok_p, ok_len, ok_rs = None, 0, 0
     if allowed is not None:
-        if str(allowed.dtype) not in ("torch.bool", "torch.uint8"):
+        if _dtype_name(allowed) not in ("bool", "uint8"):
             raise TypeError(f"token_logprobs: bool or uint8 allowed expected, got {allowed.dtype}")
         rows, width, ok_rs = _rows(allowed, "token_logprobs")
         assert width == v and rows in (1, n)
         _on_device(ctx, "token_logprobs", allowed)
-        ok_p, ok_len = allowed.data_ptr(), _span(allowed)
         if rows == 1:
             ok_rs = 0
-    ptr = [None if t is None else t.data_ptr()
-           for t in (tokens, logprobs, entropy, top_ids, top_logprobs)]
+        ok_p, ok_len = allowed.data_ptr(), (rows - 1) * ok_rs + v
     ctx.check(ctx._lib.wrs_token_logprobs(
-        ctx.handle, _dtype_code(logits), logits.data_ptr(), _span(logits), rs, n, v, ok_p, ok_len,
-        ok_rs, float(temperature), ptr[0], ptr[1], ptr[2], k, ptr[3], ptr[4]), "token_logprobs")
+        ctx.handle, _dtype_code(logits), logits.data_ptr(), (n - 1) * rs + v if n else 0, rs, n, v,
+        ok_p, ok_len, ok_rs, float(temperature), ptr[0], ptr[1], ptr[2], k, ptr[3], ptr[4]),
+        "token_logprobs")
 
 
 def layer_norm(x, gamma, beta, eps, out, ctx=None):
@@ -603,18 +634,17 @@ class KvArena:
         self._c(self._lib.wrs_kv_append(self.handle, layer, slot, pk, pv, nk // self.d_model,
                                         host), "append")
 
-    def _device_rows(self, what, *tensors):
-        """(rows, [pointer, span, stride of each]) of float32 rows of d_model."""
-        count, args = None, []
-        for t in tensors:
-            n, d, rs = _rows(t, what)
-            if _dtype_code(t) != WRS_F32:
-                raise TypeError(f"{what}: float32 rows expected, got {t.dtype}")
-            assert d == self.d_model and count in (None, n)
-            count = n
-            args += [t.data_ptr(), _span(t), rs]
-        _on_device(self.ctx, what, *tensors)
-        return count, args
+    def _device_rows(self, what, a, b):
+        """Their rows, and (pointer, elements, row stride) of each: float32 rows of d_model."""
+        n, d, rs_a = _rows(a, what)
+        n_b, d_b, rs_b = _rows(b, what)
+        if _dtype_name(a) != "float32" or _dtype_name(b) != "float32":
+            raise TypeError(f"{what}: float32 rows expected, got {a.dtype} and {b.dtype}")
+        assert d == d_b == self.d_model and n == n_b
+        device = self.ctx.device
+        if a.get_device() != device or b.get_device() != device:
+            _on_device(self.ctx, what, a, b)
+        return n, (a.data_ptr(), (n - 1) * rs_a + d, rs_a, b.data_ptr(), (n - 1) * rs_b + d, rs_b)
 
     def append_rows(self, layer, slots, counts, k, v):
         """Appends ``counts[i]`` rows of ``slots[i]`` (each slot once) in one launch
@@ -622,7 +652,7 @@ class KvArena:
         rows of any stride. :meth:`advance` takes them into the history."""
         n, args = self._device_rows("append_rows", k, v)
         assert len(slots) == len(counts) and sum(counts) == n
-        self._c(self._lib.wrs_kv_append_rows(self.handle, layer, _sizes(slots), _sizes(counts),
+        self._c(self._lib.wrs_kv_append_rows(self.handle, layer, _packed(slots), _packed(counts),
                                              len(slots), *args), "append_rows")
 
     def read_rows(self, layer, slots, first, counts, k, v):
@@ -630,8 +660,8 @@ class KvArena:
         the rows of ``k`` and ``v`` (``wrs_kv_read_rows``)."""
         n, args = self._device_rows("read_rows", k, v)
         assert len(slots) == len(counts) == len(first) and sum(counts) == n
-        self._c(self._lib.wrs_kv_read_rows(self.handle, layer, _sizes(slots), _sizes(first),
-                                           _sizes(counts), len(slots), *args), "read_rows")
+        self._c(self._lib.wrs_kv_read_rows(self.handle, layer, _packed(slots), _packed(first),
+                                           _packed(counts), len(slots), *args), "read_rows")
 
     def read_cross(self, layer, first, k, v):
         """The stored values of cross rows from ``first`` on, into the rows of ``k`` and ``v``
@@ -720,8 +750,8 @@ class KvArena:
         assert len(slots) == len(counts) and sum(counts) == n
         window = 2 ** 64 - 1 if window is None else window
         assert window > 0 and sinks >= 0
-        self._c(self._lib.wrs_attn_window_self(self.ctx.handle, self.handle, layer, _sizes(slots),
-                                               _sizes(counts), len(slots), window, sinks, *args),
+        self._c(self._lib.wrs_attn_window_self(self.ctx.handle, self.handle, layer, _packed(slots),
+                                               _packed(counts), len(slots), window, sinks, *args),
                 "window_self")
 
     def keep_rows(self, slots, counts, rows):

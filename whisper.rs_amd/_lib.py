@@ -90,9 +90,9 @@ _SIGNATURES = {
     "wrs_kv_set_len": (_int, [_vp, _sz, _sz]),
     "wrs_kv_slide_to_fit": (_int, [_vp, _sz, _sz, _sz, _szp]),
     "wrs_kv_append": (_int, [_vp, _sz, _sz, _vp, _vp, _sz, _int]),
-    "wrs_kv_append_rows": (_int, [_vp, _sz, _szp, _szp, _sz, _vp, _sz, ctypes.c_int64, _vp, _sz,
+    "wrs_kv_append_rows": (_int, [_vp, _sz, _vp, _vp, _sz, _vp, _sz, ctypes.c_int64, _vp, _sz,
                                   ctypes.c_int64]),
-    "wrs_kv_read_rows": (_int, [_vp, _sz, _szp, _szp, _szp, _sz, _vp, _sz, ctypes.c_int64, _vp,
+    "wrs_kv_read_rows": (_int, [_vp, _sz, _vp, _vp, _vp, _sz, _vp, _sz, ctypes.c_int64, _vp,
                                 _sz, ctypes.c_int64]),
     "wrs_kv_read_cross": (_int, [_vp, _sz, _sz, _sz, _vp, _sz, ctypes.c_int64, _vp, _sz,
                                  ctypes.c_int64]),
@@ -108,7 +108,7 @@ _SIGNATURES = {
     "wrs_attn_prefill_self": (_int, [_vp, _vp, _sz, _sz, _vp, _sz, _vp]),
     "wrs_attn_tree_self": (_int, [_vp, _vp, _sz, _szp, _szp, _sz, _vp, _sz, _vp, ctypes.c_int64,
                                   _vp, ctypes.c_int64]),
-    "wrs_attn_window_self": (_int, [_vp, _vp, _sz, _szp, _szp, _sz, _sz, _sz, _vp, _sz,
+    "wrs_attn_window_self": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _sz,
                                     ctypes.c_int64, _vp, _sz, ctypes.c_int64]),
     "wrs_attn_prefill_cross": (_int, [_vp, _vp, _sz, _vp, _sz, _vp]),
     "wrs_attn_prefill_cross_lse": (_int, [_vp, _vp, _sz, _vp, _sz, _vp, _vp]),

@@ -1,6 +1,6 @@
 // Log probabilities of given tokens, the entropy and the likeliest alternatives of rows of logits.
 //
-// K20 (score_rows): over the allowed entries of a row, m the largest, z_j = (x_j - m) / T:
+// K21 (score_rows): over the allowed entries of a row, m the largest, z_j = (x_j - m) / T:
 //   lp_j = z_j - ln s,  s = sum e^z,  H = ln s - sum z e^z / s,
 //   and the k largest x_j with their indices, the lowest index first among equals.
 //   A row is read once: every thread keeps the maximum of its entries (and which group of 16 held it
@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace wrs {
 namespace {
@@ -29,8 +30,13 @@ typedef uint32_t u32u __attribute__((aligned(1)));
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kGroup = 16;  // entries of a thread's group: 16-byte pieces, kThreads pieces apart
+constexpr int kSmallGroup = kScoreSmall / kThreads;  // entries of a thread of a small chunk
+static_assert(kScoreSmall <= kScoreMostTop * (kScoreChunk / kThreads), "room for every one's key");
 constexpr int kRun = kThreads / 64;  // neighbouring threads that share a maximum of the bound
+static_assert(kRun == 8, "max8");
 constexpr int kMostPieces = kScoreChunk / kThreads / 4;  // of a thread, at most (f32: 4 entries)
+static_assert(kMostPieces <= 64, "a piece a lane");
+constexpr int kMostKeys = kScoreMostTop * (kScoreChunk / kThreads);  // entries of that many threads
 constexpr int kCounterStride = 32;   // 128 bytes between merge counters
 constexpr float kLow = -1e30f;       // finite: times a weight of 0 it is 0
 
@@ -48,23 +54,28 @@ __device__ inline int index_of(uint64_t key) {
   return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
 }
 
+// A 16-byte piece of entries. T: float, _Float16 or uint16_t (bf16).
 template <typename T>
 struct Piece {
-  static constexpr int kN = 16 / sizeof(T);  // entries of 16 bytes
-};
-// Entry e of a 16-byte piece as f32. T: float, _Float16 or uint16_t (bf16).
-template <typename T>
-__device__ inline float entry(const u32x4& p, int e) {
-  const uint32_t w = p[sizeof(T) == 4 ? e : e >> 1];
-  if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(float, w);
-  } else {
-    if constexpr (__is_same(T, uint16_t))
-      return __builtin_bit_cast(float, e & 1 ? w & 0xFFFF0000u : w << 16);
+  static constexpr int kN = 16 / sizeof(T);
+  u32x4 w;
+  __device__ inline float operator[](int e) const {
+    const uint32_t x = w[sizeof(T) == 4 ? e : e >> 1];
+    if constexpr (sizeof(T) == 4)
+      return __builtin_bit_cast(float, x);
+    else if constexpr (__is_same(T, uint16_t))
+      return __builtin_bit_cast(float, e & 1 ? x & 0xFFFF0000u : x << 16);
     else
       return static_cast<float>(
-          __builtin_bit_cast(_Float16, static_cast<uint16_t>(e & 1 ? w >> 16 : w)));
+          __builtin_bit_cast(_Float16, static_cast<uint16_t>(e & 1 ? x >> 16 : x)));
   }
+};
+template <typename T>
+__device__ inline float value(T x) {
+  if constexpr (__is_same(T, uint16_t))
+    return __builtin_bit_cast(float, static_cast<uint32_t>(x) << 16);
+  else
+    return static_cast<float>(x);
 }
 
 // A row's (or chunk's) entries: x[0 .. n), entry i allowed where ok[i] is not zero.
@@ -74,121 +85,200 @@ struct Row {
   const uint8_t* ok;
   int n;
   static constexpr int kN = Piece<T>::kN;
-  // Piece p, hidden entries and those past the end at -infinity.
-  template <bool kWhole>
-  __device__ inline void load(int p, float (&v)[kN]) const {
-    const int i0 = p * kN;
-    if (kWhole || i0 + kN <= n) {
-      const u32x4 w = *reinterpret_cast<const u32x4u*>(x + i0);
+  // Piece p, entries kN p.. : hidden ones and those past the end come as -infinity. The row's last
+  // piece is read from its last kN entries on, so that nothing lies outside the row; returns the
+  // index of v[0].
+  __device__ inline int load(int p, float (&v)[kN]) const {
+    const int i0 = p * kN, at = min(i0, n - kN);
+    if (n < kN) {  // rows shorter than a piece
 #pragma unroll
-      for (int e = 0; e < kN; ++e) v[e] = entry<T>(w, e);
-      if constexpr (kMask) {
-#pragma unroll
-        for (int h = 0; h < kN / 4; ++h) {
-          const uint32_t m = *reinterpret_cast<const u32u*>(ok + i0 + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(m & (0xFFu << (8 * e)))) v[4 * h + e] = -INFINITY;
-        }
-      }
-      return;
+      for (int e = 0; e < kN; ++e)
+        v[e] = i0 + e < n && (!kMask || ok[i0 + e]) ? value(x[i0 + e]) : -INFINITY;
+      return i0;
     }
+    Raw r;
+    fetch(at, r);
+    values(r, v);
 #pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      v[e] = -INFINITY;
-      if (i0 + e < n && (!kMask || ok[i0 + e])) {
-        if constexpr (__is_same(T, uint16_t))
-          v[e] = __builtin_bit_cast(float, static_cast<uint32_t>(x[i0 + e]) << 16);
-        else
-          v[e] = static_cast<float>(x[i0 + e]);
-      }
+    for (int e = 0; e < kN; ++e)
+      if (at + e < i0) v[e] = -INFINITY;
+    return at;
+  }
+  // A piece that lies within the row, from entry `at` on, in two steps.
+  struct Raw {
+    Piece<T> x;
+    uint32_t ok[kMask ? kN / 4 : 1];
+  };
+  __device__ inline void fetch(int at, Raw& r) const {
+    r.x.w = *reinterpret_cast<const u32x4u*>(x + at);
+    if constexpr (kMask) {
+#pragma unroll
+      for (int h = 0; h < kN / 4; ++h) r.ok[h] = *reinterpret_cast<const u32u*>(ok + at + 4 * h);
+    }
+  }
+  static __device__ inline void values(const Raw& r, float (&v)[kN]) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) v[e] = r.x[e];
+    if constexpr (kMask) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (!(r.ok[e / 4] & (0xFFu << (8 * (e & 3))))) v[e] = -INFINITY;
     }
   }
 };
 
-__device__ inline float wave_max(float x) {
+// The largest of the 16 f16 entries of two pieces, two at a time (widened first: 16 conversions).
+template <typename R>
+__device__ inline float max_of_halves(const R (&r)[2]) {
+  uint32_t m = r[0].x.w[0];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-  return x;
+  for (int i = 1; i < 8; ++i) {
+    const uint32_t w = r[i >> 2].x.w[i & 3];
+    asm("v_pk_max_f16 %0, %1, %2" : "=v"(m) : "v"(m), "v"(w));
+  }
+  return fmaxf(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m))),
+               static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(m >> 16))));
+}
+
+template <int kCtrl>
+__device__ inline float dpp(float x) {
+  const int i = __builtin_bit_cast(int, x);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, kCtrl, 0xF, 0xF, false));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128;  // lanes of 16
+__device__ inline float max8(float x) {  // of 8 neighbouring lanes
+  x = fmaxf(x, dpp<kXor1>(x));
+  x = fmaxf(x, dpp<kXor2>(x));
+  return fmaxf(x, dpp<kHalfMirror>(x));
+}
+__device__ inline float wave_max(float x) {
+  x = max8(x);
+  return max_x16_x32(fmaxf(x, dpp<kRor8>(x)));
 }
 __device__ inline float wave_sum(float x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
+  x += dpp<kXor1>(x);
+  x += dpp<kXor2>(x);
+  x += dpp<kHalfMirror>(x);
+  return sum_x16_x32(x + dpp<kRor8>(x));
 }
 // How many of n keys are larger than `mine`.
 __device__ inline int rank_of(uint64_t mine, const uint64_t* keys, int n) {
-  int r = 0;
-  for (int i = 0; i < n; ++i) r += keys[i] > mine;
+  int r = 0, i = 0;
+  for (; i + 8 <= n; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r += keys[i + j] > mine;
+  }
+  for (; i < n; ++i) r += keys[i] > mine;
   return r;
 }
 
 struct Shared {
-  uint64_t keys[kScoreMostTop * (kScoreChunk / kThreads)];  // candidates
-  uint64_t first[kThreads];   // threads' first largest entries, and whose they are
+  union {
+    uint64_t keys[kMostKeys];  // candidates
+    uint64_t first[kThreads];  // before them: threads' first largest entries
+  };
   uint64_t best[kScoreMostTop];
   float run_max[64];
-  float piece[2][kMostPieces];  // sums of the pieces of the largest entry's thread
   float sums[2][kWaves];
+  float piece[2][kMostPieces];  // sums of the pieces of the thread that holds the largest entry
   float bound;
-  int first_of[kThreads], chosen[kScoreMostTop];
-  int n_first, n_keys, last;
+  int first_of[kThreads];  // whose they are
+  int chosen[kThreads];    // threads whose entries are read again (-1 - thread: holds the largest)
+  int equals[kMostPieces];  // entries of those pieces that equal it
+  int tops[kWaves];
+  int n_first, n_chosen, n_keys, last;
 };
 
-// One chunk: its largest entry m and the sums without it, both in the exp2 domain of `scale`
-// (s = sum 2^(scale (x - m)), t = sum scale (x - m) 2^(..)), and its k best entries in sh.best, keys of
-// entries that are not there 0. Every thread gets m, s and t.
-template <typename T, bool kMask>
+// One chunk: its largest entry m, the sums of the others (s = sum 2^z, t = sum z 2^z with z = scale (x
+// - m)) and its k best entries in sh.best, keys of entries that are not there 0. Every thread gets
+// m, s and t.
+//
+// Sums are kept against a reference r of the thread's, its maximum times scale as f32 rounds it, so that
+// a term's exponent is one fma (rounded once, whatever r is); what r is off by is taken back at the
+// end. Entries so large that this overflows take `plain`: a second pass over differences.
+template <typename T, bool kMask, bool kSmall>
 __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float scale, Shared& sh,
                             float& m_out, float& s_out, float& t_out) {
-  constexpr int kN = Piece<T>::kN, kTurns = kGroup / kN;
+  constexpr int kN = Piece<T>::kN, kTurns = (kSmall ? kSmallGroup : kGroup) / kN;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int pieces = (row.n + kN - 1) / kN;
-  float m = -INFINITY, s = 0.f, t = 0.f;
+  float m = -INFINITY, s = 0.f, t = 0.f, ref = kLow;
   int at = 0;  // the group that held m first
-  auto take = [&](const float (&v)[kTurns][kN], int g) __attribute__((always_inline)) {
+  float v[kTurns][kN];
+  // kClean: -infinity is unlikely among the group's entries.
+  auto take = [&](int g, float top, auto kClean) __attribute__((always_inline)) {
+    if (top > m) at = g;
+    m = fmaxf(m, top);
+    const float r = fmaxf(m * scale, kLow), d = ref - r, w0 = __builtin_amdgcn_exp2f(d);
+    ref = r;
+    t = w0 * __builtin_fmaf(d, s, t);
+    s *= w0;
+    const float t0 = t;
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float z = __builtin_fmaf(v[u][e], scale, -r), w = __builtin_amdgcn_exp2f(z);
+        s += w;
+        t = __builtin_fmaf(kClean.value ? z : fmaxf(z, kLow), w, t);
+      }
+    if (kClean.value && __any(t != t)) {
+      // An entry of -infinity, whose weight of 0 times its exponent is no number: again without.
+      t = t0;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+        for (int e = 0; e < kN; ++e) {
+          const float z = __builtin_fmaf(v[u][e], scale, -r);
+          t = __builtin_fmaf(fmaxf(z, kLow), __builtin_amdgcn_exp2f(z), t);
+        }
+    }
+  };
+  const int groups = kSmall ? 1 : (pieces + kTurns * kThreads - 1) / (kTurns * kThreads);
+  const int whole = row.n / (kN * kTurns * kThreads);  // groups with every entry in the row
+  int index[kTurns] = {};  // of v[u][0], in a small chunk
+  if constexpr (!kSmall) {
+    if (whole > 0) {
+      typename Row<T, kMask>::Raw raw[kTurns];
+      auto fetch = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u)
+          row.fetch(((g * kTurns + u) * kThreads + tid) * kN, raw[u]);
+      };
+      fetch(0);
+      for (int g = 0; g < whole; ++g) {
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) row.values(raw[u], v[u]);
+        float top = v[0][0];
+        if constexpr (__is_same(T, _Float16) && !kMask) {
+          top = max_of_halves(raw);
+        } else {
+#pragma unroll
+          for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+            for (int e = 0; e < kN; ++e) top = fmaxf(top, v[u][e]);
+        }
+        if (g + 1 < whole) fetch(g + 1);
+        take(g, top, std::integral_constant<bool, !kMask>{});
+      }
+    }
+  }
+  if (kSmall || whole < groups) {
+    const int g = kSmall ? 0 : whole;
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) index[u] = row.load((g * kTurns + u) * kThreads + tid, v[u]);
     float top = v[0][0];
 #pragma unroll
     for (int u = 0; u < kTurns; ++u)
 #pragma unroll
       for (int e = 0; e < kN; ++e) top = fmaxf(top, v[u][e]);
-    if (top > m) at = g;
-    const float m_new = fmaxf(fmaxf(m, top), -FLT_MAX);
-    const float d = fmaxf((fmaxf(m, -FLT_MAX) - m_new) * scale, kLow);
-    const float r = __builtin_amdgcn_exp2f(d);
-    t = r * __builtin_fmaf(d, s, t);
-    s *= r;
-    m = fmaxf(m, top);
-#pragma unroll
-    for (int u = 0; u < kTurns; ++u)
-#pragma unroll
-      for (int e = 0; e < kN; ++e) {
-        const float z = (v[u][e] - m_new) * scale, w = __builtin_amdgcn_exp2f(z);
-        s += w;
-        t = __builtin_fmaf(fmaxf(z, kLow), w, t);
-      }
-  };
-  const int groups = (pieces + kTurns * kThreads - 1) / (kTurns * kThreads);
-  const int whole = row.n / (kN * kTurns * kThreads);  // groups with every entry in the row
-  for (int g = 0; g < groups; ++g) {
-    float v[kTurns][kN];
-#pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      const int p = (g * kTurns + u) * kThreads + tid;
-      if (g < whole)
-        row.template load<true>(p, v[u]);
-      else
-        row.template load<false>(p, v[u]);
-    }
-    take(v, g);
+    take(g, top, std::false_type{});
   }
 
-  // A bound under the k-th largest thread's maximum: that of 64 runs of threads.
-  float run = m;
-#pragma unroll
-  for (int d = 1; d < kRun; d <<= 1) run = fmaxf(run, __shfl_xor(run, d));
+  // A bound at or below the k-th largest thread's maximum: that of 64 runs of threads.
+  const float run = max8(m);
   if (tid % kRun == 0) sh.run_max[tid / kRun] = run;
-  if (tid == 0) sh.n_first = sh.n_keys = 0;
+  if (tid == 0) sh.n_first = sh.n_chosen = sh.n_keys = 0;
   __syncthreads();
   const float mine = sh.run_max[lane];
   const float m_all = wave_max(mine);
@@ -202,71 +292,125 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
     }
     if (r == k - 1) sh.bound = mine;
   }
-  __syncthreads();
-  if (m > -INFINITY && m >= sh.bound) {
-    int index = 0;
-    bool found = false;
+  const bool odd = !(m_all * scale > kLow && m_all * scale < -kLow);  // of all threads
+  if (odd && m_all > -INFINITY) {
+    // plain: the sums against the largest entry, from differences.
+    s = t = ref = 0.f;
+    for (int g = 0; g < groups; ++g)
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-      const int p = (at * kTurns + u) * kThreads + tid;
-      float v[kN];
-      row.template load<false>(p, v);
+      for (int u = 0; u < kTurns; ++u) {
+        float x[kN];
+        row.load((g * kTurns + u) * kThreads + tid, x);
 #pragma unroll
-      for (int e = 0; e < kN; ++e)
-        if (!found && v[e] == m) {
-          found = true;
-          index = p * kN + e;
+        for (int e = 0; e < kN; ++e) {
+          const float z = (x[e] - m_all) * scale, w = __builtin_amdgcn_exp2f(z);
+          s += w;
+          t = __builtin_fmaf(fmaxf(z, kLow), w, t);
         }
-    }
-    const int i = atomicAdd(&sh.n_first, 1);
-    sh.first[i] = key_of(m, index0 + index);
-    sh.first_of[i] = tid;
+      }
   }
   __syncthreads();
-  const int n_first = sh.n_first, n_chosen = min(n_first, k);
-  if (tid < n_first) {
-    const int r = rank_of(sh.first[tid], sh.first, n_first);
-    if (r < k) {
-      sh.chosen[r] = sh.first_of[tid];
-      sh.best[r] = sh.first[tid];
-    }
+  const float bound = sh.bound;
+  const bool in = m > -INFINITY && m >= bound, is_top = in && m == m_all;
+  {
+    const uint64_t tops = __ballot(is_top);
+    if (lane == 0) sh.tops[wave] = __popcll(tops);
   }
+  if (!kSmall && in) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = is_top ? -1 - tid : tid;
   __syncthreads();
-  // Entries of the chosen threads, a piece a thread.
-  const int per = groups * kTurns;
-  if (n_chosen > 0) {
-    const uint64_t least = n_chosen == k ? sh.best[k - 1] : 0;
-    const int top_at = index_of(sh.best[0]) - index0;
+  int n_top = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) n_top += sh.tops[w];
+  float ps = 0.f, pt = 0.f;  // a small chunk: of the thread that alone holds the largest entry
+  // A piece's terms without the entries that equal the largest, which are counted.
+  auto others = [&](const float (&x)[kN], float& a, float& b, int& n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const float z = (x[e] - m_all) * scale, w = __builtin_amdgcn_exp2f(z);
+      n += x[e] == m_all;
+      a += x[e] == m_all ? 0.f : w;
+      b = __builtin_fmaf(fmaxf(z, kLow), w, b);
+    }
+  };
+  const int per = groups * kTurns;  // pieces of a thread
+  // Entries at or above the bound, whatever their index..
+  uint64_t least = key_of(bound == -INFINITY ? -FLT_MAX : bound, 0xFFFFFFFFu);
+  if constexpr (kSmall) {
+    if (in) {
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+        for (int e = 0; e < kN; ++e)
+          if (v[u][e] > -INFINITY && v[u][e] >= bound)
+            sh.keys[atomicAdd(&sh.n_keys, 1)] = key_of(v[u][e], index0 + index[u] + e);
+      if (is_top && n_top == 1) {
+        int equal = 0;
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) others(v[u], ps, pt, equal);
+        ps += static_cast<float>(equal - 1);
+      }
+    }
+  } else {
+    int n_chosen = sh.n_chosen;
+    if (n_chosen * per * kN > kMostKeys) {
+      // .. or, where that could be too many, those of the k threads whose first largest entries are the
+      // k best.
+      if (in) {
+        int first = 0;
+#pragma unroll
+        for (int u = kTurns - 1; u >= 0; --u) {
+          float x[kN];
+          const int i0 = row.load((at * kTurns + u) * kThreads + tid, x);
+#pragma unroll
+          for (int e = kN - 1; e >= 0; --e)
+            if (x[e] == m) first = i0 + e;
+        }
+        const int i = atomicAdd(&sh.n_first, 1);
+        sh.first[i] = key_of(m, index0 + first);
+        sh.first_of[i] = is_top ? -1 - tid : tid;
+      }
+      __syncthreads();
+      if (tid < n_chosen) {
+        const int r = rank_of(sh.first[tid], sh.first, n_chosen);
+        if (r < k) {
+          sh.chosen[r] = sh.first_of[tid];
+          sh.best[r] = sh.first[tid];
+        }
+      }
+      __syncthreads();
+      least = n_chosen > k ? sh.best[k - 1] : 0;
+      n_chosen = min(n_chosen, k);
+    }
+    // The chosen threads' entries again, a piece a thread.
     for (int i = tid; i < n_chosen * per; i += kThreads) {
       const int j = i / per, q = i - j * per;
-      const int p = q * kThreads + sh.chosen[j];
-      float v[kN];
-      row.template load<false>(p, v);
-      float ps = 0.f, pt = 0.f;
+      const int who = sh.chosen[j];
+      float x[kN];
+      const int i0 = row.load(q * kThreads + (who < 0 ? -1 - who : who), x);
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        const uint64_t key = key_of(v[e], index0 + p * kN + e);
-        if (v[e] > -INFINITY && key >= least) sh.keys[atomicAdd(&sh.n_keys, 1)] = key;
-        if (j == 0 && p * kN + e != top_at) {
-          const float z = (v[e] - m_all) * scale, w = __builtin_amdgcn_exp2f(z);
-          ps += w;
-          pt = __builtin_fmaf(fmaxf(z, kLow), w, pt);
-        }
+        const uint64_t key = key_of(x[e], index0 + i0 + e);
+        if (x[e] > -INFINITY && key >= least) sh.keys[atomicAdd(&sh.n_keys, 1)] = key;
       }
-      if (j == 0) {
-        sh.piece[0][q] = ps;
-        sh.piece[1][q] = pt;
+      if (who < 0 && n_top == 1) {
+        float a = 0.f, b = 0.f;
+        int equal = 0;
+        others(x, a, b, equal);
+        sh.piece[0][q] = a;
+        sh.piece[1][q] = b;
+        sh.equals[q] = equal;
       }
     }
   }
-  // The threads' sums, without the largest entry's thread.
+  // The threads' sums, against m_all: without the one that alone holds it, whose pieces follow.
   {
-    const float low = fmaxf(m_all, -FLT_MAX);
-    const float d = fmaxf((fmaxf(m, -FLT_MAX) - low) * scale, kLow);
-    const float r = __builtin_amdgcn_exp2f(d);
-    const bool out = n_chosen > 0 && tid == sh.chosen[0];
-    const float ws = wave_sum(out ? 0.f : r * s);
-    const float wt = wave_sum(out ? 0.f : r * __builtin_fmaf(d, s, t));
+    const float r_all = odd ? 0.f : m_all * scale;
+    // scale m_all - r_all, which the sums lie too high by
+    const float off = odd ? 0.f : __builtin_fmaf(m_all, scale, -r_all);
+    const float d = fmaxf(ref - r_all - off, kLow), w0 = __builtin_amdgcn_exp2f(d);
+    const bool apart = is_top && n_top == 1;
+    const float ws = wave_sum(apart ? ps : w0 * s);
+    const float wt = wave_sum(apart ? pt : w0 * __builtin_fmaf(d, s, t));
     if (lane == 0) {
       sh.sums[0][wave] = ws;
       sh.sums[1][wave] = wt;
@@ -274,26 +418,27 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   }
   __syncthreads();
   const int n_keys = sh.n_keys;
-  if (tid < k) sh.best[tid] = 0;
+  if (tid < k && tid >= n_keys) sh.best[tid] = 0;
+  for (int i = tid; i < n_keys; i += kThreads) {
+    const uint64_t key = sh.keys[i];
+    const int r = rank_of(key, sh.keys, n_keys);
+    if (r < k) sh.best[r] = key;
+  }
   s = t = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
     s += sh.sums[0][w];
     t += sh.sums[1][w];
   }
-  if (n_chosen > 0) {
-    float ps = 0.f, pt = 0.f;
-    for (int q = lane; q < per; q += 64) {
-      ps += sh.piece[0][q];
-      pt += sh.piece[1][q];
-    }
-    s += wave_sum(ps);
-    t += wave_sum(pt);
-  }
-  __syncthreads();
-  for (int i = tid; i < n_keys; i += kThreads) {
-    const int r = rank_of(sh.keys[i], sh.keys, n_keys);
-    if (r < k) sh.best[r] = sh.keys[i];
+  if (kSmall && n_top == 1) {
+    // It is left out already.
+  } else if (n_top == 1) {
+    const bool mine_too = lane < per;
+    s += wave_sum(mine_too ? sh.piece[0][lane] : 0.f) +
+         (wave_sum(mine_too ? static_cast<float>(sh.equals[lane]) : 0.f) - 1.f);
+    t += wave_sum(mine_too ? sh.piece[1][lane] : 0.f);
+  } else if (n_top > 1) {
+    s -= 1.f;
   }
   __syncthreads();
   m_out = m_all;
@@ -301,8 +446,8 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   t_out = t;
 }
 
-template <typename T, bool kMask>
-__global__ __launch_bounds__(kThreads) void score_rows(ScoreArgs a) {
+template <typename T, bool kMask, bool kSmall>
+__global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const int64_t r = blockIdx.y + static_cast<int64_t>(blockIdx.z) * 65535;
@@ -314,7 +459,7 @@ __global__ __launch_bounds__(kThreads) void score_rows(ScoreArgs a) {
   const Row<T, kMask> row = {x + i0, kMask ? ok + i0 : nullptr, min(a.chunk, a.n_vocab - i0)};
   const int k = max(a.top_k, 1);
   float m, s, t;  // of the allowed entries; s and t without the largest entry
-  scan<T, kMask>(row, i0, k, a.scale_log2, sh, m, s, t);
+  scan<T, kMask, kSmall>(row, i0, k, a.scale_log2, sh, m, s, t);
   if (a.n_chunks > 1) {
     float* const part = a.part + (r * a.n_chunks + blockIdx.x) * kScorePart;
     if (tid == 0) {
@@ -336,9 +481,18 @@ __global__ __launch_bounds__(kThreads) void score_rows(ScoreArgs a) {
     if (!sh.last) return;
     const float* const all = a.part + r * a.n_chunks * kScorePart;
     const int n = a.n_chunks * k;
+    // The chunks' sums, a chunk a lane, and their best entries.
+    const int c = tid & 63;
+    float mc = -INFINITY, sc = 0.f, tc = 0.f;
+    if (c < a.n_chunks) {
+      const float* const p = all + c * kScorePart;
+      mc = ld_agent(p);
+      sc = ld_agent(p + 1);
+      tc = ld_agent(p + 2);
+    }
     for (int i = tid; i < n; i += kThreads) {
-      const int c = i / k, j = i - c * k;
-      sh.keys[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(all + c * kScorePart + 4) + j,
+      const int from = i / k, j = i - from * k;
+      sh.keys[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(all + from * kScorePart + 4) + j,
                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if (tid < k) sh.best[tid] = 0;
@@ -350,22 +504,14 @@ __global__ __launch_bounds__(kThreads) void score_rows(ScoreArgs a) {
       if (p < k) sh.best[p] = key;
     }
     __syncthreads();
-    // The chunks' sums in their order; the one that holds the largest entry leaves its 1 out.
+    // The chunk that holds the largest entry leaves its 1 out.
     const int home = sh.best[0] ? index_of(sh.best[0]) / a.chunk : -1;
-    m = -INFINITY;
-    for (int c = 0; c < a.n_chunks; ++c) m = fmaxf(m, ld_agent(all + c * kScorePart));
-    s = t = 0.f;
-    for (int c = 0; c < a.n_chunks; ++c) {
-      const float* const p = all + c * kScorePart;
-      const float mc = ld_agent(p), tc = ld_agent(p + 2);
-      float sc = ld_agent(p + 1);
-      if (c != home && mc > -INFINITY) sc += 1.f;
-      const float d =
-          fmaxf((fmaxf(mc, -FLT_MAX) - fmaxf(m, -FLT_MAX)) * a.scale_log2, kLow);
-      const float w = __builtin_amdgcn_exp2f(d);
-      s = __builtin_fmaf(w, sc, s);
-      t = __builtin_fmaf(w, __builtin_fmaf(d, sc, tc), t);
-    }
+    if (c != home && mc > -INFINITY) sc += 1.f;
+    m = wave_max(mc);
+    const float d = fmaxf((fmaxf(mc, -FLT_MAX) - fmaxf(m, -FLT_MAX)) * a.scale_log2, kLow);
+    const float w = __builtin_amdgcn_exp2f(d);
+    s = wave_sum(w * sc);
+    t = wave_sum(w * __builtin_fmaf(d, sc, tc));
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   // A row with an allowed NaN or +infinity has no distribution; one without an entry gives none
@@ -384,14 +530,8 @@ __global__ __launch_bounds__(kThreads) void score_rows(ScoreArgs a) {
     if (a.top_logprobs) a.top_logprobs[o] = key ? logprob(value_of(key)) : odd ? NAN : -INFINITY;
   }
   if (tid == 0 && a.logprobs) {
-    float v = -INFINITY;
-    if (token >= 0 && token < a.n_vocab && (!kMask || ok[token])) {
-      if constexpr (__is_same(T, uint16_t))
-        v = __builtin_bit_cast(float, static_cast<uint32_t>(x[token]) << 16);
-      else
-        v = static_cast<float>(x[token]);
-    }
-    a.logprobs[r] = logprob(v);
+    const bool is_entry = token >= 0 && token < a.n_vocab && (!kMask || ok[token]);
+    a.logprobs[r] = logprob(is_entry ? value(x[token]) : -INFINITY);
   }
   if (tid == 64 && a.entropy)
     a.entropy[r] = odd ? NAN : none ? 0.f : ln_s - t * 0.6931471805599453f / (1.f + s);
@@ -403,8 +543,7 @@ void score_plan(ScoreArgs& a, bool split) {
   // Rows that fill the GPU are taken whole.
   int64_t chunks = 1;
   if (split) chunks = std::max<int64_t>(1, kScoreMaxWgs / std::max<int64_t>(a.n_rows, 1));
-  // Not less than 4 groups of every thread's.. entries a workgroup.
-  chunks = std::min<int64_t>(chunks, (a.n_vocab + 4095) / 4096);
+  chunks = std::min<int64_t>(chunks, (a.n_vocab + kScoreSmall - 1) / kScoreSmall);
   chunks = std::min<int64_t>(chunks, kScoreMostChunks);
   chunks = std::max<int64_t>(chunks, (a.n_vocab + kScoreChunk - 1) / kScoreChunk);
   a.chunk = static_cast<int>(((a.n_vocab + chunks - 1) / chunks + 63) / 64 * 64);
@@ -419,11 +558,14 @@ hipError_t launch_score_rows(const ScoreArgs& a, DType dt, hipStream_t s) {
   if (z > 65535) return hipErrorInvalidConfiguration;
   const dim3 grid(a.n_chunks, static_cast<unsigned>(std::min<int64_t>(a.n_rows, 65535)),
                   static_cast<unsigned>(z));
-#define WRS_SCORE(T)                                                                       \
-  if (a.allowed)                                                                           \
-    hipLaunchKernelGGL((score_rows<T, true>), grid, dim3(kThreads), 0, s, a);              \
-  else                                                                                     \
-    hipLaunchKernelGGL((score_rows<T, false>), grid, dim3(kThreads), 0, s, a)
+  const bool small = a.chunk <= kScoreSmall;
+#define WRS_SCORE_ONE(T, M, S) hipLaunchKernelGGL((score_rows<T, M, S>), grid, dim3(kThreads), 0, s, a)
+#define WRS_SCORE(T)                                                      \
+  if (a.allowed) {                                                        \
+    if (small) { WRS_SCORE_ONE(T, true, true); } else { WRS_SCORE_ONE(T, true, false); }   \
+  } else {                                                                \
+    if (small) { WRS_SCORE_ONE(T, false, true); } else { WRS_SCORE_ONE(T, false, false); } \
+  }
   switch (dt) {
     case kF32: WRS_SCORE(float); break;
     case kF16: WRS_SCORE(_Float16); break;
@@ -431,6 +573,7 @@ hipError_t launch_score_rows(const ScoreArgs& a, DType dt, hipStream_t s) {
     default: return hipErrorInvalidValue;
   }
 #undef WRS_SCORE
+#undef WRS_SCORE_ONE
   return hipGetLastError();
 }
 

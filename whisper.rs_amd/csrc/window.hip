@@ -4,20 +4,26 @@
 // K19 (window_attend): row r of a sequence stands at position p = past + r (`causal`; else every
 //   row at the last key) and sees the keys j <= p with j > p - window or j < sinks:
 //   s_j = q.k_j / 8, out = softmax(s) V over those j only.
-//   A workgroup of four waves runs one block of 16 kRT rows of one head. The block's keys are the
+//   A workgroup of four waves runs one block of 16 rows of one head. The block's keys are the
 //   first tokens' 32-key steps, then those from its first row's window to its last row's own key:
 //   steps in between are never read. Wave w takes steps w, w + 4, ... with an online softmax of its
 //   own, the waves merge their (max, sum, O) in LDS, and where a block's steps are dealt over several
 //   workgroups those merge through memory (the last to count in adds the partials up in order, so
 //   results do not depend on which it is). Only steps that hold a key hidden from some row test keys.
-//   f16 planes run on the f16 matrix pipe with operands in two parts, f32 ones on the f32 pipe.
-//   8-bit planes: codes are whole numbers that f16 and bf16 hold as they are. Scores take them as
-//   f16 against q in two f16 parts, then the keys' powers of two, whatever they are, in f32. Weights
-//   take the values' powers before they are split, into two bf16 parts: bf16 has f32's range, so rows
-//   of any scale meet in one sum, and two parts hold 2^-18 of a weight.
+//   f16 planes run on the f16 matrix pipe with f32 operands in two parts (Rows16), f32 planes on
+//   the f32 pipe. 8-bit codes are whole numbers that f16 holds as they are: they enter the same way,
+//   and the keys' powers of two go to the scores in f32, the values' to the weights before they are split.
+//   One row of q a step costs what 16 do, so few rows are bound by latency: a step of a wave takes 0.7 us
+//   from the load to the weights' product when it is alone on its SIMD (f32: 1.9), and window_plan
+//   deals a block's steps over workgroups by that. Bytes are the other bound: 16 sequences of 20 heads
+//   that see 8192 keys each (f16: 672 MB) take 121 us, 5.5 TB/s, and the 8-bit ones half the bytes in
+//   80 us, 4.3 TB/s: with as many steps in flight, each loads half. Deeper prefetch (2 to 4 steps),
+//   steps of 64 keys and 32 rows a wave were measured and are no faster (79 to 88 us; registers then
+//   allow 2 or 3 waves a SIMD instead of 4).
 #include "split16.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace wrs {
 namespace {
@@ -28,41 +34,45 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = 4;
 constexpr int kN = 32;              // keys per step
 constexpr int kPitch = 68;          // LDS pitch (floats) of a merge row
-constexpr int kCounterStride = 32;  // 128 bytes between merge counters
+constexpr int kCounterStride = 16;  // 64 bytes between merge counters
 constexpr int kMergeLoads = 8;      // partials in flight per thread in the merge
 constexpr int kRawBuffer = 0x00020000;  // buffer resource word 3: raw, 32-bit data format
 
-// The steps of rows at positions p0..p1: `sink_steps` of them from key 0 on, the others from key
-// `lo` on (a multiple of kN), up to key p1. Where the two meet, all lie from key 0 on.
+// The steps of kSize keys of rows at positions p0..p1: `sink_steps` of them from key 0 on, the others
+// from key `lo` on (a multiple of kSize), up to key p1. Where the two meet, all lie from key 0 on.
+template <int kSize>
 struct Span {
   int lo, sink_steps, n_steps;
-};
-__host__ __device__ inline Span span_of(int p0, int p1, int window, int sinks) {
-  Span s;
-  const int first = p0 - window + 1;  // window <= 2^24
-  s.lo = first > 0 ? first / kN * kN : 0;
-  s.sink_steps = (sinks < p1 + 1 ? sinks + kN - 1 : p1 + kN) / kN;
-  if (s.sink_steps * kN >= s.lo) s.lo = s.sink_steps = 0;
-  s.n_steps = s.sink_steps + (p1 - s.lo + kN) / kN;
-  return s;
-}
-
-// What a wave knows of its block.
-struct Block {
-  int p0, p1;            // positions of the block's first and last row
-  int window, sinks;
-  Span span;
-  int step0, step1;      // the workgroup's steps
-  __amdgpu_buffer_rsrc_t k, v, ks, vs;  // the head's planes, zero past key p1
-
+  __host__ __device__ inline Span(int p0, int p1, int window, int sinks) {
+    const int first = p0 - window + 1;  // window <= 2^24
+    lo = first > 0 ? first / kSize * kSize : 0;
+    sink_steps = (sinks < p1 + 1 ? sinks + kSize - 1 : p1 + kSize) / kSize;
+    if (sink_steps * kSize >= lo) lo = sink_steps = 0;
+    n_steps = sink_steps + (p1 - lo + kSize) / kSize;
+  }
   __device__ inline int key_of(int step) const {
-    return kN * step + (step < span.sink_steps ? 0 : span.lo - kN * span.sink_steps);
+    return kSize * step + (step < sink_steps ? 0 : lo - kSize * sink_steps);
+  }
+};
+
+// What a wave knows of its rows.
+struct Block {
+  int p0, p1;  // positions of the first and last row
+  int window, sinks;
+  Span<kN> span;
+  int step0, step1;  // the workgroup's steps
+  __amdgpu_buffer_rsrc_t k, v, ks, vs;  // the head's planes, zero past the last key
+
+  __device__ inline Block(int first, int last, int w, int n)
+      : p0(first), p1(last), window(w), sinks(n), span(first, last, w, n) {}
+  __device__ inline int key_of(int step) const { return span.key_of(step); }
+  // Whether some row sees one of `n` keys from j0 on.
+  __device__ inline bool any(int j0, int n) const {
+    return j0 <= p1 && (j0 + n - 1 > p0 - window || j0 < sinks);
   }
   // Whether some row of the block does not see some of `n` keys from j0 on.
   __device__ inline bool masked(int j0, int n) const {
@@ -73,19 +83,15 @@ struct Block {
   }
 };
 
-// A wave's running sums: of lane (c, g), rows 16 rt + c.
-template <int kRT>
+// A wave's running sums: of lane (c, g), row c.
 struct Sums {
-  f32x4 o[kRT][4];
-  float m[kRT], l[kRT];
+  f32x4 o[4];
+  float m, l;
   __device__ inline void clear() {
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      m[rt] = -INFINITY;
-      l[rt] = 0.f;
-    }
+    for (int dt = 0; dt < 4; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
   }
 };
 
@@ -101,11 +107,12 @@ __device__ inline f32x4 load4(const __amdgpu_buffer_rsrc_t& rs, uint32_t o) {
 
 // A wave's steps on the f32 matrix pipe, 16 keys at a time, f16 planes widened exactly: lane
 // (c, g) holds key c's values d = 16 g + 0..15, so that lane (r, g) gets scores of keys 4 g + 0..3 of
-// row r, which are the B operand of O^T += V^T P^T as they stand. o[rt][dt][e] is column 16 g + 4 e +
+// row r, which are the B operand of O^T += V^T P^T as they stand. o[dt][e] is column 16 g + 4 e +
 // dt. q: d = 16 g + 0..15 of row c, times scale * log2(e). pos: row c's position.
-template <DType kD, int kRT>
-__device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4],
-                                  const int (&pos)[kRT], int wave, int lane, Sums<kRT>& st) {
+// Steps b.step0 + wave, + waves, .. of the block's, 16 keys at a time, the next 16 on their way.
+template <DType kD>
+__device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[4], int pos,
+                                  int wave, int waves, int lane, Sums& st) {
   constexpr uint32_t kSize = kD == kF32 ? 4 : 2, kRowBytes = 64 * kSize;
   const int c = lane & 15, g = lane >> 4;
   f32x4 kn[4], vn[4];
@@ -117,22 +124,24 @@ __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4],
 #pragma unroll
     for (int i = 0; i < 4; ++i) vn[i] = load4<kD>(b.v, vo + i * kRowBytes);
   };
-  // Piece u: half u % 2 of step u / 2.
-  auto key_of = [&](int u) { return b.key_of(u >> 1) + 16 * (u & 1); };
-  int u = 2 * (b.step0 + wave);
-  const int end = 2 * b.step1;
-  if (u < end) load(key_of(u));
+  // The wave's piece n: 16 keys of its step n / kPer.
+  constexpr int kPer = kN / 16;
+  const int steps = b.step1 - b.step0 - wave;
+  const int end = steps > 0 ? kPer * ((steps + waves - 1) / waves) : 0;
+  auto key_of = [&](int n) {
+    return b.key_of(b.step0 + wave + waves * (n / kPer)) + 16 * (n % kPer);
+  };
+  if (end > 0) load(key_of(0));
   st.clear();
-  for (int next; u < end; u = next) {
-    next = u & 1 ? u + 1 + 2 * (kWaves - 1) : u + 1;
-    const int j0 = key_of(u);
+  for (int n = 0; n < end; ++n) {
+    const int j0 = key_of(n);
     f32x4 kx[4], vx[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       kx[i] = kn[i];
       vx[i] = vn[i];
     }
-    if (next < end) load(key_of(next));
+    if (n + 1 < end) load(key_of(n + 1));
     // Values that a row does not see have weight 0, and 0 times an infinity or NaN is NaN: such
     // values leave the product and are added row by row.
     const bool masked = b.masked(j0, 16);
@@ -144,63 +153,60 @@ __device__ inline void attend_f32(const Block& b, const f32x4 (&qx)[kRT][4],
         for (int e = 0; e < 4; ++e) odd |= !__builtin_isfinite(vx[i][e]);
       odd = __any(odd);
     }
+    f32x4 s0 = {}, s1 = {};
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      f32x4 s0 = {}, s1 = {};
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e], qx[i][e], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e + 1], qx[i][e + 1], s1, 0, 0, 0);
+      }
+    f32x4 s = s0 + s1;
+    int seen = 0xF;  // bit i: the row sees key j0 + 4 g + i
+    if (masked) {
+      seen = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e], qx[rt][i][e], s0, 0, 0, 0);
-          s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[i][e + 1], qx[rt][i][e + 1], s1, 0, 0, 0);
-        }
-      f32x4 s = s0 + s1;
-      int seen = 0xF;  // bit i: the row sees key j0 + 4 g + i
-      if (masked) {
-        seen = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (b.sees(pos[rt], j0 + 4 * g + i))
-            seen |= 1 << i;
-          else
-            s[i] = -INFINITY;
-      }
-      const float mx = max_x16_x32(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-      const float m_new = fmaxf(st.m[rt], mx);
-      const float alpha = st.m[rt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m[rt] - m_new);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      st.m[rt] = m_new;
-      f32x4 p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
-      st.l[rt] = __builtin_fmaf(st.l[rt], alpha, (p[0] + p[1]) + (p[2] + p[3]));
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) st.o[rt][dt] *= alpha;
-      if (odd) {
-#pragma unroll 1
-        for (int key = 0; key < 16; ++key) {
-          // Weight and sight of key j0 + key, and its row's values of this lane's columns.
-          const int i = key & 3;
-          const float mine = i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3];
-          const float pk = __shfl(mine, c + 16 * (key >> 2));
-          const bool vis = (__shfl(seen, c + 16 * (key >> 2)) >> i) & 1;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f32x4 vk = load4<kD>(b.v, static_cast<uint32_t>(j0 + key) * kRowBytes +
-                                                (16 * g + 4 * e) * kSize);
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt)
-              if (vis && !__builtin_isfinite(vk[dt])) st.o[rt][dt][e] += pk * vk[dt];
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-          st.o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-              odd && !__builtin_isfinite(vx[i][dt]) ? 0.f : vx[i][dt], p[i], st.o[rt][dt], 0, 0, 0);
+        if (b.sees(pos, j0 + 4 * g + i))
+          seen |= 1 << i;
+        else
+          s[i] = -INFINITY;
     }
+    const float mx = max_x16_x32(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    const float m_new = fmaxf(st.m, mx);
+    const float alpha = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.m - m_new);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    st.m = m_new;
+    f32x4 p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+    st.l = __builtin_fmaf(st.l, alpha, (p[0] + p[1]) + (p[2] + p[3]));
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) st.o[dt] *= alpha;
+    if (odd) {
+#pragma unroll 1
+      for (int key = 0; key < 16; ++key) {
+        // Weight and sight of key j0 + key, and its row's values of this lane's columns.
+        const int i = key & 3;
+        const float mine = i == 0 ? p[0] : i == 1 ? p[1] : i == 2 ? p[2] : p[3];
+        const float pk = __shfl(mine, c + 16 * (key >> 2));
+        const bool vis = (__shfl(seen, c + 16 * (key >> 2)) >> i) & 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4 vk = load4<kD>(b.v, static_cast<uint32_t>(j0 + key) * kRowBytes +
+                                              (16 * g + 4 * e) * kSize);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+            if (vis && !__builtin_isfinite(vk[dt])) st.o[dt][e] += pk * vk[dt];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+        st.o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+            odd && !__builtin_isfinite(vx[i][dt]) ? 0.f : vx[i][dt], p[i], st.o[dt], 0, 0, 0);
   }
 }
 
@@ -212,69 +218,244 @@ __device__ inline void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
   lo = __builtin_bit_cast(uint32_t, a + off);
   hi = __builtin_bit_cast(uint32_t, b + off);
 }
-// The same as bf16, which holds whole numbers to 256: the upper half of each f32.
-__device__ inline void codes_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  uint32_t x[4];
+__device__ inline void codes_f16(const u32x4& w, u32x4 (&out)[2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    x[i] = __builtin_bit_cast(uint32_t, static_cast<float>((w >> (8 * i)) & 0xFFu) - 128.f);
-  lo = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
-  hi = __builtin_amdgcn_perm(x[3], x[2], 0x07060302u);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t lo, hi;
+    codes_f16(w[i], lo, hi);
+    out[i >> 1][2 * (i & 1)] = lo;
+    out[i >> 1][2 * (i & 1) + 1] = hi;
+  }
 }
 // 2^(byte - 127) of byte i of four scales (255: infinity, and its codes are zeros: NaN).
 __device__ inline float scale_at(uint32_t w, int i) {
-  const uint32_t up = i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1;
-  return __builtin_bit_cast(float, up & 0x7F800000u);
-}
-// Two weights in two bf16 parts: both to nearest, the second of what the first leaves.
-__device__ inline void split_bf16(float x0, float x1, uint32_t (&out)[kParts]) {
-  const f32x2 x = {x0, x1};
-  const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
-  const f32x2 r = {x0 - __builtin_bit_cast(float, h << 16),
-                   x1 - __builtin_bit_cast(float, h & 0xFFFF0000u)};
-  out[0] = h;
-  out[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
-}
-__device__ inline f32x4 mfma_bf16(const u32x4& a, const u32x4& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_bit_cast(float, ((w >> (8 * i)) & 0xFFu) << 23);
 }
 
-// Query rows (d = 16 g + 0..15 of row c of each tile) times a power of two that puts a row's
-// largest element into [2^14, 2^15), in two f16 parts; down: its inverse.
-template <int kRT>
-__device__ inline void split_rows(const f32x4 (&qx)[kRT][4], u32x4 (&qf)[kRT][kParts][2],
-                                  float (&down)[kRT]) {
-#pragma unroll
-  for (int rt = 0; rt < kRT; ++rt) {
+// The values' operand of columns 16 dt.. from 32 rows of V in LDS: lane (c, g) gets column 16 dt + c of
+// keys 4 g + 0..3 and 16 + 4 g + 0..3, the order that the packed weights have. Rows r and r + 16 swizzle
+// alike.
+__device__ inline int value_offset(int dt, int c, int g) {
+  const int row = 4 * g + (c >> 2);
+  return row * 128 + (((2 * dt + ((c & 3) >> 1)) ^ swz(row)) * 16) + 8 * (c & 1);
+}
+__device__ inline u32x4 value_operand(const char* v) {
+  const u32x2 a = read_tr(v), b = read_tr(v + 2048);
+  return u32x4{a.x, a.y, b.x, b.y};
+}
+
+// Two weights (below 2^16) as packed f16 pairs in two parts of one unit: to nearest, and what that
+// leaves.
+__device__ inline void split_weights(float x0, float x1, uint32_t (&out)[2]) {
+  const f32x2 x = {x0, x1};
+  uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+  asm("" : "+v"(w));  // formed once, not again by each element that the rest takes
+  const f16x2 h = __builtin_bit_cast(f16x2, w);
+  float one = 1.f;
+  asm("" : "+s"(one));  // so that a remainder is one mixed fma, not a subtraction and a conversion
+  const f16x2 l = {static_cast<_Float16>(__builtin_fmaf(x0, one, -static_cast<float>(h[0]))),
+                   static_cast<_Float16>(__builtin_fmaf(x1, one, -static_cast<float>(h[1])))};
+  out[0] = w;
+  out[1] = __builtin_bit_cast(uint32_t, l);
+}
+
+// Rows of a wave on the f16 matrix pipe: lane (c, g) has row c of each tile of 16.
+//   Query rows, times a power of two that puts the largest element into [2^14, 2^15), and weights
+//   are split into two f16 parts in one unit, whose products add up in one chain: within 2^-22 of
+//   themselves, small ones within 2^-40 of the row's largest element and 2^-31 of its largest weight.
+//   Weights are taken against a reference, the row's maximum so far or less than 2^kRoom below it,
+//   so that the sums are scaled only where a score passes that (for a row's first step and hardly
+//   ever after), and times a unit 2^u, which the quotient at the end drops. 8-bit values have powers of
+//   two, which go to the weights; the largest product of the two sets the unit, so that rows of
+//   any scale meet in one sum (values above 2^-90).
+constexpr float kRoom = 8.f;
+constexpr float kUnit = 7.f;      // f16 planes: weights below 2^15
+constexpr float kMostUnit = 87.f;  // 8-bit planes: 2^24 weights of 2^kRoom stay below f32's largest
+template <bool k8>
+struct Rows16 {
+  u32x4 qf[2][2];  // d = 16 g + 8 kk + 0..7
+  float down;      // the inverse of the rows' power of two
+  f32x4 o[4];      // column 16 dt + 4 g + e
+  float m, l;
+  float unit;
+  float zero;   // what exponents are taken against: the reference (0 before there is one), less the unit
+  float limit;  // a score past this (before `down`) moves the reference
+
+  __device__ inline void start(const f32x4 (&qx)[4]) {
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) amax = fmaxf(amax, __builtin_fabsf(qx[rt][i][e]));
+      for (int e = 0; e < 4; ++e) amax = fmaxf(amax, __builtin_fabsf(qx[i][e]));
     amax = max_x16_x32(amax);
     const int e_max = static_cast<int>((__builtin_bit_cast(uint32_t, amax) >> 23) & 0xFF);
     const int sh = e_max == 0 ? 0 : clamp_exp(141 - e_max);
-    const float up = pow2(sh);
-    down[rt] = pow2(clamp_exp(-sh));
+    const float x = pow2(sh);
+    down = pow2(clamp_exp(-sh));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t w[kParts];
-      split_units(qx[rt][i >> 1][2 * (i & 1)], qx[rt][i >> 1][2 * (i & 1) + 1], up, w);
+      uint32_t w[2];
+      split2(qx[i >> 1][2 * (i & 1)], qx[i >> 1][2 * (i & 1) + 1], x, w);
 #pragma unroll
-      for (int p = 0; p < kParts; ++p) qf[rt][p][i >> 2][i & 3] = w[p];
+      for (int p = 0; p < 2; ++p) qf[p][i >> 2][i & 3] = w[p];
     }
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = limit = -INFINITY;
+    l = 0.f;
+    unit = k8 ? kMostUnit : kUnit;
+    zero = -unit;
   }
-}
 
-// A wave's steps of an f16 or 8-bit plane on the 16-bit matrix pipe. K comes from memory in operand
-// layout, V passes through the wave's own swizzled LDS rows and is read transposed; the packed weights
-// are the B operand of O^T += V^T P^T as they stand. o[rt][dt][e] is column 16 dt + 4 g + e. Returns
-// whether a sum came out infinite or NaN: parts of an infinity are not numbers, so a wave over f16
-// planes starts again with f32 operands.
-template <bool k8, int kRT>
-__device__ inline bool attend_16(const Block& b, const f32x4 (&qx)[kRT][4], const int (&pos)[kRT],
-                                 int wave, int lane, char* vw, Sums<kRT>& st) {
+  // 32 keys from j0 on: their operands (key 16 t + c, d = 16 g + 8 kk + 0..7), the powers of two of keys
+  // 16 t + 4 g + i and of their values, and values(dt), the values' operand of columns 16 dt.. .
+  template <typename V>
+  __device__ inline void step(const Block& b, int pos, int j0, int g,
+                              const u32x4 (&kf)[2][2], const float (&ks)[2][4],
+                              const float (&vs)[2][4], V values) {
+    const bool masked = b.masked(j0, kN);
+    u32x4 pf[2], va[4];
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 1; p >= 0; --p)  // the smaller part first
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          s[t] = mfma16(kf[t][kk], qf[p][kk], s[t]);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) va[dt] = values(dt);  // on their way under the softmax
+    // Register i of tile t holds key 16 t + 4 g + i.
+    if constexpr (k8) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][i] *= ks[t][i];
+    }
+    if (masked) {
+      asm volatile("");  // a branch: whole steps pay for no selection
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!b.sees(pos, j0 + 16 * t + 4 * g + i)) s[t][i] = -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]);
+    mx = fmaxf(fmaxf(mx, s[0][3]), s[1][0]);
+    mx = fmaxf(fmaxf(mx, s[1][1]), s[1][2]);
+    mx = fmaxf(mx, s[1][3]);
+    if (__any(mx > limit)) {
+      const float m_new = fmaxf(m, max_x16_x32(mx) * down), d = m_new - m;
+      // The products so far fall with the weights, so 8-bit planes' unit may rise as much.
+      const float u = k8 ? fminf(unit + floorf(d), kMostUnit) : kUnit;
+      move(m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((u - unit) - d));
+      unit = u;
+      m = m_new;
+      zero = (m_new == -INFINITY ? 0.f : m_new) - u;
+      limit = (m_new + kRoom) / down;  // a power of two
+    }
+    float p[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], down, -zero));
+    if constexpr (k8) {
+      float w[2][4];
+      auto weigh = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[t][i] = p[t][i] * vs[t][i];
+        if (masked) {
+          // A hidden row's scale may be the NaN one: it takes no part.
+          asm volatile("");
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (s[t][i] == -INFINITY) w[t][i] = 0.f;
+        }
+        float top = fmaxf(fmaxf(w[0][0], w[0][1]), w[0][2]);
+        top = fmaxf(fmaxf(top, w[0][3]), w[1][0]);
+        top = fmaxf(fmaxf(top, w[1][1]), w[1][2]);
+        return fmaxf(top, w[1][3]);
+      };
+      float top = weigh();
+      // Twice at most: a product past f32's range has e of 128, and is in range once that is taken off
+      // (a NaN row's never is).
+      for (int turn = 0; turn < 2 && __any(top > 0x1p15f); ++turn) {
+        // The largest comes to [2^7, 2^8): 2^e <= it < 2^(e + 1).
+        top = max_x16_x32(top);
+        const int e = static_cast<int>(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+        const float u = fminf(unit, unit + 7.f - static_cast<float>(e));
+        const float x = __builtin_amdgcn_exp2f(u - unit);
+        move(x);
+        zero += unit - u;
+        unit = u;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            p[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], down, -zero));
+        top = weigh();
+      }
+      l += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) +
+               ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[t][i] = w[t][i];
+    } else {
+      l += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) +
+               ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        uint32_t w[2];
+        split_weights(p[t][i], p[t][i + 1], w);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) pf[q][2 * t + (i >> 1)] = w[q];
+      }
+#pragma unroll
+    for (int p = 1; p >= 0; --p)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+        o[dt] = mfma16(va[dt], pf[p], o[dt]);
+  }
+  // The row's sums so far, times x.
+  __device__ inline void move(float x) {
+    l *= x;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[dt] *= x;
+  }
+
+  // The sums without their unit. Returns whether one came out infinite or NaN: parts of an infinity
+  // are not numbers, so a wave over f16 planes starts again with f32 operands.
+  __device__ inline bool finish() {
+    bool odd = false;
+    const float x = __builtin_amdgcn_exp2f(-unit);
+    move(x);
+    odd |= !__builtin_isfinite(l);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= !__builtin_isfinite(o[dt][e]);
+    return !k8 && __any(odd);
+  }
+};
+
+// A wave's steps of an f16 or 8-bit plane. K comes from memory in operand layout, V passes through
+// the wave's own swizzled LDS rows and is read transposed; the packed weights are the B operand of
+// O^T += V^T P^T as they stand. Returns whether the wave has to start again with f32 operands.
+template <bool k8>
+__device__ inline bool attend_16(const Block& b, const f32x4 (&qx)[4], int pos,
+                                 int wave, int lane, char* vw, Rows16<k8>& r) {
   const int c = lane & 15, g = lane >> 4;
   constexpr int kK = k8 ? 1 : 2;  // 16-byte pieces of a lane's share of a key
   constexpr int kV = k8 ? 2 : 4;  // and of the step's values
@@ -300,186 +481,113 @@ __device__ inline bool attend_16(const Block& b, const f32x4 (&qx)[kRT][4], cons
       vx[i] = __builtin_bit_cast(u32x4,
                                  __builtin_amdgcn_raw_buffer_load_b128(b.v, vo + 1024 * i, 0, 0));
   };
-  st.clear();
   int step = b.step0 + wave;
   if (step < b.step1) load(b.key_of(step));
-  u32x4 qf[kRT][kParts][2];  // d = 16 g + 8 kk + 0..7
-  float down[kRT];
-  split_rows<kRT>(qx, qf, down);
+  r.start(qx);
   for (; step < b.step1; step += kWaves) {
-    const int j0 = b.key_of(step);
-    u32x4 pf[kRT][kParts];
-    f32x4 s[kRT][2];
-    float alpha[kRT], sv[2][4];
+    u32x4 kf[2][2];
+    float kscale[2][4], vscale[2][4];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      u32x4 kf[2];
       if constexpr (k8) {
+        codes_f16(kx[t][0], kf[t]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t lo, hi;
-          codes_f16(kx[t][0][i], lo, hi);
-          kf[i >> 1][2 * (i & 1)] = lo;
-          kf[i >> 1][2 * (i & 1) + 1] = hi;
+          kscale[t][i] = scale_at(ks[t], i);
+          vscale[t][i] = scale_at(vs[t], i);
         }
       } else {
-        kf[0] = kx[t][0];
-        kf[1] = kx[t][kK - 1];
-      }
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        f32x4 sp[kParts] = {};
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) sp[p] = mfma16(kf[kk], qf[rt][p][kk], sp[p]);
-        s[rt][t] = join(sp);
-        if constexpr (k8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[rt][t][i] *= scale_at(ks[t], i);
-        }
-      }
-      if constexpr (k8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sv[t][i] = scale_at(vs[t], i);
+        kf[t][0] = kx[t][0];
+        kf[t][1] = kx[t][kK - 1];
       }
     }
     wave_sync();  // the last step's transposed reads are done
-    if constexpr (k8) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kV; ++i) {
+      if constexpr (k8) {
         const int row = 16 * i + (lane >> 2);
+        u32x4 y[2];
+        codes_f16(vx[i], y);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          u32x4 y;
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            uint32_t lo, hi;
-            codes_bf16(vx[i][2 * e + n], lo, hi);
-            y[2 * n] = lo;
-            y[2 * n + 1] = hi;
-          }
-          *reinterpret_cast<u32x4*>(vw + row * 128 + (((2 * (lane & 3) + e) ^ swz(row)) * 16)) = y;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kV; ++i) {
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<u32x4*>(vw + row * 128 + (((2 * (lane & 3) + e) ^ swz(row)) * 16)) = y[e];
+      } else {
         const int row = 8 * i + (lane >> 3);
         *reinterpret_cast<u32x4*>(vw + row * 128 + (((lane & 7) ^ swz(row)) * 16)) = vx[i];
       }
     }
     wave_sync();
     if (step + kWaves < b.step1) load(b.key_of(step + kWaves));
-    const bool masked = b.masked(j0, kN);
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      // Register i of tile t holds key 16 t + 4 g + i.
-      uint32_t seen = 0xFFu;
-      if (masked) {
-        seen = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (b.sees(pos[rt], j0 + 16 * t + 4 * g + i))
-              seen |= 1u << (4 * t + i);
-            else
-              s[rt][t][i] = -INFINITY;
-      }
-      float mx = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][t][i]);
-      // Maxima are kept in the units of the parts' sums: times down, a power of two, exact.
-      const float m_new = fmaxf(st.m[rt], max_x16_x32(mx));
-      alpha[rt] = st.m[rt] == -INFINITY
-                      ? 0.f
-                      : __builtin_amdgcn_exp2f((st.m[rt] - m_new) * down[rt]);
-      st.m[rt] = m_new;
-      const float md = m_new == -INFINITY ? 0.f : m_new * down[rt];
-      float ls = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], down[rt], -md));
-          float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i + 1], down[rt], -md));
-          ls += p0 + p1;
-          uint32_t w[kParts];
-          if constexpr (k8) {
-            // A hidden key's scale may be the NaN one: it takes no part.
-            p0 *= masked && !(seen >> (4 * t + i) & 1) ? 0.f : sv[t][i];
-            p1 *= masked && !(seen >> (4 * t + i + 1) & 1) ? 0.f : sv[t][i + 1];
-            split_bf16(p0, p1, w);
-          } else {
-            split_units(p0, p1, kWeightUp, w);
-          }
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) pf[rt][p][2 * t + (i >> 1)] = w[p];
-        }
-      st.l[rt] = __builtin_fmaf(st.l[rt], alpha[rt], ls);
-    }
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
-      u32x2 t[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = 16 * e + 4 * g + (c >> 2);
-        t[e] = read_tr(vw + row * 128 + (((2 * dt + ((c & 3) >> 1)) ^ swz(row)) * 16) + 8 * (c & 1));
-      }
-      const u32x4 va = {t[0].x, t[0].y, t[1].x, t[1].y};
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        f32x4 y;
-        if constexpr (k8) {
-          y = mfma_bf16(va, pf[rt][1], f32x4{0.f, 0.f, 0.f, 0.f});
-          y = mfma_bf16(va, pf[rt][0], y);
-        } else {
-          f32x4 x[kParts];
-#pragma unroll
-          for (int p = 0; p < kParts; ++p) x[p] = mfma16(va, pf[rt][p], f32x4{0.f, 0.f, 0.f, 0.f});
-          y = join(x);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st.o[rt][dt][e] = __builtin_fmaf(st.o[rt][dt][e], alpha[rt], y[e]);
-      }
-    }
+    r.step(b, pos, b.key_of(step), g, kf, kscale, vscale, [&](int dt) __attribute__((always_inline)) {
+      return value_operand(vw + value_offset(dt, c, g));
+    });
   }
-  bool odd = false;
-#pragma unroll
-  for (int rt = 0; rt < kRT; ++rt) {
-    odd |= !__builtin_isfinite(st.l[rt]);
-    st.m[rt] *= down[rt];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
-      if constexpr (!k8) st.o[rt][dt] *= 1.f / kWeightUp;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) odd |= !__builtin_isfinite(st.o[rt][dt][e]);
-    }
-  }
-  return !k8 && __any(odd);
+  return r.finish();
 }
 
-template <DType kD, int kRT>
-__global__ __launch_bounds__(64 * kWaves, 2) void window_attend(WindowArgs a) {
-  constexpr int kRows = 16 * kRT;
+// The head's planes: rows past the `keys` first read as zero (scales by whole words: their planes
+// are padded to 64).
+template <DType kD>
+__device__ inline void set_planes(const WindowArgs& a, int64_t plane, uint32_t keys, Block& b) {
+  constexpr uint32_t kRowBytes = kD == kF32 ? 256 : kD == kF16 ? 128 : 64;
+  auto rows_of = [&](const void* p, int64_t stride, uint32_t range) __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(static_cast<const char*>(p)) + plane * stride, 0, range, kRawBuffer);
+  };
+  b.k = rows_of(a.k, a.plane_rows * kRowBytes, keys * kRowBytes);
+  b.v = rows_of(a.v, a.plane_rows * kRowBytes, keys * kRowBytes);
+  if constexpr (kD == kI8) {
+    b.ks = rows_of(a.k_scale, a.scale_rows, (keys + 3u) & ~3u);
+    b.vs = rows_of(a.v_scale, a.scale_rows, (keys + 3u) & ~3u);
+  }
+}
+// Query row r0 + c of a sequence (of `rows`): d = 16 g + 0..15, times scale * log2(e), and
+// where they stand (rows past the last one are zero and stand at the last key, p1).
+__device__ inline void load_rows(const WindowArgs& a, int t, int h, int r0, int p1, int c, int g,
+                                 f32x4 (&qx)[4], int& pos) {
+  const int past = a.past[t], rows = a.rows[t];
+  const int r = r0 + c;
+  pos = a.causal ? min(past + r, p1) : past - 1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) qx[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (r < rows) {
+    const float* qp = a.q + (a.row0[t] + r) * a.q_rs + h * 64 + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qx[i] = *reinterpret_cast<const f32x4u*>(qp + 4 * i) * a.scale_log2;
+  }
+}
+
+// The square root of what sums against `m` weigh against `all` (at or above it): a sum whose weight is
+// past f32's range may still count, where its values are as much larger.
+__device__ inline float half_weight(float m, float all) {
+  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (m - all));
+}
+
+template <DType kD>
+__global__ __launch_bounds__(64 * kWaves, 4) void window_attend(WindowArgs a) {
+  constexpr int kRows = 16;
   __shared__ __attribute__((aligned(128))) char vs[kD == kF32 ? 1 : kWaves][kN * 128];
   __shared__ __attribute__((aligned(16))) float mo[kWaves][kRows * kPitch];  // a wave's O rows
   __shared__ float ml[kWaves][2][kRows];  // and their max and sum
   __shared__ int last_flag;
 
-  // The workgroups of one head's keys, which read the same rows, share an XCD's L2 (a sequence's
-  // row of the grid is a multiple of the XCDs).
+  // Chunks: the workgroups of one head's keys, which read the same rows, share an XCD's L2 (a
+  // sequence's row of the grid is a multiple of the XCDs). Whole blocks: the last ones of all heads
+  // first, which have the most keys (1000 rows on each other, 20 heads, 8-bit: 17.7 us, 22.1 with
+  // the heads on an XCD each).
   const int t = blockIdx.y;
-  const int lid = xcd_remap(blockIdx.x, gridDim.x);
-  if (lid >= a.n_wgs[t]) return;
   const int past = a.past[t], rows = a.rows[t];
   const int n_blk = a.n_blk[t], n_split = a.n_split[t];
-  int blk, split;
-  const int hs = divide(lid, n_blk, a.blk_inv[t], blk);
-  const int h = divide(hs, n_split, a.split_inv[t], split);
+  const int lid = n_split > 1 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
+  if (lid >= a.n_wgs[t]) return;
+  int blk, split = 0, h;
+  if (n_split > 1) {
+    const int hs = divide(lid, n_blk, a.blk_inv[t], blk);
+    h = divide(hs, n_split, a.split_inv[t], split);
+  } else {
+    blk = n_blk - 1 - divide(lid, a.n_heads, a.head_inv, h);
+  }
   const int row0 = blk * kRows;
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -487,77 +595,49 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attend(WindowArgs a) {
   const int c = lane & 15, g = lane >> 4;
   const int64_t q_row = a.row0[t];
 
-  Block b;
-  b.p0 = a.causal ? past + row0 : past - 1;
-  b.p1 = a.causal ? past + min(row0 + kRows, rows) - 1 : past - 1;
-  b.window = a.window;
-  b.sinks = a.sinks;
-  b.span = span_of(b.p0, b.p1, a.window, a.sinks);
+  Block b(a.causal ? past + row0 : past - 1,
+          a.causal ? past + min(row0 + kRows, rows) - 1 : past - 1, a.window, a.sinks);
   b.step0 = split * a.chunk;
   b.step1 = min(b.step0 + a.chunk, b.span.n_steps);
-  // The head's planes: rows past the last key read as zero (scales by whole words: their planes
-  // are padded to 64).
-  constexpr uint32_t kRowBytes = kD == kF32 ? 256 : kD == kF16 ? 128 : 64;
-  const int64_t plane = a.plane[t] + h;
-  auto rows_of = [&](const void* p, int64_t stride, uint32_t range) __attribute__((always_inline)) {
-    return __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(static_cast<const char*>(p)) + plane * stride, 0, range, kRawBuffer);
-  };
-  const uint32_t keys = static_cast<uint32_t>(b.p1) + 1u;
-  b.k = rows_of(a.k, a.plane_rows * kRowBytes, keys * kRowBytes);
-  b.v = rows_of(a.v, a.plane_rows * kRowBytes, keys * kRowBytes);
-  if constexpr (kD == kI8) {
-    b.ks = rows_of(a.k_scale, a.scale_rows, (keys + 3u) & ~3u);
-    b.vs = rows_of(a.v_scale, a.scale_rows, (keys + 3u) & ~3u);
-  }
+  set_planes<kD>(a, a.plane[t] + h, static_cast<uint32_t>(b.p1) + 1u, b);
+  f32x4 qx[4];
+  int pos;
+  load_rows(a, t, h, row0, b.p1, c, g, qx, pos);
 
-  // Query rows: d = 16 g + 0..15 of row c of each tile, times scale * log2(e).
-  f32x4 qx[kRT][4];
-  int pos[kRT];
+  Sums st;
+  bool f32_order = true;  // which column o[dt][e] is
+  if constexpr (kD != kF32) {
+    Rows16<kD == kI8> r;
+    f32_order = attend_16<kD == kI8>(b, qx, pos, wave, lane, vs[wave], r);
 #pragma unroll
-  for (int rt = 0; rt < kRT; ++rt) {
-    const int r = row0 + 16 * rt + c;
-    pos[rt] = a.causal ? min(past + r, b.p1) : past - 1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) qx[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (r < rows) {
-      const float* qp = a.q + (q_row + r) * a.q_rs + h * 64 + 16 * g;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        qx[rt][i] = *reinterpret_cast<const f32x4u*>(qp + 4 * i) * a.scale_log2;
-    }
+    for (int dt = 0; dt < 4; ++dt) st.o[dt] = r.o[dt];
+    st.m = r.m;
+    st.l = r.l;
   }
-
-  Sums<kRT> st;
-  bool f32_order = true;  // which column o[rt][dt][e] is
-  if constexpr (kD == kF32) {
-    attend_f32<kD, kRT>(b, qx, pos, wave, lane, st);
-  } else {
-    f32_order = attend_16<kD == kI8, kRT>(b, qx, pos, wave, lane, vs[wave], st);
-    if constexpr (kD == kF16) {
-      if (f32_order) attend_f32<kD, kRT>(b, qx, pos, wave, lane, st);
+  if constexpr (kD != kI8) {
+    if (f32_order) {
+      // The rows again, rather than kept through the steps.
+      if (kD == kF16) load_rows(a, t, h, row0, b.p1, c, g, qx, pos);
+      attend_f32<kD>(b, qx, pos, wave, kWaves, lane, st);
     }
   }
 
   // The waves' rows meet in LDS.
+  st.l = sum_x16_x32(st.l);
+  float* const row = &mo[wave][(c) * kPitch];
+  const f32x4(&o)[4] = st.o;
+  if (f32_order) {
 #pragma unroll
-  for (int rt = 0; rt < kRT; ++rt) {
-    st.l[rt] = sum_x16_x32(st.l[rt]);
-    float* const row = &mo[wave][(16 * rt + c) * kPitch];
-    const f32x4(&o)[4] = st.o[rt];
-    if (f32_order) {
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<f32x4*>(row + 16 * g + 4 * e) =
+          f32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
+  } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<f32x4*>(row + 16 * g + 4 * e) =
-            f32x4{o[0][e], o[1][e], o[2][e], o[3][e]};
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4*>(row + 16 * dt + 4 * g) = o[dt];
-    }
-    if (g == 0) {
-      ml[wave][0][16 * rt + c] = st.m[rt];
-      ml[wave][1][16 * rt + c] = st.l[rt];
-    }
+    for (int dt = 0; dt < 4; ++dt) *reinterpret_cast<f32x4*>(row + 16 * dt + 4 * g) = o[dt];
+  }
+  if (g == 0) {
+    ml[wave][0][c] = st.m;
+    ml[wave][1][c] = st.l;
   }
   __syncthreads();
   // Thread (r, kCols columns from d0 on) adds the waves up, and the last of a block's chunks
@@ -584,11 +664,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attend(WindowArgs a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       // A wave without a maximum saw no key, or NaN scores only (sums of NaN, which 0 keeps).
-      const float x = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M);
-      L = __builtin_fmaf(lw[w], x, L);
+      const float x = half_weight(mw[w], M);
+      L = __builtin_fmaf(lw[w] * x, x, L);
 #pragma unroll
       for (int e = 0; e < kCols; ++e)
-        acc[e] = __builtin_fmaf(mo[w][r * kPitch + d0 + e], x, acc[e]);
+        acc[e] = __builtin_fmaf(mo[w][r * kPitch + d0 + e] * x, x, acc[e]);
     }
   }
   if (n_split == 1) {
@@ -630,17 +710,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attend(WindowArgs a) {
     float Mb = M;
 #pragma unroll
     for (int j = 0; j < kMergeLoads; ++j) Mb = fmaxf(Mb, ms[j]);
-    const float x = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - Mb);
-    L *= x;
+    const float x = half_weight(M, Mb);
+    L = L * x * x;
 #pragma unroll
-    for (int e = 0; e < kCols; ++e) acc[e] *= x;
+    for (int e = 0; e < kCols; ++e) acc[e] = acc[e] * x * x;
 #pragma unroll
     for (int j = 0; j < kMergeLoads; ++j) {
       if (s0 + j >= n_split) break;
-      const float w = ms[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[j] - Mb);
-      L = __builtin_fmaf(ls[j], w, L);
+      const float w = half_weight(ms[j], Mb);
+      L = __builtin_fmaf(ls[j] * w, w, L);
 #pragma unroll
-      for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(as[j][e], w, acc[e]);
+      for (int e = 0; e < kCols; ++e) acc[e] = __builtin_fmaf(as[j][e] * w, w, acc[e]);
     }
     M = Mb;
   }
@@ -648,32 +728,194 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attend(WindowArgs a) {
   if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Rows of a block.
-int block_rows(const WindowArgs& a, DType) {
+// K20 (window_tiles): the same for many rows. A workgroup of four waves takes 64 rows of one head, 16 a
+//   wave, and goes through their keys in tiles of 64 that pass through LDS once for all four, so that K
+//   and V are read and widened for 64 rows; a wave leaves out the halves of a tile that none of its rows
+//   see. No merge: a wave has its rows to itself. Blocks start with the last ones of every head, which
+//   see the most keys (4000 rows on each other, 20 heads, f16: 99 us; heads in turn: 175).
+//   Bound by what a wave issues (the softmax and the split of its weights, vector pipe 55%, next to
+//   29% of the matrix pipe): 4000 rows take 41 GFLOP each for scores and outputs (two parts), 0.83
+//   PFLOP/s, of 1.26 that a large product reaches here. 32 rows a wave halve the LDS reads, but leave 2 or
+//   3 waves a SIMD and half the blocks (110 us; 1500 rows: 39 us, 26 with 16 rows a wave).
+constexpr int kTile = 64;
+constexpr int kTileRows = 64;
+__device__ inline int kswz(int r) { return (r >> 1) & 7; }  // 16 rows' equal chunks hit distinct banks
+
+template <bool k8>
+__global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs a) {
+  constexpr int kPieces = k8 ? 1 : 2;  // 16-byte pieces of a tile's K (or V) a thread
+  constexpr DType kD = k8 ? kI8 : kF16;
+  __shared__ __attribute__((aligned(128))) char kt[2][kTile * 128], vt[2][kTile * 128];
+  __shared__ __attribute__((aligned(16))) float st[2][2][k8 ? kTile : 4];  // K's and V's powers of two
+  const int t = blockIdx.y;
+  const int lid = blockIdx.x;
+  if (lid >= a.n_wgs[t]) return;
+  const int past = a.past[t], rows = a.rows[t];
+  int h;
+  const int blk = a.n_blk[t] - 1 - divide(lid, a.n_heads, a.head_inv, h);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int first = blk * kTileRows, row0 = first + 16 * wave;
+  // The block's tiles, and the wave's rows (a wave past the last row only loads).
+  const int p1 = a.causal ? past + min(first + kTileRows, rows) - 1 : past - 1;
+  const Span<kTile> span(a.causal ? past + first : past - 1, p1, a.window, a.sinks);
+  const bool idle = row0 >= rows;
+  Block b(a.causal ? past + min(row0, rows - 1) : past - 1,
+          a.causal ? past + min(row0 + 16, rows) - 1 : past - 1, a.window, a.sinks);
+  b.step0 = 0;
+  b.step1 = b.span.n_steps;
+  set_planes<kD>(a, a.plane[t] + h, static_cast<uint32_t>(p1) + 1u, b);
+
+  u32x4 kx[kPieces], vx[kPieces];
+  uint32_t sx = 0;
+  auto load = [&](int j0) __attribute__((always_inline)) {
+    const uint32_t o = static_cast<uint32_t>(j0) * (64u * kPieces) + 16u * tid;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      kx[i] = __builtin_bit_cast(u32x4,
+                                 __builtin_amdgcn_raw_buffer_load_b128(b.k, o + 4096 * i, 0, 0));
+      vx[i] = __builtin_bit_cast(u32x4,
+                                 __builtin_amdgcn_raw_buffer_load_b128(b.v, o + 4096 * i, 0, 0));
+    }
+    if constexpr (k8) {
+      if (tid < 2 * kTile) {
+        const uint32_t so = static_cast<uint32_t>(j0 + (tid & (kTile - 1)));
+        sx = tid < kTile ? __builtin_amdgcn_raw_buffer_load_b8(b.ks, so, 0, 0)
+                         : __builtin_amdgcn_raw_buffer_load_b8(b.vs, so, 0, 0);
+      }
+    }
+  };
+  auto put = [&](char* p, int row, int chunk, int swizzle, const u32x4& x)
+                 __attribute__((always_inline)) {
+    *reinterpret_cast<u32x4*>(p + row * 128 + ((chunk ^ swizzle) * 16)) = x;
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+    if constexpr (k8) {
+      const int row = tid >> 2, chunk = 2 * (tid & 3);
+      u32x4 y[2];
+      codes_f16(kx[0], y);
+      put(kt[buf], row, chunk, kswz(row), y[0]);
+      put(kt[buf], row, chunk + 1, kswz(row), y[1]);
+      codes_f16(vx[0], y);
+      put(vt[buf], row, chunk, swz(row & 31), y[0]);
+      put(vt[buf], row, chunk + 1, swz(row & 31), y[1]);
+      if (tid < 2 * kTile) st[buf][tid >= kTile][tid & (kTile - 1)] = scale_at(sx, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int row = 32 * i + (tid >> 3), chunk = tid & 7;
+        put(kt[buf], row, chunk, kswz(row), kx[i]);
+        put(vt[buf], row, chunk, swz(row & 31), vx[i]);
+      }
+    }
+  };
+  load(span.key_of(0));
+  f32x4 qx[4];
+  int pos;
+  load_rows(a, t, h, row0, b.p1, c, g, qx, pos);
+  Rows16<k8> r;
+  r.start(qx);
+  store(0);
+  if (span.n_steps > 1) load(span.key_of(1));
+  __syncthreads();
+  // A lane's places in a tile: its share of a key, and the values of its columns.
+  int k_at[2], v_at[4];
+#pragma unroll
+  for (int kk = 0; kk < 2; ++kk) k_at[kk] = c * 128 + (((2 * g + kk) ^ kswz(c)) * 16);
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) v_at[dt] = value_offset(dt, c, g);
+  for (int i = 0; i < span.n_steps; ++i) {
+    const int buf = i & 1;
+    if (i + 1 < span.n_steps) {
+      store(buf ^ 1);  // last read before the last barrier
+      if (i + 2 < span.n_steps) load(span.key_of(i + 2));
+    }
+    const char *const kp = kt[buf], *const vp = vt[buf];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int j0 = span.key_of(i) + kN * half;
+      if (idle || !b.any(j0, kN)) continue;
+      u32x4 kf[2][2];
+      float ks[2][4], vs[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = kN * half + 16 * u;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+          kf[u][kk] = *reinterpret_cast<const u32x4*>(kp + k_at[kk] + 128 * at);
+        if constexpr (k8) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(&st[buf][0][at + 4 * g]);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(&st[buf][1][at + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ks[u][e] = x[e];
+            vs[u][e] = y[e];
+          }
+        }
+      }
+      r.step(b, pos, j0, g, kf, ks, vs, [&](int dt) __attribute__((always_inline)) {
+        return value_operand(vp + v_at[dt] + 4096 * half);
+      });
+    }
+    __syncthreads();
+  }
+  bool f32_order = r.finish();  // which column o[dt][e] is
+  if constexpr (!k8) {
+    if (f32_order) {
+      Sums sums;
+      load_rows(a, t, h, row0, b.p1, c, g, qx, pos);  // again, rather than kept so long
+      attend_f32<kD>(b, qx, pos, 0, 1, lane, sums);
+      r.l = sums.l;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) r.o[dt] = sums.o[dt];
+    }
+  }
+  const float l = sum_x16_x32(r.l), inv = l == 0.f ? 0.f : 1.f / l;
+  const int row = row0 + c;
+  if (row >= rows) return;
+  float* const op = a.o + (a.row0[t] + row) * a.o_rs + h * 64;
+  const f32x4(&o)[4] = r.o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 x = f32_order ? f32x4{o[0][i], o[1][i], o[2][i], o[3][i]} : o[i];
+    *reinterpret_cast<f32x4u*>(op + (f32_order ? 16 * g + 4 * i : 16 * i + 4 * g)) = x * inv;
+  }
+}
+
+// Rows of a block: tiles where they fill the GPU. Measured with 20 heads of rows on each other, tiles
+// against blocks of 16: f16 1000 rows (320 tiles) 19.3 us against 19.7, 4000 rows 99 against 183, 8
+// heads of 1500 rows (192 tiles) 23.4 against 17.8; 8-bit 1500 rows (480) 35 against 29, 2500 rows (800)
+// 60 against 66, 4000 rows 113 against 146. Calls of at most 32 rows a sequence would leave half a tile.
+int block_rows(const WindowArgs& a, DType dt) {
+  int64_t wide = 0;
   int most = 0;
-  for (int t = 0; t < a.n_seqs; ++t) most = std::max(most, a.rows[t]);
-  return most > 16 ? 32 : 16;
+  for (int t = 0; t < a.n_seqs; ++t) {
+    most = std::max(most, a.rows[t]);
+    wide += static_cast<int64_t>((a.rows[t] + kTileRows - 1) / kTileRows) * a.n_heads;
+  }
+  return dt != kF32 && wide >= (dt == kI8 ? 640 : 256) && most > 32 ? kTileRows : 16;
+}
+
+// Steps of the longest block of a sequence, at most.
+int most_steps(const WindowArgs& a, int t, int rows) {
+  const int p1 = a.past[t] - 1 + (a.causal ? a.rows[t] : 0), wide = std::min(a.rows[t], rows);
+  const Span<kN> s(a.causal ? p1 - wide + 1 : p1, p1, a.window, a.sinks);
+  // A block before the last may begin its window at another place within a step.
+  return std::min(s.n_steps + (a.rows[t] > rows ? 1 : 0), (p1 + kN) / kN);
 }
 
 }  // namespace
 
 int64_t window_plan(WindowArgs& a, DType dt, bool split) {
   const int rows = block_rows(a, dt);
-  int64_t blocks = 0, work = 0;
-  int steps[kWindowMaxSeqs], longest = 1;  // of a sequence's longest block, at most
+  int steps[kWindowMaxSeqs], longest = 1;
   for (int t = 0; t < a.n_seqs; ++t) {
     a.n_blk[t] = (a.rows[t] + rows - 1) / rows;
-    const int64_t b = static_cast<int64_t>(a.n_blk[t]) * a.n_heads;
-    const int p1 = a.past[t] - 1 + (a.causal ? a.rows[t] : 0);
-    const int wide = std::min(a.rows[t], rows);
-    const Span s = span_of(a.causal ? p1 - wide + 1 : p1, p1, a.window, a.sinks);
-    // A block before the last may begin its window at another place within a step.
-    steps[t] = s.n_steps + (a.n_blk[t] > 1 ? 1 : 0);
-    steps[t] = std::min(steps[t], (p1 + kN) / kN);
-    blocks += b;
-    work += b * steps[t];
+    steps[t] = most_steps(a, t, rows);
     longest = std::max(longest, steps[t]);
   }
+  a.head_inv = inverse(a.n_heads);
   int64_t widest = 0;
   auto lay = [&](int64_t chunk) {
     int64_t sum = 0;
@@ -692,13 +934,29 @@ int64_t window_plan(WindowArgs& a, DType dt, bool split) {
     widest = (widest + 7) / 8 * 8;
     return sum;
   };
-  const int whole = dt == kF32 ? 10 : 16, least = dt == kF32 ? 4 : 8;
-  if (split && blocks < kTreeMaxWgs && longest > whole) {
-    int64_t chunk = std::max<int64_t>(least, (work + kTreeMaxWgs - 1) / kTreeMaxWgs);
-    for (chunk = (chunk + 3) / 4 * 4; chunk < longest; chunk += 4)
-      if (lay(chunk) <= kTreeMaxWgs) return widest;
+  int64_t chunk = longest;
+  if (split && rows == 16) {
+    // What a launch takes, in us, next to its fixed 3.5: the fullest CU's workgroups share it (a step
+    // alone 0.7, f32 1.9), and chunks cost their merge, in turns of kMergeLoads.
+    const float alone = dt == kF32 ? 0.95f : 0.25f, each = dt == kF32 ? 0.95f : 0.45f;
+    float best = 0.f;
+    for (int n = 1; n <= 256; n += n < 4 ? 1 : n & (n - 1) ? n / 3 : n / 2) {
+      const int64_t c = ((longest + n - 1) / n + 3) / 4 * 4;
+      int64_t wgs = 0;
+      for (int t = 0; t < a.n_seqs; ++t)
+        wgs += static_cast<int64_t>(a.n_blk[t]) * a.n_heads * ((steps[t] + c - 1) / c);
+      if (n > 1 && wgs > 2 * kTreeMaxWgs) break;  // what the scratch takes, of 16 rows
+      float us = static_cast<float>(c / 4) * (alone + each * static_cast<float>((wgs + 255) / 256));
+      if (n > 1)
+        us += 1.1f + 0.7f * static_cast<float>((n + kMergeLoads - 1) / kMergeLoads) +
+              static_cast<float>(wgs) / 240.f;
+      if (n == 1 || us < best) {
+        best = us;
+        chunk = n == 1 ? longest : c;
+      }
+    }
   }
-  lay(longest);
+  lay(chunk);
   return widest;
 }
 
@@ -706,17 +964,15 @@ hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipS
   if (wgs <= 0) return hipSuccess;
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(wgs), a.n_seqs), block(64 * kWaves);
-  const bool few = block_rows(a, dt) == 16;
-#define WRS_WINDOW(D, RT) hipLaunchKernelGGL((window_attend<D, RT>), grid, block, 0, s, a)
+  const bool tiles = block_rows(a, dt) == kTileRows;
+#define WRS_WINDOW(K) hipLaunchKernelGGL(K, grid, block, 0, s, a)
   switch (dt) {
     case kF16:
-      if (few) { WRS_WINDOW(kF16, 1); } else { WRS_WINDOW(kF16, 2); }
+      if (tiles) { WRS_WINDOW(window_tiles<false>); } else { WRS_WINDOW(window_attend<kF16>); }
       break;
-    case kF32:
-      if (few) { WRS_WINDOW(kF32, 1); } else { WRS_WINDOW(kF32, 2); }
-      break;
+    case kF32: WRS_WINDOW(window_attend<kF32>); break;
     case kI8:
-      if (few) { WRS_WINDOW(kI8, 1); } else { WRS_WINDOW(kI8, 2); }
+      if (tiles) { WRS_WINDOW(window_tiles<true>); } else { WRS_WINDOW(window_attend<kI8>); }
       break;
     default: return hipErrorInvalidValue;
   }

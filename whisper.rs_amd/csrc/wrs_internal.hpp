@@ -312,7 +312,7 @@ struct WindowArgs {
   int past[kWindowMaxSeqs], rows[kWindowMaxSeqs];  // rows >= 1; past >= 1 where not causal
   // By window_plan, as TreeArgs has them; chunk counts steps.
   int n_wgs[kWindowMaxSeqs], wg0[kWindowMaxSeqs], n_blk[kWindowMaxSeqs], n_split[kWindowMaxSeqs];
-  uint32_t blk_inv[kWindowMaxSeqs], split_inv[kWindowMaxSeqs];
+  uint32_t blk_inv[kWindowMaxSeqs], split_inv[kWindowMaxSeqs], head_inv;
 };
 int64_t window_plan(WindowArgs& a, DType dt, bool split);
 hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipStream_t s);
@@ -325,7 +325,8 @@ hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipS
 // without `split` only rows past kScoreChunk entries are dealt.
 constexpr int kScoreMostTop = 32;
 constexpr int kScoreChunk = 65536;   // entries of one workgroup, at most
-constexpr int kScoreMaxWgs = 512;    // of a launch that splits rows which fit a workgroup
+constexpr int kScoreSmall = 4096;    // entries of a workgroup that keeps them in registers, at most
+constexpr int kScoreMaxWgs = 128;    // of a launch that splits rows which fit a workgroup
 constexpr int kScoreMostChunks = 64;  // of a row
 constexpr int kScorePart = 4 + 2 * kScoreMostTop;  // floats: m, s, t, and the best entries' keys
 struct ScoreArgs {
