@@ -263,7 +263,8 @@ __device__ inline void split_weights(float x0, float x1, uint32_t (&out)[2]) {
 //   Query rows, times a power of two that puts the largest element into [2^14, 2^15), and weights
 //   are split into two f16 parts in one unit, whose products add up in one chain: within 2^-22 of
 //   themselves, small ones within 2^-40 of the row's largest element and 2^-31 of its largest weight.
-//   Weights are taken against a reference, the row's maximum so far or less than 2^kRoom below it,
+//   Weights are taken against a reference, the row's maximum so far or less than kRoom below it (a whole
+//   number, so that what is taken off the exponents is the reference that sums are joined by, exactly),
 //   so that the sums are scaled only where a score passes that (for a row's first step and hardly
 //   ever after), and times a unit 2^u, which the quotient at the end drops. 8-bit values have powers of
 //   two, which go to the weights; the largest product of the two sets the unit, so that rows of
@@ -348,9 +349,9 @@ struct Rows16 {
     mx = fmaxf(fmaxf(mx, s[1][1]), s[1][2]);
     mx = fmaxf(mx, s[1][3]);
     if (__any(mx > limit)) {
-      const float m_new = fmaxf(m, max_x16_x32(mx) * down), d = m_new - m;
+      const float m_new = fmaxf(m, ceilf(max_x16_x32(mx) * down)), d = m_new - m;
       // The products so far fall with the weights, so 8-bit planes' unit may rise as much.
-      const float u = k8 ? fminf(unit + floorf(d), kMostUnit) : kUnit;
+      const float u = k8 ? fminf(unit + d, kMostUnit) : kUnit;
       move(m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((u - unit) - d));
       unit = u;
       m = m_new;
