@@ -134,6 +134,37 @@ def test_long_rows_of_many_slots(wrs, ctx):
     assert same(gk, stored(k, "i8")) and same(gv, stored(v, "i8"))
 
 
+@pytest.mark.parametrize("name", ["f16", "f32", "i8"])
+@pytest.mark.parametrize("heads,counts", [(3, [16, 1, 0, 15]), (5, [64, 65, 1]), (1, [129, 63]),
+                                          (8, [33000, 100])])
+def test_many_rows_of_a_slot(wrs, ctx, name, heads, counts):
+    """Blocks of rows of a head, the longest ones read past the caches; from odd rows on, in wider
+    rows at an odd dword; what lies around stays."""
+    d, n, slots = heads * D, sum(counts), len(counts)
+    note(f"rows of a head {name} {heads} {counts}")
+    ar = wrs.KvArena(1, slots, heads, max(counts) + 4, 0, ctx=ctx, dtype=_dtype(wrs, name))
+    before = normal(3 * slots, d, seed=50)
+    ar.append_rows(0, list(range(slots)), [3] * slots, before, before)
+    for i in range(slots):
+        ar.advance(i, 3)
+    wide = normal(n, 2 * d + 3, seed=51)
+    k, v = wide[:, 1:d + 1], wide[:, d + 3:]
+    ar.append_rows(0, list(range(slots)), counts, k, v)
+    out = torch.full((n + 2, 2 * d + 3), 9.0, device="cuda")
+    gk, gv = out[1:-1, 2:d + 2], out[1:-1, d + 2:2 * d + 2]
+    for i, c in enumerate(counts):
+        ar.advance(i, c)
+    ar.read_rows(0, list(range(slots)), [3] * slots, counts, gk, gv)
+    old_k, old_v = torch.zeros_like(before), torch.zeros_like(before)
+    ar.read_rows(0, list(range(slots)), [0] * slots, [3] * slots, old_k, old_v)
+    torch.cuda.synchronize()
+    assert same(gk, stored(k.contiguous(), name)) and same(gv, stored(v.contiguous(), name))
+    assert same(old_k, stored(before, name)) and same(old_v, stored(before, name))
+    gk.fill_(9.0)
+    gv.fill_(9.0)
+    assert (out == 9.0).all()
+
+
 def fill(wrs, ctx, layers, slots, heads, rows, max_ctx, seed=0):
     ar = wrs.KvArena(layers, slots, heads, max_ctx, 0, ctx=ctx, dtype=wrs.WRS_I8)
     data = {}

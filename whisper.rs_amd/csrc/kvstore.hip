@@ -14,6 +14,13 @@
 //   take a row of a head, 4 values each, and find its largest magnitude by DPP (as bit patterns:
 //   a NaN is the largest).
 // K18 (kv_read): the stored values as f32, the same way round.
+//   Bound by memory. From kManyRows rows on a workgroup takes 64 rows of one head, whose codes and
+//   scales are contiguous and no other workgroup's (rows of all heads in turn: a scale's line is
+//   written by many). What is read back is written past the caches (non-temporal), and so is read what
+//   is stored if it is more than they keep. 44012 rows of 12 heads to 8 bits and back (339 MB
+//   each way): 64 us and 50 us, 5.3 and 6.8 TB/s; by rows of all heads 70 and 68, without the
+//   non-temporal forms 68 and 67. 1500 rows of 20 heads: 5.5 and 4.2 us (non-temporal loads: 5.8).
+//   A step's 5 rows take 2.8 and 2.5 us, what an empty launch does.
 #include "wrs_internal.hpp"
 
 #include <algorithm>
@@ -71,15 +78,28 @@ __device__ inline f32x4 decode4(uint32_t w, uint32_t byte) {
   return x;
 }
 
-constexpr int kTurns = 4;  // pieces of 4 values that a thread has in flight, 256 apart
+constexpr int kTurns = 4;  // pieces of 4 values that a thread has in flight
+constexpr int kBlockRows = 16 * kTurns;
+constexpr int kManyRows = 16;
+constexpr int64_t kOnce = 128 << 20;  // bytes that are read past the caches
 
-// Piece t of a slot's rows: 4 columns of row t / (16 heads).
-template <DType kD, bool kStore>
+// A workgroup takes 1024 pieces of 4 columns: the next ones of rows of all heads, or those of
+// kBlockRows rows of a head.
+enum class Order { kAllHeads, kByHead, kByHeadOnce };
+template <DType kD, bool kStore, Order kOrder>
 __global__ __launch_bounds__(256) void kv_rows(KvSlotRows a) {
-  const int u = blockIdx.z, per_row = a.n_heads * 16;
-  const int64_t n = static_cast<int64_t>(a.count[u]) * per_row;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (256 * kTurns) + threadIdx.x;
-  if (t0 - threadIdx.x >= n) return;
+  constexpr bool kByHead = kOrder != Order::kAllHeads;
+  const int u = blockIdx.z, rows_here = a.count[u], sub = threadIdx.x >> 4;
+  // The block's first row of a head and that head, or its first row in turn.
+  int64_t first;
+  int head = 0;
+  if constexpr (kByHead)
+    first = static_cast<int64_t>(kBlockRows) *
+            divide(static_cast<int>(blockIdx.x), a.n_heads, a.heads_inv, head);
+  else
+    first = static_cast<int64_t>(kBlockRows) * blockIdx.x;
+  const int64_t n = kByHead ? rows_here : static_cast<int64_t>(rows_here) * a.n_heads;
+  if (first >= n) return;
   float* const rows = (blockIdx.y ? a.v_rows : a.k_rows) + a.row0[u] * (blockIdx.y ? a.v_rs : a.k_rs);
   const int64_t rs = blockIdx.y ? a.v_rs : a.k_rs;
   char* const plane = static_cast<char*>(blockIdx.y ? a.v : a.k);
@@ -90,17 +110,20 @@ __global__ __launch_bounds__(256) void kv_rows(KvSlotRows a) {
   float* p[kTurns];
 #pragma unroll
   for (int j = 0; j < kTurns; ++j) {
-    const int64_t t = t0 + 256 * j;
-    // Threads past the end take the last piece's place (whole rows of 16 lanes: n is a multiple).
-    const int64_t tc = t < n ? t : n - 16 + (threadIdx.x & 15);
-    int col;
-    const int row = divide(static_cast<int>(tc >> 4), a.n_heads, a.heads_inv, col);
+    // Lanes past the end take the last row (16 lanes together).
+    const int t = static_cast<int>(min(first + 16 * j + sub, n - 1));
+    int col = head, row = t;
+    if constexpr (!kByHead) row = divide(t, a.n_heads, a.heads_inv, col);
     const int64_t r = a.plane[u] + col;  // plane of (slot, head)
     at[j] = (r * a.plane_rows + a.pos[u] + row) * 64 + 4 * (threadIdx.x & 15);
     sc[j] = r * a.scale_rows + a.pos[u] + row;
     p[j] = rows + row * rs + col * 64 + 4 * (threadIdx.x & 15);
     if constexpr (kStore) {
-      x[j] = *reinterpret_cast<const f32x4u*>(p[j]);
+      const f32x4u* const from = reinterpret_cast<const f32x4u*>(p[j]);
+      if constexpr (kOrder == Order::kByHeadOnce)
+        x[j] = __builtin_nontemporal_load(from);
+      else
+        x[j] = *from;
     } else if constexpr (kD == kF32) {
       x[j] = *reinterpret_cast<const f32x4*>(plane + 4 * at[j]);
     } else if constexpr (kD == kF16) {
@@ -113,10 +136,14 @@ __global__ __launch_bounds__(256) void kv_rows(KvSlotRows a) {
 #pragma unroll
   for (int j = 0; j < kTurns; ++j) {
     if (kStore && kD == kI8) w[j] = encode4(x[j], byte[j]);  // every lane of a row
-    if (t0 + 256 * j >= n) continue;
+    if (first + 16 * j + sub >= n) continue;
     if constexpr (!kStore) {
       if constexpr (kD == kI8) x[j] = decode4(w[j], byte[j]);
-      *reinterpret_cast<f32x4u*>(p[j]) = x[j];
+      f32x4u* const to = reinterpret_cast<f32x4u*>(p[j]);
+      if constexpr (kByHead)
+        __builtin_nontemporal_store(x[j], to);
+      else
+        *to = x[j];
     } else if constexpr (kD == kF32) {
       *reinterpret_cast<f32x4*>(plane + 4 * at[j]) = x[j];
     } else if constexpr (kD == kF16) {
@@ -220,17 +247,34 @@ __global__ __launch_bounds__(64 * kKeepWaves) void kv8_keep_rows(KeepArgs<kSlots
 
 hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStream_t s) {
   int most = 0;
-  for (int u = 0; u < a.n_slots; ++u) most = std::max(most, a.count[u]);
-  const int64_t pieces = static_cast<int64_t>(most) * a.n_heads * 16;
-  if (pieces <= 0) return hipSuccess;
-  if (static_cast<int64_t>(most) * a.n_heads > 0x7fffffff) return hipErrorInvalidConfiguration;
-  const int64_t blocks = (pieces + 256 * kTurns - 1) / (256 * kTurns);
+  int64_t all = 0;
+  for (int u = 0; u < a.n_slots; ++u) {
+    most = std::max(most, a.count[u]);
+    all += a.count[u];
+  }
+  if (most <= 0 || a.n_heads <= 0) return hipSuccess;
+  const int64_t rows = static_cast<int64_t>(most) * a.n_heads;
+  if (rows > 0x7fffffff - kBlockRows) return hipErrorInvalidConfiguration;
+  const bool by_head = most >= kManyRows, once = all * a.n_heads * 512 > kOnce;
+  const int64_t blocks = by_head ? (most + kBlockRows - 1) / kBlockRows * static_cast<int64_t>(a.n_heads)
+                                 : (rows + kBlockRows - 1) / kBlockRows;
   const dim3 grid(static_cast<unsigned>(blocks), 2, a.n_slots);
-#define WRS_KV_ROWS(D)                                                               \
-  if (store)                                                                         \
-    hipLaunchKernelGGL((kv_rows<D, true>), grid, dim3(256), 0, s, a);                \
-  else                                                                               \
-    hipLaunchKernelGGL((kv_rows<D, false>), grid, dim3(256), 0, s, a)
+#define WRS_KV_ROWS_ONE(D, S, O) \
+  hipLaunchKernelGGL((kv_rows<D, S, Order::O>), grid, dim3(256), 0, s, a)
+#define WRS_KV_ROWS(D)                                                        \
+  if (!by_head) {                                                             \
+    if (store) {                                                              \
+      WRS_KV_ROWS_ONE(D, true, kAllHeads);                                    \
+    } else {                                                                  \
+      WRS_KV_ROWS_ONE(D, false, kAllHeads);                                   \
+    }                                                                         \
+  } else if (!store) {                                                        \
+    WRS_KV_ROWS_ONE(D, false, kByHead);                                       \
+  } else if (once) {                                                          \
+    WRS_KV_ROWS_ONE(D, true, kByHeadOnce);                                    \
+  } else {                                                                    \
+    WRS_KV_ROWS_ONE(D, true, kByHead);                                        \
+  }
   switch (dt) {
     case kF32: WRS_KV_ROWS(kF32); break;
     case kF16: WRS_KV_ROWS(kF16); break;
@@ -238,6 +282,7 @@ hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStr
     default: return hipErrorInvalidValue;
   }
 #undef WRS_KV_ROWS
+#undef WRS_KV_ROWS_ONE
   return hipGetLastError();
 }
 
