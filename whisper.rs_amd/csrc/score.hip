@@ -205,8 +205,9 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   float m = -INFINITY, s = 0.f, t = 0.f, ref = kLow;
   int at = 0;  // the group that held m first
   float v[kTurns][kN];
-  // kClean: -infinity is unlikely among the group's entries.
-  auto take = [&](int g, float top, auto kClean) __attribute__((always_inline)) {
+  // Entries of the group g, `top` the largest. kClean: -infinity is unlikely among them.
+  auto take = [&](int g, const auto& x, float top, auto kClean) __attribute__((always_inline)) {
+    constexpr int kPieces = sizeof(x) / sizeof(x[0]);
     if (top > m) at = g;
     m = fmaxf(m, top);
     const float r = fmaxf(m * scale, kLow), d = ref - r, w0 = __builtin_amdgcn_exp2f(d);
@@ -215,10 +216,10 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
     s *= w0;
     const float t0 = t;
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u)
+    for (int u = 0; u < kPieces; ++u)
 #pragma unroll
       for (int e = 0; e < kN; ++e) {
-        const float z = __builtin_fmaf(v[u][e], scale, -r), w = __builtin_amdgcn_exp2f(z);
+        const float z = __builtin_fmaf(x[u][e], scale, -r), w = __builtin_amdgcn_exp2f(z);
         s += w;
         t = __builtin_fmaf(kClean.value ? z : fmaxf(z, kLow), w, t);
       }
@@ -226,10 +227,10 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
       // An entry of -infinity, whose weight of 0 times its exponent is no number: again without.
       t = t0;
 #pragma unroll
-      for (int u = 0; u < kTurns; ++u)
+      for (int u = 0; u < kPieces; ++u)
 #pragma unroll
         for (int e = 0; e < kN; ++e) {
-          const float z = __builtin_fmaf(v[u][e], scale, -r);
+          const float z = __builtin_fmaf(x[u][e], scale, -r);
           t = __builtin_fmaf(fmaxf(z, kLow), __builtin_amdgcn_exp2f(z), t);
         }
     }
@@ -259,20 +260,28 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
             for (int e = 0; e < kN; ++e) top = fmaxf(top, v[u][e]);
         }
         if (g + 1 < whole) fetch(g + 1);
-        take(g, top, std::integral_constant<bool, !kMask>{});
+        take(g, v, top, std::integral_constant<bool, !kMask>{});
       }
     }
   }
-  if (kSmall || whole < groups) {
-    const int g = kSmall ? 0 : whole;
+  if constexpr (kSmall) {
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) index[u] = row.load((g * kTurns + u) * kThreads + tid, v[u]);
+    for (int u = 0; u < kTurns; ++u) index[u] = row.load(u * kThreads + tid, v[u]);
     float top = v[0][0];
 #pragma unroll
     for (int u = 0; u < kTurns; ++u)
 #pragma unroll
       for (int e = 0; e < kN; ++e) top = fmaxf(top, v[u][e]);
-    take(g, top, std::false_type{});
+    take(0, v, top, std::false_type{});
+  } else if (whole < groups) {
+    for (int q = whole * kTurns; q * kThreads + 64 * wave < pieces; ++q) {
+      float x[1][kN];
+      row.load(q * kThreads + tid, x[0]);
+      float top = x[0][0];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) top = fmaxf(top, x[0][e]);
+      take(whole, x, top, std::false_type{});
+    }
   }
 
   // A bound at or below the k-th largest thread's maximum: that of 64 runs of threads.
@@ -517,6 +526,7 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
   // A row with an allowed NaN or +infinity has no distribution; one without an entry gives none
   // of its tokens.
   const bool odd = s != s || m == INFINITY, none = !odd && m == -INFINITY;
+  if (tid >= 128) return;  // two waves write
   const float ln_s = log1pf(s);
   auto logprob = [&](float v) {
     if (odd) return NAN;
