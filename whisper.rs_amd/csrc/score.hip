@@ -40,16 +40,19 @@ constexpr int kMostKeys = kScoreMostTop * (kScoreChunk / kThreads);  // entries 
 constexpr int kCounterStride = 32;   // 128 bytes between merge counters
 constexpr float kLow = -1e30f;       // finite: times a weight of 0 it is 0
 
-// An entry's order as an unsigned number: by value, the lower index first among equals.
-__device__ inline uint64_t key_of(float x, uint32_t index) {
+// A value's order as an unsigned number, and an entry's: by value, the lower index first among
+// equals.
+__device__ inline uint32_t order_of(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);  // one zero
-  const uint32_t o = u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
-  return static_cast<uint64_t>(o) << 32 | (0xFFFFFFFFu - index);
+  return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
-__device__ inline float value_of(uint64_t key) {
-  const uint32_t o = static_cast<uint32_t>(key >> 32);
+__device__ inline float value_of(uint32_t o) {
   return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
+__device__ inline uint64_t key_of(float x, uint32_t index) {
+  return static_cast<uint64_t>(order_of(x)) << 32 | (0xFFFFFFFFu - index);
+}
+__device__ inline float value_of(uint64_t key) { return value_of(static_cast<uint32_t>(key >> 32)); }
 __device__ inline int index_of(uint64_t key) {
   return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(key));
 }
@@ -161,24 +164,60 @@ __device__ inline float wave_sum(float x) {
   x += dpp<kHalfMirror>(x);
   return sum_x16_x32(x + dpp<kRor8>(x));
 }
-// How many of n keys are larger than `mine`.
-__device__ inline int rank_of(uint64_t mine, const uint64_t* keys, int n) {
-  int r = 0, i = 0;
-  for (; i + 8 <= n; i += 8) {
+// The sum over 8 neighbouring lanes.
+__device__ inline int sum8(int x) {
+  x += __builtin_amdgcn_update_dpp(x, x, kXor1, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(x, x, kXor2, 0xF, 0xF, false);
+  return x + __builtin_amdgcn_update_dpp(x, x, kHalfMirror, 0xF, 0xF, false);
+}
+// Calls f(rank, key) for each of n keys, 8 lanes to a key, with how many keys are larger; in one lane
+// of the 8. The array goes on for 31 more.
+template <typename F>
+__device__ inline void rank_all(const uint64_t* keys, int n, F f) {
+  const int part = threadIdx.x & 7;
+  for (int q = threadIdx.x >> 3; q - static_cast<int>(threadIdx.x >> 3) < n; q += kThreads / 8) {
+    const uint64_t mine = keys[min(q, n - 1)];
+    int r = 0;
+    for (int i = part; i < n; i += 32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r += keys[i + j] > mine;
+      for (int j = 0; j < 32; j += 8) r += keys[i + j] > mine && i + j < n;
+    }
+    r = sum8(r);
+    if (part == 0 && q < n) f(r, mine);
   }
-  for (; i < n; ++i) r += keys[i] > mine;
-  return r;
+}
+// Puts the kCount keys of each lane that `in` names behind those in the list.
+template <int kCount>
+__device__ inline void append(const uint64_t (&key)[kCount], const bool (&in)[kCount], uint64_t* list,
+                              int* n) {
+  uint64_t who[kCount];
+  int all = 0;
+#pragma unroll
+  for (int e = 0; e < kCount; ++e) {
+    who[e] = __ballot(in[e]);
+    all += __popcll(who[e]);
+  }
+  if (all == 0) return;  // the whole wave
+  int at = 0;
+  if ((threadIdx.x & 63) == 0) at = atomicAdd(n, all);
+  at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+  for (int e = 0; e < kCount; ++e) {
+    const int before = __builtin_amdgcn_mbcnt_hi(
+        static_cast<uint32_t>(who[e] >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who[e]), 0));
+    if (in[e]) list[at + before] = key[e];
+    at += __popcll(who[e]);
+  }
 }
 
 struct Shared {
   union {
-    uint64_t keys[kMostKeys];  // candidates
+    uint64_t keys[kMostKeys + 32];  // candidates
     uint64_t first[kThreads];  // before them: threads' first largest entries
   };
-  uint64_t best[kScoreMostTop];
-  float run_max[64];
+  uint64_t best[kScoreMostTop], least;
+  uint32_t run_max[64];  // in order_of's numbers, the low bits a number of the run's own
+  float wave_max[kWaves];
   float sums[2][kWaves];
   float piece[2][kMostPieces];  // sums of the pieces of the thread that holds the largest entry
   float bound;
@@ -196,9 +235,10 @@ struct Shared {
 // Sums are kept against a reference r of the thread's, its maximum times scale as f32 rounds it, so that
 // a term's exponent is one fma (rounded once, whatever r is); what r is off by is taken back at the
 // end. Entries so large that this overflows take `plain`: a second pass over differences.
-template <typename T, bool kMask, bool kSmall>
+// early() is called while few other loads are on their way.
+template <typename T, bool kMask, bool kSmall, typename F>
 __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float scale, Shared& sh,
-                            float& m_out, float& s_out, float& t_out) {
+                            F early, float& m_out, float& s_out, float& t_out) {
   constexpr int kN = Piece<T>::kN, kTurns = (kSmall ? kSmallGroup : kGroup) / kN;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int pieces = (row.n + kN - 1) / kN;
@@ -285,22 +325,25 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   }
 
   // A bound at or below the k-th largest thread's maximum: that of 64 runs of threads.
-  const float run = max8(m);
+  // The 64 are told apart by their low bits; the bound has none of them, so it lies at or below.
+  const uint32_t run = (order_of(max8(m)) & ~63u) | (63u - (tid / kRun));
   if (tid % kRun == 0) sh.run_max[tid / kRun] = run;
+  const float wave_top = wave_max(m);
+  if (lane == 0) sh.wave_max[wave] = wave_top;
   if (tid == 0) sh.n_first = sh.n_chosen = sh.n_keys = 0;
+  early();
   __syncthreads();
-  const float mine = sh.run_max[lane];
-  const float m_all = wave_max(mine);
-  if (wave == 0) {
+  {
     int r = 0;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) {
-      const float other = __builtin_bit_cast(
-          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i));
-      r += other > mine || (other == mine && i < lane);
-    }
-    if (r == k - 1) sh.bound = mine;
+    for (int i = 0; i < kRun; ++i) r += sh.run_max[kRun * (tid % kRun) + i] > run;
+    r = sum8(r);
+    // Cut down, -infinity is a NaN.
+    if (tid % kRun == 0 && r == k - 1) sh.bound = fmaxf(value_of(run & ~63u), -INFINITY);
   }
+  float m_all = sh.wave_max[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, sh.wave_max[w]);
   const bool odd = !(m_all * scale > kLow && m_all * scale < -kLow);  // of all threads
   if (odd && m_all > -INFINITY) {
     // plain: the sums against the largest entry, from differences.
@@ -345,13 +388,17 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   // Entries at or above the bound, whatever their index..
   uint64_t least = key_of(bound == -INFINITY ? -FLT_MAX : bound, 0xFFFFFFFFu);
   if constexpr (kSmall) {
+    uint64_t key[kTurns * kN];
+    bool with[kTurns * kN];
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        key[u * kN + e] = key_of(v[u][e], index0 + index[u] + e);
+        with[u * kN + e] = v[u][e] > -INFINITY && v[u][e] >= bound;
+      }
+    append(key, with, sh.keys, &sh.n_keys);
     if (in) {
-#pragma unroll
-      for (int u = 0; u < kTurns; ++u)
-#pragma unroll
-        for (int e = 0; e < kN; ++e)
-          if (v[u][e] > -INFINITY && v[u][e] >= bound)
-            sh.keys[atomicAdd(&sh.n_keys, 1)] = key_of(v[u][e], index0 + index[u] + e);
       if (is_top && n_top == 1) {
         int equal = 0;
 #pragma unroll
@@ -379,13 +426,13 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
         sh.first_of[i] = is_top ? -1 - tid : tid;
       }
       __syncthreads();
-      if (tid < n_chosen) {
-        const int r = rank_of(sh.first[tid], sh.first, n_chosen);
-        if (r < k) {
-          sh.chosen[r] = sh.first_of[tid];
-          sh.best[r] = sh.first[tid];
-        }
-      }
+      rank_all(sh.first, n_chosen, [&](int r, uint64_t key) __attribute__((always_inline)) {
+        if (r < k) sh.best[r] = key;
+      });
+      __syncthreads();
+      if (tid < n_chosen)
+        for (int r = 0; r < min(n_chosen, k); ++r)
+          if (sh.best[r] == sh.first[tid]) sh.chosen[r] = sh.first_of[tid];
       __syncthreads();
       least = n_chosen > k ? sh.best[k - 1] : 0;
       n_chosen = min(n_chosen, k);
@@ -428,11 +475,9 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   __syncthreads();
   const int n_keys = sh.n_keys;
   if (tid < k && tid >= n_keys) sh.best[tid] = 0;
-  for (int i = tid; i < n_keys; i += kThreads) {
-    const uint64_t key = sh.keys[i];
-    const int r = rank_of(key, sh.keys, n_keys);
+  rank_all(sh.keys, n_keys, [&](int r, uint64_t key) __attribute__((always_inline)) {
     if (r < k) sh.best[r] = key;
-  }
+  });
   s = t = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
@@ -468,7 +513,11 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
   const Row<T, kMask> row = {x + i0, kMask ? ok + i0 : nullptr, min(a.chunk, a.n_vocab - i0)};
   const int k = max(a.top_k, 1);
   float m, s, t;  // of the allowed entries; s and t without the largest entry
-  scan<T, kMask, kSmall>(row, i0, k, a.scale_log2, sh, m, s, t);
+  float given = -INFINITY;  // the token's logit
+  scan<T, kMask, kSmall>(row, i0, k, a.scale_log2, sh, [&]() __attribute__((always_inline)) {
+    if (tid == 0 && a.logprobs && token >= 0 && token < a.n_vocab && (!kMask || ok[token]))
+      given = value(x[token]);
+  }, m, s, t);
   if (a.n_chunks > 1) {
     float* const part = a.part + (r * a.n_chunks + blockIdx.x) * kScorePart;
     if (tid == 0) {
@@ -499,19 +548,38 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
       sc = ld_agent(p + 1);
       tc = ld_agent(p + 2);
     }
-    for (int i = tid; i < n; i += kThreads) {
-      const int from = i / k, j = i - from * k;
-      sh.keys[i] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(all + from * kScorePart + 4) + j,
-                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The k best are at or above the largest of the chunks' k-th ones, as few others are.
+    if (tid == 0) {
+      sh.n_keys = 0;
+      sh.least = 0;
     }
     if (tid < k) sh.best[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kThreads) {
-      const uint64_t key = sh.keys[i];
-      if (key == 0) continue;
-      const int p = rank_of(key, sh.keys, n);
-      if (p < k) sh.best[p] = key;
+    constexpr int kMine = (kScoreMostTop * kScoreMostChunks + kThreads - 1) / kThreads;
+    uint64_t mine[kMine];
+#pragma unroll
+    for (int q = 0; q < kMine; ++q) {
+      const int i = q * kThreads + tid, from = i / k, j = i - from * k;
+      mine[q] = 0;
+      if (i < n) {
+        mine[q] = __hip_atomic_load(
+            reinterpret_cast<const uint64_t*>(all + from * kScorePart + 4) + j, __ATOMIC_RELAXED,
+            __HIP_MEMORY_SCOPE_AGENT);
+        if (j == k - 1 && mine[q])
+          atomicMax(reinterpret_cast<unsigned long long*>(&sh.least), mine[q]);
+      }
     }
+    __syncthreads();
+    const uint64_t least = sh.least;
+    bool with[kMine];
+#pragma unroll
+    for (int q = 0; q < kMine; ++q) with[q] = mine[q] && mine[q] >= least;
+    append(mine, with, sh.keys, &sh.n_keys);
+    __syncthreads();
+    const int n_keys = sh.n_keys;
+    rank_all(sh.keys, n_keys, [&](int p, uint64_t key) __attribute__((always_inline)) {
+      if (p < k) sh.best[p] = key;
+    });
     __syncthreads();
     // The chunk that holds the largest entry leaves its 1 out.
     const int home = sh.best[0] ? index_of(sh.best[0]) / a.chunk : -1;
@@ -539,10 +607,7 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
     if (a.top_ids) a.top_ids[o] = key ? index_of(key) : -1;
     if (a.top_logprobs) a.top_logprobs[o] = key ? logprob(value_of(key)) : odd ? NAN : -INFINITY;
   }
-  if (tid == 0 && a.logprobs) {
-    const bool is_entry = token >= 0 && token < a.n_vocab && (!kMask || ok[token]);
-    a.logprobs[r] = logprob(is_entry ? value(x[token]) : -INFINITY);
-  }
+  if (tid == 0 && a.logprobs) a.logprobs[r] = logprob(given);
   if (tid == 64 && a.entropy)
     a.entropy[r] = odd ? NAN : none ? 0.f : ln_s - t * 0.6931471805599453f / (1.f + s);
 }
