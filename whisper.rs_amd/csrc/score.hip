@@ -6,14 +6,20 @@
 //   A row is read once: every thread keeps the maximum of its entries (and which group of 16 held it
 //   first) and its sums relative to that maximum. The k largest entries then lie in the k threads
 //   whose maxima are the k largest under the same order (value, then index): a bound from 64 maxima of
-//   neighbouring threads leaves few threads, these look their group up again for the index, and the
-//   entries of the k chosen ones, a few hundred bytes each, are read again, an entry at or above the
-//   k-th chosen maximum being one of at most k * (entries of a thread) candidates. Nothing else depends
-//   on values, so equal logits cost what others do.
+//   neighbouring threads leaves few threads, and the entries of the chosen ones, a few hundred bytes
+//   each, are read again (where the bound leaves many, after the index of their largest entry has
+//   left k of them). Nothing else depends on values, so equal logits cost what others do.
 //   s is kept without the largest entry's 1 (its thread's entries are summed again, a piece a thread),
 //   and ln s = log1p of it: a token of probability 1 - 1e-7 has its log probability to 2^-22 too.
 //   Few rows split over several workgroups, which merge through memory (the last to count in joins
-//   the parts in order; sums and order do not depend on which it is).
+//   the parts in order; sums and order do not depend on which it is). Chunks of at most kScoreSmall
+//   entries stay in registers.
+//   Bound: many rows by what a wave issues for an entry (exponent, sum, entropy: 4 instructions and a
+//   half, one of them v_exp_f32) next to the bytes: 7168 rows of 51865 f16 (744 MB) 158 us, 4.7 TB/s,
+//   f32 rows of the same bytes 132 us, 5.6; prefetch of 2 or 3 groups is no faster (163 and 171 us).
+//   Rows of less than a workgroup a CU by latency: of the 8.9 us of 5 masked rows of 51866 f32 (13 chunks
+//   of 5 rows), 0.5 are the logits, 3.5 bound, candidates and their order, 2.3 the parts' way through
+//   memory, 1.9 the merge's candidates and 0.9 the results.
 #include "wrs_internal.hpp"
 
 #include <algorithm>
@@ -215,7 +221,8 @@ struct Shared {
     uint64_t keys[kMostKeys + 32];  // candidates
     uint64_t first[kThreads];  // before them: threads' first largest entries
   };
-  uint64_t best[kScoreMostTop], least;
+  uint64_t best[kScoreMostTop];
+  uint32_t least;
   uint32_t run_max[64];  // in order_of's numbers, the low bits a number of the run's own
   float wave_max[kWaves];
   float sums[2][kWaves];
@@ -361,19 +368,7 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
         }
       }
   }
-  __syncthreads();
-  const float bound = sh.bound;
-  const bool in = m > -INFINITY && m >= bound, is_top = in && m == m_all;
-  {
-    const uint64_t tops = __ballot(is_top);
-    if (lane == 0) sh.tops[wave] = __popcll(tops);
-  }
-  if (!kSmall && in) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = is_top ? -1 - tid : tid;
-  __syncthreads();
-  int n_top = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) n_top += sh.tops[w];
-  float ps = 0.f, pt = 0.f;  // a small chunk: of the thread that alone holds the largest entry
+  const bool is_top = m > -INFINITY && m == m_all;
   // A piece's terms without the entries that equal the largest, which are counted.
   auto others = [&](const float (&x)[kN], float& a, float& b, int& n) __attribute__((always_inline)) {
 #pragma unroll
@@ -384,10 +379,40 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
       b = __builtin_fmaf(fmaxf(z, kLow), w, b);
     }
   };
+  // A thread's sums s and t, against m_all.
+  auto joined = [&](float& a, float& b) __attribute__((always_inline)) {
+    const float r_all = odd ? 0.f : m_all * scale;
+    // scale m_all - r_all, which the sums lie too high by
+    const float off = odd ? 0.f : __builtin_fmaf(m_all, scale, -r_all);
+    const float d = fmaxf(ref - r_all - off, kLow), w0 = __builtin_amdgcn_exp2f(d);
+    a = w0 * s;
+    b = w0 * __builtin_fmaf(d, s, t);
+  };
+  auto add_up = [&](float a, float b) __attribute__((always_inline)) {
+    const float ws = wave_sum(a), wt = wave_sum(b);
+    if (lane == 0) {
+      sh.sums[0][wave] = ws;
+      sh.sums[1][wave] = wt;
+    }
+  };
+  int n_top = 0;
   const int per = groups * kTurns;  // pieces of a thread
-  // Entries at or above the bound, whatever their index..
-  uint64_t least = key_of(bound == -INFINITY ? -FLT_MAX : bound, 0xFFFFFFFFu);
   if constexpr (kSmall) {
+    // Threads that hold the largest entry leave out all that equal it, and count them.
+    float a, b;
+    int equal = 0;
+    joined(a, b);
+    if (is_top) {
+      a = b = 0.f;
+#pragma unroll
+      for (int u = 0; u < kTurns; ++u) others(v[u], a, b, equal);
+    }
+    add_up(a, b);
+    int of_wave = 0;
+    if (__any(is_top)) of_wave = static_cast<int>(wave_sum(static_cast<float>(equal)));
+    if (lane == 0) sh.tops[wave] = of_wave;
+    __syncthreads();
+    const float bound = sh.bound;
     uint64_t key[kTurns * kN];
     bool with[kTurns * kN];
 #pragma unroll
@@ -398,15 +423,18 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
         with[u * kN + e] = v[u][e] > -INFINITY && v[u][e] >= bound;
       }
     append(key, with, sh.keys, &sh.n_keys);
-    if (in) {
-      if (is_top && n_top == 1) {
-        int equal = 0;
-#pragma unroll
-        for (int u = 0; u < kTurns; ++u) others(v[u], ps, pt, equal);
-        ps += static_cast<float>(equal - 1);
-      }
-    }
   } else {
+    const int of_wave = __popcll(__ballot(is_top));
+    if (lane == 0) sh.tops[wave] = of_wave;
+    __syncthreads();
+    const float bound = sh.bound;
+    const bool in = m > -INFINITY && m >= bound;
+    if (in) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = is_top ? -1 - tid : tid;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) n_top += sh.tops[w];
+    // Entries at or above the bound, whatever their index..
+    uint64_t least = key_of(bound == -INFINITY ? -FLT_MAX : bound, 0xFFFFFFFFu);
     int n_chosen = sh.n_chosen;
     if (n_chosen * per * kN > kMostKeys) {
       // .. or, where that could be too many, those of the k threads whose first largest entries are the
@@ -457,20 +485,11 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
         sh.equals[q] = equal;
       }
     }
-  }
-  // The threads' sums, against m_all: without the one that alone holds it, whose pieces follow.
-  {
-    const float r_all = odd ? 0.f : m_all * scale;
-    // scale m_all - r_all, which the sums lie too high by
-    const float off = odd ? 0.f : __builtin_fmaf(m_all, scale, -r_all);
-    const float d = fmaxf(ref - r_all - off, kLow), w0 = __builtin_amdgcn_exp2f(d);
+    // The threads' sums, without the one that alone holds the largest entry, whose pieces follow.
+    float a, b;
+    joined(a, b);
     const bool apart = is_top && n_top == 1;
-    const float ws = wave_sum(apart ? ps : w0 * s);
-    const float wt = wave_sum(apart ? pt : w0 * __builtin_fmaf(d, s, t));
-    if (lane == 0) {
-      sh.sums[0][wave] = ws;
-      sh.sums[1][wave] = wt;
-    }
+    add_up(apart ? 0.f : a, apart ? 0.f : b);
   }
   __syncthreads();
   const int n_keys = sh.n_keys;
@@ -484,8 +503,11 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
     s += sh.sums[0][w];
     t += sh.sums[1][w];
   }
-  if (kSmall && n_top == 1) {
-    // It is left out already.
+  if constexpr (kSmall) {
+    int equal = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) equal += sh.tops[w];
+    s += static_cast<float>(max(equal - 1, 0));
   } else if (n_top == 1) {
     const bool mine_too = lane < per;
     s += wave_sum(mine_too ? sh.piece[0][lane] : 0.f) +
@@ -513,10 +535,14 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
   const Row<T, kMask> row = {x + i0, kMask ? ok + i0 : nullptr, min(a.chunk, a.n_vocab - i0)};
   const int k = max(a.top_k, 1);
   float m, s, t;  // of the allowed entries; s and t without the largest entry
-  float given = -INFINITY;  // the token's logit
+  float given = 0.f;  // the token's logit
+  uint8_t given_ok = 1;
   scan<T, kMask, kSmall>(row, i0, k, a.scale_log2, sh, [&]() __attribute__((always_inline)) {
-    if (tid == 0 && a.logprobs && token >= 0 && token < a.n_vocab && (!kMask || ok[token]))
-      given = value(x[token]);
+    if (tid == 0 && a.logprobs) {
+      const int at = min(max(token, 0), a.n_vocab - 1);
+      given = value(x[at]);
+      if (kMask) given_ok = ok[at];
+    }
   }, m, s, t);
   if (a.n_chunks > 1) {
     float* const part = a.part + (r * a.n_chunks + blockIdx.x) * kScorePart;
@@ -538,9 +564,8 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
     __syncthreads();
     if (!sh.last) return;
     const float* const all = a.part + r * a.n_chunks * kScorePart;
-    const int n = a.n_chunks * k;
-    // The chunks' sums, a chunk a lane, and their best entries.
-    const int c = tid & 63;
+    // A chunk a lane: their sums, and the best entries j = wave, wave + 8, .. of each.
+    const int c = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     float mc = -INFINITY, sc = 0.f, tc = 0.f;
     if (c < a.n_chunks) {
       const float* const p = all + c * kScorePart;
@@ -548,32 +573,29 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
       sc = ld_agent(p + 1);
       tc = ld_agent(p + 2);
     }
-    // The k best are at or above the largest of the chunks' k-th ones, as few others are.
-    if (tid == 0) {
-      sh.n_keys = 0;
-      sh.least = 0;
-    }
-    if (tid < k) sh.best[tid] = 0;
-    __syncthreads();
-    constexpr int kMine = (kScoreMostTop * kScoreMostChunks + kThreads - 1) / kThreads;
-    uint64_t mine[kMine];
+    constexpr int kMine = (kScoreMostTop + kWaves - 1) / kWaves;
+    uint64_t mine[kMine] = {};
 #pragma unroll
     for (int q = 0; q < kMine; ++q) {
-      const int i = q * kThreads + tid, from = i / k, j = i - from * k;
-      mine[q] = 0;
-      if (i < n) {
-        mine[q] = __hip_atomic_load(
-            reinterpret_cast<const uint64_t*>(all + from * kScorePart + 4) + j, __ATOMIC_RELAXED,
-            __HIP_MEMORY_SCOPE_AGENT);
-        if (j == k - 1 && mine[q])
-          atomicMax(reinterpret_cast<unsigned long long*>(&sh.least), mine[q]);
-      }
+      const int j = wave + kWaves * q;
+      if (j < k && c < a.n_chunks)
+        mine[q] = __hip_atomic_load(reinterpret_cast<const uint64_t*>(all + c * kScorePart + 4) + j,
+                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
+    if (tid == 0) sh.n_keys = sh.least = 0;
+    if (tid < k) sh.best[tid] = 0;
     __syncthreads();
-    const uint64_t least = sh.least;
+    // The k best are at or above the largest of the chunks' k-th ones.
+#pragma unroll
+    for (int q = 0; q < kMine; ++q)
+      if (wave + kWaves * q == k - 1 && mine[q])
+        atomicMax(&sh.least, static_cast<uint32_t>(mine[q] >> 32));
+    __syncthreads();
+    const uint32_t least = sh.least;
     bool with[kMine];
 #pragma unroll
-    for (int q = 0; q < kMine; ++q) with[q] = mine[q] && mine[q] >= least;
+    for (int q = 0; q < kMine; ++q)
+      with[q] = mine[q] && static_cast<uint32_t>(mine[q] >> 32) >= least;
     append(mine, with, sh.keys, &sh.n_keys);
     __syncthreads();
     const int n_keys = sh.n_keys;
@@ -607,7 +629,10 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
     if (a.top_ids) a.top_ids[o] = key ? index_of(key) : -1;
     if (a.top_logprobs) a.top_logprobs[o] = key ? logprob(value_of(key)) : odd ? NAN : -INFINITY;
   }
-  if (tid == 0 && a.logprobs) a.logprobs[r] = logprob(given);
+  if (tid == 0 && a.logprobs) {
+    const bool is_entry = token >= 0 && token < a.n_vocab && given_ok != 0;
+    a.logprobs[r] = logprob(is_entry ? given : -INFINITY);
+  }
   if (tid == 64 && a.entropy)
     a.entropy[r] = odd ? NAN : none ? 0.f : ln_s - t * 0.6931471805599453f / (1.f + s);
 }
@@ -615,7 +640,8 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
 }  // namespace
 
 void score_plan(ScoreArgs& a, bool split) {
-  // Rows that fill the GPU are taken whole.
+  // A workgroup a CU and no more: f32 rows of 51865 entries, a workgroup a row, up to 256 and up to
+  // 520 workgroups: 16 rows 9.0, 8.1, 8.2 us, 40 rows 9.8, 9.4, 11.1 us, 130 rows 11.2, 11.2, 15.9 us.
   int64_t chunks = 1;
   if (split) chunks = std::max<int64_t>(1, kScoreMaxWgs / std::max<int64_t>(a.n_rows, 1));
   chunks = std::min<int64_t>(chunks, (a.n_vocab + kScoreSmall - 1) / kScoreSmall);

@@ -326,7 +326,7 @@ hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipS
 constexpr int kScoreMostTop = 32;
 constexpr int kScoreChunk = 65536;   // entries of one workgroup, at most
 constexpr int kScoreSmall = 4096;    // entries of a workgroup that keeps them in registers, at most
-constexpr int kScoreMaxWgs = 128;    // of a launch that splits rows which fit a workgroup
+constexpr int kScoreMaxWgs = 256;    // of a launch that splits rows which fit a workgroup
 constexpr int kScoreMostChunks = 64;  // of a row
 constexpr int kScorePart = 4 + 2 * kScoreMostTop;  // floats: m, s, t, and the best entries' keys
 struct ScoreArgs {
