@@ -105,9 +105,11 @@ const char *wrs_attn_status_string(int status);
  * idle, which split k through another fixed buffer (~8 MB on 256 CUs) under the same
  * rule;
  * and fused norms of decode rows over many features (wrs_linear_fused), likewise
- * (reserving linear_tokens allocates both). Tree attention splits long caches through
- * a third one (~4 MB, which reserving heads with decode rows and keys allocates too)
- * and, captured before it exists, runs unsplit. Switching streams
+ * (reserving linear_tokens allocates both). Tree and window attention, every attention
+ * over 8-bit arenas and token scores split long keys and rows through a third one (~4 MB,
+ * which reserving heads with decode rows and keys allocates too) and, captured before it
+ * exists, run unsplit. wrs_kv_set_cross_proj into an 8-bit arena takes f32 rows of a layer
+ * that its first call outside capture allocates. Switching streams
  * (wrs_attn_set_stream) drains the old stream unless either stream is
  * recording a graph. Zero fields are ignored; reserving never shrinks.
  * Synchronous. */
@@ -201,9 +203,11 @@ int wrs_attn_prefill(wrs_attn_ctx *ctx, int q_dtype, const void *q, const wrs_la
  * largest (of each head), and rows with an infinity or NaN read as NaN. A row has a
  * scale to itself, so storing, moving, cutting and sliding rows never rounds
  * another one, and rows that were read back store as the same codes. Attention runs on
- * the codes (q split in two f16 parts, weights in two bf16 parts: 2^-22 and 2^-18), the
- * cross calls with any 16-byte aligned q and any rows as on f16 arenas; a row of q
- * with an infinity or NaN gives NaN. Planes hold up to 2^24 - 4096 rows.
+ * the codes, q and the products of weight and value scale in two f16 parts each (2^-22,
+ * small ones within 2^-40 of the row's largest element and 2^-31 of its largest product, for
+ * values of 2^-80 and more and keys below 2^100), the cross calls with any 16-byte aligned q and any rows as
+ * on f16 arenas; a row of q with an infinity or NaN gives NaN. Planes hold up to
+ * 2^24 - 4096 rows.
  * wrs_attn_decode_cross_noalloc, the _lse pair, wrs_attn_capture_cross_heads and
  * wrs_attn_tree_self return WRS_EUNSUPPORTED on them. */
 
@@ -283,7 +287,8 @@ int wrs_kv_read_cross(wrs_kv *kv, size_t layer, size_t first, size_t n, float *k
  * layer, decoder.rs:136-139); 0 after wrs_kv_invalidate_cross. */
 int wrs_kv_cross_len(wrs_kv *kv, size_t layer, size_t *n_audio);
 /* Raw device pointers of the arena planes (for tests and fused callers);
- * elements are of the arena's dtype, the slot stride in elements. */
+ * elements are of the arena's dtype, the slot stride in elements. 8-bit arenas give their
+ * codes (stored plus 128); what they stand for is what wrs_kv_read_rows gives. */
 int wrs_kv_self_planes(wrs_kv *kv, void **k, void **v, size_t *slot_stride_elems);
 int wrs_kv_cross_planes(wrs_kv *kv, void **k, void **v);
 
@@ -356,11 +361,11 @@ int wrs_attn_tree_self(wrs_attn_ctx *ctx, wrs_kv *kv, size_t layer, const size_t
  * and sees the keys up to its own that are among the first `sinks` or among the last `window`
  * (p - window < key <= p; window >= 1, SIZE_MAX: every key). Keys that no row of a block sees are
  * not read. Rows of q and out ([sum of counts][d_model] f32, device) lie q_row_stride and
- * out_row_stride elements apart; q_len and out_len are the buffers' lengths in elements. Values of
- * keys that a row does not see never reach it, infinities and NaN among them; a row whose visible
+ * out_row_stride elements apart (out may be q itself); q_len and out_len are the buffers' lengths
+ * in elements. A slot may come twice. Values of keys that a row does not see never reach it, infinities and NaN among them; a row whose visible
  * scores are all -infinity is zero, and one with a NaN among them NaN. Any arena, up to
- * 2^24 - 4096 keys; f16 arenas take q and the weights in two f16 parts (2^-22 down to 2^-28 of the
- * row's largest), f32 ones whole, 8-bit ones as above. Slots, counts and lengths are read
+ * 2^24 - 4096 keys; f16 arenas take q and the weights in two f16 parts (2^-22, small ones
+ * within 2^-40 and 2^-31 of the row's largest), f32 ones whole, 8-bit ones as above. Slots, counts and lengths are read
  * when the call is made: a replayed graph keeps them. Long keys of few rows split over
  * workgroups through the buffer of tree attention. No reference counterpart: its decoder
  * sees the whole cache and drops the oldest tokens (decoder.rs:248-263). */

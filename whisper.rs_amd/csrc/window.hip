@@ -268,7 +268,7 @@ __device__ inline void split_weights(float x0, float x1, uint32_t (&out)[2]) {
 //   so that the sums are scaled only where a score passes that (for a row's first step and hardly
 //   ever after), and times a unit 2^u, which the quotient at the end drops. 8-bit values have powers of
 //   two, which go to the weights; the largest product of the two sets the unit, so that rows of
-//   any scale meet in one sum (values above 2^-90).
+//   any scale meet in one sum (values of 2^-80 and more to 2^-22 of the largest product).
 constexpr float kRoom = 8.f;
 constexpr float kUnit = 7.f;      // f16 planes: weights below 2^15
 constexpr float kMostUnit = 87.f;  // 8-bit planes: 2^24 weights of 2^kRoom stay below f32's largest
