@@ -233,11 +233,14 @@ __device__ inline float scale_at(uint32_t w, int i) {
 }
 
 // The values' operand of columns 16 dt.. from 32 rows of V in LDS: lane (c, g) gets column 16 dt + c of
-// keys 4 g + 0..3 and 16 + 4 g + 0..3, the order that the packed weights have. Rows r and r + 16 swizzle
-// alike.
+// keys 4 g + 0..3 and 16 + 4 g + 0..3, the order that the packed weights have. Chunk c of 16 bytes of row r
+// sits at c ^ vswz(r): four rows' pairs of chunks, and two rows' chunks of one parity (which a wave
+// stores together from 8-bit codes: with rows of one parity 32 of 100 LDS cycles a step were conflicts),
+// hit distinct banks. Rows r and r + 16 swizzle alike.
+__device__ inline int vswz(int r) { return (2 * (r & 3)) | (r & 1); }
 __device__ inline int value_offset(int dt, int c, int g) {
   const int row = 4 * g + (c >> 2);
-  return row * 128 + (((2 * dt + ((c & 3) >> 1)) ^ swz(row)) * 16) + 8 * (c & 1);
+  return row * 128 + (((2 * dt + ((c & 3) >> 1)) ^ vswz(row)) * 16) + 8 * (c & 1);
 }
 __device__ inline u32x4 value_operand(const char* v) {
   const u32x2 a = read_tr(v), b = read_tr(v + 2048);
@@ -511,10 +514,10 @@ __device__ inline bool attend_16(const Block& b, const f32x4 (&qx)[4], int pos,
         codes_f16(vx[i], y);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          *reinterpret_cast<u32x4*>(vw + row * 128 + (((2 * (lane & 3) + e) ^ swz(row)) * 16)) = y[e];
+          *reinterpret_cast<u32x4*>(vw + row * 128 + (((2 * (lane & 3) + e) ^ vswz(row)) * 16)) = y[e];
       } else {
         const int row = 8 * i + (lane >> 3);
-        *reinterpret_cast<u32x4*>(vw + row * 128 + (((lane & 7) ^ swz(row)) * 16)) = vx[i];
+        *reinterpret_cast<u32x4*>(vw + row * 128 + (((lane & 7) ^ vswz(row)) * 16)) = vx[i];
       }
     }
     wave_sync();
@@ -799,15 +802,15 @@ __global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs a) {
       put(kt[buf], row, chunk, kswz(row), y[0]);
       put(kt[buf], row, chunk + 1, kswz(row), y[1]);
       codes_f16(vx[0], y);
-      put(vt[buf], row, chunk, swz(row & 31), y[0]);
-      put(vt[buf], row, chunk + 1, swz(row & 31), y[1]);
+      put(vt[buf], row, chunk, vswz(row), y[0]);
+      put(vt[buf], row, chunk + 1, vswz(row), y[1]);
       if (tid < 2 * kTile) st[buf][tid >= kTile][tid & (kTile - 1)] = scale_at(sx, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
         const int row = 32 * i + (tid >> 3), chunk = tid & 7;
         put(kt[buf], row, chunk, kswz(row), kx[i]);
-        put(vt[buf], row, chunk, swz(row & 31), vx[i]);
+        put(vt[buf], row, chunk, vswz(row), vx[i]);
       }
     }
   };
