@@ -177,6 +177,23 @@ def fill(wrs, ctx, layers, slots, heads, rows, max_ctx, seed=0):
     return ar, data
 
 
+def test_rows_from_the_host(wrs, ctx):
+    heads, n = 2, 37
+    ar = wrs.KvArena(2, 2, heads, 40, 40, ctx=ctx, dtype=wrs.WRS_I8)
+    k, v = normal(n, heads * D, seed=61), normal(n, heads * D, seed=62)
+    note("rows from the host")
+    ar.append(1, 1, k.cpu().numpy(), v.cpu().numpy())
+    ar.advance(1, n)
+    ar.set_cross(1, v.cpu().numpy(), k.cpu().numpy())
+    gk, gv = torch.zeros_like(k), torch.zeros_like(v)
+    ar.read_rows(1, [1], [0], [n], gk, gv)
+    ck, cv = torch.zeros_like(k), torch.zeros_like(v)
+    ar.read_cross(1, 0, ck, cv)
+    torch.cuda.synchronize()
+    assert same(gk, stored(k, "i8")) and same(gv, stored(v, "i8"))
+    assert same(ck, stored(v, "i8")) and same(cv, stored(k, "i8"))
+
+
 @pytest.mark.parametrize("rows", [1, 63, 257, 600])
 def test_copy_slot_8_bit(wrs, ctx, rows):
     ar, data = fill(wrs, ctx, 2, 3, 2, rows, 601)

@@ -110,6 +110,12 @@ def test_rows_longer_than_a_workgroup_takes(wrs, ctx, n, v):
     check(wrs, ctx, x, some_tokens(n, v, 2), 9)
 
 
+def test_more_rows_than_a_grid_is_wide(wrs, ctx):
+    note("70001 rows")
+    x = logits_of(70001, 33, "f16", seed=3)
+    check(wrs, ctx, x, some_tokens(70001, 33, 4), 3)
+
+
 @pytest.mark.parametrize("temperature", [0.2, 0.4, 0.7, 1.0, 3.0, 1e-6, 1e6])
 def test_temperature(wrs, ctx, temperature):
     note(f"temperature {temperature}")

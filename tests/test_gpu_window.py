@@ -414,6 +414,24 @@ def test_cross_rows_8_bit(wrs, ctx, rows, frames):
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("frames", [1, 64, 100])
+def test_many_cross_rows_8_bit(wrs, ctx, frames):
+    """Tiles whose rows all see every key."""
+    heads, rows = 16, 2600
+    d = heads * D
+    ar = wrs.KvArena(1, 1, heads, 8, 100, ctx=ctx, dtype=wrs.WRS_I8)
+    k, v = normal(frames, d, seed=46), normal(frames, d, seed=47)
+    ar.set_cross(0, k, v)
+    q, out = normal(rows, d, seed=48), torch.zeros(rows, d, device="cuda")
+    note(f"many cross rows {frames}")
+    ar.prefill_cross(0, q, out)
+    torch.cuda.synchronize()
+    kk, vv = stored(k, "i8"), stored(v, "i8")
+    hide = torch.zeros(rows, frames, dtype=torch.bool, device="cuda")
+    want, worst = attend64(q, kk, vv, hide)
+    assert (out.double() - want).abs().max().item() <= tolerance("i8", worst, vv, frames)
+
+
 @pytest.mark.parametrize("past", [0, 1, 31, 223, 600, 4000])
 def test_self_rows_8_bit(wrs, ctx, past):
     note(f"self i8 {past}")
