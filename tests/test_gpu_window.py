@@ -169,6 +169,9 @@ CASES = [
     (2, [5003], [19], 2048, 16),
     (1, [9000], [2], 9001, 0),
     (2, [2900, 2897, 2894], [33, 28, 30], 448, 1),
+    (4, [6000, 5000, 4100], [3, 1, 17], 5000, 4),
+    (4, [8000, 10, 0], [1, 40, 9], 5000, 4),
+    (2, [4000] * 9 + [30], [1] * 9 + [200], 3000, 5),
 ]
 
 
@@ -344,7 +347,7 @@ def test_errors_do_not_add_up(wrs, ctx, name, past, rows, window):
 @pytest.mark.parametrize("window,sinks", [(200, 5), (10 ** 6, 0), (33, 130)])
 def test_many_rows(wrs, ctx, name, window, sinks):
     """Enough rows for tiles, sequences of a few rows among them."""
-    rows = 1030 if name == "f16" else 2600  # 256 and 640 blocks of 64 rows and more
+    rows = 1500 if name == "f16" else 3300
     note(f"many rows {name} {window}")
     Session(wrs, ctx, name, 16, [37, 300, 0, 513], [rows, 3, 0, 70], seed=41).check(window, sinks)
 

@@ -562,6 +562,25 @@ __device__ inline void load_rows(const WindowArgs& a, int t, int h, int r0, int 
   }
 }
 
+// The workgroup's sequence, and which of the sequence's workgroups it is. There is none without one:
+// with a grid as wide as the widest sequence the dispatcher put the others' workgroups on few CUs
+// (16 single tokens over 8192 keys and a text of 256 rows, 20 heads, f16: 533 us, now 141).
+__device__ inline int sequence_of(const WindowArgs& a, int& lid) {
+  lid = a.remap ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
+  if (a.n_seqs == 1) return 0;
+  if (a.like) {
+    return divide(lid, a.n_wgs[0], a.wgs_inv, lid);
+  }
+  // Those past the last sequence start past every workgroup.
+  int t = -1;
+  for (int i = 0; i < a.n_seqs; i += 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t += a.wg0[i + j] <= lid;
+  }
+  lid -= a.wg0[t];
+  return t;
+}
+
 // The square root of what sums against `m` weigh against `all` (at or above it): a sum whose weight is
 // past f32's range may still count, where its values are as much larger.
 __device__ inline float half_weight(float m, float all) {
@@ -576,15 +595,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void window_attend(WindowArgs a) {
   __shared__ float ml[kWaves][2][kRows];  // and their max and sum
   __shared__ int last_flag;
 
-  // Chunks: the workgroups of one head's keys, which read the same rows, share an XCD's L2 (a
-  // sequence's row of the grid is a multiple of the XCDs). Whole blocks: the last ones of all heads
-  // first, which have the most keys (1000 rows on each other, 20 heads, 8-bit: 17.7 us, 22.1 with
-  // the heads on an XCD each).
-  const int t = blockIdx.y;
+  // Chunks of one sequence or of like ones: the workgroups of one head's keys, which read the same rows,
+  // share an XCD's L2. Whole blocks: the last ones of all heads first, which have the most keys
+  // (1000 rows on each other, 20 heads, 8-bit: 17.7 us, 22.1 with the heads on an XCD each).
+  int lid;
+  const int t = sequence_of(a, lid);
   const int past = a.past[t], rows = a.rows[t];
   const int n_blk = a.n_blk[t], n_split = a.n_split[t];
-  const int lid = n_split > 1 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
-  if (lid >= a.n_wgs[t]) return;
   int blk, split = 0, h;
   if (n_split > 1) {
     const int hs = divide(lid, n_blk, a.blk_inv[t], blk);
@@ -751,9 +768,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs a) {
   constexpr DType kD = k8 ? kI8 : kF16;
   __shared__ __attribute__((aligned(128))) char kt[2][kTile * 128], vt[2][kTile * 128];
   __shared__ __attribute__((aligned(16))) float st[2][2][k8 ? kTile : 4];  // K's and V's powers of two
-  const int t = blockIdx.y;
-  const int lid = blockIdx.x;
-  if (lid >= a.n_wgs[t]) return;
+  int lid;
+  const int t = sequence_of(a, lid);
   const int past = a.past[t], rows = a.rows[t];
   int h;
   const int blk = a.n_blk[t] - 1 - divide(lid, a.n_heads, a.head_inv, h);
@@ -887,18 +903,31 @@ __global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs a) {
   }
 }
 
-// Rows of a block: tiles where they fill the GPU. Measured with 20 heads of rows on each other, tiles
-// against blocks of 16: f16 1000 rows (320 tiles) 19.3 us against 19.7, 4000 rows 99 against 183, 8
-// heads of 1500 rows (192 tiles) 23.4 against 17.8; 8-bit 1500 rows (480) 35 against 29, 2500 rows (800)
-// 60 against 66, 4000 rows 113 against 146. Calls of at most 32 rows a sequence would leave half a tile.
+// Rows of a block: 64 where their tiles of 64 keys, in whole blocks, come to 150 times the longest block's
+// own (8-bit planes, of which blocks of 16 rows read half the bytes: 400), so that no block runs on
+// alone. Measured, tiles against blocks of 16 at so many times: 20 heads of rows on each other, f16 1000
+// rows (170) 19.3 us against 19.7, 1500 (250) 26 against 34, 4000 (630) 99 against 183; 8 heads of 1500
+// rows (100) 23.4 against 17.8, 3500 (220) 54 against 61; 8-bit 1500 rows (250) 35 against 29, 2500 (410)
+// 60 against 66, 4000 (630) 107 against 146. A single token is 1/64 of a block: 39 of them over 8192 keys
+// with a text of 64 or 256 rows, 8-bit, 192 and 192 us against 179 and 168 (with 2000 rows 287 and 237; 16 of
+// them with 2000 rows, f16 (163) 172 us against 242, 8-bit (163) 208 and 153).
 int block_rows(const WindowArgs& a, DType dt) {
-  int64_t wide = 0;
-  int most = 0;
+  if (dt == kF32) return 16;
+  int64_t work = 0;
+  int longest = 1;
   for (int t = 0; t < a.n_seqs; ++t) {
-    most = std::max(most, a.rows[t]);
-    wide += static_cast<int64_t>((a.rows[t] + kTileRows - 1) / kTileRows) * a.n_heads;
+    auto steps = [&](int row0, int row1) {
+      const int p1 = a.past[t] - 1 + (a.causal ? row1 : 0);
+      return Span<kTile>(a.causal ? a.past[t] + row0 : p1, p1, a.window, a.sinks).n_steps;
+    };
+    const int rows = a.rows[t], part = std::min(rows, kTileRows);
+    const int last = steps(rows - part, rows);
+    work += static_cast<int64_t>(rows) * (steps(0, part) + last);
+    longest = std::max(longest, last);
   }
-  return dt != kF32 && wide >= (dt == kI8 ? 640 : 256) && most > 32 ? kTileRows : 16;
+  return work * a.n_heads / (2 * kTileRows) >= (dt == kI8 ? 400 : 150) * static_cast<int64_t>(longest)
+             ? kTileRows
+             : 16;
 }
 
 // Steps of the longest block of a sequence, at most.
@@ -914,16 +943,17 @@ int most_steps(const WindowArgs& a, int t, int rows) {
 int64_t window_plan(WindowArgs& a, DType dt, bool split) {
   const int rows = block_rows(a, dt);
   int steps[kWindowMaxSeqs], longest = 1;
+  int64_t work = 0;
   for (int t = 0; t < a.n_seqs; ++t) {
     a.n_blk[t] = (a.rows[t] + rows - 1) / rows;
     steps[t] = most_steps(a, t, rows);
     longest = std::max(longest, steps[t]);
+    work += static_cast<int64_t>(a.n_blk[t]) * a.n_heads * steps[t];
   }
   a.head_inv = inverse(a.n_heads);
-  int64_t widest = 0;
   auto lay = [&](int64_t chunk) {
     int64_t sum = 0;
-    widest = 0;
+    a.like = a.remap = 1;
     a.chunk = static_cast<int>(chunk);
     for (int t = 0; t < a.n_seqs; ++t) {
       a.n_split[t] = static_cast<int>((steps[t] + chunk - 1) / chunk);
@@ -933,9 +963,11 @@ int64_t window_plan(WindowArgs& a, DType dt, bool split) {
       const int64_t n = static_cast<int64_t>(a.n_blk[t]) * a.n_heads * a.n_split[t];
       a.n_wgs[t] = static_cast<int>(std::min<int64_t>(n, 0x7fffffff));
       sum += n;
-      widest = std::max(widest, n);
+      a.like &= a.n_wgs[t] == a.n_wgs[0];
+      a.remap &= a.n_split[t] > 1;
     }
-    widest = (widest + 7) / 8 * 8;
+    for (int t = a.n_seqs; t < kWindowMaxSeqs; ++t) a.wg0[t] = 0x7fffffff;
+    a.wgs_inv = inverse(a.n_wgs[0]);
     return sum;
   };
   int64_t chunk = longest;
@@ -945,12 +977,14 @@ int64_t window_plan(WindowArgs& a, DType dt, bool split) {
     const float alone = dt == kF32 ? 0.95f : 0.25f, each = dt == kF32 ? 0.95f : 0.45f;
     float best = 0.f;
     for (int n = 1; n <= 256; n += n < 4 ? 1 : n & (n - 1) ? n / 3 : n / 2) {
-      const int64_t c = ((longest + n - 1) / n + 3) / 4 * 4;
+      const int c = ((longest + n - 1) / n + kWaves - 1) / kWaves * kWaves;
       int64_t wgs = 0;
       for (int t = 0; t < a.n_seqs; ++t)
         wgs += static_cast<int64_t>(a.n_blk[t]) * a.n_heads * ((steps[t] + c - 1) / c);
       if (n > 1 && wgs > 2 * kTreeMaxWgs) break;  // what the scratch takes, of 16 rows
-      float us = static_cast<float>(c / 4) * (alone + each * static_cast<float>((wgs + 255) / 256));
+      const int64_t turn = static_cast<int64_t>(c) * 256;
+      float us = static_cast<float>(c / kWaves) *
+                 (alone + each * static_cast<float>(std::max<int64_t>((work + turn - 1) / turn, 1)));
       if (n > 1)
         us += 1.1f + 0.7f * static_cast<float>((n + kMergeLoads - 1) / kMergeLoads) +
               static_cast<float>(wgs) / 240.f;
@@ -960,14 +994,13 @@ int64_t window_plan(WindowArgs& a, DType dt, bool split) {
       }
     }
   }
-  lay(chunk);
-  return widest;
+  return lay(chunk);
 }
 
 hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipStream_t s) {
   if (wgs <= 0) return hipSuccess;
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
-  const dim3 grid(static_cast<unsigned>(wgs), a.n_seqs), block(64 * kWaves);
+  const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kWaves);
   const bool tiles = block_rows(a, dt) == kTileRows;
 #define WRS_WINDOW(K) hipLaunchKernelGGL(K, grid, block, 0, s, a)
   switch (dt) {

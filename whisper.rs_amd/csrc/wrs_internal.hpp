@@ -313,6 +313,9 @@ struct WindowArgs {
   // By window_plan, as TreeArgs has them; chunk counts steps.
   int n_wgs[kWindowMaxSeqs], wg0[kWindowMaxSeqs], n_blk[kWindowMaxSeqs], n_split[kWindowMaxSeqs];
   uint32_t blk_inv[kWindowMaxSeqs], split_inv[kWindowMaxSeqs], head_inv;
+  // Whether every sequence has n_wgs[0] workgroups, and whether those go to the XCDs by heads.
+  int like, remap;
+  uint32_t wgs_inv;
 };
 int64_t window_plan(WindowArgs& a, DType dt, bool split);
 hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipStream_t s);
