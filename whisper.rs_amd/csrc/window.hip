@@ -941,7 +941,7 @@ int most_steps(const WindowArgs& a, int t, int rows) {
 }  // namespace
 
 int64_t window_plan(WindowArgs& a, DType dt, bool split) {
-  const int rows = block_rows(a, dt);
+  const int rows = a.block_rows = block_rows(a, dt);
   int steps[kWindowMaxSeqs], longest = 1;
   int64_t work = 0;
   for (int t = 0; t < a.n_seqs; ++t) {
@@ -1001,7 +1001,7 @@ hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipS
   if (wgs <= 0) return hipSuccess;
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kWaves);
-  const bool tiles = block_rows(a, dt) == kTileRows;
+  const bool tiles = a.block_rows == kTileRows;
 #define WRS_WINDOW(K) hipLaunchKernelGGL(K, grid, block, 0, s, a)
   switch (dt) {
     case kF16:

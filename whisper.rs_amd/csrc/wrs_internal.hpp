@@ -296,7 +296,8 @@ hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStrea
 // (plane_rows rows of 64 f16, f32, or 8-bit codes with scale_rows scales). With `causal` row i stands
 // at position past[t] + i, otherwise every row at past[t] - 1, and sees the keys j up to it with
 // j > position - window or j < sinks. past + rows < 2^24 - 4095 and window <= 2^24. window_plan lays
-// out the launch as tree_plan does, with the same scratch.
+// out the launch and returns its workgroups; with `split` keys may be dealt over several of them,
+// through the scratch of tree attention.
 constexpr int kWindowMaxSeqs = 64;  // per launch
 struct WindowArgs {
   const float* q;
@@ -313,8 +314,9 @@ struct WindowArgs {
   // By window_plan, as TreeArgs has them; chunk counts steps.
   int n_wgs[kWindowMaxSeqs], wg0[kWindowMaxSeqs], n_blk[kWindowMaxSeqs], n_split[kWindowMaxSeqs];
   uint32_t blk_inv[kWindowMaxSeqs], split_inv[kWindowMaxSeqs], head_inv;
-  // Whether every sequence has n_wgs[0] workgroups, and whether those go to the XCDs by heads.
-  int like, remap;
+  // Rows of a block; whether every sequence has n_wgs[0] workgroups, and whether those go to the
+  // XCDs by heads.
+  int block_rows, like, remap;
   uint32_t wgs_inv;
 };
 int64_t window_plan(WindowArgs& a, DType dt, bool split);
