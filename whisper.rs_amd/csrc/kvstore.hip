@@ -86,8 +86,8 @@ constexpr int64_t kOnce = 128 << 20;  // bytes that are read past the caches
 // A workgroup takes 1024 pieces of 4 columns: the next ones of rows of all heads, or those of
 // kBlockRows rows of a head.
 enum class Order { kAllHeads, kByHead, kByHeadOnce };
-template <DType kD, bool kStore, Order kOrder>
-__global__ __launch_bounds__(256) void kv_rows(KvSlotRows a) {
+template <DType kD, bool kStore, Order kOrder, int kSlots>
+__global__ __launch_bounds__(256) void kv_rows(KvSlotRows<kSlots> a) {
   constexpr bool kByHead = kOrder != Order::kAllHeads;
   const int u = blockIdx.z, rows_here = a.count[u], sub = threadIdx.x >> 4;
   // The block's first row of a head and that head, or its first row in turn.
@@ -245,7 +245,8 @@ __global__ __launch_bounds__(64 * kKeepWaves) void kv8_keep_rows(KeepArgs<kSlots
 
 }  // namespace
 
-hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStream_t s) {
+template <int kSlots>
+hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store, hipStream_t s) {
   int most = 0;
   int64_t all = 0;
   for (int u = 0; u < a.n_slots; ++u) {
@@ -260,7 +261,7 @@ hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStr
                                  : (rows + kBlockRows - 1) / kBlockRows;
   const dim3 grid(static_cast<unsigned>(blocks), 2, a.n_slots);
 #define WRS_KV_ROWS_ONE(D, S, O) \
-  hipLaunchKernelGGL((kv_rows<D, S, Order::O>), grid, dim3(256), 0, s, a)
+  hipLaunchKernelGGL((kv_rows<D, S, Order::O, kSlots>), grid, dim3(256), 0, s, a)
 #define WRS_KV_ROWS(D)                                                        \
   if (!by_head) {                                                             \
     if (store) {                                                              \
@@ -285,6 +286,8 @@ hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStr
 #undef WRS_KV_ROWS_ONE
   return hipGetLastError();
 }
+template hipError_t launch_kv_slot_rows(const KvSlotRows<kRowSlots>&, DType, bool, hipStream_t);
+template hipError_t launch_kv_slot_rows(const KvSlotRows<kRowFewSlots>&, DType, bool, hipStream_t);
 
 hipError_t launch_kv8_copy(const Kv8Planes& to, const Kv8Planes& from, int n_layers, int n_heads,
                            int len, hipStream_t s) {

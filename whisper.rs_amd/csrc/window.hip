@@ -531,8 +531,8 @@ __device__ inline bool attend_16(const Block& b, const f32x4 (&qx)[4], int pos,
 
 // The head's planes: rows past the `keys` first read as zero (scales by whole words: their planes
 // are padded to 64).
-template <DType kD>
-__device__ inline void set_planes(const WindowArgs& a, int64_t plane, uint32_t keys, Block& b) {
+template <DType kD, int kSeqs>
+__device__ inline void set_planes(const WindowArgs<kSeqs>& a, int64_t plane, uint32_t keys, Block& b) {
   constexpr uint32_t kRowBytes = kD == kF32 ? 256 : kD == kF16 ? 128 : 64;
   auto rows_of = [&](const void* p, int64_t stride, uint32_t range) __attribute__((always_inline)) {
     return __builtin_amdgcn_make_buffer_rsrc(
@@ -547,7 +547,8 @@ __device__ inline void set_planes(const WindowArgs& a, int64_t plane, uint32_t k
 }
 // Query row r0 + c of a sequence (of `rows`): d = 16 g + 0..15, times scale * log2(e), and
 // where they stand (rows past the last one are zero and stand at the last key, p1).
-__device__ inline void load_rows(const WindowArgs& a, int t, int h, int r0, int p1, int c, int g,
+template <int kSeqs>
+__device__ inline void load_rows(const WindowArgs<kSeqs>& a, int t, int h, int r0, int p1, int c, int g,
                                  f32x4 (&qx)[4], int& pos) {
   const int past = a.past[t], rows = a.rows[t];
   const int r = r0 + c;
@@ -565,7 +566,8 @@ __device__ inline void load_rows(const WindowArgs& a, int t, int h, int r0, int 
 // The workgroup's sequence, and which of the sequence's workgroups it is. There is none without one:
 // with a grid as wide as the widest sequence the dispatcher put the others' workgroups on few CUs
 // (16 single tokens over 8192 keys and a text of 256 rows, 20 heads, f16: 533 us, now 141).
-__device__ inline int sequence_of(const WindowArgs& a, int& lid) {
+template <int kSeqs>
+__device__ inline int sequence_of(const WindowArgs<kSeqs>& a, int& lid) {
   lid = a.remap ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
   if (a.n_seqs == 1) return 0;
   if (a.like) {
@@ -587,8 +589,8 @@ __device__ inline float half_weight(float m, float all) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (m - all));
 }
 
-template <DType kD>
-__global__ __launch_bounds__(64 * kWaves, 4) void window_attend(WindowArgs a) {
+template <DType kD, int kSeqs>
+__global__ __launch_bounds__(64 * kWaves, 4) void window_attend(WindowArgs<kSeqs> a) {
   constexpr int kRows = 16;
   __shared__ __attribute__((aligned(128))) char vs[kD == kF32 ? 1 : kWaves][kN * 128];
   __shared__ __attribute__((aligned(16))) float mo[kWaves][kRows * kPitch];  // a wave's O rows
@@ -762,8 +764,8 @@ constexpr int kTile = 64;
 constexpr int kTileRows = 64;
 __device__ inline int kswz(int r) { return (r >> 1) & 7; }  // 16 rows' equal chunks hit distinct banks
 
-template <bool k8>
-__global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs a) {
+template <bool k8, int kSeqs>
+__global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs<kSeqs> a) {
   constexpr int kPieces = k8 ? 1 : 2;  // 16-byte pieces of a tile's K (or V) a thread
   constexpr DType kD = k8 ? kI8 : kF16;
   __shared__ __attribute__((aligned(128))) char kt[2][kTile * 128], vt[2][kTile * 128];
@@ -911,7 +913,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void window_tiles(WindowArgs a) {
 // 60 against 66, 4000 (630) 107 against 146. A single token is 1/64 of a block: 39 of them over 8192 keys
 // with a text of 64 or 256 rows, 8-bit, 192 and 192 us against 179 and 168 (with 2000 rows 287 and 237; 16 of
 // them with 2000 rows, f16 (163) 172 us against 242, 8-bit (163) 208 and 153).
-int block_rows(const WindowArgs& a, DType dt) {
+template <int kSeqs>
+int block_rows(const WindowArgs<kSeqs>& a, DType dt) {
   if (dt == kF32) return 16;
   int64_t work = 0;
   int longest = 1;
@@ -931,7 +934,8 @@ int block_rows(const WindowArgs& a, DType dt) {
 }
 
 // Steps of the longest block of a sequence, at most.
-int most_steps(const WindowArgs& a, int t, int rows) {
+template <int kSeqs>
+int most_steps(const WindowArgs<kSeqs>& a, int t, int rows) {
   const int p1 = a.past[t] - 1 + (a.causal ? a.rows[t] : 0), wide = std::min(a.rows[t], rows);
   const Span<kN> s(a.causal ? p1 - wide + 1 : p1, p1, a.window, a.sinks);
   // A block before the last may begin its window at another place within a step.
@@ -940,9 +944,10 @@ int most_steps(const WindowArgs& a, int t, int rows) {
 
 }  // namespace
 
-int64_t window_plan(WindowArgs& a, DType dt, bool split) {
+template <int kSeqs>
+int64_t window_plan(WindowArgs<kSeqs>& a, DType dt, bool split) {
   const int rows = a.block_rows = block_rows(a, dt);
-  int steps[kWindowMaxSeqs], longest = 1;
+  int steps[kSeqs], longest = 1;
   int64_t work = 0;
   for (int t = 0; t < a.n_seqs; ++t) {
     a.n_blk[t] = (a.rows[t] + rows - 1) / rows;
@@ -966,7 +971,7 @@ int64_t window_plan(WindowArgs& a, DType dt, bool split) {
       a.like &= a.n_wgs[t] == a.n_wgs[0];
       a.remap &= a.n_split[t] > 1;
     }
-    for (int t = a.n_seqs; t < kWindowMaxSeqs; ++t) a.wg0[t] = 0x7fffffff;
+    for (int t = a.n_seqs; t < kSeqs; ++t) a.wg0[t] = 0x7fffffff;
     a.wgs_inv = inverse(a.n_wgs[0]);
     return sum;
   };
@@ -997,24 +1002,32 @@ int64_t window_plan(WindowArgs& a, DType dt, bool split) {
   return lay(chunk);
 }
 
-hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipStream_t s) {
+template <int kSeqs>
+hipError_t launch_window_attend(const WindowArgs<kSeqs>& a, DType dt, int64_t wgs, hipStream_t s) {
   if (wgs <= 0) return hipSuccess;
   if (wgs > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid(static_cast<unsigned>(wgs)), block(64 * kWaves);
   const bool tiles = a.block_rows == kTileRows;
-#define WRS_WINDOW(K) hipLaunchKernelGGL(K, grid, block, 0, s, a)
+#define WRS_WINDOW(K, ...) hipLaunchKernelGGL((K<__VA_ARGS__, kSeqs>), grid, block, 0, s, a)
   switch (dt) {
     case kF16:
-      if (tiles) { WRS_WINDOW(window_tiles<false>); } else { WRS_WINDOW(window_attend<kF16>); }
+      if (tiles) { WRS_WINDOW(window_tiles, false); } else { WRS_WINDOW(window_attend, kF16); }
       break;
-    case kF32: WRS_WINDOW(window_attend<kF32>); break;
+    case kF32: WRS_WINDOW(window_attend, kF32); break;
     case kI8:
-      if (tiles) { WRS_WINDOW(window_tiles<true>); } else { WRS_WINDOW(window_attend<kI8>); }
+      if (tiles) { WRS_WINDOW(window_tiles, true); } else { WRS_WINDOW(window_attend, kI8); }
       break;
     default: return hipErrorInvalidValue;
   }
 #undef WRS_WINDOW
   return hipGetLastError();
 }
+
+template int64_t window_plan(WindowArgs<kWindowMaxSeqs>&, DType, bool);
+template int64_t window_plan(WindowArgs<kWindowFewSeqs>&, DType, bool);
+template hipError_t launch_window_attend(const WindowArgs<kWindowMaxSeqs>&, DType, int64_t,
+                                         hipStream_t);
+template hipError_t launch_window_attend(const WindowArgs<kWindowFewSeqs>&, DType, int64_t,
+                                         hipStream_t);
 
 }  // namespace wrs

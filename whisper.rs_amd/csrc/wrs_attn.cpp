@@ -905,8 +905,9 @@ void free_planes(wrs_kv* kv) {
 }
 
 // Rows of the arena's self or cross planes, no slot's yet, and one slot's (first plane `plane`).
-wrs::KvSlotRows slot_rows(const wrs_kv* kv, bool cross) {
-  wrs::KvSlotRows a;
+template <int kSlots>
+wrs::KvSlotRows<kSlots> slot_rows(const wrs_kv* kv, bool cross) {
+  wrs::KvSlotRows<kSlots> a;
   a.k = cross ? kv->k_cross : kv->k_self;
   a.v = cross ? kv->v_cross : kv->v_self;
   a.k_scale = cross ? kv->k_cross_scale : kv->k_self_scale;
@@ -919,7 +920,8 @@ wrs::KvSlotRows slot_rows(const wrs_kv* kv, bool cross) {
   a.n_slots = 0;
   return a;
 }
-void add_rows(wrs::KvSlotRows& a, size_t plane, size_t row0, size_t pos, size_t count) {
+template <int kSlots>
+void add_rows(wrs::KvSlotRows<kSlots>& a, size_t plane, size_t row0, size_t pos, size_t count) {
   const int u = a.n_slots++;
   a.plane[u] = static_cast<int64_t>(plane);
   a.row0[u] = static_cast<int64_t>(row0);
@@ -932,7 +934,7 @@ void add_rows(wrs::KvSlotRows& a, size_t plane, size_t row0, size_t pos, size_t 
 int write_rows(wrs_attn_ctx* c, wrs_kv* kv, const float* k_src, const float* v_src, size_t n,
                void* k, void* v, size_t off, size_t plane, size_t pos) {
   if (kv->i8()) {
-    wrs::KvSlotRows a = slot_rows(kv, k == kv->k_cross);
+    auto a = slot_rows<wrs::kRowFewSlots>(kv, k == kv->k_cross);
     a.k_rows = const_cast<float*>(k_src);
     a.v_rows = const_cast<float*>(v_src);
     a.k_rs = a.v_rs = static_cast<int64_t>(kv->d_model());
@@ -1345,13 +1347,14 @@ int check_rows(wrs_attn_ctx* c, const wrs_kv* kv, size_t n, const float* p, size
 }
 
 // Rows of several slots into the arena (first: nullptr, at the slots' lengths) or out of it, their
-// arguments checked; kRowSlots of them to a launch.
-int move_slot_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* first,
-                   const size_t* counts, size_t n_slots, float* k, int64_t k_rs, float* v,
-                   int64_t v_rs) {
+// arguments checked; kSlots of them to a launch.
+template <int kSlots>
+int launch_slot_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* first,
+                     const size_t* counts, size_t n_slots, float* k, int64_t k_rs, float* v,
+                     int64_t v_rs) {
   wrs_attn_ctx* c = kv->ctx;
   DeviceGuard g(c->device);
-  wrs::KvSlotRows a = slot_rows(kv, false);
+  auto a = slot_rows<kSlots>(kv, false);
   a.k_rows = k;
   a.v_rows = v;
   a.k_rs = k_rs;
@@ -1362,12 +1365,20 @@ int move_slot_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* 
       add_rows(a, (layer * kv->n_slots + slots[i]) * kv->n_heads, row,
                first ? first[i] : kv->len[slots[i]], counts[i]);
     row += counts[i];
-    if (a.n_slots == wrs::kRowSlots || i + 1 == n_slots) {
+    if (a.n_slots == kSlots || i + 1 == n_slots) {
       WRS_HIP(c, wrs::launch_kv_slot_rows(a, kv->plane_type(), !first, c->stream));
       a.n_slots = 0;
     }
   }
   return WRS_OK;
+}
+
+template <typename... A>
+int move_slot_rows(wrs_kv* kv, size_t layer, const size_t* slots, const size_t* first,
+                   const size_t* counts, size_t n_slots, A... args) {
+  const auto f = n_slots <= wrs::kRowFewSlots ? launch_slot_rows<wrs::kRowFewSlots>
+                                              : launch_slot_rows<wrs::kRowSlots>;
+  return f(kv, layer, slots, first, counts, n_slots, args...);
 }
 
 }  // namespace
@@ -1448,7 +1459,7 @@ int wrs_kv_read_cross(wrs_kv* kv, size_t layer, size_t first, size_t n, float* k
   rc = check_rows(c, kv, n, v_rows, v_len, v_row_stride);
   if (rc) return rc;
   DeviceGuard g(c->device);
-  wrs::KvSlotRows a = slot_rows(kv, true);
+  auto a = slot_rows<wrs::kRowFewSlots>(kv, true);
   a.k_rows = k_rows;
   a.v_rows = v_rows;
   a.k_rs = k_row_stride;
@@ -1568,11 +1579,11 @@ namespace {
 // Attention of rows that see a window and the first keys, on K19: n_seqs sequences of count(i) rows
 // whose first plane is plane(i) and whose history is past(i) (window_plan's terms). At most
 // kRowsMaxKeys keys each, checked before.
-template <typename P, typename L, typename C>
-int window_rows(wrs_attn_ctx* c, const wrs_kv* kv, bool cross, bool causal, size_t window,
-                size_t sinks, size_t n_seqs, P plane, L past, C count, const float* q, int64_t q_rs,
-                float* out, int64_t o_rs) {
-  wrs::WindowArgs a;
+template <int kSeqs, typename P, typename L, typename C>
+int window_launches(size_t n_seqs, wrs_attn_ctx* c, const wrs_kv* kv, bool cross, bool causal,
+                    size_t window, size_t sinks, P plane, L past, C count, const float* q,
+                    int64_t q_rs, float* out, int64_t o_rs) {
+  wrs::WindowArgs<kSeqs> a;
   a.q = q;
   a.o = out;
   a.k = cross ? kv->k_cross : kv->k_self;
@@ -1593,7 +1604,7 @@ int window_rows(wrs_attn_ctx* c, const wrs_kv* kv, bool cross, bool causal, size
   size_t row = 0;
   for (size_t i = 0; i < n_seqs;) {
     a.n_seqs = 0;
-    for (; i < n_seqs && a.n_seqs < wrs::kWindowMaxSeqs; ++i) {
+    for (; i < n_seqs && a.n_seqs < kSeqs; ++i) {
       if (count(i) == 0) continue;
       const int t = a.n_seqs++;
       a.plane[t] = static_cast<int64_t>(plane(i));
@@ -1613,13 +1624,19 @@ int window_rows(wrs_attn_ctx* c, const wrs_kv* kv, bool cross, bool causal, size
   return WRS_OK;
 }
 
+template <typename... A>
+int window_rows(size_t n_seqs, A... args) {
+  return n_seqs <= wrs::kWindowFewSeqs ? window_launches<wrs::kWindowFewSeqs>(n_seqs, args...)
+                                       : window_launches<wrs::kWindowMaxSeqs>(n_seqs, args...);
+}
+
 // Rows of a slot's cache with every key up to their own, rows of cross-attention with every key:
 // an 8-bit arena's attention. q and out: packed rows.
 int self_rows_i8(wrs_attn_ctx* c, const wrs_kv* kv, size_t layer, const size_t* slots, size_t n_slots,
                  size_t count, const float* q, float* out) {
   const int64_t dm = static_cast<int64_t>(kv->d_model());
   return window_rows(
-      c, kv, false, true, SIZE_MAX, 0, n_slots,
+      n_slots, c, kv, false, true, SIZE_MAX, 0,
       [&](size_t i) { return (layer * kv->n_slots + slots[i]) * kv->n_heads; },
       [&](size_t i) { return kv->len[slots[i]]; }, [&](size_t) { return count; }, q, dm, out, dm);
 }
@@ -1627,7 +1644,7 @@ int cross_rows_i8(wrs_attn_ctx* c, const wrs_kv* kv, size_t layer, const float* 
                   float* out) {
   const int64_t dm = static_cast<int64_t>(kv->d_model());
   return window_rows(
-      c, kv, true, false, SIZE_MAX, 0, 1, [&](size_t) { return layer * kv->n_heads; },
+      1, c, kv, true, false, SIZE_MAX, 0, [&](size_t) { return layer * kv->n_heads; },
       [&](size_t) { return kv->cross_len[layer]; }, [&](size_t) { return n; }, q, dm, out, dm);
 }
 
@@ -2003,7 +2020,7 @@ int wrs_attn_window_self(wrs_attn_ctx* c, wrs_kv* kv, size_t layer, const size_t
   if (rc) return rc;
   DeviceGuard g(c->device);
   return window_rows(
-      c, kv, false, true, window, sinks, n_slots,
+      n_slots, c, kv, false, true, window, sinks,
       [&](size_t i) { return (layer * kv->n_slots + slots[i]) * kv->n_heads; },
       [&](size_t i) { return kv->len[slots[i]]; }, [&](size_t i) { return counts[i]; }, q,
       q_row_stride, out, out_row_stride);

@@ -298,7 +298,11 @@ hipError_t launch_tree_attend(const TreeArgs& a, DType dt, int64_t wgs, hipStrea
 // j > position - window or j < sinks. past + rows < 2^24 - 4095 and window <= 2^24. window_plan lays
 // out the launch and returns its workgroups; with `split` keys may be dealt over several of them,
 // through the scratch of tree attention.
+// Arguments are copied per launch: those of few sequences are small (64: a call of one row 6.1 us from
+// Python, 8: 5.7).
 constexpr int kWindowMaxSeqs = 64;  // per launch
+constexpr int kWindowFewSeqs = 8;
+template <int kSeqs>
 struct WindowArgs {
   const float* q;
   float* o;  // row r at o + r*o_rs
@@ -309,18 +313,20 @@ struct WindowArgs {
   float scale_log2;  // (1/8) * log2(e)
   float* part;
   unsigned* counters;
-  int64_t plane[kWindowMaxSeqs], row0[kWindowMaxSeqs];
-  int past[kWindowMaxSeqs], rows[kWindowMaxSeqs];  // rows >= 1; past >= 1 where not causal
+  int64_t plane[kSeqs], row0[kSeqs];
+  int past[kSeqs], rows[kSeqs];  // rows >= 1; past >= 1 where not causal
   // By window_plan, as TreeArgs has them; chunk counts steps.
-  int n_wgs[kWindowMaxSeqs], wg0[kWindowMaxSeqs], n_blk[kWindowMaxSeqs], n_split[kWindowMaxSeqs];
-  uint32_t blk_inv[kWindowMaxSeqs], split_inv[kWindowMaxSeqs], head_inv;
+  int n_wgs[kSeqs], wg0[kSeqs], n_blk[kSeqs], n_split[kSeqs];
+  uint32_t blk_inv[kSeqs], split_inv[kSeqs], head_inv;
   // Rows of a block; whether every sequence has n_wgs[0] workgroups, and whether those go to the
   // XCDs by heads.
   int block_rows, like, remap;
   uint32_t wgs_inv;
 };
-int64_t window_plan(WindowArgs& a, DType dt, bool split);
-hipError_t launch_window_attend(const WindowArgs& a, DType dt, int64_t wgs, hipStream_t s);
+template <int kSeqs>
+int64_t window_plan(WindowArgs<kSeqs>& a, DType dt, bool split);
+template <int kSeqs>
+hipError_t launch_window_attend(const WindowArgs<kSeqs>& a, DType dt, int64_t wgs, hipStream_t s);
 
 // Log probabilities of given tokens, entropies and the top_k likeliest entries of rows of logits
 // (f32, f16 or bf16, row r at r*row_stride) over the entries whose allowed byte is not zero (nullptr:
@@ -557,6 +563,8 @@ hipError_t launch_kv_keep_rows(const KeepArgs<kSlots, kMoves>& a, hipStream_t s)
 // f32: count[u] rows from row row0[u] of k_rows and v_rows (k_rs and v_rs apart, head h at + h*64)
 // against rows pos[u].. of planes plane[u] + h, each plane_rows rows of 64 (and scale_rows scales).
 constexpr int kRowSlots = 64;  // per launch
+constexpr int kRowFewSlots = 8;
+template <int kSlots>
 struct KvSlotRows {
   float *k_rows, *v_rows;  // only read where rows are stored
   int64_t k_rs, v_rs;
@@ -565,10 +573,11 @@ struct KvSlotRows {
   int64_t plane_rows, scale_rows;
   int n_heads, n_slots;
   uint32_t heads_inv;  // 2^32 / n_heads, as divide() takes it
-  int64_t plane[kRowSlots], row0[kRowSlots];
-  int pos[kRowSlots], count[kRowSlots];
+  int64_t plane[kSlots], row0[kSlots];
+  int pos[kSlots], count[kSlots];
 };
-hipError_t launch_kv_slot_rows(const KvSlotRows& a, DType dt, bool store, hipStream_t s);
+template <int kSlots>
+hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store, hipStream_t s);
 // The planes of an 8-bit arena's slot: plane (l, h) is plane l*layer + h, of `rows` rows of codes
 // and `scale_rows` scales.
 struct Kv8Planes {
