@@ -17,9 +17,9 @@
 //   from the load to the weights' product when it is alone on its SIMD (f32: 1.9), and window_plan
 //   deals a block's steps over workgroups by that. Bytes are the other bound: 16 sequences of 20 heads
 //   that see 8192 keys each (f16: 672 MB) take 121 us, 5.5 TB/s, and the 8-bit ones half the bytes in
-//   80 us, 4.3 TB/s: with as many steps in flight, each loads half. Deeper prefetch (2 to 4 steps),
-//   steps of 64 keys and 32 rows a wave were measured and are no faster (79 to 88 us; registers then
-//   allow 2 or 3 waves a SIMD instead of 4).
+//   80 us, 4.3 TB/s (three caches in turn; two, of which the L3 keeps a part, 68): with as many steps in
+//   flight, each loads half. Deeper prefetch (2 to 4 steps), steps of 64 keys and 32 rows a wave were
+//   measured and are no faster (79 to 88 us; registers then allow 2 or 3 waves a SIMD instead of 4).
 #include "split16.hpp"
 
 #include <algorithm>
