@@ -269,3 +269,54 @@ def test_the_widest_and_the_narrowest_window(wrs, name, window):
     assert torch.equal(s.q, out)
     s.arena.close()
     c.close()
+
+
+@pytest.mark.parametrize("name,rows", [("f32", 9_000_000), ("f16", 16_000_000), ("i8", 16_000_000)])
+def test_far_rows_of_a_long_cache(wrs, name, rows):
+    """Planes of gigabytes: rows behind 2^31 bytes of their plane, planes behind 2^32 bytes."""
+    c = wrs.Context(0)
+    c.use_torch_stream()
+    heads, n, new = 5, 100, 3
+    d = heads * D
+    note(f"far rows {name}")
+    ar = wrs.KvArena(1, 1, heads, rows, 0, ctx=c, dtype=_dtype(wrs, name))
+    past = rows - n
+    ar.set_len(0, 0)
+    ar.advance(0, past)
+    k, v, q = (normal(n, d, seed=s) for s in (1, 2, 3))
+    ar.append_rows(0, [0], [n], k, v)
+    ar.advance(0, n - new)
+    gk, gv = torch.zeros_like(k), torch.zeros_like(v)
+    ar.read_rows(0, [0], [past], [n], gk, gv)
+    out = torch.zeros(new, d, device="cuda")
+    ar.window_self(0, [0], [new], 60, 0, q[:new], out)
+    torch.cuda.synchronize()
+    kk, vv = stored(k, name), stored(v, name)
+    assert torch.equal(gk.double(), kk) and torch.equal(gv.double(), vv)
+    hide = hidden(n - new, new, 60, 0)
+    for h in range(heads):
+        at = slice(h * D, (h + 1) * D)
+        s = torch.where(hide, -torch.inf, q[:new, at].double() @ kk[:, at].T.contiguous() / 8)
+        want = torch.softmax(s, 1) @ vv[:, at]
+        # weights to 2^-16 of themselves (sums of |q k| / 8 below 9), on both sides
+        assert (out[:, at].double() - want).abs().max().item() <= 2.0 ** -15 * vv.abs().max().item()
+    ar.close()
+    c.close()
+
+
+def test_logits_rows_far_apart(wrs):
+    c = wrs.Context(0)
+    c.use_torch_stream()
+    stride, v = 1_200_000_000, 5000
+    note("far logits")
+    x = torch.empty(3, stride, dtype=torch.float16, device="cuda")[:, :v]
+    x.copy_(normal(3, v, seed=5))
+    tokens = torch.tensor([0, 2500, 4999], device="cuda").int()
+    lp, ids = torch.zeros(3, device="cuda"), torch.zeros(3, 1, dtype=torch.int32, device="cuda")
+    wrs.token_logprobs(x, tokens, lp, top_ids=ids, ctx=c)
+    torch.cuda.synchronize()
+    want = torch.log_softmax(x.double(), 1)
+    # exponents below 2^4: 2^-20; the sum's logarithm 2^-22
+    assert (lp.double() - want[torch.arange(3), tokens.long()]).abs().max().item() <= 2.0 ** -19
+    assert torch.equal(ids[:, 0].long(), want.argmax(1))
+    c.close()
