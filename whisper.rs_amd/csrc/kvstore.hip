@@ -14,13 +14,14 @@
 //   take a row of a head, 4 values each, and find its largest magnitude by DPP (as bit patterns:
 //   a NaN is the largest).
 // K18 (kv_read): the stored values as f32, the same way round.
-//   Bound by memory. From kManyRows rows on a workgroup takes 64 rows of one head, whose codes and
-//   scales are contiguous and no other workgroup's (rows of all heads in turn: a scale's line is
+//   Bound by memory. From kManyRows rows on a workgroup takes 32 rows of one head, whose codes and
+//   scales are contiguous and hardly another workgroup's (rows of all heads in turn: a scale's line is
 //   written by many). What is read back is written past the caches (non-temporal), and so is read what
 //   is stored if it is more than they keep. 44012 rows of 12 heads to 8 bits and back (339 MB
-//   each way): 64 us and 50 us, 5.3 and 6.8 TB/s; by rows of all heads 70 and 68, without the
-//   non-temporal forms 68 and 67. 1500 rows of 20 heads: 5.5 and 4.2 us (non-temporal loads: 5.8).
-//   A step's 5 rows take 2.8 and 2.5 us, what an empty launch does.
+//   each way): 62 us and 50 us, 5.4 and 6.8 TB/s; by rows of all heads 70 and 68, without the
+//   non-temporal forms 68 and 67, 16 or 64 rows a workgroup 72 and 47, 64 and 50. 1500 rows of 20 heads:
+//   5.2 and 4.4 us (non-temporal loads: 5.8). A step's 5 rows take 2.4 and 2.3 us, what an empty
+//   launch does (64 rows of all heads a workgroup: 2.7 and 2.4).
 #include "wrs_internal.hpp"
 
 #include <algorithm>
@@ -78,17 +79,16 @@ __device__ inline f32x4 decode4(uint32_t w, uint32_t byte) {
   return x;
 }
 
-constexpr int kTurns = 4;  // pieces of 4 values that a thread has in flight
-constexpr int kBlockRows = 16 * kTurns;
 constexpr int kManyRows = 16;
 constexpr int64_t kOnce = 128 << 20;  // bytes that are read past the caches
 
-// A workgroup takes 1024 pieces of 4 columns: the next ones of rows of all heads, or those of
-// kBlockRows rows of a head.
+// A workgroup takes rows of a head, 16 lanes each: the next 16 of all heads', or 32 of one head.
 enum class Order { kAllHeads, kByHead, kByHeadOnce };
+constexpr int block_rows(bool by_head) { return by_head ? 32 : 16; }
 template <DType kD, bool kStore, Order kOrder, int kSlots>
 __global__ __launch_bounds__(256) void kv_rows(KvSlotRows<kSlots> a) {
   constexpr bool kByHead = kOrder != Order::kAllHeads;
+  constexpr int kBlockRows = block_rows(kByHead), kTurns = kBlockRows / 16;
   const int u = blockIdx.z, rows_here = a.count[u], sub = threadIdx.x >> 4;
   // The block's first row of a head and that head, or its first row in turn.
   int64_t first;
@@ -255,10 +255,11 @@ hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store
   }
   if (most <= 0 || a.n_heads <= 0) return hipSuccess;
   const int64_t rows = static_cast<int64_t>(most) * a.n_heads;
-  if (rows > 0x7fffffff - kBlockRows) return hipErrorInvalidConfiguration;
+  if (rows > 0x7fffffff - 64) return hipErrorInvalidConfiguration;
   const bool by_head = most >= kManyRows, once = all * a.n_heads * 512 > kOnce;
-  const int64_t blocks = by_head ? (most + kBlockRows - 1) / kBlockRows * static_cast<int64_t>(a.n_heads)
-                                 : (rows + kBlockRows - 1) / kBlockRows;
+  const int block = block_rows(by_head);
+  const int64_t blocks = by_head ? (most + block - 1) / block * static_cast<int64_t>(a.n_heads)
+                                 : (rows + block - 1) / block;
   const dim3 grid(static_cast<unsigned>(blocks), 2, a.n_slots);
 #define WRS_KV_ROWS_ONE(D, S, O) \
   hipLaunchKernelGGL((kv_rows<D, S, Order::O, kSlots>), grid, dim3(256), 0, s, a)
