@@ -320,3 +320,25 @@ def test_logits_rows_far_apart(wrs):
     assert (lp.double() - want[torch.arange(3), tokens.long()]).abs().max().item() <= 2.0 ** -19
     assert torch.equal(ids[:, 0].long(), want.argmax(1))
     c.close()
+
+
+def test_a_cache_of_too_many_keys_is_refused(wrs):
+    c = wrs.Context(0)
+    c.use_torch_stream()
+    note("too many keys")
+    ar = wrs.KvArena(1, 1, 1, 2 ** 24 + 10, 0, ctx=c)
+    q, out = torch.zeros(1, D, device="cuda"), torch.full((1, D), 3.0, device="cuda")
+    ar.advance(0, 2 ** 24 - 4096)
+    with pytest.raises(RuntimeError, match="too long"):
+        ar.window_self(0, [0], [1], 5, 0, q, out)
+    ar.set_len(0, 2 ** 24 - 4097)
+    ar.append_rows(0, [0], [1], q + 1.0, q + 2.0)
+    torch.cuda.synchronize()
+    assert (out == 3.0).all()
+    ar.window_self(0, [0], [1], 1, 0, q, out)  # the last key there is room for, alone
+    torch.cuda.synchronize()
+    assert (out == 2.0).all()
+    with pytest.raises(RuntimeError, match="too long"):
+        wrs.KvArena(1, 1, 1, 2 ** 24, 0, ctx=c, dtype=wrs.WRS_I8)
+    ar.close()
+    c.close()
