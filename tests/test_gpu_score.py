@@ -208,6 +208,62 @@ def test_values_that_are_no_numbers(wrs, ctx, n):
             check(wrs, ctx, x[:1], some_tokens(1, v, 9), 4, allowed=ok)
 
 
+def check_far(wrs, ctx, x, tokens, k, allowed=None, temperature=1.0):
+    """check(), of rows whose smallest terms may lie below 2^-126: those come as zero, which is off by
+    v 2^-126 < 1e-33 in the sum and 88 times that in the entropy. Log probabilities past f32's range are
+    -infinity."""
+    lp, h, ids, top = score(wrs, ctx, x, tokens, k, allowed, temperature)
+    w_lp, w_h, w_ids, w_top = expect(x, tokens, k, allowed, temperature)
+    most = torch.finfo(torch.float32).max
+    for got, want in ((lp, w_lp), (top, w_top)):
+        want = torch.where(want < -most, -INF, want)
+        small = (want.abs() < 1e-27) & ((got.double() - want).abs() <= 1e-33 + 2e-5 * want.abs())
+        assert close(torch.where(small, 0.0, got), torch.where(small, 0.0, want))
+    assert ((h.double() - w_h).abs() <= 4e-5 * w_h + 1e-31).all()
+    assert torch.equal(ids.long(), w_ids)
+
+
+def far_rows(dtype, far):
+    """Rows with entries far from zero, or far from each other, all finite in `dtype`."""
+    v = 51865
+    x = logits_of(6, v, "f32", seed=5)
+    x[0, 1501:] = far          # all but the first ones held down by a finite mask
+    x[1, :v - 9] = far         # all but the last ones
+    x[2] += far                # every entry there
+    x[3, 1::2] = far
+    x[4] = far                 # all equal
+    x[5, 100:200] -= far / 2   # some far up
+    return x.to(DT[dtype])
+
+
+@pytest.mark.parametrize("dtype,far", [
+    *(("f32", f) for f in (-1e7, -1e9, -3e9, -1e10, -2e10, -5e10, -1e12, -3e15, -1e20, -1e25, -9e29, -1e32)),
+    ("bf16", -1e10), ("bf16", -3e15), ("bf16", -1e29), ("f16", -65504.0)])
+@pytest.mark.parametrize("copies", [1, 60])
+def test_entries_far_from_zero(wrs, ctx, dtype, far, copies):
+    """Masks of any finite value, rows split over workgroups and whole."""
+    x = far_rows(dtype, far).repeat(copies, 1)
+    tokens = some_tokens(x.shape[0], x.shape[1], 11)
+    ok = torch.ones(1, x.shape[1], dtype=torch.bool, device="cuda")
+    for temperature in (1.0, 0.7):
+        note(f"far entries {dtype} {far} {copies} {temperature}")
+        t = float(torch.tensor(temperature, dtype=torch.float32))
+        check_far(wrs, ctx, x, tokens, 5, temperature=t)
+        check_far(wrs, ctx, x, tokens, 5, allowed=ok, temperature=t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("temperature", [1e-7, 1e-8, 1e-9, 3e-10, 1e-11, 1e-20, 1e-30, 1e-37])
+@pytest.mark.parametrize("n", [3, 300])
+def test_temperatures_next_to_zero(wrs, ctx, dtype, temperature, n):
+    note(f"cold {dtype} {temperature} {n}")
+    x = logits_of(n, 9001, dtype, seed=8)
+    x[0, 100:] = x[0, 0]
+    x[1] = x[1, 0]  # all equal
+    t = float(torch.tensor(temperature, dtype=torch.float32))
+    check_far(wrs, ctx, x, some_tokens(n, 9001, 12), 5, temperature=t)
+
+
 def test_confident_rows_keep_their_precision(wrs, ctx):
     """Log probabilities close to 0, with the likeliest entry anywhere."""
     v = 51865

@@ -44,7 +44,9 @@ constexpr int kMostPieces = kScoreChunk / kThreads / 4;  // of a thread, at most
 static_assert(kMostPieces <= 64, "a piece a lane");
 constexpr int kMostKeys = kScoreMostTop * (kScoreChunk / kThreads);  // entries of that many threads
 constexpr int kCounterStride = 32;   // 128 bytes between merge counters
-constexpr float kLow = -1e30f;       // finite: times a weight of 0 it is 0
+// Exponents below it are 0: finite, so that times a weight of 0 it is 0. References lie at or above it,
+// and below -kLow where the sums against them are used.
+constexpr float kLow = -0x1p24f;
 
 // A value's order as an unsigned number, and an entry's: by value, the lower index first among
 // equals.
@@ -240,8 +242,10 @@ struct Shared {
 // m, s and t.
 //
 // Sums are kept against a reference r of the thread's, its maximum times scale as f32 rounds it, so that
-// a term's exponent is one fma (rounded once, whatever r is); what r is off by is taken back at the
-// end. Entries so large that this overflows take `plain`: a second pass over differences.
+// a term's exponent is one fma (rounded once, whatever r is); what r is off by, half a unit of f32 at
+// 2^24 at most, is taken back at the end. Farther out it is off by more than a sum's range takes (2^9
+// at 2^33), so a thread whose entries all lie below -2^24 adds 0 against that, and where the largest
+// entry of all lies outside `plain` takes a second pass over differences.
 // early() is called while few other loads are on their way.
 template <typename T, bool kMask, bool kSmall, typename F>
 __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float scale, Shared& sh,
@@ -351,7 +355,7 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
   float m_all = sh.wave_max[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, sh.wave_max[w]);
-  const bool odd = !(m_all * scale > kLow && m_all * scale < -kLow);  // of all threads
+  const bool odd = !(m_all * scale > kLow && m_all * scale < -kLow);  // the same in all threads
   if (odd && m_all > -INFINITY) {
     // plain: the sums against the largest entry, from differences.
     s = t = ref = 0.f;
