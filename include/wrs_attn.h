@@ -95,7 +95,7 @@ const char *wrs_attn_status_string(int status);
  * reference allocates per call on the host). Device-resident entry points
  * never allocate once their sizes are reserved; a call that would grow
  * scratch while the context's stream records a graph fails with
- * WRS_ECAPTURE instead. Four exceptions need no reservation:
+ * WRS_ECAPTURE instead. These need no reservation, but where said:
  * 16-bit prefill grids of fewer 128-query blocks than half the CUs merge
  * blocks split over two workgroups through a fixed context buffer (~9 MB on
  * 256 CUs), allocated by the first such call outside capture; during capture
@@ -108,8 +108,10 @@ const char *wrs_attn_status_string(int status);
  * (reserving linear_tokens allocates both). Tree and window attention, every attention
  * over 8-bit arenas and token scores split long keys and rows through a third one (~4 MB,
  * which reserving heads with decode rows and keys allocates too) and, captured before it
- * exists, run unsplit. wrs_kv_set_cross_proj into an 8-bit arena takes f32 rows of a layer
- * that its first call outside capture allocates. Switching streams
+ * exists, run unsplit (but token scores past 65536 entries a row: WRS_ECAPTURE).
+ * wrs_kv_set_cross_proj into an 8-bit arena takes its f32 rows through a fixed buffer of 16 MB,
+ * which reserving linear_tokens or the first such call outside capture allocates; captured
+ * before, it fails with WRS_ECAPTURE. Switching streams
  * (wrs_attn_set_stream) drains the old stream unless either stream is
  * recording a graph. Zero fields are ignored; reserving never shrinks.
  * Synchronous. */

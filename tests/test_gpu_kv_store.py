@@ -366,3 +366,97 @@ def test_refusals(wrs, ctx):
         assert ar._lib.wrs_kv_read_rows(ar.handle, 0, zero, zero, three, 1, k, kl, kr, v, vl,
                                         vr) == wrs.WRS_EINVAL
     assert torch.equal(before, read(ar, 0, 0, 0, 16)[0])
+
+
+# ---- cross projections: their f32 rows pass through memory that the context keeps ----------------
+
+
+def projections(layers, d, seed):
+    wk = [normal(d, d, seed=seed + i, sigma=d ** -0.5).half() for i in range(layers)]
+    wv = [normal(d, d, seed=seed + 20 + i, sigma=d ** -0.5).half() for i in range(layers)]
+    bv = [normal(d, seed=seed + 40 + i) for i in range(layers)]
+    return wk, wv, bv
+
+
+def cross(ar, layer, frames):
+    k, v = (torch.zeros(frames, ar.d_model, device="cuda") for _ in range(2))
+    ar.read_cross(layer, 0, k, v)
+    return k, v
+
+
+@pytest.mark.parametrize("ready", ["eager", "reserved"])
+def test_a_captured_cross_projection_keeps_its_rows(wrs, ready):
+    """A projection captured for a few frames replays after eager ones of more frames and of wider
+    arenas on the same context."""
+    heads, frames, layers = 2, 40, 2
+    d = heads * D
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        c = wrs.Context(0)
+        c.use_torch_stream()
+        small = wrs.KvArena(layers, 1, heads, 1, frames, ctx=c, dtype=wrs.WRS_I8)
+        plain = wrs.KvArena(layers, 1, heads, 1, frames, ctx=c, dtype=wrs.WRS_F32)
+        wide = wrs.KvArena(1, 1, 20, 1, 1500, ctx=c, dtype=wrs.WRS_I8)
+        ws, wide_ws = projections(layers, d, 1), projections(1, 20 * D, 100)
+        enc, wide_enc = normal(frames, d, seed=7).half(), normal(1500, 20 * D, seed=8).half()
+        stream.synchronize()
+        note(f"captured cross projection {ready}")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            with pytest.raises(RuntimeError, match="reserve"):
+                small.set_cross_proj(enc, *ws)
+            enc.mul_(1.0)
+        if ready == "eager":
+            small.set_cross_proj(enc, *ws)
+        else:
+            c.reserve(linear_tokens=frames, linear_n_in=d)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            small.set_cross_proj(enc, *ws)
+        wide.set_cross_proj(wide_enc, *wide_ws)
+        before = [t.clone() for t in cross(wide, 0, 1500)]
+        others = torch.full((4, 4 << 20), 7.0, device="cuda")  # 64 MB that take what was freed
+        for turn in range(4):
+            enc.copy_(normal(frames, d, seed=60 + turn))
+            g.replay()
+            if turn % 2:
+                wide.set_cross_proj(wide_enc, *wide_ws)
+            plain.set_cross_proj(enc, *ws)
+            for layer in range(layers):
+                for x, y in zip(cross(small, layer, frames), cross(plain, layer, frames)):
+                    assert torch.equal(x.double(), stored(y, "i8"))
+            for x, y in zip(before, cross(wide, 0, 1500)):
+                assert torch.equal(x, y)
+            stream.synchronize()
+            assert (others == 7.0).all()
+        del g
+        for ar in (small, plain, wide):
+            ar.close()
+        c.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("frames", [512, 517, 1100])
+def test_a_cross_projection_of_many_pieces(wrs, ctx, dtype, frames):
+    """64 heads: 512 rows at a time. A stored value is off by half a code, at most 1/127.5 of its row's
+    largest, and by the product's own error. That is at most (4096 + 4) 2^-24 of the terms' absolute sum,
+    which for these terms is below 64 |largest| / 1.5: below 2^-6.5, and as a walk of rounded sums rather
+    its square root's share, 64 2^-24 times 43: 2^-12."""
+    heads = 64
+    d = heads * D
+    wk, wv, bv = projections(1, d, 3)
+    wide = normal(frames, d + 8, seed=frames).to(dtype)
+    enc = wide[:, :d]
+    ar = wrs.KvArena(1, 1, heads, 1, frames + 3, ctx=ctx, dtype=wrs.WRS_I8)
+    note(f"cross projection in pieces {dtype} {frames}")
+    ar.set_cross_proj(enc, wk, wv, bv)
+    torch.cuda.synchronize()
+    assert ar.cross_len(0) == frames
+    k, v = cross(ar, 0, frames)
+    torch.cuda.synchronize()
+    for got, w, b in ((k, wk[0], 0.0), (v, wv[0], bv[0].double())):
+        want = (enc.double() @ w.double().T.contiguous() + b).reshape(frames, heads, D)
+        largest = want.abs().amax(2, keepdim=True)
+        err = (got.double().reshape(frames, heads, D) - want).abs()
+        assert (err <= largest * (1 / 127.5 + 2.0 ** -10)).all()
+    ar.close()

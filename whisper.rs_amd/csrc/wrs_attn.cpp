@@ -80,7 +80,8 @@ struct wrs_attn_ctx {
   size_t tree_part_bytes = 0;
   unsigned* tree_counters = nullptr;
   size_t tree_counter_bytes = 0;
-  float* cross_rows = nullptr;  // 8-bit arenas: projected cross K and V of a layer, before rounding
+  // Projected cross K and V of an 8-bit arena before rounding: a piece of a layer's rows, of one size.
+  float* cross_rows = nullptr;
   size_t cross_rows_bytes = 0;
   // Prefill schedule overrides (wrs_attn_set_schedule).
   int prefill_queries = 0;
@@ -306,6 +307,12 @@ int tree_scratch(wrs_attn_ctx* c) {
   if (rc) return rc;
   return grow(c, reinterpret_cast<void**>(&c->tree_counters), &c->tree_counter_bytes,
               wrs::kTreeCounterWords * sizeof(unsigned), true);
+}
+// And for the cross projections of 8-bit arenas, which take their rows through it in pieces: it holds
+// K and V of an encoder window of 1500 frames of 20 heads. Such a call cannot do without.
+constexpr size_t kCrossRowsBytes = size_t{16} << 20;
+int cross_rows_scratch(wrs_attn_ctx* c) {
+  return grow(c, reinterpret_cast<void**>(&c->cross_rows), &c->cross_rows_bytes, kCrossRowsBytes, false);
 }
 // And for the rows of fused decode projections that are normalized first.
 int ln_rows_scratch(wrs_attn_ctx* c) {
@@ -752,6 +759,8 @@ int wrs_attn_reserve(wrs_attn_ctx* c, const wrs_reserve* r) {
   }
   if (r->linear_tokens && r->linear_n_in) {
     rc = ln_rows_scratch(c);
+    if (rc) return rc;
+    rc = cross_rows_scratch(c);
     if (rc) return rc;
   }
   if (r->linear_tokens > static_cast<size_t>(wrs::kGemvMaxRows) && r->linear_n_in) {
@@ -2486,33 +2495,42 @@ int wrs_kv_set_cross_proj(wrs_kv* kv, int x_dtype, const void* enc, size_t enc_l
     DeviceGuard g(c->device);
     wrs::LinearArgs a{};
     const size_t dm = kv->d_model();
-    int rc = linear_prepare(c, x_dtype, enc, enc_row_stride, n_audio, dm, dm, a);
-    if (rc) return rc;
     if (kv->i8()) {
-      // A layer at a time: projected as f32 rows, then rounded into its planes.
-      const size_t half = align_up(n_audio * dm * sizeof(float), 256);
-      rc = grow(c, reinterpret_cast<void**>(&c->cross_rows), &c->cross_rows_bytes, 2 * half, false);
+      // A piece of a layer at a time: projected as f32 rows, then rounded into its planes.
+      const size_t most = kCrossRowsBytes / 2 / (dm * sizeof(float));
+      if (most == 0) return fail(c, WRS_EUNSUPPORTED, "projection shape too large");
+      const size_t piece = std::min(n_audio, most < 64 ? most : most / 64 * 64);
+      const size_t esize = x_dtype == WRS_F32 ? 4 : 2;
+      int rc = cross_rows_scratch(c);
       if (rc) return rc;
       float* const k = c->cross_rows;
-      float* const v = k + half / sizeof(float);
+      float* const v = k + kCrossRowsBytes / 2 / sizeof(float);
       a.out_rs = static_cast<int64_t>(dm);
       a.out_hs = 64;
       a.n_groups = 2;
-      for (size_t l = 0; l < kv->n_layers; ++l) {
-        a.w[0] = static_cast<const _Float16*>(w_k[l]);
-        a.bias[0] = nullptr;
-        a.out[0] = k;
-        a.w[1] = static_cast<const _Float16*>(w_v[l]);
-        a.bias[1] = b_v ? b_v[l] : nullptr;
-        a.out[1] = v;
-        WRS_HIP(c, wrs::launch_linear_f16w(a, wrs::kF32, c->stream));
-        rc = write_rows(c, kv, k, v, n_audio, kv->k_cross, kv->v_cross, kv->cross_off(l),
-                        kv->n_audio_max * 64, 0);
+      for (size_t r0 = 0; r0 < n_audio; r0 += piece) {
+        const size_t n = std::min(piece, n_audio - r0);
+        const char* x = static_cast<const char*>(enc) + r0 * static_cast<size_t>(enc_row_stride) * esize;
+        rc = linear_prepare(c, x_dtype, x, enc_row_stride, n, dm, dm, a);
         if (rc) return rc;
+        for (size_t l = 0; l < kv->n_layers; ++l) {
+          a.w[0] = static_cast<const _Float16*>(w_k[l]);
+          a.bias[0] = nullptr;
+          a.out[0] = k;
+          a.w[1] = static_cast<const _Float16*>(w_v[l]);
+          a.bias[1] = b_v ? b_v[l] : nullptr;
+          a.out[1] = v;
+          WRS_HIP(c, wrs::launch_linear_f16w(a, wrs::kF32, c->stream));
+          rc = write_rows(c, kv, k, v, n, kv->k_cross, kv->v_cross, kv->cross_off(l),
+                          kv->n_audio_max * 64, r0);
+          if (rc) return rc;
+        }
       }
       for (size_t l = 0; l < kv->n_layers; ++l) kv->cross_len[l] = n_audio;
       return WRS_OK;
     }
+    int rc = linear_prepare(c, x_dtype, enc, enc_row_stride, n_audio, dm, dm, a);
+    if (rc) return rc;
     a.out_rs = 64;  // [head][n_audio_max][64] planes
     a.out_hs = static_cast<int64_t>(kv->n_audio_max * 64);
     // decoder.rs:433-442: K without bias, V with cross_attn_v_b; every layer's
