@@ -208,6 +208,81 @@ def test_values_that_are_no_numbers(wrs, ctx, n):
             check(wrs, ctx, x[:1], some_tokens(1, v, 9), 4, allowed=ok)
 
 
+def rows_of_many_candidates(v, dtype):
+    """Rows of which many entries lie close to the best ones or equal them."""
+    i = torch.arange(v, device="cuda")
+    g = torch.Generator().manual_seed(13)
+    noise = torch.randint(0, 40, (v,), generator=g).cuda()
+    ulp = {"f32": 2.0 ** -23, "f16": 2.0 ** -10, "bf16": 2.0 ** -7}[dtype]
+    low = -65504.0
+    rows = [
+        torch.ones(v, device="cuda"),
+        1 + noise * ulp,                                    # a narrow band
+        (noise % 3).float(),                                # three values
+        torch.where(i % 2048 < 128, 5 + (i % 7) * ulp, 0),  # all entries of some threads, f32
+        torch.where(i % 4096 < 200, 5.0, low),
+        torch.where(i < min(1501, v), noise * 0.125, low),  # the others held down
+        torch.where(i >= v - 9, i % 5, low),                # fewer than are asked for, then equal ones
+        torch.where(i == v // 2, 1.0, low),
+        -(i // 64).float(),                                 # falling steps
+        (i // 600).float(),                                 # rising ones
+    ]
+    return torch.stack([r.float() for r in rows]).to(DT[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("v", [300, 2049, 4096, 4097, 8191, 51865, 262144])
+@pytest.mark.parametrize("k", [1, 5, 32])
+def test_many_candidates(wrs, ctx, dtype, v, k):
+    x = rows_of_many_candidates(v, dtype)
+    n = x.shape[0]
+    note(f"many candidates {dtype} {v} {k}")
+    ok = torch.rand(n, v, generator=torch.Generator().manual_seed(v)) < 0.6
+    for copies in (1, 30):  # rows split over workgroups where they are long, and whole
+        rows = x.repeat(copies, 1)
+        tokens = some_tokens(n * copies, v, 3)
+        check(wrs, ctx, rows, tokens, k)
+        if copies == 1:
+            check(wrs, ctx, rows, tokens, k, allowed=ok.cuda())
+            for row in range(n):
+                check(wrs, ctx, rows[row:row + 1], tokens[row:row + 1], k)
+
+
+def time_of(call):
+    """The least of several means over queued calls, in us."""
+    for _ in range(3):
+        call()
+    best = float("inf")
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(20):
+            call()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 50)
+    return best
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n,v,k", [(5, 51866, 10), (1, 51866, 32), (600, 4096, 7), (1, 262144, 32),
+                                   (130, 51865, 32)])
+def test_time_does_not_depend_on_values(wrs, ctx, dtype, n, v, k):
+    """Rows of many candidates take no more than three times what random ones do (ranked one against all
+    the others they took up to two hundred times that)."""
+    outs = [torch.zeros(n, k, dtype=torch.int32, device="cuda"), torch.zeros(n, k, device="cuda")]
+    h = torch.zeros(n, device="cuda")
+
+    def took(x):
+        return time_of(lambda: wrs.token_logprobs(x, entropy=h, top_ids=outs[0], top_logprobs=outs[1],
+                                                  ctx=ctx))
+    note(f"times {dtype} {n} {v} {k}")
+    usual = took(logits_of(n, v, dtype, seed=1))
+    for i, row in enumerate(rows_of_many_candidates(v, dtype)):
+        us = took(row.repeat(n, 1))
+        assert us <= 3 * usual, f"row {i}: {us:.1f} us, random values {usual:.1f}"
+
+
 def check_far(wrs, ctx, x, tokens, k, allowed=None, temperature=1.0):
     """check(), of rows whose smallest terms may lie below 2^-126: those come as zero, which is off by
     v 2^-126 < 1e-33 in the sum and 88 times that in the entropy. Log probabilities past f32's range are

@@ -8,7 +8,11 @@
 //   whose maxima are the k largest under the same order (value, then index): a bound from 64 maxima of
 //   neighbouring threads leaves few threads, and the entries of the chosen ones, a few hundred bytes
 //   each, are read again (where the bound leaves many, after the index of their largest entry has
-//   left k of them). Nothing else depends on values, so equal logits cost what others do.
+//   left k of them). Candidates are ranked one against all the others; of more than 256 (equal or nearly
+//   equal entries, a row held down by a finite mask) only those of k threads are. 5 rows of 51866 f32
+//   entries, 10 alternatives: random ones 9.0 us, equal ones 13.5, all but 1501 held down 11.8 (820 both,
+//   ranked whole); 600 rows of 4096, 32 alternatives 8.1 and 18.9 (1492). One row of 262144, 32
+//   alternatives, whose chunks' best ones are more than 256: 15 us, ranked whole 118.
 //   s is kept without the largest entry's 1 (its thread's entries are summed again, a piece a thread),
 //   and ln s = log1p of it: a token of probability 1 - 1e-7 has its log probability to 2^-22 too.
 //   Few rows split over several workgroups, which merge through memory (the last to count in joins
@@ -43,6 +47,7 @@ static_assert(kRun == 8, "max8");
 constexpr int kMostPieces = kScoreChunk / kThreads / 4;  // of a thread, at most (f32: 4 entries)
 static_assert(kMostPieces <= 64, "a piece a lane");
 constexpr int kMostKeys = kScoreMostTop * (kScoreChunk / kThreads);  // entries of that many threads
+constexpr int kMostRanked = 256;  // keys that are ranked one against all the others, at most
 constexpr int kCounterStride = 32;   // 128 bytes between merge counters
 // Exponents below it are 0: finite, so that times a weight of 0 it is 0. References lie at or above it,
 // and below -kLow where the sums against them are used.
@@ -219,23 +224,73 @@ __device__ inline void append(const uint64_t (&key)[kCount], const bool (&in)[kC
 }
 
 struct Shared {
-  union {
-    uint64_t keys[kMostKeys + 32];  // candidates
-    uint64_t first[kThreads];  // before them: threads' first largest entries
-  };
-  uint64_t best[kScoreMostTop];
+  uint64_t keys[kMostKeys + 32];  // candidates
+  uint64_t best[kScoreMostTop], bound_key;
   uint32_t least;
   uint32_t run_max[64];  // in order_of's numbers, the low bits a number of the run's own
   float wave_max[kWaves];
   float sums[2][kWaves];
   float piece[2][kMostPieces];  // sums of the pieces of the thread that holds the largest entry
   float bound;
-  int first_of[kThreads];  // whose they are
   int chosen[kThreads];    // threads whose entries are read again (-1 - thread: holds the largest)
   int equals[kMostPieces];  // entries of those pieces that equal it
   int tops[kWaves];
   int n_first, n_chosen, n_keys, last;
 };
+
+// The k-th best of the threads' keys (0: none), 0 if there are fewer. Takes the room of the candidates
+// and leaves none of them. Keys lie in the k runs of 8 threads whose best ones are the k best, so that
+// 8 k of them are ranked, however many there are.
+static_assert(kScoreMostTop * kRun <= kMostRanked, "runs of k");
+__device__ inline uint64_t kth_best(uint64_t mine, int k, Shared& sh) {
+  const int tid = threadIdx.x;
+  unsigned long long run = mine;
+#pragma unroll
+  for (int x = 1; x < kRun; x <<= 1) run = max(run, __shfl_xor(run, x));
+  __syncthreads();  // what was listed is read
+  if (tid % kRun == 0) sh.keys[tid / kRun] = run;
+  if (tid == 0) {
+    sh.bound_key = 0;
+    sh.n_keys = sh.n_first = 0;
+  }
+  __syncthreads();
+  int r = 0;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) r += sh.keys[kRun * (tid % kRun) + i] > run;
+  r = sum8(r);
+  if (tid % kRun == 0 && r == k - 1) sh.bound_key = run;
+  __syncthreads();
+  uint64_t* const list = sh.keys + kThreads / kRun;
+  const uint64_t key[1] = {mine};
+  const bool in[1] = {mine != 0 && mine >= sh.bound_key};
+  append(key, in, list, &sh.n_first);
+  __syncthreads();
+  const int n = sh.n_first;
+  rank_all(list, n, [&](int r, uint64_t key) __attribute__((always_inline)) {
+    if (r == k - 1) sh.best[r] = key;
+  });
+  __syncthreads();
+  return n < k ? 0 : sh.best[k - 1];
+}
+// Leaves the candidates that may be among the k best: those of k threads, 8 each.
+__device__ inline void cut(int k, Shared& sh) {
+  constexpr int kMine = kMostKeys / kThreads;
+  static_assert(kMine * kScoreMostTop <= kMostRanked, "keys that are left");
+  const int n = sh.n_keys;
+  uint64_t key[kMine], mine = 0;
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) {
+    const int i = threadIdx.x + kThreads * j;
+    key[j] = i < n ? sh.keys[i] : 0;
+    mine = key[j] > mine ? key[j] : mine;
+  }
+  const uint64_t least = kth_best(mine, k, sh);
+  bool in[kMine];
+#pragma unroll
+  for (int j = 0; j < kMine; ++j) in[j] = key[j] != 0 && key[j] >= least;
+  append(key, in, sh.keys, &sh.n_keys);
+  __syncthreads();
+}
 
 // One chunk: its largest entry m, the sums of the others (s = sum 2^z, t = sum z 2^z with z = scale (x
 // - m)) and its k best entries in sh.best, keys of entries that are not there 0. Every thread gets
@@ -443,6 +498,7 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
     if (n_chosen * per * kN > kMostKeys) {
       // .. or, where that could be too many, those of the k threads whose first largest entries are the
       // k best.
+      uint64_t mine = 0;
       if (in) {
         int first = 0;
 #pragma unroll
@@ -453,21 +509,14 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
           for (int e = kN - 1; e >= 0; --e)
             if (x[e] == m) first = i0 + e;
         }
-        const int i = atomicAdd(&sh.n_first, 1);
-        sh.first[i] = key_of(m, index0 + first);
-        sh.first_of[i] = is_top ? -1 - tid : tid;
+        mine = key_of(m, index0 + first);
       }
+      least = kth_best(mine, k, sh);
+      if (tid == 0) sh.n_chosen = 0;
       __syncthreads();
-      rank_all(sh.first, n_chosen, [&](int r, uint64_t key) __attribute__((always_inline)) {
-        if (r < k) sh.best[r] = key;
-      });
+      if (in && mine >= least) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = is_top ? -1 - tid : tid;
       __syncthreads();
-      if (tid < n_chosen)
-        for (int r = 0; r < min(n_chosen, k); ++r)
-          if (sh.best[r] == sh.first[tid]) sh.chosen[r] = sh.first_of[tid];
-      __syncthreads();
-      least = n_chosen > k ? sh.best[k - 1] : 0;
-      n_chosen = min(n_chosen, k);
+      n_chosen = sh.n_chosen;
     }
     // The chosen threads' entries again, a piece a thread.
     for (int i = tid; i < n_chosen * per; i += kThreads) {
@@ -496,6 +545,7 @@ __device__ inline void scan(const Row<T, kMask>& row, int index0, int k, float s
     add_up(apart ? 0.f : a, apart ? 0.f : b);
   }
   __syncthreads();
+  if (sh.n_keys > kMostRanked) cut(k, sh);
   const int n_keys = sh.n_keys;
   if (tid < k && tid >= n_keys) sh.best[tid] = 0;
   rank_all(sh.keys, n_keys, [&](int r, uint64_t key) __attribute__((always_inline)) {
@@ -602,6 +652,7 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
       with[q] = mine[q] && static_cast<uint32_t>(mine[q] >> 32) >= least;
     append(mine, with, sh.keys, &sh.n_keys);
     __syncthreads();
+    if (sh.n_keys > kMostRanked) cut(k, sh);
     const int n_keys = sh.n_keys;
     rank_all(sh.keys, n_keys, [&](int p, uint64_t key) __attribute__((always_inline)) {
       if (p < k) sh.best[p] = key;
