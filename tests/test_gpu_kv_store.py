@@ -460,3 +460,67 @@ def test_a_cross_projection_of_many_pieces(wrs, ctx, dtype, frames):
         err = (got.double().reshape(frames, heads, D) - want).abs()
         assert (err <= largest * (1 / 127.5 + 2.0 ** -10)).all()
     ar.close()
+
+
+# ---- slots of unlike lengths -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("name", ["f16", "f32", "i8"])
+@pytest.mark.parametrize("counts", [[1] * 40 + [500], [500] + [1] * 69, [1] * 7 + [500],
+                                    [300] + [1] * 15, [i * 7 % 97 for i in range(70)], [15, 1, 2, 9],
+                                    [0, 16, 0, 1, 33, 0], [2] * 63 + [65, 1]])
+def test_unlike_slots_in_one_call(wrs, ctx, name, counts):
+    heads = 7
+    d, n, n_slots = heads * D, sum(counts), len(counts)
+    ar = wrs.KvArena(1, n_slots, heads, 512, 0, ctx=ctx, dtype=_dtype(wrs, name))
+    slots = [(11 * i + 3) % n_slots if n_slots % 11 else n_slots - 1 - i for i in range(n_slots)]
+    pasts = [i % 12 for i in range(n_slots)]
+    guard = torch.full((512, d), 2.0, device="cuda")
+    for s, p in zip(slots, pasts):
+        ar.append_rows(0, [s], [512], guard, guard)
+        ar.advance(s, p)
+    k, v = normal(n, d, seed=n), normal(n, d, seed=n + 1)
+    note(f"unlike {name} {counts[:4]}")
+    ar.append_rows(0, slots, counts, k, v)
+    row = 0
+    for s, p, c in zip(slots, pasts, counts):
+        gk, gv = read(ar, 0, s, 0, 512)
+        for got, x in ((gk, k), (gv, v)):
+            want = guard.double()
+            want[p:p + c] = stored(x[row:row + c].contiguous(), name) if c else want[p:p + c]
+            assert same(got, want)
+        row += c
+    gk, gv = (torch.zeros(n, d, device="cuda") for _ in range(2))
+    ar.read_rows(0, slots, pasts, counts, gk, gv)
+    torch.cuda.synchronize()
+    assert same(gk, stored(k, name)) and same(gv, stored(v, name))
+    ar.close()
+
+
+@pytest.mark.parametrize("name", ["f16", "i8"])
+def test_single_tokens_beside_a_text_cost_little(wrs, ctx, name):
+    heads, text, singles = 20, 8191, 15
+    d = heads * D
+    ar = wrs.KvArena(1, singles + 1, heads, text, 0, ctx=ctx, dtype=_dtype(wrs, name))
+    k, v = (torch.randn(text + singles, d, device="cuda") for _ in range(2))
+
+    def took(call):
+        for _ in range(3):
+            call()
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(20):
+                call()
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 50)
+        return best
+
+    note(f"mixed append {name}")
+    alone = took(lambda: ar.append_rows(0, [0], [text], k[:text], v[:text]))
+    slots, counts = list(range(singles + 1)), [text] + [1] * singles
+    mixed = took(lambda: ar.append_rows(0, slots, counts, k, v))
+    assert mixed <= 1.8 * alone, (mixed, alone)
+    ar.close()

@@ -85,19 +85,35 @@ constexpr int64_t kOnce = 128 << 20;  // bytes that are read past the caches
 // A workgroup takes rows of a head, 16 lanes each: the next 16 of all heads', or 32 of one head.
 enum class Order { kAllHeads, kByHead, kByHeadOnce };
 constexpr int block_rows(bool by_head) { return by_head ? 32 : 16; }
-template <DType kD, bool kStore, Order kOrder, int kSlots>
+// Workgroups that a slot's K (or V) rows take.
+__host__ __device__ inline int slot_blocks(bool by_head, int rows, int n_heads) {
+  const int n = block_rows(by_head);
+  return by_head ? (rows + n - 1) / n * n_heads : (rows * n_heads + n - 1) / n;
+}
+// kInTurn: the slots' workgroups follow each other; else each has as many as the longest one.
+template <DType kD, bool kStore, Order kOrder, bool kInTurn, int kSlots>
 __global__ __launch_bounds__(256) void kv_rows(KvSlotRows<kSlots> a) {
   constexpr bool kByHead = kOrder != Order::kAllHeads;
   constexpr int kBlockRows = block_rows(kByHead), kTurns = kBlockRows / 16;
-  const int u = blockIdx.z, rows_here = a.count[u], sub = threadIdx.x >> 4;
+  int u = blockIdx.z, block = blockIdx.x;
+  if constexpr (kInTurn) {
+    // Slots past the last one start past every workgroup.
+    u = -1;
+    for (int i = 0; i < a.n_slots; i += 8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u += a.wg0[i + j] <= block;
+    }
+    block -= a.wg0[u];
+  }
+  const int rows_here = a.count[u], sub = threadIdx.x >> 4;
   // The block's first row of a head and that head, or its first row in turn.
   int64_t first;
   int head = 0;
   if constexpr (kByHead)
     first = static_cast<int64_t>(kBlockRows) *
-            divide(static_cast<int>(blockIdx.x), a.n_heads, a.heads_inv, head);
+            divide(block, a.n_heads, a.heads_inv, head);
   else
-    first = static_cast<int64_t>(kBlockRows) * blockIdx.x;
+    first = static_cast<int64_t>(kBlockRows) * block;
   const int64_t n = kByHead ? rows_here : static_cast<int64_t>(rows_here) * a.n_heads;
   if (first >= n) return;
   float* const rows = (blockIdx.y ? a.v_rows : a.k_rows) + a.row0[u] * (blockIdx.y ? a.v_rs : a.k_rs);
@@ -246,7 +262,8 @@ __global__ __launch_bounds__(64 * kKeepWaves) void kv8_keep_rows(KeepArgs<kSlots
 }  // namespace
 
 template <int kSlots>
-hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store, hipStream_t s) {
+hipError_t launch_kv_slot_rows(KvSlotRows<kSlots>& a, DType dt, bool store, hipStream_t s) {
+  static_assert(kSlots % 8 == 0, "read 8 at a time");
   int most = 0;
   int64_t all = 0;
   for (int u = 0; u < a.n_slots; ++u) {
@@ -254,28 +271,42 @@ hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store
     all += a.count[u];
   }
   if (most <= 0 || a.n_heads <= 0) return hipSuccess;
-  const int64_t rows = static_cast<int64_t>(most) * a.n_heads;
-  if (rows > 0x7fffffff - 64) return hipErrorInvalidConfiguration;
+  if (static_cast<int64_t>(most) * a.n_heads > 0x7fffffff - 64) return hipErrorInvalidConfiguration;
   const bool by_head = most >= kManyRows, once = all * a.n_heads * 512 > kOnce;
-  const int block = block_rows(by_head);
-  const int64_t blocks = by_head ? (most + block - 1) / block * static_cast<int64_t>(a.n_heads)
-                                 : (rows + block - 1) / block;
-  const dim3 grid(static_cast<unsigned>(blocks), 2, a.n_slots);
-#define WRS_KV_ROWS_ONE(D, S, O) \
-  hipLaunchKernelGGL((kv_rows<D, S, Order::O, kSlots>), grid, dim3(256), 0, s, a)
+  const int widest = slot_blocks(by_head, most, a.n_heads);
+  int64_t sum = 0;
+  for (int u = 0; u < kSlots; ++u) {
+    a.wg0[u] = u < a.n_slots ? static_cast<int>(std::min<int64_t>(sum, 0x7fffffff)) : 0x7fffffff;
+    if (u < a.n_slots) sum += slot_blocks(by_head, a.count[u], a.n_heads);
+  }
+  // A grid as wide as the longest slot for each of them has empty workgroups, of which 5000 cost 1 us; slots
+  // in turn cost a search (2 to 5% where few are empty). In turn and wide, 20 heads, 8-bit: a text of
+  // 8191 rows and 15 single tokens 19 and 49 us, 2 of them 19.5 and 21.5, 1500 rows and 7 single tokens
+  // 5.6 and 6.7, 3 pieces of 100 rows 6.1 and 5.7; 16 slots of 1, 101, .. 1501 rows 25.1 and 24.3.
+  const int64_t wide = widest * static_cast<int64_t>(a.n_slots);
+  const bool in_turn = by_head && sum <= 0x7fffffff && 2 * wide > 5 * sum && wide - sum > 4096;
+  const dim3 grid(static_cast<unsigned>(in_turn ? sum : widest), 2, in_turn ? 1 : a.n_slots);
+#define WRS_KV_ROWS_ONE(D, S, O, T) \
+  hipLaunchKernelGGL((kv_rows<D, S, Order::O, T, kSlots>), grid, dim3(256), 0, s, a)
+#define WRS_KV_ROWS_STORE(D, O, T)                                            \
+  if (store) {                                                                \
+    WRS_KV_ROWS_ONE(D, true, O, T);                                           \
+  } else {                                                                    \
+    WRS_KV_ROWS_ONE(D, false, O, T);                                          \
+  }
 #define WRS_KV_ROWS(D)                                                        \
   if (!by_head) {                                                             \
-    if (store) {                                                              \
-      WRS_KV_ROWS_ONE(D, true, kAllHeads);                                    \
+    WRS_KV_ROWS_STORE(D, kAllHeads, false);                                   \
+  } else if (store && once) {                                                 \
+    if (in_turn) {                                                            \
+      WRS_KV_ROWS_ONE(D, true, kByHeadOnce, true);                            \
     } else {                                                                  \
-      WRS_KV_ROWS_ONE(D, false, kAllHeads);                                   \
+      WRS_KV_ROWS_ONE(D, true, kByHeadOnce, false);                           \
     }                                                                         \
-  } else if (!store) {                                                        \
-    WRS_KV_ROWS_ONE(D, false, kByHead);                                       \
-  } else if (once) {                                                          \
-    WRS_KV_ROWS_ONE(D, true, kByHeadOnce);                                    \
+  } else if (in_turn) {                                                       \
+    WRS_KV_ROWS_STORE(D, kByHead, true);                                      \
   } else {                                                                    \
-    WRS_KV_ROWS_ONE(D, true, kByHead);                                        \
+    WRS_KV_ROWS_STORE(D, kByHead, false);                                     \
   }
   switch (dt) {
     case kF32: WRS_KV_ROWS(kF32); break;
@@ -284,11 +315,12 @@ hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store
     default: return hipErrorInvalidValue;
   }
 #undef WRS_KV_ROWS
+#undef WRS_KV_ROWS_STORE
 #undef WRS_KV_ROWS_ONE
   return hipGetLastError();
 }
-template hipError_t launch_kv_slot_rows(const KvSlotRows<kRowSlots>&, DType, bool, hipStream_t);
-template hipError_t launch_kv_slot_rows(const KvSlotRows<kRowFewSlots>&, DType, bool, hipStream_t);
+template hipError_t launch_kv_slot_rows(KvSlotRows<kRowSlots>&, DType, bool, hipStream_t);
+template hipError_t launch_kv_slot_rows(KvSlotRows<kRowFewSlots>&, DType, bool, hipStream_t);
 
 hipError_t launch_kv8_copy(const Kv8Planes& to, const Kv8Planes& from, int n_layers, int n_heads,
                            int len, hipStream_t s) {

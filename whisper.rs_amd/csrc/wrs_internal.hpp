@@ -575,9 +575,10 @@ struct KvSlotRows {
   uint32_t heads_inv;  // 2^32 / n_heads, as divide() takes it
   int64_t plane[kSlots], row0[kSlots];
   int pos[kSlots], count[kSlots];
+  int wg0[kSlots];  // by the launch: the slots' first workgroups, where they follow each other
 };
 template <int kSlots>
-hipError_t launch_kv_slot_rows(const KvSlotRows<kSlots>& a, DType dt, bool store, hipStream_t s);
+hipError_t launch_kv_slot_rows(KvSlotRows<kSlots>& a, DType dt, bool store, hipStream_t s);
 // The planes of an 8-bit arena's slot: plane (l, h) is plane l*layer + h, of `rows` rows of codes
 // and `scale_rows` scales.
 struct Kv8Planes {
