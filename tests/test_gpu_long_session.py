@@ -271,6 +271,26 @@ def test_the_widest_and_the_narrowest_window(wrs, name, window):
     c.close()
 
 
+@pytest.mark.parametrize("name", ["f16", "f32", "i8"])
+def test_windows_past_64_bits(wrs, name):
+    """Counts of keys that no size_t holds are all of the keys."""
+    c = wrs.Context(0)
+    c.use_torch_stream()
+    s = Session(wrs, c, name, 2, [130], [3], seed=13)
+    note(f"huge windows {name}")
+    outs = []
+    for window, sinks in ((None, 0), (2 ** 64, 0), (2 ** 64 + 3, 0), (2, 2 ** 64), (5, 2 ** 70 + 1)):
+        out = torch.zeros(3, 2 * D, device="cuda")
+        s.arena.window_self(1, [0], [3], window, sinks, s.q, out)
+        outs.append(out)
+    torch.cuda.synchronize()
+    want, tol = s.expect(10 ** 6, 0)
+    for out in outs:
+        assert (out.double() - want).abs().max().item() <= tol
+    s.arena.close()
+    c.close()
+
+
 @pytest.mark.parametrize("name,rows", [("f32", 9_000_000), ("f16", 16_000_000), ("i8", 16_000_000)])
 def test_far_rows_of_a_long_cache(wrs, name, rows):
     """Planes of gigabytes: rows behind 2^31 bytes of their plane, planes behind 2^32 bytes."""

@@ -748,7 +748,9 @@ class KvArena:
         stride."""
         n, args = self._device_rows("window_self", q, out)
         assert len(slots) == len(counts) and sum(counts) == n
-        window = 2 ** 64 - 1 if window is None else window
+        # Past size_t ctypes would drop the upper bits.
+        window = 2 ** 64 - 1 if window is None else min(window, 2 ** 64 - 1)
+        sinks = min(sinks, 2 ** 64 - 1)
         assert window > 0 and sinks >= 0
         self._c(self._lib.wrs_attn_window_self(self.ctx.handle, self.handle, layer, _packed(slots),
                                                _packed(counts), len(slots), window, sinks, *args),
