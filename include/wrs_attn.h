@@ -202,12 +202,12 @@ int wrs_attn_prefill(wrs_attn_ctx *ctx, int q_dtype, const void *q, const wrs_la
  * Or 8-bit codes (WRS_I8; no reference counterpart), for long sessions: a row of
  * a head is 64 whole numbers times a power of two, the least that leaves none past
  * 127, so 65 bytes against 128 or 256; a value is off by at most 2/255 of its row's
- * largest (of each head), and rows with an infinity or NaN read as NaN. A row has a
+ * largest (of each head; by 2^-127 where that is below 2^-120), and rows with an infinity or NaN read as NaN. A row has a
  * scale to itself, so storing, moving, cutting and sliding rows never rounds
  * another one, and rows that were read back store as the same codes. Attention runs on
  * the codes, q and the products of weight and value scale in two f16 parts each (2^-22,
  * small ones within 2^-40 of the row's largest element and 2^-31 of its largest product, for
- * values of 2^-80 and more and keys below 2^100), the cross calls with any 16-byte aligned q and any rows as
+ * values of 2^-80 to 2^100 and keys below 2^100), the cross calls with any 16-byte aligned q and any rows as
  * on f16 arenas; a row of q with an infinity or NaN gives NaN. Planes hold up to
  * 2^24 - 4096 rows.
  * wrs_attn_decode_cross_noalloc, the _lse pair, wrs_attn_capture_cross_heads and

@@ -696,7 +696,9 @@ __global__ __launch_bounds__(kThreads, 8) void score_rows(ScoreArgs a) {
 
 void score_plan(ScoreArgs& a, bool split) {
   // A workgroup a CU and no more: f32 rows of 51865 entries, a workgroup a row, up to 256 and up to
-  // 520 workgroups: 16 rows 9.0, 8.1, 8.2 us, 40 rows 9.8, 9.4, 11.1 us, 130 rows 11.2, 11.2, 15.9 us.
+  // 520 workgroups: 16 rows 9.0, 8.1, 8.2 us, 40 rows 9.8, 9.4, 11.1 us, 130 rows 11.2, 11.2, 15.9 us. With
+  // one, two and three workgroups a row 86 rows take 8.5, 9.5 and 10.2 us, 130 9.0, 11.7 and 11.0, 200 10.9,
+  // 14.0 and 15.7 (with a mask each 10.5, 10.9, 11.7; 10.9, 14.3, 12.8; 13.0, 17.0, 18.0).
   int64_t chunks = 1;
   if (split) chunks = std::max<int64_t>(1, kScoreMaxWgs / std::max<int64_t>(a.n_rows, 1));
   chunks = std::min<int64_t>(chunks, (a.n_vocab + kScoreSmall - 1) / kScoreSmall);
